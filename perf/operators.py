@@ -321,7 +321,7 @@ def _cross(s):
     return {"out": out}
 
 
-_LEAST = 2.0 ** -47  # a token of less weight beside the likeliest one is never drawn
+_LEAST = 2.0 ** -45  # a token of less weight beside the likeliest one is never drawn
 
 
 def _sample(s):
