@@ -20,6 +20,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // device error word bits (read and cleared by nllb_attn_sync)
 constexpr int NLLB_DEV_ERR_TIMEOUT = 1;
 constexpr int NLLB_DEV_ERR_BAD_PARENT = 2;
+constexpr int NLLB_DEV_ERR_BAD_PAGE = 4;    // page number outside the pool
+constexpr int NLLB_DEV_ERR_BAD_LENGTH = 8;  // start or length outside its buffer or bound
 
 // ~1 s at 2 GHz: far above any legitimate wait for a copy of a few KB.
 constexpr long long kWaitBudgetCycles = 2000000000LL;

@@ -13,6 +13,7 @@
 #include "attn_internal.h"
 #include "device_common.cuh"
 #include "kernels.h"
+#include "rows.h"
 
 using namespace nllb;
 
@@ -104,6 +105,9 @@ int check_device_error(nllb_attn_ctx* c) {
     NLLB_CK(cudaMemset(c->err, 0, sizeof(int)));
     if (e & NLLB_DEV_ERR_TIMEOUT)
         return fail(NLLB_ATTN_ETIMEOUT, "a kernel's bounded wait for a bulk copy gave up");
+    if (e & NLLB_DEV_ERR_BAD_PAGE) return fail(NLLB_ATTN_EINVAL, "page number outside [0, n_pages)");
+    if (e & NLLB_DEV_ERR_BAD_LENGTH)
+        return fail(NLLB_ATTN_EINVAL, "a sequence's start or length lies outside its buffer or bound");
     return fail(NLLB_ATTN_EINVAL, "reorder: parent index outside [0, n_beams)");
 }
 
@@ -242,6 +246,7 @@ int nllb_attn_create(int device, const nllb_attn_dims* dims, nllb_attn_ctx** out
     NLLB_CKC(cudaSetDevice(device));
     NLLB_CKC(configure_decode_kernels());
     NLLB_CKC(configure_prefill_kernels());
+    NLLB_CKC(configure_rows_kernels());
     NLLB_CKC(cudaStreamCreateWithFlags(&c->own_stream, cudaStreamNonBlocking));
     c->stream = c->own_stream;
     const nllb_attn_dims& d = c->d;

@@ -55,6 +55,37 @@ class KernelProfile(ctypes.Structure):
                 ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
 
 
+F32, F16, BF16 = range(3)
+
+
+class PagedArgs(ctypes.Structure):
+    _fields_ = ([(n, _fp) for n in ("q", "k_new", "v_new", "k_pages", "v_pages", "out", "q_start", "q_len", "kv_len",
+                                    "page_table")]
+                + [(n, ctypes.c_int) for n in ("dtype", "head_dim", "n_heads", "n_kv_heads", "n_seq", "q_rows",
+                                               "max_q", "max_kv", "n_pages", "page_size", "page_table_stride")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int64) for n in (
+                    "q_stride_row", "q_stride_head", "out_stride_row", "out_stride_head", "k_new_stride_row",
+                    "k_new_stride_head", "v_new_stride_row", "v_new_stride_head", "k_stride_page", "k_stride_slot",
+                    "k_stride_head", "v_stride_page", "v_stride_slot", "v_stride_head")])
+
+
+class CrossRowsArgs(ctypes.Structure):
+    _fields_ = ([(n, _fp) for n in ("q", "k", "v", "out", "q_start", "q_len", "kv_start", "kv_len", "key_mask")]
+                + [(n, ctypes.c_int) for n in ("dtype", "head_dim", "n_heads", "n_kv_heads", "n_seq", "q_rows",
+                                               "kv_rows", "max_q", "max_kv")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int64) for n in (
+                    "q_stride_row", "q_stride_head", "k_stride_row", "k_stride_head", "v_stride_row",
+                    "v_stride_head", "out_stride_row", "out_stride_head")])
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("logits", _fp), ("ld", ctypes.c_longlong), ("dtype", ctypes.c_int), ("vocab", ctypes.c_int),
+                ("rows", ctypes.c_int), ("temperature", _fp), ("top_k", _fp), ("top_p", _fp), ("min_p", _fp),
+                ("u", _fp), ("out_tok", _fp), ("out_logp", _fp)]
+
+
 PROF_CLASSES = 14
 
 SIGNATURES = {
@@ -81,6 +112,8 @@ SIGNATURES = {
                                            ctypes.c_int64, ctypes.c_int64]),
     "nllb_attn_cross": (_c_int, [_c_void_p, _c_int, _c_int, _fp, _fp]),
     "nllb_attn_cross_host": (_c_int, [_c_void_p, _c_int, _c_int, _fp, _fp]),
+    "nllb_attn_paged": (_c_int, [_c_void_p, ctypes.POINTER(PagedArgs)]),
+    "nllb_attn_cross_rows": (_c_int, [_c_void_p, ctypes.POINTER(CrossRowsArgs)]),
     "nllb_attention_head": (None, [_fp, _fp, _fp, _fp, _fp, _fp, _c_int, _c_int]),
     "nllb_attention_head_flash": (None, [_fp, _fp, _fp, _fp, _fp, _c_int, _c_int]),
     "nllb_attn_last_status": (_c_int, []),
@@ -107,6 +140,7 @@ SIGNATURES = {
                                       _c_void_p]),
     "nllb_logsoftmax_topk_ws_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
     "nllb_logsoftmax_topk": (_c_int, [_fp, ctypes.c_longlong, _c_int, _c_int, _c_int, _fp, _fp, _fp, _c_void_p]),
+    "nllb_sample": (_c_int, [ctypes.POINTER(SampleArgs), _c_void_p]),
 }
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -156,6 +190,31 @@ def ptr(x) -> Optional[int]:
             raise ValueError("array must be C-contiguous")
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)!r}")
+
+
+def _dtype_code(x) -> int:
+    try:
+        return {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}[str(x.dtype)]
+    except KeyError:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, not {x.dtype}") from None
+
+
+def _rows(x, name, like, axes):
+    """Address of a tensor of rows whose last axis is contiguous."""
+    if x.dim() != axes or x.dtype != like.dtype or x.shape[-1] != like.shape[-1] or x.device != like.device:
+        raise ValueError(f"{name} must have {axes} axes and the type, last size and device of q")
+    if x.numel() and x.stride(-1) != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+    return x.data_ptr()
+
+
+def _ints(x, name, n, like, dtype="torch.int32"):
+    """Address of a contiguous device array of n entries (None passes NULL)."""
+    if x is None:
+        return None
+    if str(x.dtype) != dtype or x.numel() != n or not x.is_contiguous() or x.device != like.device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} entries on q's device")
+    return x.data_ptr()
 
 
 class Context:
@@ -263,6 +322,87 @@ class Context:
     def cross_host(self, layer, n_sent, q, out) -> None:
         _check(self.lib, self.lib.nllb_attn_cross_host(self.handle, layer, n_sent, ptr(q),
                                                        ptr(out)), "cross_host")
+
+
+    # -- many query rows against keys of another length --
+    @staticmethod
+    def paged_args(q, k_pages, v_pages, page_table, kv_len, out, k_new=None, v_new=None, q_start=None, q_len=None,
+                   max_q=None, max_kv=None, scale=None) -> PagedArgs:
+        """Arguments of :meth:`paged` from torch CUDA tensors, which the caller
+        keeps alive: q, out [rows][heads][dim], k_new, v_new
+        [rows][kv_heads][dim], pages [n_pages][page_size][kv_heads][dim] (any
+        strides, the last axis contiguous), page_table [n_seq][entries] int32.
+        max_q defaults to q's rows / n_seq without q_len and to q's rows with
+        it, max_kv to what the table holds, scale to dim ** -0.5."""
+        n_seq, (rows, heads, dim) = kv_len.numel(), q.shape
+        n_pages, page, kv_heads = k_pages.shape[:3]
+        if out.shape != q.shape or v_pages.shape != k_pages.shape:
+            raise ValueError("out must have q's shape, v_pages k_pages's")
+        if (k_new is None) != (v_new is None):
+            raise ValueError("k_new and v_new go together")
+        if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32" or page_table.shape[0] != n_seq \
+                or (page_table.numel() and page_table.stride(1) != 1) or page_table.device != q.device:
+            raise ValueError("page_table must be an int32 tensor [n_seq][entries] on q's device")
+        # (a one-row table's stride may be anything: its entries bound it)
+        table_ld = page_table.stride(0) if n_seq > 1 else page_table.shape[1]
+        if max_q is None:
+            max_q = rows if q_len is not None else rows // max(n_seq, 1)
+        if max_kv is None:
+            max_kv = page_table.shape[1] * page
+        if max_kv > page_table.shape[1] * page:
+            raise ValueError("page_table has too few entries for max_kv")
+        a = PagedArgs(q=_rows(q, "q", q, 3), out=_rows(out, "out", q, 3), k_pages=_rows(k_pages, "k_pages", q, 4),
+                      v_pages=_rows(v_pages, "v_pages", q, 4), q_start=_ints(q_start, "q_start", n_seq, q),
+                      q_len=_ints(q_len, "q_len", n_seq, q), kv_len=_ints(kv_len, "kv_len", n_seq, q),
+                      page_table=page_table.data_ptr(), dtype=_dtype_code(q), head_dim=dim, n_heads=heads,
+                      n_kv_heads=kv_heads, n_seq=n_seq, q_rows=rows, max_q=max_q, max_kv=max_kv, n_pages=n_pages,
+                      page_size=page, page_table_stride=table_ld, scale=dim ** -0.5 if scale is None else scale,
+                      q_stride_row=q.stride(0), q_stride_head=q.stride(1),
+                      out_stride_row=out.stride(0), out_stride_head=out.stride(1),
+                      k_stride_page=k_pages.stride(0), k_stride_slot=k_pages.stride(1),
+                      k_stride_head=k_pages.stride(2), v_stride_page=v_pages.stride(0),
+                      v_stride_slot=v_pages.stride(1), v_stride_head=v_pages.stride(2))
+        if k_new is not None:
+            if k_new.shape != (rows, kv_heads, dim) or v_new.shape != k_new.shape:
+                raise ValueError("k_new and v_new must be [q rows][kv_heads][dim]")
+            a.k_new, a.v_new = _rows(k_new, "k_new", q, 3), _rows(v_new, "v_new", q, 3)
+            a.k_new_stride_row, a.k_new_stride_head = k_new.stride(0), k_new.stride(1)
+            a.v_new_stride_row, a.v_new_stride_head = v_new.stride(0), v_new.stride(1)
+        return a
+
+    def paged(self, args: PagedArgs) -> None:
+        """nllb_attn_paged: a chunk of new tokens over a paged cache."""
+        _check(self.lib, self.lib.nllb_attn_paged(self.handle, ctypes.byref(args)), "nllb_attn_paged")
+
+    @staticmethod
+    def cross_rows_args(q, k, v, out, kv_len, q_start=None, q_len=None, kv_start=None, max_q=None, max_kv=None,
+                        key_mask=None, scale=None) -> CrossRowsArgs:
+        """Arguments of :meth:`cross_rows` from torch CUDA tensors, which the
+        caller keeps alive: q, out [rows][heads][dim], k, v
+        [kv_rows][kv_heads][dim] (any strides, the last axis contiguous),
+        key_mask [kv_rows] uint8.  max_q and max_kv default to rows / n_seq
+        without the lengths' starts and to all rows with them."""
+        n_seq, (rows, heads, dim), (kv_rows, kv_heads) = kv_len.numel(), q.shape, k.shape[:2]
+        if out.shape != q.shape or v.shape != k.shape:
+            raise ValueError("out must have q's shape, v k's")
+        if max_q is None:
+            max_q = rows if q_len is not None else rows // max(n_seq, 1)
+        if max_kv is None:
+            max_kv = kv_rows if kv_start is not None else kv_rows // max(n_seq, 1)
+        return CrossRowsArgs(
+            q=_rows(q, "q", q, 3), k=_rows(k, "k", q, 3), v=_rows(v, "v", q, 3), out=_rows(out, "out", q, 3),
+            q_start=_ints(q_start, "q_start", n_seq, q), q_len=_ints(q_len, "q_len", n_seq, q),
+            kv_start=_ints(kv_start, "kv_start", n_seq, q), kv_len=_ints(kv_len, "kv_len", n_seq, q),
+            key_mask=_ints(key_mask, "key_mask", kv_rows, q, "torch.uint8"), dtype=_dtype_code(q), head_dim=dim,
+            n_heads=heads, n_kv_heads=kv_heads, n_seq=n_seq, q_rows=rows, kv_rows=kv_rows, max_q=max_q,
+            max_kv=max_kv, scale=dim ** -0.5 if scale is None else scale,
+            q_stride_row=q.stride(0), q_stride_head=q.stride(1), k_stride_row=k.stride(0), k_stride_head=k.stride(1),
+            v_stride_row=v.stride(0), v_stride_head=v.stride(1), out_stride_row=out.stride(0),
+            out_stride_head=out.stride(1))
+
+    def cross_rows(self, args: CrossRowsArgs) -> None:
+        """nllb_attn_cross_rows: target rows over encoder states of another length."""
+        _check(self.lib, self.lib.nllb_attn_cross_rows(self.handle, ctypes.byref(args)), "nllb_attn_cross_rows")
 
 
 def attention_head_flash(Q, K, V, mask, out, seq_len: int, head_dim: int = 64) -> int:
@@ -406,6 +546,30 @@ def logsoftmax_topk(logits, k=8, vocab=None, stream=None):
     _check(lib, lib.nllb_logsoftmax_topk(ptr(logits), logits.stride(0), V, rows, k, ptr(tok), ptr(lp), ptr(ws),
                                          stream), "nllb_logsoftmax_topk")
     return tok, lp
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_tok=None, out_logp=None,
+           stream=None):
+    """nllb_sample on torch CUDA tensors: logits [rows][vocab] (rows may be
+    strided), u [rows] fp32; temperature, top_p, min_p [rows] fp32 and top_k
+    [rows] int32 or None.  Returns (tokens [rows] int32, log-probabilities
+    [rows] fp32)."""
+    lib = load()
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("the rows of logits must be contiguous")
+    if out_tok is None or out_logp is None:
+        import torch
+        out_tok = torch.empty(rows, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
+        out_logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
+    f = "torch.float32"
+    a = SampleArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _dtype_code(logits), vocab, rows,
+                   _ints(temperature, "temperature", rows, logits, f), _ints(top_k, "top_k", rows, logits),
+                   _ints(top_p, "top_p", rows, logits, f), _ints(min_p, "min_p", rows, logits, f),
+                   _ints(u, "u", rows, logits, f), _ints(out_tok, "out_tok", rows, logits),
+                   _ints(out_logp, "out_logp", rows, logits, f))
+    _check(lib, lib.nllb_sample(ctypes.byref(a), stream), "nllb_sample")
+    return out_tok, out_logp
 
 
 class PreparedLinear:

@@ -22,6 +22,8 @@
  *    run, copy outputs back and return once the outputs are written, the way
  *    the reference's call sites use their stack and heap buffers.
  *  - fp32 in, fp32 out.  head_dim must be 64 (NLLB-200: 16 heads x 64).
+ *    (nllb_attn_paged and nllb_attn_cross_rows also take 16-bit types and
+ *    heads of 128; their rows lie at the strides of their arguments.)
  *  - Rows of q/k/v/out hold all heads, head h at columns [64h, 64h+64), as the
  *    reference's projections produce them (decoder.c:57-59, encoder.c:159-163).
  *  - One context belongs to one device and is used by one host thread at a
@@ -194,6 +196,95 @@ NLLB_ATTN_API int nllb_attn_cross(nllb_attn_ctx* ctx, int layer, int n_sentences
                     const float* q, float* out);
 NLLB_ATTN_API int nllb_attn_cross_host(nllb_attn_ctx* ctx, int layer, int n_sentences,
                          const float* q, float* out);
+
+/* ---- many query rows against keys of another length ----------------------
+ * Two calls for a decoder that draws its tokens (nllb_sample) or scores given
+ * target rows: a chunk of new tokens over a paged cache, and target rows over
+ * encoder states.  No counterpart in the reference, whose decoder moves one
+ * token at a time (decoder.c:48-152).
+ *
+ * Types: q, k, v and out are all fp32, all fp16 or all bf16.  Scores, softmax
+ * sums and outputs are accumulated in fp32 and an output is rounded once.
+ * The weights of 16-bit calls of many rows are rounded to the type before
+ * their product with V; fp32 calls of many rows split q, k and v into two
+ * fp16 parts, which keeps fp32 accuracy for |q|, |k|, |v| < 65504.
+ * n_heads is a multiple of n_kv_heads: query head h reads key head
+ * h / (n_heads / n_kv_heads).  head_dim is 64 or 128.
+ * Sequence s has q_len[s] query rows from row q_start[s] of q and out
+ * (device arrays; q_len NULL: max_q rows each, q_start NULL: s * max_q).
+ * Rows of q and out that belong to no sequence are neither read nor written.
+ * Strides count elements; every row must start on 16 bytes (out may not
+ * overlap an input).  max_q and max_kv bound the lengths: they size the
+ * launch, larger lengths on the device are refused there.  A length, start
+ * or page number outside its bound or buffer sets the device error word
+ * (nllb_attn_sync then returns NLLB_ATTN_EINVAL): a sequence with a bad
+ * length or start is left out, a key on a bad page is left out of the
+ * attention.  The calls allocate nothing and may be captured into a graph. */
+#define NLLB_F32  0
+#define NLLB_F16  1
+#define NLLB_BF16 2
+
+/* A chunk of new tokens over a paged cache.  Slot r of page p, key head g is
+ * at k_pages + p*k_stride_page + r*k_stride_slot + g*k_stride_head; key j of
+ * sequence s lies in slot j % page_size of page
+ * page_table[s*page_table_stride + j / page_size].  kv_len[s] counts the keys
+ * with the chunk: new token i stands at position kv_len[s] - q_len[s] + i and
+ *    out_i = sum_{j <= its position} softmax_j(scale * q_i . k_j) v_j.
+ * With k_new and v_new (both or neither; rows as q's) the call also writes
+ * the chunk's keys and values into their slots; without, they are there
+ * already.  The slots written belong to one sequence each: a page that two
+ * sequences of a call share may only hold keys from before both chunks.
+ * Entries of page_table past a sequence's last page are not read. */
+typedef struct {
+    const void* q;
+    const void* k_new;
+    const void* v_new;
+    void*       k_pages;
+    void*       v_pages;
+    void*       out;
+    const int*  q_start;
+    const int*  q_len;
+    const int*  kv_len;
+    const int*  page_table;
+    int dtype, head_dim, n_heads, n_kv_heads;
+    int n_seq, q_rows, max_q, max_kv;
+    int n_pages, page_size, page_table_stride;
+    float scale;
+    int64_t q_stride_row, q_stride_head;
+    int64_t out_stride_row, out_stride_head;
+    int64_t k_new_stride_row, k_new_stride_head;
+    int64_t v_new_stride_row, v_new_stride_head;
+    int64_t k_stride_page, k_stride_slot, k_stride_head;
+    int64_t v_stride_page, v_stride_slot, v_stride_head;
+} nllb_attn_paged_args;
+
+NLLB_ATTN_API int nllb_attn_paged(nllb_attn_ctx* ctx, const nllb_attn_paged_args* args);
+
+/* Target rows over encoder states of another length: every query row of
+ * sequence s attends to its kv_len[s] key rows from row kv_start[s] of k and v
+ * (kv_start NULL: s * max_kv), except those whose byte of key_mask (indexed
+ * like the rows of k; NULL: none) is 0.  Hidden rows, and rows past the
+ * lengths, are never read.  A sequence without a visible key gives zeros. */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    void*       out;
+    const int*  q_start;
+    const int*  q_len;
+    const int*  kv_start;
+    const int*  kv_len;
+    const uint8_t* key_mask;
+    int dtype, head_dim, n_heads, n_kv_heads;
+    int n_seq, q_rows, kv_rows, max_q, max_kv;
+    float scale;
+    int64_t q_stride_row, q_stride_head;
+    int64_t k_stride_row, k_stride_head;
+    int64_t v_stride_row, v_stride_head;
+    int64_t out_stride_row, out_stride_head;
+} nllb_attn_cross_rows_args;
+
+NLLB_ATTN_API int nllb_attn_cross_rows(nllb_attn_ctx* ctx, const nllb_attn_cross_rows_args* args);
 
 /* ---- drop-ins for the declared single-head API (pico.h:85-92) -----------
  * Same signatures and meaning as the reference's attention_head

@@ -195,6 +195,48 @@ NLLB_ATTN_API size_t nllb_logsoftmax_topk_ws_bytes(int vocab, int rows, int k);
 NLLB_ATTN_API int nllb_logsoftmax_topk(const float* logits, long long ld, int vocab, int rows, int k,
                                        int* out_tok, float* out_logp, void* ws, void* stream);
 
+/* ---- drawing tokens ---------------------------------------------------------
+ * One token for each row of logits (row r at logits + r*ld, `vocab` entries of
+ * `dtype` NLLB_F32, NLLB_F16 or NLLB_BF16), from a given uniform number u[r]
+ * in [0, 1).  No counterpart in the reference, which only searches.  With
+ * temperature T and m the row's largest logit, token i weighs
+ * w_i = exp((l_i - m) / T), taken as 0 below 2^-45.  Of the tokens, ordered by
+ * falling logit and then rising index, remain
+ *   the first top_k;
+ *   of these the shortest run whose weights sum to at least top_p of theirs;
+ *   of these the ones with w_i >= min_p, and the first in any case;
+ * and the token drawn is the lowest index at which the sum of the remaining
+ * weights up to and including it exceeds u times their whole sum.
+ * out_logp (may be NULL): its log-probability among the remaining tokens.
+ * temperature, top_k, top_p, min_p: device arrays of one entry per row, or
+ * NULL for 1, 0, 1, 0.  T = 0 takes the first token of the order (logp 0),
+ * T below 2^-100 counts as 2^-100;
+ * top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 cut nothing, top_p <= 0
+ * keeps one token, min_p above 1 counts as 1; NaN in top_p or min_p cuts
+ * nothing, u is clamped into [0, 1) and NaN counts as 0.  A NaN logit counts
+ * as -inf; logits of +inf share all the weight.  A row with no logit above
+ * -inf, or with a temperature that is negative, infinite or NaN, gives token
+ * -1 and logp -inf.
+ * Weights are summed as integer multiples of 2^-44, so a result does not
+ * depend on the order of the additions.  Device pointers; asynchronous on
+ * `stream` (a cudaStream_t, NULL = default); nothing is allocated, the logits
+ * are not modified.  At most NLLB_SAMPLE_MAX_VOCAB entries a row (more:
+ * NLLB_ATTN_ECAPACITY). */
+#define NLLB_SAMPLE_MAX_VOCAB 524288
+typedef struct {
+    const void*  logits;
+    long long    ld;
+    int          dtype, vocab, rows;
+    const float* temperature;
+    const int*   top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* u;
+    int*         out_tok;
+    float*       out_logp;
+} nllb_sample_args;
+NLLB_ATTN_API int nllb_sample(const nllb_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
