@@ -39,6 +39,9 @@ enum class RowType { f32 = 0, f16 = 1, bf16 = 2 };
 
 // Per-device kernel attributes; call once per device.
 cudaError_t configure_rows_kernels();
+cudaError_t configure_rows_tc();
 cudaError_t launch_rows(const RowsParams& p, RowType type, int head_dim, bool paged, int num_sms, cudaStream_t st);
+// the tensor-core form (rows_tc.cu), for launch_rows
+cudaError_t launch_rows_tc(const RowsParams& p, RowType type, int head_dim, bool paged, int num_sms, cudaStream_t st);
 
 }  // namespace nllb

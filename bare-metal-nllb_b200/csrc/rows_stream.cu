@@ -290,10 +290,13 @@ cudaError_t configure_rows_kernels() {
     cudaError_t e = configure_type<float>();
     if (e == cudaSuccess) e = configure_type<__half>();
     if (e == cudaSuccess) e = configure_type<__nv_bfloat16>();
+    if (e == cudaSuccess) e = configure_rows_tc();
     return e;
 }
 
 cudaError_t launch_rows(const RowsParams& p, RowType type, int head_dim, bool paged, int num_sms, cudaStream_t st) {
+    // more rows than one CTA of this kernel takes would read the keys again
+    if ((long long)p.max_q * p.group > 8) return launch_rows_tc(p, type, head_dim, paged, num_sms, st);
     switch (type) {
         case RowType::f32: return launch_by_dim<float>(p, head_dim, paged, num_sms, st);
         case RowType::f16: return launch_by_dim<__half>(p, head_dim, paged, num_sms, st);
