@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         tc_fence_after();
         if (n_split == 1) {
             if (ok && any) {
-                const float inv = l > 0.f ? 1.0f / l : 0.f;  // no visible key: zeros
+                const float inv = 1.0f / l;
                 T* dst = static_cast<T*>(p.out) + (long long)(sq.q0 + tok) * p.o_row +
                          (long long)(g * p.group + row % p.group) * p.o_head;
 #pragma unroll
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         for (int i = 0; i < 32; i += VEC) {
                             float x[VEC];
 #pragma unroll
-                            for (int e = 0; e < VEC; ++e) x[e] = l > 0.f ? o[i + e] * inv : 0.f;
+                            for (int e = 0; e < VEC; ++e) x[e] = l == 0.f ? 0.f : o[i + e] * inv;  // no visible key: zeros
                             *reinterpret_cast<uint4*>(dst + c + i) = rows_pack<T>(x);
                         }
                     }
@@ -343,9 +343,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<float4*>(st + c + i) =
-                            l > 0.f ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
-                *reinterpret_cast<float4*>(st + D) = make_float4(l > 0.f ? m : -INFINITY, ok ? l : -1.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(st + D) = make_float4(l == 0.f ? -INFINITY : m, ok ? l : -1.f, 0.f, 0.f);
             }
         }
     } else if (warp < NQ * 4 + kLoaders / 32) {
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 for (int z = 0; z < n_split; ++z) {
                     const float w = ex2_approx(ld_cluster_f32(map_rank(st + r * C::LD + D, z)) - off);
                     const float lz = ld_cluster_f32(map_rank(st + r * C::LD + D + 1, z));
-                    good = good && lz >= 0.f;  // a split that gave up says so
+                    good = good && !(lz < 0.f);  // a split that gave up says so
                     sum = fmaf(w, lz, sum);
 #pragma unroll
                     for (int e = 0; e < VEC; e += 4) {
@@ -586,9 +586,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         x[e + 2] = fmaf(w, f.z, x[e + 2]), x[e + 3] = fmaf(w, f.w, x[e + 3]);
                     }
                 }
-                const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                const float inv = 1.f / sum;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) x[e] *= inv;
+                for (int e = 0; e < VEC; ++e) x[e] = sum == 0.f ? 0.f : x[e] * inv;
                 T* dst = static_cast<T*>(p.out) + (long long)(sq.q0 + row / p.group) * p.o_row +
                          (long long)(g * p.group + row % p.group) * p.o_head;
                 if (good) *reinterpret_cast<uint4*>(dst + c * VEC) = rows_pack<T>(x);

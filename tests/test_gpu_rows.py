@@ -376,6 +376,19 @@ def test_cross_rows_hidden_keys_may_hold_anything(ctx):
             c.verify("hidden")
 
 
+def test_cross_rows_nan_query_stays_in_its_row(ctx):
+    for dtype in TYPES:
+        for lens in ("tokens", "rows", "few rows over many keys"):
+            c = Cross(CROSS[lens], 4, 2, 64, dtype)
+            c.run(ctx)
+            plain = c.out.clone()
+            c.q[1, 1] = float("nan")
+            c.run(ctx)
+            assert torch.isnan(c.out[1, 1]).all()
+            c.out[1, 1] = plain[1, 1]
+            assert torch.equal(c.out, plain)
+
+
 def test_cross_rows_everything_hidden_gives_zeros(ctx):
     for dtype in TYPES:
         for n in (1, 200):
