@@ -27,21 +27,16 @@
 
 #include "rows.cuh"
 
-#ifndef ROWS_RING
-#define ROWS_RING 3
-#endif
-#ifndef ROWS_WARPS
-#define ROWS_WARPS 4
-#endif
-#ifndef ROWS_FEW
-#define ROWS_FEW 1
-#endif
-
 namespace nllb {
 namespace {
 
-constexpr int kRing = ROWS_RING;         // key blocks in a warp's ring
-constexpr int kRowsMax = 16;     // query rows of one CTA at most
+constexpr int kRowsMax = 16;  // query rows of one CTA at most
+constexpr int kRing = 2;      // key blocks in a warp's ring
+// Warps of a CTA with several, by the bytes of a block of K and V: as many as shared memory has room for, since more
+// warps of short rings beat fewer of long ones (64 sequences over 200..8191 keys, 4 rows of 128: 7 x 2 blocks of 16 KB
+// 106 us, 6 x 2 113, 5 x 2 148, 4 x 3 145; one over 99990 keys, 8 rows of 64: 14 x 2 blocks of 8 KB 31.5 us, 12 x 2
+// 36.2, 8 x 3 37.6, 6 x 4 48.1).
+constexpr int kWarps8 = 14, kWarps16 = 7;
 constexpr float kWeightExp = 7.0f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
@@ -89,10 +84,14 @@ struct Cfg {
     static constexpr int ROW = D * (int)sizeof(T);      // bytes of a key row
     static constexpr int CH = ROW / 16;                 // its 16-byte chunks = lanes to a row
     static constexpr int KPW = 32 / CH;                 // rows a warp copies at a time
-    static constexpr int BLK = ROW == 512 ? 16 : 32;    // keys of a block
-    static constexpr uint32_t HALF = BLK * ROW;         // K (or V) of a block
-    static constexpr uint32_t RING = kRing * 2 * HALF;  // of one warp
     static constexpr bool MMA = sizeof(T) == 2 && R > 1;
+    // Keys of a block: 16 of 256 bytes and more, which makes room for more warps (fp32 heads of 64: 161 us instead of
+    // 174; memories of 18..512 rows of 128, a warp each: 100 instead of 122 us), except for the matrix products of
+    // many warps, which take 32 (106 us instead of 123 for the 64 sequences above).
+    static constexpr int BLK = ROW == 512 || (ROW == 256 && (!MMA || NW == 1)) ? 16 : 32;
+    static constexpr uint32_t HALF = BLK * ROW;         // K (or V) of a block
+    static constexpr int MANY = 2 * HALF <= 8192 ? kWarps8 : kWarps16;
+    static constexpr uint32_t RING = kRing * 2 * HALF;  // of one warp
     static constexpr int LD = D + 4;                    // a row's state: m, l, -, -, D sums
     static constexpr uint32_t STATES = (NW + 1) * R * LD * 4;  // the warps', then the CTA's; over the rings
     static constexpr uint32_t SMEM = NW * RING > STATES ? NW * RING : STATES;
@@ -219,9 +218,9 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
         // this lane's part of the ldmatrix addresses
         const int mr = lane & 7, mm = lane >> 3;  // row of matrix mm
         run([&](int b, uint32_t seen, uint32_t kb) {
-            float sc[4][4];
+            float sc[BLK / 8][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {  // 8 keys
+            for (int n = 0; n < BLK / 8; ++n) {  // 8 keys
                 sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
                 for (int k = 0; k < D / 32; ++k) {
@@ -232,17 +231,18 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
                 }
             }
             const int j0 = b * BLK;
-            const bool whole = seen == 0xffffffffu && (!PAGED || j0 + BLK <= past);
-            uint32_t pf[2][4];
+            const bool whole = seen == (BLK == 32 ? 0xffffffffu : 0xffffu) && (!PAGED || j0 + BLK <= past);
+            uint32_t pf[BLK / 16][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h >= HALVES) {
-                    pf[0][1] = pf[0][3] = pf[1][1] = pf[1][3] = 0u;
+#pragma unroll
+                    for (int k = 0; k < BLK / 16; ++k) pf[k][1] = pf[k][3] = 0u;
                     continue;
                 }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < BLK / 8; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float& x = sc[n][2 * h + e];
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) o[i][2 * h] *= corr, o[i][2 * h + 1] *= corr;
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int n = 0; n < BLK / 8; ++n) {
                     const float x = exp2f(sc[n][2 * h] - off), y = exp2f(sc[n][2 * h + 1] - off);
                     l[h] += x + y;
                     pf[n >> 1][(n & 1) * 2 + h] = pack2<T>(x, y);
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
             }
             const uint32_t vb = kb + C::HALF;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)  // 16 keys
+            for (int k = 0; k < BLK / 16; ++k)  // 16 keys
 #pragma unroll
                 for (int n = 0; n < D / 16; ++n) {  // 16 dims: matrices (keys 0-7, 8-15) x (dims 0-7, 8-15)
                     uint32_t f[4];
@@ -471,11 +471,11 @@ cudaError_t launch_by_units(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long units = ((long long)p.max_q * p.group + R - 1) / R * p.kv_heads * p.n_seq;
     // A warp alone per unit where that already fills the SMs and the keys are few; else four warps, and as many
     // splits as give every SM work, none with less than a block per warp, one cluster at most.
-    if (units >= 8LL * num_sms && p.max_kv <= 1024) return launch_one<T, D, R, PAGED, ROWS_FEW>(p, 1, st);
-    constexpr int step = ROWS_WARPS * Cfg<T, D, R, ROWS_WARPS>::BLK;
+    if (units >= 8LL * num_sms && p.max_kv <= 1024) return launch_one<T, D, R, PAGED, 1>(p, 1, st);
+    constexpr int MANY = Cfg<T, D, R, 0>::MANY, step = MANY * Cfg<T, D, R, 0>::BLK;
     int n_split = 1;
     while (n_split < 16 && units * n_split < 2LL * num_sms && p.max_kv > step * n_split) n_split *= 2;
-    return launch_one<T, D, R, PAGED, ROWS_WARPS>(p, n_split, st);
+    return launch_one<T, D, R, PAGED, MANY>(p, n_split, st);
 }
 
 template <typename T, int D, bool PAGED>
@@ -509,10 +509,10 @@ cudaError_t configure_one() {
 
 template <typename T, int D, int R>
 cudaError_t configure_rows() {
-    cudaError_t e = configure_one<T, D, R, false, ROWS_FEW>();
-    if (e == cudaSuccess) e = configure_one<T, D, R, true, ROWS_FEW>();
-    if (e == cudaSuccess) e = configure_one<T, D, R, false, ROWS_WARPS>();
-    if (e == cudaSuccess) e = configure_one<T, D, R, true, ROWS_WARPS>();
+    cudaError_t e = configure_one<T, D, R, false, 1>();
+    if (e == cudaSuccess) e = configure_one<T, D, R, true, 1>();
+    if (e == cudaSuccess) e = configure_one<T, D, R, false, Cfg<T, D, R, 0>::MANY>();
+    if (e == cudaSuccess) e = configure_one<T, D, R, true, Cfg<T, D, R, 0>::MANY>();
     return e;
 }
 
