@@ -41,6 +41,8 @@ static_assert(NLLB_SAMPLE_MAX_VOCAB == 1 << kIndexBits, "an index fits the compo
 // the first histogram covers (m - l) / T up to 33: exp(-33) < 2^-45 weighs 0
 constexpr float kSpan = 33.0f;
 
+constexpr int kList = kBins / 2;  // candidates that rank 0 finishes alone, in the place of the masses
+
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSlice = NLLB_SAMPLE_MAX_VOCAB / kMaxCluster;
 constexpr int kMaxChunks = kMaxSlice / 128;  // fp32's chunks are the shortest
@@ -66,13 +68,17 @@ struct Shared {
     double tab[64];            // 2^(j/64)
     u64 chunk[kMaxChunks];     // kept weight of each chunk of the slice
     u64 warp_sum[kWarpsS];
-    u64 total, sum;            // of a scan; of this CTA's kept weight
-    u64 found_before, found_value;
+    u64 sum;                   // this CTA's kept weight
+    u64 found_before;
     uint32_t found_cnt;
     int found_bin;
     float best;                // this CTA's largest logit
     uint32_t key_lo, key_hi;   // this CTA's range of keys in the border step
     float red[kWarpsS];
+    u64 z, above;              // this CTA's weight, in all and above the window
+    int win_lo, win_hi;        // steps the border by weight lies between
+    uint32_t listed;           // (rank 0) candidates gathered
+    int first_best;            // this CTA's lowest index of the largest logit
 };
 
 __device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
@@ -130,6 +136,23 @@ __device__ __forceinline__ T minus_inf() {
     else return __ushort_as_bfloat16((unsigned short)0xff80u);
 }
 
+__device__ __forceinline__ float key_logit(uint32_t k) {  // the inverse of order_key
+    return __uint_as_float((k & 0x80000000u) ? k : 0x7fffffffu - k);
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t x) {
+    uint32_t v;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(v) : "r"(addr), "r"(x) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 x) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(x) : "memory");
+}
+
 template <typename T>
 struct alignas(16) Vec {
     T x[16 / sizeof(T)];
@@ -161,6 +184,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid < 64) sh.tab[tid] = exp2((double)tid / 64.0);
+    if (tid == 0) sh.z = sh.above = 0, sh.listed = 0, sh.first_best = INT_MAX;
     pdl_wait_primary();
 
     const uint32_t C = cluster_size(), rank = cluster_ctarank();
@@ -206,10 +230,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
 
     // ---- the row's settings
     float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
-    int k = a.top_k ? __ldg(a.top_k + row) : 0;
-    float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
-    float min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
+    const int k = a.top_k ? __ldg(a.top_k + row) : 0;
+    const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
+    const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
     float u = __ldg(a.u + row);
+    u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;  // (NaN too)
     const bool usable = m > -INFINITY && temp >= 0.0f && temp < INFINITY;
     if (!usable) {  // (uniform over the cluster)
         if (rank == 0 && tid == 0) {
@@ -219,20 +244,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         cluster_sync_all();
         return;
     }
-    if (temp == 0.0f) temp = 1.0f, k = 1;  // the first of the order, whatever the weights
-    temp = fmaxf(temp, 0x1p-100f);         // keeps the factors below finite
-    const double md = m, scale = 64.0 * 1.4426950408889634074 / (double)temp;
-    const float to_bin = (float)kBins / (kSpan * temp);
-    // Step of the first histogram; steps rise as logits fall, in fp32 as well
-    // as in exact arithmetic, since every operation rounds monotonically.
-    auto step_of = [&](float l) -> int {
-        if (l == m) return 0;
-        const float d = (m - l) * to_bin;
-        return d < (float)kBins ? (int)d : kBins;
-    };
-    auto wt = [&](float l) { return weight(l, m, md, scale, sh.tab); };
 
-    // f(l, local index) for every element of the slice
+    // f(l, local index) for every element of the slice, a warp's lanes together
     auto each = [&](auto&& f) {
         for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
             const Vec<T> v = data[ch * 32 + lane];
@@ -240,60 +253,158 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             for (int e = 0; e < VEC; ++e) f(as_float(v.x[e]), (ch * 32 + lane) * VEC + e);
         }
     };
-    auto composite = [&](float l, int i) { return ((u64)order_key(l) << kIndexBits) | (u64)(first + i); };
 
-    // Sums the cluster's histograms and finds the first bin at which the sum of
-    // the values (counts, or masses) up to and including it, from `base` on,
-    // reaches target(sum of all).  All CTAs compute the same; found_bin -1 if
-    // no bin does.
-    auto search = [&](bool by_mass, u64 base, auto&& target) {
+    if (temp == 0.0f) {  // the first of the order
+        int at = INT_MAX;
+        each([&](float l, int i) {
+            if (l == m) at = min(at, first + i);
+        });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) atomicMin(&sh.first_best, at);
         cluster_sync_all();
-        const int share = kBins / (int)C;
-        if (C > 1) {
-            for (int b = tid; b < share; b += kThreads) {
-                uint32_t c = 0;
-                u64 w = 0;
-                for (uint32_t z = 0; z < C; ++z) {
-                    uint32_t x;
-                    asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                                 : "=r"(x) : "r"(map_rank(&sh.cnt[rank * share + b], z)) : "memory");
-                    c += x;
-                    if (by_mass) w += ld_cluster_u64(map_rank(&sh.mass[rank * share + b], z));
-                }
-                sh.tot_cnt[b] = c;
-                if (by_mass) sh.tot_mass[b] = w;
-            }
-            cluster_sync_all();
+        if (rank == 0 && tid == 0) {
+            for (uint32_t z = 0; z < C; ++z) at = min(at, (int)ld_cluster_u32(map_rank(&sh.first_best, z)));
+            a.out_tok[row] = at;
+            if (a.out_logp) a.out_logp[row] = 0.0f;
         }
-        constexpr int PER = kBins / kThreads;
-        uint32_t c[PER];
-        u64 v[PER], mine = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int b = tid * PER + i;
-            if (C > 1) {
-                const uint32_t z = (uint32_t)(b / share), at = (uint32_t)(b % share);
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c[i]) : "r"(map_rank(&sh.tot_cnt[at], z)) : "memory");
-                v[i] = by_mass ? ld_cluster_u64(map_rank(&sh.tot_mass[at], z)) : (u64)c[i];
-            } else {
-                c[i] = sh.cnt[b];
-                v[i] = by_mass ? sh.mass[b] : (u64)c[i];
-            }
-            mine += v[i];
+        cluster_sync_all();
+        return;
+    }
+
+    temp = fmaxf(temp, 0x1p-100f);  // keeps the factors below finite
+    const double md = m, scale = 64.0 * 1.4426950408889634074 / (double)temp;
+    const float to_bin = (float)kBins / (kSpan * temp);
+    // Place of a logit on the scale of the first histogram, in steps.  Places
+    // rise as logits fall, in fp32 as well as in exact arithmetic, since every
+    // operation rounds monotonically; so do the finer places below.
+    auto place = [&](float l) -> float { return l == m ? 0.0f : (m - l) * to_bin; };
+    auto step_of = [&](float l) -> int {
+        const float d = place(l);
+        return d < (float)kBins ? (int)d : kBins;
+    };
+    auto wt = [&](float l) { return weight(l, m, md, scale, sh.tab); };
+    auto composite = [&](float l, int i) { return ((u64)order_key(l) << kIndexBits) | (u64)(first + i); };
+    u64 least = 1;  // min-p as a weight
+    if (min_p > 0.0f) {
+        const double t = ceil((double)fminf(min_p, 1.0f) * (double)(1ull << kWeightBits));
+        least = t > 1.0 ? (u64)t : 1;
+    }
+    auto share_of = [&](u64 whole) -> u64 {  // the weight that top-p asks for
+        const double t = ceil((double)fmaxf(top_p, 0.0f) * (double)whole);
+        const u64 want = t < (double)whole ? (u64)t : whole;
+        return want > 0 ? want : 1;
+    };
+    auto threshold = [&](u64 whole) -> u64 {  // the token is the first whose running sum is above it
+        const double t = (double)u * (double)whole;
+        return t < (double)whole ? min((u64)t, whole - 1) : whole - 1;
+    };
+    auto answer = [&](int token, float l, u64 whole) {
+        a.out_tok[row] = token;
+        if (a.out_logp) {
+            const double x = l == m ? 0.0 : ((double)l - md) / (double)temp;
+            a.out_logp[row] = (float)(x - log((double)whole * (1.0 / (double)(1ull << kWeightBits))));
         }
+    };
+
+    // ---- sums over the CTA
+    auto block_scan = [&](u64 mine, u64& all) -> u64 {  // sum of the threads before this one
         const u64 inc = warp_scan_u64(mine, lane);
-        if (lane == 31) sh.warp_sum[warp] = inc;
-        if (tid == 0) sh.found_bin = -1;
         __syncthreads();
-        u64 before = base, all = base;
+        if (lane == 31) sh.warp_sum[warp] = inc;
+        __syncthreads();
+        u64 before = inc - mine;
+        all = 0;
 #pragma unroll
         for (int w = 0; w < kWarpsS; ++w) {
             const u64 x = sh.warp_sum[w];
             if (w < warp) before += x;
             all += x;
         }
-        before += inc - mine;
-        const u64 want = target(all);
+        return before;
+    };
+    auto block_scan_d = [&](double mine, double& all) -> double {  // up to and including this one
+        double inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+        }
+        __syncthreads();
+        if (lane == 31) sh.warp_sum[warp] = (u64)__double_as_longlong(inc);
+        __syncthreads();
+        double before = 0.0;
+        all = 0.0;
+#pragma unroll
+        for (int w = 0; w < kWarpsS; ++w) {
+            const double x = __longlong_as_double((long long)sh.warp_sum[w]);
+            if (w < warp) before += x;
+            all += x;
+        }
+        return before + inc;
+    };
+    // Sum over the cluster of a value each thread has a part of (two at once).
+    auto cluster_sums = [&](u64 x, u64 y, u64& sx, u64& sy) {
+        x = warp_sum_u64(x), y = warp_sum_u64(y);
+        if (lane == 0) {
+            atomicAdd(&sh.z, x);
+            atomicAdd(&sh.above, y);
+        }
+        cluster_sync_all();
+        sx = sy = 0;
+        for (uint32_t z = 0; z < C; ++z) {
+            sx += ld_cluster_u64(map_rank(&sh.z, z));
+            sy += ld_cluster_u64(map_rank(&sh.above, z));
+        }
+    };
+
+    // ---- histograms over the cluster
+    constexpr int PER = kBins / kThreads;  // a thread's bins, PER tid ...
+    uint32_t c[PER];                       // their counts, in the cluster
+    auto clear = [&](bool by_mass) {
+        for (int b = tid; b < kBins; b += kThreads) {
+            sh.cnt[b] = 0;
+            if (by_mass) sh.mass[b] = 0;
+        }
+        __syncthreads();
+    };
+    // Sums the CTAs' histograms: each CTA a share of the bins, then all read all.
+    auto collect = [&](bool by_mass, u64 (&v)[PER]) {
+        cluster_sync_all();
+        const int share = kBins / (int)C;
+        if (C > 1) {
+            for (int b = tid; b < share; b += kThreads) {
+                uint32_t n0 = 0;
+                u64 w = 0;
+                for (uint32_t z = 0; z < C; ++z) {
+                    n0 += ld_cluster_u32(map_rank(&sh.cnt[rank * share + b], z));
+                    if (by_mass) w += ld_cluster_u64(map_rank(&sh.mass[rank * share + b], z));
+                }
+                sh.tot_cnt[b] = n0;
+                if (by_mass) sh.tot_mass[b] = w;
+            }
+            cluster_sync_all();
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int b = tid * PER + i;
+            if (C > 1) {
+                const uint32_t z = (uint32_t)(b / share), at = (uint32_t)(b % share);
+                c[i] = ld_cluster_u32(map_rank(&sh.tot_cnt[at], z));
+                v[i] = by_mass ? ld_cluster_u64(map_rank(&sh.tot_mass[at], z)) : (u64)c[i];
+            } else {
+                c[i] = sh.cnt[b];
+                v[i] = by_mass ? sh.mass[b] : (u64)c[i];
+            }
+        }
+    };
+    // The first bin at which the sum of the values up to and including it, from
+    // `base` on, reaches `want`; found_bin -1 if none does.
+    auto find = [&](const u64 (&v)[PER], u64 base, u64 want) {
+        u64 mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) mine += v[i];
+        u64 before = base + block_scan(mine, all);
+        if (tid == 0 && !(base < want && want <= base + all)) sh.found_bin = -1;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (before < want && want <= before + v[i]) {
@@ -303,39 +414,39 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             }
             before += v[i];
         }
-        if (tid == 0) sh.total = all;
         __syncthreads();
-        return want;
     };
-    auto clear = [&](bool by_mass) {
-        for (int b = tid; b < kBins; b += kThreads) {
-            sh.cnt[b] = 0;
-            if (by_mass) sh.mass[b] = 0;
+    // Steps between which the sum of the weights reaches top_p of the whole,
+    // from the counts alone: within a step the weights differ by a factor of
+    // exp(kSpan / kBins) at most.
+    auto window = [&] {
+        double lo[PER], hi[PER], lo_mine = 0.0, hi_mine = 0.0, lo_all, hi_all;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float x = (float)(tid * PER + i), w = kSpan / (float)kBins;
+            lo[i] = (double)c[i] * (double)expf(-(x + 1.01f) * w);
+            hi[i] = (double)c[i] * (double)expf(-fmaxf(x - 0.01f, 0.0f) * w);
+            lo_mine += lo[i], hi_mine += hi[i];
+        }
+        if (tid == 0) sh.win_lo = sh.win_hi = kBins - 1;
+        double lo_sum = block_scan_d(lo_mine, lo_all) - lo_mine, hi_sum = block_scan_d(hi_mine, hi_all) - hi_mine;
+        const double p = (double)fmaxf(top_p, 0.0f);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            lo_sum += lo[i], hi_sum += hi[i];
+            if (lo_sum >= (p + 1e-5) * (lo_sum + fmax(hi_all - hi_sum, 0.0)) && c[i] > 0)
+                atomicMin(&sh.win_hi, tid * PER + i);
+            if (hi_sum >= (p - 1e-5) * (hi_sum + fmax(lo_all - lo_sum, 0.0))) atomicMin(&sh.win_lo, tid * PER + i);
         }
         __syncthreads();
     };
 
-    // The composite up to which the elements (of those <= limit) are kept:
-    // the first at which the count, or the weight, of the elements up to it
-    // reaches target(whole).  Unchanged limit if none does.
-    auto border = [&](bool by_mass, u64 limit, auto&& target) -> u64 {
-        clear(by_mass);
-        each([&](float l, int i) {
-            const int b = step_of(l);
-            if (b < kBins && composite(l, i) <= limit) {
-                atomicAdd(&sh.cnt[b], 1u);
-                if (by_mass) atomicAdd(&sh.mass[b], wt(l));
-            }
-        });
-        const u64 want = search(by_mass, 0, target);
-        const int b = sh.found_bin;
-        if (b < 0) return limit;
-        u64 base = sh.found_before;
-        bool one = sh.found_cnt == 1;
-        // the keys of that step
+    // The composite of the element at which the sum reaches `want`, among the
+    // elements (of composite <= limit) that in(l) picks, `base` before them.
+    auto refine = [&](auto&& in, bool by_mass, bool one, u64 base, u64 want, u64 limit) -> u64 {
         uint32_t lo = 0xffffffffu, hi = 0;
         each([&](float l, int i) {
-            if (step_of(l) == b && composite(l, i) <= limit) {
+            if (in(l) && composite(l, i) <= limit) {
                 lo = min(lo, order_key(l));
                 hi = max(hi, order_key(l));
             }
@@ -350,48 +461,195 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         }
         cluster_sync_all();
         for (uint32_t z = 0; z < C; ++z) {
-            uint32_t x, y;
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(map_rank(&sh.key_lo, z)) : "memory");
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(y) : "r"(map_rank(&sh.key_hi, z)) : "memory");
-            lo = min(lo, x);
-            hi = max(hi, y);
+            lo = min(lo, ld_cluster_u32(map_rank(&sh.key_lo, z)));
+            hi = max(hi, ld_cluster_u32(map_rank(&sh.key_hi, z)));
         }
         u64 from = (u64)lo << kIndexBits, to = ((u64)hi << kIndexBits) | ((1u << kIndexBits) - 1u);
         while (!one) {
-            to = to < limit ? to : limit;
+            to = min(to, limit);
             const int bits = 64 - __clzll((long long)(to - from));
             const int shift = max(0, bits - kBinBits);
             clear(by_mass);
             each([&](float l, int i) {
-                const u64 c = composite(l, i);
-                if (c >= from && c <= to) {
-                    const int x = (int)((c - from) >> shift);
-                    atomicAdd(&sh.cnt[x], 1u);
-                    if (by_mass) atomicAdd(&sh.mass[x], wt(l));
+                const u64 x = composite(l, i);
+                if (x >= from && x <= to) {
+                    const int b = (int)((x - from) >> shift);
+                    atomicAdd(&sh.cnt[b], 1u);
+                    if (by_mass) atomicAdd(&sh.mass[b], wt(l));
                 }
             });
-            search(by_mass, base, [&](u64) { return want; });
+            u64 v[PER];
+            collect(by_mass, v);
+            find(v, base, want);
             base = sh.found_before;
             from += (u64)sh.found_bin << shift;
             to = from + ((1ull << shift) - 1ull);
             one = sh.found_cnt == 1 || shift == 0;
-            __syncthreads();  // the next search's writes wait for these reads
         }
-        return to < limit ? to : limit;
+        return min(to, limit);
     };
 
-    u64 limit = ~0ull;
-    if (k > 0 && k < a.vocab) limit = border(false, limit, [&](u64) { return (u64)k; });
-    if (top_p < 1.0f)
-        limit = border(true, limit, [&](u64 all) {
-            const double t = ceil((double)fmaxf(top_p, 0.0f) * (double)all);
-            const u64 want = t < (double)all ? (u64)t : all;
-            return want > 0 ? want : 1;
-        });
-    u64 least = 1;
-    if (min_p > 0.0f) {
-        const double t = ceil((double)fminf(min_p, 1.0f) * (double)(1ull << kWeightBits));
-        least = t > 1.0 ? (u64)t : 1;
+    const bool cut_k = k > 0 && k < a.vocab, cut_p = top_p < 1.0f;
+    u64 limit = ~0ull;  // the composite of the last element kept
+    if (cut_k || cut_p) {
+        auto count = [&] {
+            clear(false);
+            each([&](float l, int i) {
+                const int b = step_of(l);
+                if (b < kBins && composite(l, i) <= limit) atomicAdd(&sh.cnt[b], 1u);
+            });
+        };
+        u64 v[PER];
+        count();
+        collect(false, v);
+        int last = -1;       // the steps up to it hold everything kept
+        u64 n_list = 0;      // elements in them
+        bool by_k = false;   // ... since top-k ends in it
+        if (cut_k) {
+            find(v, 0, (u64)k);
+            if (sh.found_bin >= 0) {
+                by_k = true;
+                last = sh.found_bin;
+                n_list = sh.found_before + sh.found_cnt;
+            }
+        }
+        if (!by_k && cut_p) {
+            window();
+            last = sh.win_hi;
+            u64 mine = 0, all;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (tid * PER + i <= last) mine += c[i];
+            (void)block_scan(mine, all);
+            n_list = all;
+        }
+        if (last >= 0 && n_list <= kList) {
+            // ---- few candidates: rank 0 takes them all and finishes alone
+            u64 whole = 0, unused = 0;
+            if (!by_k) {
+                u64 z = 0;
+                each([&](float l, int) { z += wt(l); });
+                cluster_sums(z, 0, whole, unused);
+            }
+            each([&](float l, int i) {
+                const bool in = step_of(l) <= last;
+                const unsigned who = __ballot_sync(0xffffffffu, in);
+                if (who) {
+                    uint32_t at = 0;
+                    if (lane == 0) at = add_cluster_u32(map_rank(&sh.listed, 0), __popc(who));
+                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+                    if (in && at < kList) st_cluster_u64(map_rank(&sh.mass[at], 0), composite(l, i));
+                }
+            });
+            cluster_sync_all();
+            if (rank != 0) return;  // (nobody reads this CTA's shared memory any more)
+            const int n = (int)n_list;
+            int n2 = 64;
+            while (n2 < n) n2 *= 2;
+            auto sort = [&] {  // sh.mass[0 .. n2) rising
+                for (int size = 2; size <= n2; size *= 2)
+                    for (int stride = size / 2; stride > 0; stride /= 2) {
+                        __syncthreads();
+                        for (int t = tid; t < n2 / 2; t += kThreads) {
+                            const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+                            const u64 x = sh.mass[i], y = sh.mass[j];
+                            if ((x > y) == ((i & size) == 0)) sh.mass[i] = y, sh.mass[j] = x;
+                        }
+                    }
+                __syncthreads();
+            };
+            for (int i = n + tid; i < n2; i += kThreads) sh.mass[i] = ~0ull;
+            sort();
+            // weights in the order, the cuts, then the kept ones in the order of their indices
+            constexpr int EACH = kList / kThreads;
+            u64 w[EACH], x[EACH], mine = 0, all;
+            const int n_k = by_k ? min(n, k) : n;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int i = tid * EACH + e;
+                x[e] = i < n_k ? sh.mass[i] : ~0ull;
+                w[e] = i < n_k ? wt(key_logit((uint32_t)(x[e] >> kIndexBits))) : 0;
+                mine += w[e];
+            }
+            u64 before = block_scan(mine, all);
+            const u64 want = cut_p ? share_of(by_k ? all : whole) : ~0ull;
+            mine = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int i = tid * EACH + e;
+                const u64 weighs = w[e];
+                if (!(before < want && (weighs >= least || i == 0))) w[e] = 0;
+                before += weighs;
+                mine += w[e];
+                if (i < n2) {
+                    sh.mass[i] = w[e] ? (x[e] & ((1ull << kIndexBits) - 1ull)) << 32 | (u64)i : ~0ull;
+                    sh.mass[kList + i] = w[e];
+                    sh.cnt[i] = (uint32_t)(x[e] >> kIndexBits);
+                }
+            }
+            (void)block_scan(mine, all);
+            sort();
+            mine = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int i = tid * EACH + e;
+                x[e] = i < n2 ? sh.mass[i] : ~0ull;
+                w[e] = x[e] != ~0ull ? sh.mass[kList + (uint32_t)x[e]] : 0;
+                mine += w[e];
+            }
+            u64 unused_all;
+            before = block_scan(mine, unused_all);
+            const u64 thr = threshold(all);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                if (before <= thr && thr < before + w[e])
+                    answer((int)(x[e] >> 32), key_logit(sh.cnt[(uint32_t)x[e]]), all);
+                before += w[e];
+            }
+            return;
+        }
+        if (by_k)
+            limit = refine([&](float l) { return step_of(l) == last; }, false, sh.found_cnt == 1, sh.found_before,
+                           (u64)k, limit);
+        if (cut_p) {
+            if (by_k) {
+                __syncthreads();
+                count();
+                collect(false, v);
+                window();
+            }
+            // exact weights: of everything, of what lies above the window, and in 2048 steps within it
+            const int lo = sh.win_lo, hi = sh.win_hi;
+            const float finer = (float)kBins / (float)(hi - lo + 1);
+            auto fine = [&](float l) { return min(max((int)((place(l) - (float)lo) * finer), 0), kBins - 1); };
+            clear(true);
+            u64 z = 0, above = 0;
+            each([&](float l, int i) {
+                const int b = step_of(l);
+                if (b < kBins && composite(l, i) <= limit) {
+                    const u64 w = wt(l);
+                    z += w;
+                    if (b < lo) above += w;
+                    else if (b <= hi) {
+                        const int f = fine(l);
+                        atomicAdd(&sh.cnt[f], 1u);
+                        atomicAdd(&sh.mass[f], w);
+                    }
+                }
+            });
+            u64 all_z, all_above;
+            cluster_sums(z, above, all_z, all_above);
+            collect(true, v);
+            const u64 want = share_of(all_z);
+            find(v, all_above, want);
+            const int f = sh.found_bin;
+            limit = refine(
+                [&](float l) {
+                    const int b = step_of(l);
+                    return b >= lo && b <= hi && fine(l) == f;
+                },
+                true, sh.found_cnt == 1, sh.found_before, want, limit);
+        }
     }
     auto kept = [&](float l, int i) -> u64 {
         if (composite(l, i) > limit) return 0;
@@ -426,9 +684,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         if (z == rank) own = s;
         all += s;
     }
-    u = u > 0.0f ? u : 0.0f;  // (NaN too)
-    const double t = fmin((double)u, 1.0) * (double)all;
-    const u64 thr = t < (double)all ? min((u64)t, all - 1) : all - 1;  // the first running sum above thr
+    const u64 thr = threshold(all);
     if (warp == 0 && before <= thr && thr < before + own) {
         // the chunk, 32 at a time, then the element within it
         u64 at = before;
@@ -465,11 +721,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
                     l = as_float(v.x[e]);
                 }
             }
-            a.out_tok[row] = first + (ch0 * 32 + lane) * VEC + found;
-            if (a.out_logp) {
-                const double x = l == m ? 0.0 : ((double)l - md) / (double)temp;
-                a.out_logp[row] = (float)(x - log((double)all * (1.0 / (double)(1ull << kWeightBits))));
-            }
+            answer(first + (ch0 * 32 + lane) * VEC + found, l, all);
         }
     }
     cluster_sync_all();  // no CTA leaves while another reads its shared memory
