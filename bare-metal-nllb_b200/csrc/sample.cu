@@ -26,6 +26,12 @@
 #include "device_common.cuh"
 #include "nllb_translate.h"
 
+#ifndef SAMPLE_C
+#define SAMPLE_C 16
+#endif
+#ifndef SAMPLE_T
+#define SAMPLE_T 512
+#endif
 namespace nllb {
 int set_error(int status, const std::string& msg);  // nllb_attn.cu
 
@@ -33,7 +39,7 @@ namespace {
 
 using u64 = unsigned long long;
 
-constexpr int kThreads = 512, kWarpsS = kThreads / 32;
+constexpr int kThreads = SAMPLE_T, kWarpsS = kThreads / 32;
 constexpr int kBins = 2048, kBinBits = 11;
 constexpr int kWeightBits = 44;
 constexpr int kIndexBits = 19;
@@ -43,8 +49,8 @@ constexpr float kSpan = 33.0f;
 
 constexpr int kList = kBins / 2;  // candidates that rank 0 finishes alone, in the place of the masses
 
-constexpr int kMaxCluster = 16;
-constexpr int kMaxSlice = NLLB_SAMPLE_MAX_VOCAB / kMaxCluster;
+constexpr int kMaxCluster = SAMPLE_C;
+constexpr int kMaxSlice = NLLB_SAMPLE_MAX_VOCAB / 16 * 16 / kMaxCluster > 40960 ? 40960 : NLLB_SAMPLE_MAX_VOCAB / kMaxCluster;
 constexpr int kMaxChunks = kMaxSlice / 128;  // fp32's chunks are the shortest
 
 struct Args {
@@ -65,7 +71,6 @@ struct Shared {
     u64 tot_mass[kBins / 2];  // this CTA's share of the bins, summed over the cluster (two CTAs or more)
     uint32_t cnt[kBins];
     uint32_t tot_cnt[kBins / 2];
-    double tab[64];            // 2^(j/64)
     u64 chunk[kMaxChunks];     // kept weight of each chunk of the slice
     u64 warp_sum[kWarpsS];
     u64 sum;                   // this CTA's kept weight
@@ -78,6 +83,8 @@ struct Shared {
     u64 z, above;              // this CTA's weight, in all and above the window
     int win_lo, win_hi;        // steps the border by weight lies between
     uint32_t listed;           // (rank 0) candidates gathered
+    uint64_t loaded;           // barrier of the copy of the slice
+    int failed;
     int first_best;            // this CTA's lowest index of the largest logit
 };
 
@@ -98,29 +105,39 @@ __device__ __forceinline__ uint32_t order_key(float l) {
     return (b & 0x80000000u) ? b : 0x7fffffffu - b;
 }
 
-// exp((l - m) / T) in units of 2^-kWeightBits.  y = 64 log2 of it is split as
-// n + f, n a whole number and |f| <= 1/2; 2^(y/64) = 2^(n >> 6) *
-// 2^((n & 63) / 64) * exp(f ln2 / 64), the middle factor from a table and the
-// last by its series to the fifth power (Tang, 1989: the remainder is below
-// 4e-17), all in fp64: a token's border may lie anywhere between its
-// neighbours', and fp32 sums over 256206 tokens place it too coarsely.
-__device__ __forceinline__ u64 weight(float l, float m, double md, double scale, const double* tab) {
-    if (l == m) return 1ull << kWeightBits;
-    const double y = ((double)l - md) * scale;
-    if (!(y > -64.0 * (kWeightBits + 2))) return 0;
+// exp((l - m) / T) in units of 2^-kWeightBits, by a whole warp.  y = 32 log2
+// of it = l scale + shift is split as n + f, n a whole number and |f| <= 1/2;
+// 2^(y/32) = 2^(n >> 5) * 2^((n & 31) / 32) * exp(f ln2 / 32), the middle
+// factor from a table of 32 that the warp's lanes hold (a shuffle reads it;
+// from shared memory the look-ups' bank conflicts cost more than all the rest)
+// and the last by its series to the fourth power (Tang, 1989: the remainder is
+// below 1.3e-12), in fp64: a token's border may lie anywhere between its
+// neighbours', and fp32 sums over 256206 tokens place it too coarsely.  There
+// are ten fp64 operations, which bound the pass over all weights.
+struct Weigher {
+    float m;
+    double scale, shift;
+    double tab;  // 2^(lane/32), with the units' exponent
+    float to_bin;
+};
+__device__ __forceinline__ u64 weight(float l, const Weigher& g) {
+    const double y = fma((double)l, g.scale, g.shift);
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double t = y + magic;
     const int n = __double2loint(t);
-    const double r = (y - (t - magic)) * (0.693147180559945309417 / 64.0);
-    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    e = fma(r, e, 1.0 / 6.0);
-    e = fma(r, e, 0.5);
-    e = fma(r, e, 1.0);
-    e = fma(r, e, 1.0);
-    const double p2 = __hiloint2double((1023 + kWeightBits + (n >> 6)) << 20, 0);
-    const double w = tab[n & 63] * e * p2;
+    const double f = y - (t - magic);
+    constexpr double a = 0.693147180559945309417 / 32.0;
+    double p = fma(f, a * a * a * a / 24.0, a * a * a / 6.0);
+    p = fma(f, p, a * a / 2.0);
+    p = fma(f, p, a);
+    p *= f;
+    const int hi = __shfl_sync(0xffffffffu, __double2hiint(g.tab), n & 31);
+    const int lo = __shfl_sync(0xffffffffu, __double2loint(g.tab), n & 31);
+    const double x = __hiloint2double(hi + (int)((unsigned)(n >> 5) << 20), lo);
     // w < 2^52: adding 2^52 rounds it to a whole number in the low bits
-    return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+    const u64 w = (u64)__double_as_longlong(fma(x, p, x) + 4503599627370496.0) & 0xfffffffffffffull;
+    const float d = (g.m - l) * g.to_bin;  // past the last step (NaN for two infinities) nothing is left
+    return l == g.m ? 1ull << kWeightBits : d < (float)kBins ? w : 0;
 }
 
 template <typename T>
@@ -183,8 +200,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid < 64) sh.tab[tid] = exp2((double)tid / 64.0);
-    if (tid == 0) sh.z = sh.above = 0, sh.listed = 0, sh.first_best = INT_MAX;
+    if (tid == 0) sh.z = sh.above = 0, sh.listed = 0, sh.first_best = INT_MAX, sh.failed = 0;
     pdl_wait_primary();
 
     const uint32_t C = cluster_size(), rank = cluster_ctarank();
@@ -196,23 +212,40 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
 
     // ---- the slice into shared memory, NaN as -inf, and its largest logit
     float best = -INFINITY;
-    {
-        const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+    const int n_vec = vec ? n / VEC : 0;  // whole vectors come by one bulk copy
+    if (n_vec > 0 && tid == 0) {
+        mbar_init(&sh.loaded, 1);
+        fence_barrier_init();
+        mbar_arrive_expect_tx(&sh.loaded, (uint32_t)n_vec * 16u);
+        bulk_g2s(data, src, (uint32_t)n_vec * 16u, &sh.loaded);
+    }
+    for (int i = n_vec + tid; i < n_chunks * 32; i += kThreads) {
+        Vec<T> v;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v.x[e] = i * VEC + e < n ? src[i * VEC + e] : minus_inf<T>();
+        data[i] = v;
+    }
+    __syncthreads();
+    if (n_vec > 0 && !mbar_wait_bounded(&sh.loaded, 0)) {
+        sh.failed = 1;
+        (void)mbar_wait_bounded(&sh.loaded, 0);  // the copy may still be on its way
+    }
+    __syncthreads();
 #pragma unroll 4
-        for (int i = tid; i < n_chunks * 32; i += kThreads) {
-            Vec<T> v;
-            if (vec && (i + 1) * VEC <= n) {
-                *reinterpret_cast<uint4*>(&v) = __ldcs(reinterpret_cast<const uint4*>(src) + i);
-            } else {
+    for (int i = tid; i < n_chunks * 32; i += kThreads) {
+        Vec<T> v = data[i];
+        bool nan = false;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v.x[e] = i * VEC + e < n ? src[i * VEC + e] : minus_inf<T>();
-            }
+        for (int e = 0; e < VEC; ++e) {
+            const float l = as_float(v.x[e]);
+            nan |= l != l;
+            best = fmaxf(best, l);  // (fmaxf passes over NaN)
+        }
+        if (nan) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float l = as_float(v.x[e]);
-                if (l != l) v.x[e] = minus_inf<T>();
-                best = fmaxf(best, l);  // (fmaxf passes over NaN)
-            }
+            for (int e = 0; e < VEC; ++e)
+                if (as_float(v.x[e]) != as_float(v.x[e])) v.x[e] = minus_inf<T>();
             data[i] = v;
         }
     }
@@ -222,11 +255,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     __syncthreads();
     if (tid == 0) {
         for (int w = 1; w < kWarpsS; ++w) best = fmaxf(best, sh.red[w]);
-        sh.best = best;
+        sh.best = sh.failed ? __int_as_float(0x7fc00000) : best;  // NaN: a copy did not come
     }
     cluster_sync_all();
     float m = -INFINITY;
-    for (uint32_t z = 0; z < C; ++z) m = fmaxf(m, ld_cluster_f32(map_rank(&sh.best, z)));
+    bool failed = false;
+    for (uint32_t z = 0; z < C; ++z) {
+        const float x = ld_cluster_f32(map_rank(&sh.best, z));
+        failed |= x != x;
+        m = fmaxf(m, x);
+    }
 
     // ---- the row's settings
     float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
@@ -235,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
     float u = __ldg(a.u + row);
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;  // (NaN too)
-    const bool usable = m > -INFINITY && temp >= 0.0f && temp < INFINITY;
+    const bool usable = !failed && m > -INFINITY && temp >= 0.0f && temp < INFINITY;
     if (!usable) {  // (uniform over the cluster)
         if (rank == 0 && tid == 0) {
             a.out_tok[row] = -1;
@@ -272,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     }
 
     temp = fmaxf(temp, 0x1p-100f);  // keeps the factors below finite
-    const double md = m, scale = 64.0 * 1.4426950408889634074 / (double)temp;
+    const double md = m;
     const float to_bin = (float)kBins / (kSpan * temp);
     // Place of a logit on the scale of the first histogram, in steps.  Places
     // rise as logits fall, in fp32 as well as in exact arithmetic, since every
@@ -282,7 +320,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         const float d = place(l);
         return d < (float)kBins ? (int)d : kBins;
     };
-    auto wt = [&](float l) { return weight(l, m, md, scale, sh.tab); };
+    Weigher weigher;
+    weigher.m = m, weigher.to_bin = to_bin;
+    weigher.scale = 32.0 * 1.4426950408889634074 / (double)temp;
+    weigher.shift = -md * weigher.scale;
+    weigher.tab = exp2((double)lane / 32.0 + (double)kWeightBits);
+    auto wt = [&](float l) { return weight(l, weigher); };  // by all lanes of a warp
     auto composite = [&](float l, int i) { return ((u64)order_key(l) << kIndexBits) | (u64)(first + i); };
     u64 least = 1;  // min-p as a weight
     if (min_p > 0.0f) {
@@ -472,10 +515,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             clear(by_mass);
             each([&](float l, int i) {
                 const u64 x = composite(l, i);
-                if (x >= from && x <= to) {
-                    const int b = (int)((x - from) >> shift);
-                    atomicAdd(&sh.cnt[b], 1u);
-                    if (by_mass) atomicAdd(&sh.mass[b], wt(l));
+                const bool in = x >= from && x <= to;
+                if (__any_sync(0xffffffffu, in)) {
+                    const u64 w = by_mass ? wt(l) : 0;
+                    if (in) {
+                        const int b = (int)((x - from) >> shift);
+                        atomicAdd(&sh.cnt[b], 1u);
+                        if (by_mass) atomicAdd(&sh.mass[b], w);
+                    }
                 }
             });
             u64 v[PER];
@@ -568,7 +615,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             for (int e = 0; e < EACH; ++e) {
                 const int i = tid * EACH + e;
                 x[e] = i < n_k ? sh.mass[i] : ~0ull;
-                w[e] = i < n_k ? wt(key_logit((uint32_t)(x[e] >> kIndexBits))) : 0;
+                const u64 weighs = wt(key_logit((uint32_t)(x[e] >> kIndexBits)));
+                w[e] = i < n_k ? weighs : 0;
                 mine += w[e];
             }
             u64 before = block_scan(mine, all);
@@ -626,8 +674,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             u64 z = 0, above = 0;
             each([&](float l, int i) {
                 const int b = step_of(l);
+                const u64 w = wt(l);
                 if (b < kBins && composite(l, i) <= limit) {
-                    const u64 w = wt(l);
                     z += w;
                     if (b < lo) above += w;
                     else if (b <= hi) {
@@ -652,9 +700,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         }
     }
     auto kept = [&](float l, int i) -> u64 {
-        if (composite(l, i) > limit) return 0;
+        const bool in = composite(l, i) <= limit;
+        if (!__any_sync(0xffffffffu, in)) return 0;
         const u64 w = wt(l);
-        return w >= least ? w : 0;
+        return in && w >= least ? w : 0;
     };
 
     // ---- the kept weight of each chunk, of this CTA, of the row

@@ -216,7 +216,7 @@ NLLB_ATTN_API int nllb_logsoftmax_topk(const float* logits, long long ld, int vo
  * nothing, u is clamped into [0, 1) and NaN counts as 0.  A NaN logit counts
  * as -inf; logits of +inf share all the weight.  A row with no logit above
  * -inf, or with a temperature that is negative, infinite or NaN, gives token
- * -1 and logp -inf.
+ * -1 and logp -inf (so does a row whose bounded device wait gave up).
  * Weights are summed as integer multiples of 2^-44, so a result does not
  * depend on the order of the additions.  Device pointers; asynchronous on
  * `stream` (a cudaStream_t, NULL = default); nothing is allocated, the logits
