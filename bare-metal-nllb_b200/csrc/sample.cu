@@ -699,21 +699,36 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
                 true, sh.found_cnt == 1, sh.found_before, want, limit);
         }
     }
-    auto kept = [&](float l, int i) -> u64 {
-        const bool in = composite(l, i) <= limit;
-        if (!__any_sync(0xffffffffu, in)) return 0;
-        const u64 w = wt(l);
-        return in && w >= least ? w : 0;
-    };
-
     // ---- the kept weight of each chunk, of this CTA, of the row
+    const bool whole_row = limit == ~0ull;
+    const float last_l = key_logit((uint32_t)(limit >> kIndexBits));
+    const int last_i = (int)(limit & ((1ull << kIndexBits) - 1ull)) - first;
+    // the weights of vector `at` of the slice that are kept, and their sum
+    auto kept = [&](int at, const Vec<T>& v, u64 (&w)[VEC]) -> u64 {
+        bool in[VEC], any = false;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float l = as_float(v.x[e]);
+            in[e] = whole_row || l > last_l || (l == last_l && at * VEC + e <= last_i);
+            any |= in[e];
+            w[e] = 0;
+        }
+        u64 sum = 0;
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const u64 x = wt(as_float(v.x[e]));
+                if (in[e] && x >= least) w[e] = x;
+                sum += w[e];
+            }
+        }
+        return sum;
+    };
     u64 mine = 0;
     for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
-        const Vec<T> v = data[ch * 32 + lane];
-        u64 s = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s += kept(as_float(v.x[e]), (ch * 32 + lane) * VEC + e);
-        s = warp_sum_u64(s);
+        u64 w[VEC];
+        u64 s = kept(ch * 32 + lane, data[ch * 32 + lane], w);
+        if (__any_sync(0xffffffffu, s != 0)) s = warp_sum_u64(s);
         if (lane == 0) sh.chunk[ch] = s;
         mine += s;
     }
@@ -751,12 +766,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             at += __shfl_sync(0xffffffffu, inc, 31);
         }
         const Vec<T> v = data[ch0 * 32 + lane];
-        u64 w[VEC], s = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            w[e] = kept(as_float(v.x[e]), (ch0 * 32 + lane) * VEC + e);
-            s += w[e];
-        }
+        u64 w[VEC];
+        const u64 s = kept(ch0 * 32 + lane, v, w);
         const u64 inc = warp_scan_u64(s, lane);
         u64 run = at + inc - s;
         if (run <= thr && thr < run + s) {
