@@ -26,8 +26,8 @@
 #include "device_common.cuh"
 #include "nllb_translate.h"
 
-#ifndef SAMPLE_C
-#define SAMPLE_C 16
+#ifndef SAMPLE_B
+#define SAMPLE_B 131072
 #endif
 #ifndef SAMPLE_T
 #define SAMPLE_T 512
@@ -49,9 +49,10 @@ constexpr float kSpan = 33.0f;
 
 constexpr int kList = kBins / 2;  // candidates that rank 0 finishes alone, in the place of the masses
 
-constexpr int kMaxCluster = SAMPLE_C;
-constexpr int kMaxSlice = NLLB_SAMPLE_MAX_VOCAB / 16 * 16 / kMaxCluster > 40960 ? 40960 : NLLB_SAMPLE_MAX_VOCAB / kMaxCluster;
-constexpr int kMaxChunks = kMaxSlice / 128;  // fp32's chunks are the shortest
+constexpr int kMaxCluster = 16;
+constexpr int kSliceBytes = SAMPLE_B;           // of a row that one CTA holds at most
+constexpr int kMaxChunks = kSliceBytes / 512;  // a chunk is a 16-byte vector per lane
+static_assert(NLLB_SAMPLE_MAX_VOCAB / kMaxCluster * 4 <= kSliceBytes, "every row fits a cluster");
 
 struct Args {
     const void* logits;
@@ -121,7 +122,11 @@ struct Weigher {
     float to_bin;
 };
 __device__ __forceinline__ u64 weight(float l, const Weigher& g) {
-    const double y = fma((double)l, g.scale, g.shift);
+    // l as a double by whole-number operations: the conversion instruction runs at a quarter of their rate and bound
+    // this pass (subnormals and infinities, which come out finite, weigh the same or are told below)
+    const uint32_t b = __float_as_uint(l);
+    const double ld = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+    const double y = fma(ld, g.scale, g.shift);
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double t = y + magic;
     const int n = __double2loint(t);
@@ -788,20 +793,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
 }
 
 template <typename T>
-size_t smem_bytes(int slice) {
-    return (sizeof(Shared) + 15) / 16 * 16 + (size_t)slice * sizeof(T);
-}
-
-template <typename T>
-cudaError_t launch(Args a, int rows, cudaStream_t st) {
+cudaError_t launch(Args a, int rows, int num_sms, cudaStream_t st) {
     constexpr int CHUNK = 32 * 16 / (int)sizeof(T);
+    // The smallest cluster that holds a row; while there are SMs to spare, larger ones down to 4096 entries a CTA.
     int C = 1;
-    while (C < kMaxCluster && a.vocab > 8192 * C) C *= 2;
-    a.slice = ((a.vocab + C - 1) / C + CHUNK - 1) / CHUNK * CHUNK;
-    const size_t smem = smem_bytes<T>(a.slice);
+    auto slice = [&] { return ((a.vocab + C - 1) / C + CHUNK - 1) / CHUNK * CHUNK; };
+    while (slice() * (int)sizeof(T) > kSliceBytes ||
+           (C < kMaxCluster && (long long)rows * C * 2 <= num_sms && a.vocab > 4096 * C))
+        C *= 2;
+    a.slice = slice();
+    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)a.slice * sizeof(T);
     // (the largest slice's bytes, whatever this call's: calls of two threads do not undo each other's)
     cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem_bytes<T>(kMaxSlice));
+                                         (int)((sizeof(Shared) + 15) / 16 * 16 + kSliceBytes));
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -844,9 +848,13 @@ extern "C" int nllb_sample(const nllb_sample_args* s, void* stream) {
     a.temperature = s->temperature, a.top_k = s->top_k, a.top_p = s->top_p, a.min_p = s->min_p, a.u = s->u;
     a.out_tok = s->out_tok, a.out_logp = s->out_logp;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = s->dtype == NLLB_F32   ? launch<float>(a, s->rows, st)
-                          : s->dtype == NLLB_F16 ? launch<__half>(a, s->rows, st)
-                                                 : launch<__nv_bfloat16>(a, s->rows, st);
+    int device = 0, num_sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess)
+        e = s->dtype == NLLB_F32   ? launch<float>(a, s->rows, num_sms, st)
+            : s->dtype == NLLB_F16 ? launch<__half>(a, s->rows, num_sms, st)
+                                   : launch<__nv_bfloat16>(a, s->rows, num_sms, st);
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_sample: ") + cudaGetErrorString(e));
     return NLLB_ATTN_OK;
 }
