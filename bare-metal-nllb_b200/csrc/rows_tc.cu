@@ -48,18 +48,16 @@ struct Cfg {
     static constexpr uint32_t OPER = PART * PARTS;
     // key tiles in flight: what leaves room for two CTAs per SM with one query tile, or fills the SM with two
     static constexpr int ST = F32 ? 1 : (NQ == 2 ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1));
-    // Fetch groups (K or V of a tile) in flight per thread beside the one being issued.  A group is handed over when
-    // group + LAG has been issued, which waits for the buffer of group + LAG - 2 ST: for K of tile j + 1 that may be
-    // K of tile j, whose products are done, but not V of tile j, which the second query tile still needs.
-    static constexpr int LAG = ST == 4 ? 3 : ST;
+    static constexpr int WORDS = 2 * ST + 2;  // key tiles whose visible keys are kept
     static constexpr uint32_t SQ = 0, SK = NQ * OPER, SV = SK + ST * OPER, SAUX = SV + ST * OPER;
-    static constexpr uint32_t PTRS = SAUX, VALID = PTRS + 4 * 128 * 8, BARS = VALID + 2 * ST * 16;
-    static constexpr int N_BARS = 4 * ST + 3 * NQ + 1;
+    static constexpr uint32_t PTRS = SAUX, VALID = PTRS + 4 * 128 * 8, BARS = VALID + WORDS * 16;
+    static constexpr int N_BARS = 4 * ST + 4 * NQ + 1;
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
     static constexpr int THREADS = NQ * 128 + kLoaders + 32;
     static constexpr uint32_t TMEM = NQ == 2 ? 512 : 256;  // S: 128 columns per tile, O: D per tile
     static constexpr int CTAS = NQ == 2 || (F32 && D == 128) ? 1 : 2;
+    static constexpr bool HOLD = NQ == 2;  // a row's scores stay in registers between their maximum and the weights
     static constexpr int LD = D + 4;  // fp32 row of a split's state: D sums, then m, l
     static_assert(NQ * 128 + NQ * D <= (int)TMEM, "tensor memory");
     static_assert(128 * LD * 4 <= (int)SAUX || NQ == 2, "a split's state fits over the operands");
@@ -71,12 +69,56 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0));
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives on `bar` (one of its expected arrivals) once this thread's copies so far have landed.  Their writes are
+// plain ones: who waits on the barrier fences before the tensor cores read them.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// A row's 128 scores (warp-wide), under one wait.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float* v) {
+    uint32_t r[128];
+#define NLLB_TMEM_LD32(T, R)                                                                                  \
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                    \
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "                    \
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"    \
+                 : "=r"(R[0]), "=r"(R[1]), "=r"(R[2]), "=r"(R[3]), "=r"(R[4]), "=r"(R[5]), "=r"(R[6]),        \
+                   "=r"(R[7]), "=r"(R[8]), "=r"(R[9]), "=r"(R[10]), "=r"(R[11]), "=r"(R[12]), "=r"(R[13]),    \
+                   "=r"(R[14]), "=r"(R[15]), "=r"(R[16]), "=r"(R[17]), "=r"(R[18]), "=r"(R[19]), "=r"(R[20]), \
+                   "=r"(R[21]), "=r"(R[22]), "=r"(R[23]), "=r"(R[24]), "=r"(R[25]), "=r"(R[26]), "=r"(R[27]), \
+                   "=r"(R[28]), "=r"(R[29]), "=r"(R[30]), "=r"(R[31])                                         \
+                 : "r"(T))
+    NLLB_TMEM_LD32(taddr, r);
+    NLLB_TMEM_LD32(taddr + 32, (r + 32));
+    NLLB_TMEM_LD32(taddr + 64, (r + 64));
+    NLLB_TMEM_LD32(taddr + 96, (r + 96));
+#undef NLLB_TMEM_LD32
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // D[128 x N] (+)= A . B, A from tensor memory.
@@ -98,6 +140,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -128,6 +179,18 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = pack2<__half>(a - ha, b - hb);
 }
 
+// 8 fp32 values as a 16-byte chunk of each part of an operand.
+template <uint32_t PART>
+__device__ __forceinline__ void split_store(unsigned char* to, const float4& a, const float4& b) {
+    uint4 hi, lo;
+    split2(a.x, a.y, hi.x, lo.x);
+    split2(a.z, a.w, hi.y, lo.y);
+    split2(b.x, b.y, hi.z, lo.z);
+    split2(b.z, b.w, hi.w, lo.w);
+    *reinterpret_cast<uint4*>(to) = hi;
+    *reinterpret_cast<uint4*>(to + PART) = lo;
+}
+
 template <typename T, int D, int NQ, bool PAGED>
 __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     rows_tc_kernel(const RowsParams p, int n_split) {
@@ -138,7 +201,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     unsigned char* sm = smem_raw + (base - raw);
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + C::BARS);
     uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
-    uint64_t *s_full = v_empty + ST, *p_full = s_full + NQ, *o_full = p_full + NQ, *done = o_full + NQ;
+    uint64_t *s_full = v_empty + ST, *p_full = s_full + NQ, *o_full = p_full + NQ, *q_full = o_full + NQ;
+    uint64_t* done = q_full + NQ;
     uint32_t* slot = reinterpret_cast<uint32_t*>(sm + C::SLOT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::SLOT + 4);
     const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::VALID);
@@ -168,6 +232,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             for (int i = 0; i < NQ; ++i) {
                 mbar_init(s_full + i, 1);
                 mbar_init(p_full + i, kTile);
+                mbar_init(q_full + i, kTile);
                 mbar_init(o_full + i, 1);
             }
             mbar_init(done, 1);
@@ -224,6 +289,39 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         const uint32_t lane_off = (uint32_t)(lq * 32) << 16;
         const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + NQ * 128 + (uint32_t)t * D;
         const float sl = p.scale_log2;
+        // this tile's queries, 16 bytes (fp32: 32) at a time
+        if (n > 0) {
+            const int lt = tid - t * kTile;
+            constexpr int CH = D / 8;
+#pragma unroll
+            for (int i0 = 0; i0 < CH; i0 += 8) {
+                const T* src[8];
+                float4 a[C::F32 ? 8 : 1], b[C::F32 ? 8 : 1];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int x = lt + (i0 + i) * kTile, r = row0 + t * kTile + x / CH, tk = r / p.group;
+                    src[i] = r < rows ? static_cast<const T*>(p.q) + (long long)(sq.q0 + tk) * p.q_row +
+                                            (long long)(g * p.group + (r - tk * p.group)) * p.q_head + (x % CH) * 8
+                                      : nullptr;
+                    if constexpr (C::F32) {
+                        a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (src[i]) {
+                            a[i] = __ldg(reinterpret_cast<const float4*>(src[i]));
+                            b[i] = __ldg(reinterpret_cast<const float4*>(src[i]) + 1);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int x = lt + (i0 + i) * kTile;
+                    const uint32_t at = C::SQ + t * C::OPER + chunk_off(x / CH, x % CH);
+                    if constexpr (C::F32) split_store<C::PART>(sm + at, a[i], b[i]);
+                    else cp_async16(base + at, src[i] ? src[i] : static_cast<const T*>(p.q), src[i] != nullptr);
+                }
+            }
+            if constexpr (C::F32) mbar_arrive(q_full + t);
+            else cp_arrive(q_full + t);
+        }
         float m = -INFINITY, l = 0.f;  // m: the maximum in use, in units of the scaled score
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
@@ -231,7 +329,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             if (j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;  // long over: its product came first
             tc_fence_after();
             if (any) {
-                const uint32_t* vw = valid + (j % (2 * ST)) * 4;
+                const uint32_t* vw = valid + (j % C::WORDS) * 4;
                 const int left = lim - (j0 + j) * kTile;  // visible keys of this tile, before the valid bits
                 uint32_t bits[4];
 #pragma unroll
@@ -239,21 +337,31 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     const int x = min(max(left - 32 * c, 0), 32);
                     bits[c] = vw[c] & (x == 32 ? 0xffffffffu : (1u << x) - 1u);
                 }
+                // (one copy of the row's work for whole tiles, one for those with hidden keys)
+                const bool whole = __all_sync(0xffffffffu, (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu);
+                float v[C::HOLD ? 128 : 64];
                 float mx = -INFINITY;
+                auto hide = [&](float* x, uint32_t w) {
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    float v[2][32];
-                    tmem_ld32x2(tS + 32 * c, tS + 32 * c + 32, v[0], v[1]);
+                    for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1u ? x[i] : -INFINITY;
+                };
+                if constexpr (C::HOLD) {
+                    tmem_ld128(tS, v);
+                    if (!whole) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (bits[c + h] == 0xffffffffu) {
+                        for (int c = 0; c < 4; ++c) hide(v + 32 * c, bits[c]);
+                    }
+                    float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[h][i]);
-                        } else {
+                    for (int i = 0; i < 128; i += 2) y[(i >> 1) & 3] = fmaxf(y[(i >> 1) & 3], fmaxf(v[i], v[i + 1]));
+                    mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+                } else {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                mx = fmaxf(mx, (bits[c + h] >> i) & 1u ? v[h][i] : -INFINITY);
-                        }
+                    for (int c = 0; c < 4; c += 2) {
+                        tmem_ld32x2(tS + 32 * c, tS + 32 * c + 32, v, v + 32);
+                        if (!whole) hide(v, bits[c]), hide(v + 32, bits[c + 1]);
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, v[i]);
                     }
                 }
                 const float mn = mx * sl;
@@ -265,45 +373,40 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     l *= corr;
                     if (j > 0) {
 #pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            tmem_ld32(tO + c, o);
-                            uint32_t r[2][16];
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tO + c, o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) r[i >> 4][i & 15] = __float_as_uint(o[i] * corr);
-                            tmem_st16(tO + c, r[0]);
-                            tmem_st16(tO + c + 16, r[1]);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            tmem_st16(tO + c, o);
                         }
                     }
                 }
                 const float off = (m == -INFINITY ? 0.f : m) - kWeightExp;
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    tmem_ld32(tS + 32 * c, v);
-                    if (bits[c] != 0xffffffffu) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = (bits[c] >> i) & 1u ? v[i] : -INFINITY;
+                    float* x = v + (C::HOLD ? 32 * c : 32 * (c & 1));
+                    if constexpr (!C::HOLD) {
+                        // (the second half is still in registers only for c = 2, 3, so all are read again)
+                        if ((c & 1) == 0) {
+                            tmem_ld32x2(tS + 32 * c, tS + 32 * c + 32, v, v + 32);
+                            if (!whole) hide(v, bits[c]), hide(v + 32, bits[c + 1]);
+                        }
                     }
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t hi[16], lo[C::F32 ? 16 : 1];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        v[i] = ex2_approx(fmaf(v[i], sl, -off));
-                        sum[i & 3] += v[i];
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    uint32_t hi[16];
-                    if constexpr (C::F32) {
-                        uint32_t lo[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
-                        tmem_st16(tS + 32 * c + 16, lo);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) hi[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sl, sl), make_float2(-off, -off));
+                        const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                        sum[i & 1] = add2(sum[i & 1], e);
+                        if constexpr (C::F32) split2(e.x, e.y, hi[i], lo[i]);
+                        else hi[i] = pack2<T>(e.x, e.y);
                     }
                     tmem_st16(tS + 32 * c, hi);
+                    if constexpr (C::F32) tmem_st16(tS + 32 * c + 16, lo);
                 }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
             }
             tc_fence_before();
@@ -366,12 +469,6 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 : "memory");
             return all != 0;
         };
-        auto q_row = [&](int r) -> const T* {
-            const int row = row0 + r;
-            if (row >= rows) return nullptr;
-            return static_cast<const T*>(p.q) + (long long)(sq.q0 + row / p.group) * p.q_row +
-                   (long long)(g * p.group + row % p.group) * p.q_head;
-        };
         // row addresses of key tile j, a row per thread (the first warp takes two), and which rows are visible
         auto addresses = [&](int j) {
             uint64_t* at = ptrs + (j & 1) * 256;
@@ -383,111 +480,67 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 at[r] = seen ? reinterpret_cast<uint64_t>(k) : 0;
                 at[128 + r] = seen ? reinterpret_cast<uint64_t>(v) : 0;
                 const uint32_t word = __ballot_sync(0xffffffffu, seen);
-                if (lane == 0) vw[(j % (2 * ST)) * 4 + (r >> 5)] = word;
+                if (lane == 0) vw[(j % C::WORDS) * 4 + (r >> 5)] = word;
             }
         };
+        // body(j, the tile's row addresses): both copies of a tile, the next tile's addresses under way
         bool ok = true;
-        if constexpr (!C::F32) {
-            constexpr int CH = D / 8;  // 16-byte chunks of a row
-#pragma unroll 4
-            // (without keys nothing is fetched: a split's state may be written at once)
-            for (int i = n > 0 ? lt : NQ * kTile * CH; i < NQ * kTile * CH; i += kLoaders) {
-                const int r = i / CH, c = i % CH;
-                const T* src = q_row(r);
-                cp_async16(base + C::SQ + (r / kTile) * C::OPER + chunk_off(r % kTile, c),
-                           src ? src + c * 8 : static_cast<const T*>(p.q), src != nullptr);
-            }
-            // group x = 2 j fetches K of tile j (the first with Q), 2 j + 1 its V
-            auto arrive = [&](int x) {
-                fence_async_smem();
-                mbar_arrive((x & 1 ? v_full : k_full) + (x >> 1) % ST);
-            };
+        auto tiles_of = [&](auto&& body) {
+            if (n > 0) addresses(0);
             for (int j = 0; j < n; ++j) {
-                addresses(j);
                 if (!(ok = loaders_sync(ok))) break;
-                const uint64_t* at = ptrs + (j & 1) * 256;
-                const int st = j % ST;
+                if (j + 1 < n) addresses(j + 1);
+                body(j, ptrs + (j & 1) * 256);
+            }
+        };
+        constexpr int CH = D / 8, PASSES = (kTile * CH + kLoaders - 1) / kLoaders;  // chunks of 8 elements
+        tiles_of([&](int j, const uint64_t* at) {
+            const int st = j % ST;
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    if (j >= ST) ok = ok && wait((kv ? v_empty : k_empty) + st, ((j / ST) - 1) & 1);
+            for (int kv = 0; kv < 2; ++kv) {
+                uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
+                const uint32_t dst = (kv ? C::SV : C::SK) + st * C::OPER;
+                if constexpr (!C::F32) {
+                    if (j >= ST) ok = ok && wait(empty, ((j / ST) - 1) & 1);
                     if (!ok) continue;  // to the next barrier, which all then leave together
-                    const uint32_t dst = base + (kv ? C::SV : C::SK) + st * C::OPER;
 #pragma unroll
-                    for (int i = 0; i < (kTile * CH + kLoaders - 1) / kLoaders; ++i) {
+                    for (int i = 0; i < PASSES; ++i) {
                         const int x = lt + i * kLoaders, r = x / CH, c = x % CH;
                         if (x >= kTile * CH) break;
                         const T* src = reinterpret_cast<const T*>(at[kv * 128 + r]);
-                        cp_async16(dst + chunk_off(r, c), src ? src + c * 8 : static_cast<const T*>(p.q),
+                        cp_async16(base + dst + chunk_off(r, c), src ? src + c * 8 : static_cast<const T*>(p.q),
                                    src != nullptr);
                     }
-                    cp_commit();
-                    if (2 * j + kv >= C::LAG) {
-                        cp_wait<C::LAG>();
-                        arrive(2 * j + kv - C::LAG);
-                    }
-                }
-            }
-            if (ok && n > 0) {
-                if constexpr (C::LAG >= 3)
-                    if (n > 1) cp_wait<2>(), arrive(2 * n - 3);
-                if constexpr (C::LAG >= 2) cp_wait<1>(), arrive(2 * n - 2);
-                cp_wait<0>(), arrive(2 * n - 1);
-            }
-            cp_wait<0>();
-        } else {
-            // fp32: 32 bytes (8 elements) of a row per thread become a chunk of each part
-            constexpr int CH = D / 8, PASSES = (kTile * CH + kLoaders - 1) / kLoaders, BATCH = 6;
-            auto store = [&](uint32_t dst, int r, int c, const float4& a, const float4& b) {
-                uint4 hi, lo;
-                split2(a.x, a.y, hi.x, lo.x);
-                split2(a.z, a.w, hi.y, lo.y);
-                split2(b.x, b.y, hi.z, lo.z);
-                split2(b.z, b.w, hi.w, lo.w);
-                unsigned char* to = sm + dst + chunk_off(r, c);
-                *reinterpret_cast<uint4*>(to) = hi;
-                *reinterpret_cast<uint4*>(to + C::PART) = lo;
-            };
-            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto fetch = [&](uint32_t dst, auto&& row_of, uint64_t* empty, uint32_t parity, bool must_wait) {
+                    cp_arrive(full);
+                } else {
+                    // fp32: 32 bytes of a row per thread become a chunk of each part
+                    constexpr int BATCH = 11;
 #pragma unroll
-                for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
-                    float4 a[BATCH], b[BATCH];
+                    for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
+                        float4 a[BATCH], b[BATCH];
 #pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        const int x = lt + (i0 + i) * kLoaders;
-                        const T* src = x < kTile * CH ? row_of(x / CH) : nullptr;
-                        a[i] = b[i] = zero;
-                        if (src) {
-                            const float4* f = reinterpret_cast<const float4*>(src) + (x % CH) * 2;
-                            a[i] = __ldg(f), b[i] = __ldg(f + 1);
+                        for (int i = 0; i < BATCH; ++i) {
+                            const int x = lt + (i0 + i) * kLoaders;
+                            const T* src = x < kTile * CH ? reinterpret_cast<const T*>(at[kv * 128 + x / CH]) : nullptr;
+                            a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (src) {
+                                const float4* f = reinterpret_cast<const float4*>(src) + (x % CH) * 2;
+                                a[i] = __ldg(f), b[i] = __ldg(f + 1);
+                            }
+                        }
+                        if (i0 == 0 && j >= ST) ok = ok && wait(empty, ((j / ST) - 1) & 1);
+                        if (!ok) break;
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) {
+                            const int x = lt + (i0 + i) * kLoaders;
+                            if (x < kTile * CH) split_store<C::PART>(sm + dst + chunk_off(x / CH, x % CH), a[i], b[i]);
                         }
                     }
-                    if (i0 == 0 && must_wait && !(ok = wait(empty, parity))) return;
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        const int x = lt + (i0 + i) * kLoaders;
-                        if (x < kTile * CH) store(dst, x / CH, x % CH, a[i], b[i]);
-                    }
-                }
-            };
-            if (n > 0) fetch(C::SQ, q_row, nullptr, 0, false);
-            for (int j = 0; j < n; ++j) {
-                addresses(j);
-                if (!(ok = loaders_sync(ok))) break;
-                const uint64_t* at = ptrs + (j & 1) * 256;
-                const int st = j % ST;
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    if (!ok) continue;  // to the next barrier, which all then leave together
-                    fetch((kv ? C::SV : C::SK) + st * C::OPER,
-                          [&](int r) { return reinterpret_cast<const T*>(at[kv * 128 + r]); },
-                          (kv ? v_empty : k_empty) + st, ((j / ST) - 1) & 1, j >= ST);
-                    if (!ok) continue;
-                    fence_async_smem();
-                    mbar_arrive((kv ? v_full : k_full) + st);
+                    if (ok) mbar_arrive(full);
                 }
             }
-        }
+        });
+        if constexpr (!C::F32) cp_wait_all();
     } else if (lane == 0) {
         // ---- products
         constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
@@ -522,24 +575,28 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         };
         bool ok = true;
         if (n > 0 && (ok = wait_one(k_full, 0))) {
-            tc_fence_after();
-            for (int t = 0; t < NQ; ++t) {
+            for (int t = 0; t < NQ && ok; ++t) {
+                if (!(ok = wait_one(q_full + t, 0))) break;
+                fence_async_smem();  // what the copies wrote
+                tc_fence_after();
                 scores(t, 0);
                 tc_commit(s_full + t);
             }
-            tc_commit(k_empty);
+            if (ok) tc_commit(k_empty);
         }
         for (int j = 0; j < n && ok; ++j) {
             const int st = j % ST, nx = (j + 1) % ST;
             for (int t = 0; t < NQ && ok; ++t) {
                 if (t == 0 && !(ok = wait_one(v_full + st, (j / ST) & 1))) break;
                 if (!(ok = wait_one(p_full + t, j & 1))) break;
+                fence_async_smem();
                 tc_fence_after();
                 output(t, st, j > 0);
                 tc_commit(o_full + t);
                 if (t == NQ - 1) tc_commit(v_empty + st);  // before the wait for K, which may come after the next V
                 if (j + 1 < n) {
                     if (t == 0 && !(ok = wait_one(k_full + nx, ((j + 1) / ST) & 1))) break;
+                    fence_async_smem();
                     tc_fence_after();
                     scores(t, nx);
                     tc_commit(s_full + t);
