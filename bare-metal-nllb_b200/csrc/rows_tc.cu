@@ -51,7 +51,10 @@ struct Cfg {
     static constexpr int WORDS = 2 * ST + 2;  // key tiles whose visible keys are kept
     static constexpr uint32_t SQ = 0, SK = NQ * OPER, SV = SK + ST * OPER, SAUX = SV + ST * OPER;
     static constexpr uint32_t PTRS = SAUX, VALID = PTRS + 4 * 128 * 8, BARS = VALID + WORDS * 16;
-    static constexpr int N_BARS = 4 * ST + 4 * NQ + 1;
+    // P beside S in tensor memory, where there is room: the next scores can then be taken as soon as a row is read
+    static constexpr bool AHEAD = NQ == 2 && D == 64;
+    static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D;
+    static constexpr int N_BARS = 4 * ST + 5 * NQ + 1;
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
     static constexpr int THREADS = NQ * 128 + kLoaders + 32;
@@ -59,7 +62,7 @@ struct Cfg {
     static constexpr int CTAS = NQ == 2 || (F32 && D == 128) ? 1 : 2;
     static constexpr bool HOLD = NQ == 2;  // a row's scores stay in registers between their maximum and the weights
     static constexpr int LD = D + 4;  // fp32 row of a split's state: D sums, then m, l
-    static_assert(NQ * 128 + NQ * D <= (int)TMEM, "tensor memory");
+    static_assert(NQ * 128 + NQ * D + (AHEAD ? NQ * 64 : 0) <= (int)TMEM, "tensor memory");
     static_assert(128 * LD * 4 <= (int)SAUX || NQ == 2, "a split's state fits over the operands");
 };
 
@@ -158,6 +161,12 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2^x, -inf -> +0
     return y;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + C::BARS);
     uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
     uint64_t *s_full = v_empty + ST, *p_full = s_full + NQ, *o_full = p_full + NQ, *q_full = o_full + NQ;
-    uint64_t* done = q_full + NQ;
+    uint64_t *s_read = q_full + NQ, *done = s_read + NQ;
     uint32_t* slot = reinterpret_cast<uint32_t*>(sm + C::SLOT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::SLOT + 4);
     const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::VALID);
@@ -233,6 +242,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 mbar_init(s_full + i, 1);
                 mbar_init(p_full + i, kTile);
                 mbar_init(q_full + i, kTile);
+                mbar_init(s_read + i, kTile);
                 mbar_init(o_full + i, 1);
             }
             mbar_init(done, 1);
@@ -287,7 +297,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         const int tok = row / p.group;
         const int lim = there ? (PAGED ? sq.kvn - sq.qn + tok + 1 : sq.kvn) : 0;
         const uint32_t lane_off = (uint32_t)(lq * 32) << 16;
-        const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + NQ * 128 + (uint32_t)t * D;
+        const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + C::O_COL + (uint32_t)t * D;
+        // the weights of 32 keys: 16 columns (and fp32's low parts in the next 16)
+        auto p_at = [&](int c) { return C::AHEAD ? tmem + lane_off + C::P_COL + t * 64 + 16 * c : tS + 32 * c; };
         const float sl = p.scale_log2;
         // this tile's queries, 16 bytes (fp32: 32) at a time
         if (n > 0) {
@@ -326,7 +338,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
             if (!(ok = wait(s_full + t, j & 1))) break;
-            if (j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;  // long over: its product came first
+            if (!C::AHEAD && j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;  // over: its product came first
             tc_fence_after();
             if (any) {
                 const uint32_t* vw = valid + (j % C::WORDS) * 4;
@@ -347,28 +359,35 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 };
                 if constexpr (C::HOLD) {
                     tmem_ld128(tS, v);
+                    if constexpr (C::AHEAD) {
+                        tc_fence_before();
+                        mbar_arrive(s_read + t);
+                    }
                     if (!whole) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c) hide(v + 32 * c, bits[c]);
                     }
                     float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2) y[(i >> 1) & 3] = fmaxf(y[(i >> 1) & 3], fmaxf(v[i], v[i + 1]));
-                    mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+                    for (int i = 0; i < 128; i += 2) y[(i >> 1) & 3] = max_nan(y[(i >> 1) & 3], max_nan(v[i], v[i + 1]));
+                    mx = max_nan(max_nan(y[0], y[1]), max_nan(y[2], y[3]));
                 } else {
 #pragma unroll
                     for (int c = 0; c < 4; c += 2) {
                         tmem_ld32x2(tS + 32 * c, tS + 32 * c + 32, v, v + 32);
                         if (!whole) hide(v, bits[c]), hide(v + 32, bits[c + 1]);
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, v[i]);
+                        for (int i = 0; i < 64; ++i) mx = max_nan(mx, v[i]);
                     }
                 }
+                if (C::AHEAD && j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;  // P and O are free
+                if (C::AHEAD) tc_fence_after();
                 const float mn = mx * sl;
-                const bool grown = mn > m + kGrow || (m == -INFINITY && mn > -INFINITY);
+                const bool grown = !(mn <= m + kGrow);  // a NaN makes the whole row NaN
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float to = fmaxf(m, mn);
-                    const float corr = m == -INFINITY ? 0.f : ex2_approx(m - to);
+                    // (a row's own affair: what its neighbours hold changes none of its roundings)
+                    const float to = grown ? max_nan(m, mn) : m;
+                    const float corr = m == to ? 1.f : m == -INFINITY ? 0.f : ex2_approx(m - to);
                     m = to;
                     l *= corr;
                     if (j > 0) {
@@ -403,11 +422,15 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         if constexpr (C::F32) split2(e.x, e.y, hi[i], lo[i]);
                         else hi[i] = pack2<T>(e.x, e.y);
                     }
-                    tmem_st16(tS + 32 * c, hi);
-                    if constexpr (C::F32) tmem_st16(tS + 32 * c + 16, lo);
+                    tmem_st16(p_at(c), hi);
+                    if constexpr (C::F32) tmem_st16(p_at(c) + 16, lo);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
+            } else if (C::AHEAD) {
+                mbar_arrive(s_read + t);
+                // not a tile ahead of the other warps, whose arrivals would be taken for this one's
+                if (j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;
             }
             tc_fence_before();
             mbar_arrive(p_full + t);
@@ -561,10 +584,10 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             }
         };
         auto output = [&](int t, int st, bool accumulate) {
-            const uint32_t v = base + C::SV + st * C::OPER, o = tmem + NQ * 128 + t * D;
+            const uint32_t v = base + C::SV + st * C::OPER, o = tmem + C::O_COL + t * D;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                const uint32_t a = tmem + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8;
+                const uint32_t a = C::AHEAD ? tmem + C::P_COL + t * 64 + ks * 8 : tmem + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8;
                 const uint64_t b = umma_desc_k_sw128(v + ks * 2048) ^ lead;
                 tc_mma_f16_ta(o, a, b, id_o, accumulate || ks > 0);
                 if constexpr (C::F32) {
@@ -586,6 +609,22 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         }
         for (int j = 0; j < n && ok; ++j) {
             const int st = j % ST, nx = (j + 1) % ST;
+            // scores of the next key tile: K has come and (AHEAD) the row's last ones are read
+            auto next = [&](int t) -> bool {
+                if (j + 1 >= n) return true;
+                if (t == 0 && !wait_one(k_full + nx, ((j + 1) / ST) & 1)) return false;
+                if (C::AHEAD && !wait_one(s_read + t, j & 1)) return false;
+                fence_async_smem();
+                tc_fence_after();
+                scores(t, nx);
+                tc_commit(s_full + t);
+                if (t == NQ - 1) tc_commit(k_empty + nx);
+                return true;
+            };
+            if constexpr (C::AHEAD) {
+                for (int t = 0; t < NQ && ok; ++t) ok = next(t);
+                if (!ok) break;
+            }
             for (int t = 0; t < NQ && ok; ++t) {
                 if (t == 0 && !(ok = wait_one(v_full + st, (j / ST) & 1))) break;
                 if (!(ok = wait_one(p_full + t, j & 1))) break;
@@ -593,16 +632,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 tc_fence_after();
                 output(t, st, j > 0);
                 tc_commit(o_full + t);
-                if (t == NQ - 1) tc_commit(v_empty + st);  // before the wait for K, which may come after the next V
-                if (j + 1 < n) {
-                    if (t == 0 && !(ok = wait_one(k_full + nx, ((j + 1) / ST) & 1))) break;
-                    fence_async_smem();
-                    tc_fence_after();
-                    scores(t, nx);
-                    tc_commit(s_full + t);
-                }
+                if (t == NQ - 1) tc_commit(v_empty + st);
+                if constexpr (!C::AHEAD) ok = next(t);  // P lies over S
             }
-            if (ok && j + 1 < n) tc_commit(k_empty + nx);
         }
         // whatever was issued is over before tensor memory is given back
         tc_commit(done);

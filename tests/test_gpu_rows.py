@@ -165,6 +165,19 @@ def test_paged_matches_64_bits(ctx, lens, heads, kv_heads, dim, dtype):
     assert torch.equal(c.k_pages, k) and torch.equal(c.v_pages, v)  # the chunk's slots and no others
 
 
+# enough (sequence, key head) pairs that a CTA takes two query tiles: tails of one row, of a whole and of half a tile
+MANY = [(129, 0), (256, 300), (257, 3), (130, 1000), (384, 64), (300, 127), (1, 9), (0, 0), (200, 700), (385, 31)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 16, 64), (16, 16, 128), (24, 12, 64), (36, 12, 128)])
+def test_paged_many_chunks(ctx, heads, kv_heads, dim, dtype):
+    c = Paged(MANY, heads, kv_heads, dim, 32, dtype, seed=heads + dim)
+    c.run(ctx)
+    ctx.sync()
+    c.verify("many chunks")
+
+
 @pytest.mark.parametrize("page", [1, 7, 48, 128])
 @pytest.mark.parametrize("hnd", [False, True], ids=["nhd", "hnd"])
 @pytest.mark.parametrize("lens", ["tokens", "chunks"])
@@ -365,6 +378,16 @@ def test_cross_rows_matches_64_bits(ctx, lens, heads, kv_heads, dim, dtype, hide
     ctx.sync()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 16, 64), (16, 16, 128), (24, 12, 64)])
+@pytest.mark.parametrize("hide", [0.0, 0.3, 0.99])
+def test_cross_rows_many_sequences(ctx, heads, kv_heads, dim, dtype, hide):
+    c = Cross([(n, t) for n, t in MANY], heads, kv_heads, dim, dtype, seed=heads + dim, hide=hide)
+    c.run(ctx)
+    c.verify("many sequences")
+    ctx.sync()
+
+
 def test_cross_rows_hidden_keys_may_hold_anything(ctx):
     for dtype in TYPES:
         for lens in ("tokens", "rows"):
@@ -386,6 +409,19 @@ def test_cross_rows_nan_query_stays_in_its_row(ctx):
             c.run(ctx)
             assert torch.isnan(c.out[1, 1]).all()
             c.out[1, 1] = plain[1, 1]
+            assert torch.equal(c.out, plain)
+
+
+def test_cross_rows_nan_key_reaches_the_rows_that_see_it(ctx):
+    for dtype in TYPES:
+        for key in (0, 5, 6, 7, 70):  # whichever way its weight is taken
+            c = Cross([(200, 74), (140, 90)], 4, 2, 64, dtype)
+            c.run(ctx)
+            plain = c.out.clone()
+            c.k[key, 1] = float("nan")  # read by query heads 2 and 3 of the first sequence
+            c.run(ctx)
+            assert torch.isnan(c.out[:200, 2:]).all()
+            c.out[:200, 2:] = plain[:200, 2:]
             assert torch.equal(c.out, plain)
 
 
