@@ -33,11 +33,29 @@ __device__ __forceinline__ bool rows_sequence(const RowsParams& p, int s, RowsSe
     return ok;
 }
 
-// Where key `j` of the sequence lies (j < kvn), for K and for V.  False: its
-// page number is outside the pool (flagged), or the mask hides the key.
+// j / page by a multiplication: page_mul = ceil(2^page_shr / page), exact for
+// j < 2^30 (rows_api.cu).
+__device__ __forceinline__ int rows_page(const RowsParams& p, int j) {
+    return (int)((unsigned long long)(uint32_t)j * p.page_mul >> p.page_shr);
+}
+
+// What has to be looked up to place key `j` of the sequence (j < kvn): its
+// page number, or its byte of the mask.  Apart from rows_at, so that it can be
+// asked for ahead of its use.
+template <bool PAGED>
+__device__ __forceinline__ int rows_entry(const RowsParams& p, const RowsSeq& q, int s, int j) {
+    if (PAGED) {
+        if (p.k_new && j >= q.kvn - q.qn) return 0;
+        return __ldg(p.table + (long long)s * p.table_ld + rows_page(p, j));
+    }
+    return p.mask ? __ldg(p.mask + q.kv0 + j) : 1;
+}
+
+// Where key `j` lies, for K and for V.  False: its page number is outside the
+// pool (flagged), or the mask hides the key.
 template <typename T, bool PAGED>
-__device__ __forceinline__ bool rows_key(const RowsParams& p, const RowsSeq& q, int s, int g, int j, const T*& k,
-                                         const T*& v) {
+__device__ __forceinline__ bool rows_at(const RowsParams& p, const RowsSeq& q, int g, int j, int entry, const T*& k,
+                                        const T*& v) {
     if (PAGED) {
         const int first_new = q.kvn - q.qn;
         if (p.k_new && j >= first_new) {  // the chunk's own rows are read where they come from
@@ -46,21 +64,25 @@ __device__ __forceinline__ bool rows_key(const RowsParams& p, const RowsSeq& q, 
             v = static_cast<const T*>(p.v_new) + r * p.vn_row + (long long)g * p.vn_head;
             return true;
         }
-        const int pg = __ldg(p.table + (long long)s * p.table_ld + j / p.page);
-        if ((unsigned)pg >= (unsigned)p.n_pages) {
+        if ((unsigned)entry >= (unsigned)p.n_pages) {
             atomicOr(p.err, NLLB_DEV_ERR_BAD_PAGE);
             return false;
         }
-        const long long slot = j % p.page;
-        k = static_cast<const T*>(p.k) + pg * p.k_page + slot * p.k_row + (long long)g * p.k_head;
-        v = static_cast<const T*>(p.v) + pg * p.v_page + slot * p.v_row + (long long)g * p.v_head;
+        const long long slot = j - rows_page(p, j) * p.page;
+        k = static_cast<const T*>(p.k) + entry * p.k_page + slot * p.k_row + (long long)g * p.k_head;
+        v = static_cast<const T*>(p.v) + entry * p.v_page + slot * p.v_row + (long long)g * p.v_head;
         return true;
     }
     const long long r = q.kv0 + j;
-    if (p.mask && __ldg(p.mask + r) == 0) return false;
     k = static_cast<const T*>(p.k) + r * p.k_row + (long long)g * p.k_head;
     v = static_cast<const T*>(p.v) + r * p.v_row + (long long)g * p.v_head;
-    return true;
+    return entry != 0;
+}
+
+template <typename T, bool PAGED>
+__device__ __forceinline__ bool rows_key(const RowsParams& p, const RowsSeq& q, int s, int g, int j, const T*& k,
+                                         const T*& v) {
+    return rows_at<T, PAGED>(p, q, g, j, rows_entry<PAGED>(p, q, s, j), k, v);
 }
 
 // The chunk's rows of tokens [t0, t1) of key head g go into their pages.
@@ -71,12 +93,12 @@ __device__ __forceinline__ void rows_append(const RowsParams& p, const RowsSeq& 
     constexpr int CH = D * (int)sizeof(T) / 16;
     for (int i = tid; i < (t1 - t0) * CH; i += n_threads) {
         const int t = t0 + i / CH, c = i % CH, j = q.kvn - q.qn + t;
-        const int pg = __ldg(p.table + (long long)s * p.table_ld + j / p.page);
+        const int at = rows_page(p, j), pg = __ldg(p.table + (long long)s * p.table_ld + at);
         if ((unsigned)pg >= (unsigned)p.n_pages) {
             atomicOr(p.err, NLLB_DEV_ERR_BAD_PAGE);
             continue;
         }
-        const long long r = q.q0 + t, slot = j % p.page;
+        const long long r = q.q0 + t, slot = j - at * p.page;
         const uint4 kv = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + r * p.kn_row +
                                                                (long long)g * p.kn_head) + c);
         const uint4 vv = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + r * p.vn_row +

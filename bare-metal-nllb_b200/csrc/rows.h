@@ -31,6 +31,8 @@ struct RowsParams {
     int n_seq, kv_heads, group;
     int q_rows, kv_rows, max_q, max_kv;
     int table_ld, n_pages, page;
+    uint32_t page_mul;  // j / page = j * page_mul >> page_shr
+    int page_shr;
     float scale_log2;  // scale * log2(e)
     int* err;
 };

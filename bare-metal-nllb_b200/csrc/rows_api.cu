@@ -68,6 +68,7 @@ int nllb_attn_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a) {
         return bad("q, k_pages, v_pages, out, page_table and kv_len are required");
     if (!a->k_new != !a->v_new) return bad("k_new and v_new go together");
     if (a->n_pages < 1 || a->page_size < 1) return bad("n_pages and page_size must be >= 1");
+    if (a->page_size > (1 << 30)) return set_error(NLLB_ATTN_ECAPACITY, "page_size above 2^30");
     if ((long long)a->page_table_stride * a->page_size < a->max_kv)
         return bad("page_table_stride * page_size must reach max_kv");
     if (!a->q_start && (long long)a->n_seq * a->max_q > a->q_rows) return bad("q_rows must reach n_seq * max_q");
@@ -89,6 +90,12 @@ int nllb_attn_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a) {
     p.n_seq = a->n_seq, p.kv_heads = a->n_kv_heads, p.group = a->n_heads / a->n_kv_heads;
     p.q_rows = a->q_rows, p.max_q = a->max_q, p.max_kv = a->max_kv;
     p.table_ld = a->page_table_stride, p.n_pages = a->n_pages, p.page = a->page_size;
+    // With 2^(b-1) < page <= 2^b the multiplier ceil(2^(30+b) / page) is too large by less than 1, so the quotient of a
+    // j < 2^30 by less than 2^30 / 2^(30+b) <= 1 / page: it stays below the next whole number.
+    int b = 0;
+    while ((1LL << b) < a->page_size) ++b;
+    p.page_shr = 30 + b;
+    p.page_mul = (uint32_t)(((1ULL << p.page_shr) + (uint64_t)a->page_size - 1) / (uint64_t)a->page_size);
     p.scale_log2 = a->scale * kLog2e;
     return launch(c, p, a->dtype, a->head_dim, true);
 }

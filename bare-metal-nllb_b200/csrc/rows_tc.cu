@@ -30,6 +30,15 @@
 
 #include "rows.cuh"
 
+#ifndef ROWS_EXP
+#define ROWS_EXP 0
+#endif
+#ifndef ROWS_WPT1
+#define ROWS_WPT1 8
+#endif
+#ifndef ROWS_WPT2
+#define ROWS_WPT2 4
+#endif
 namespace nllb {
 namespace {
 
@@ -48,19 +57,21 @@ struct Cfg {
     static constexpr uint32_t OPER = PART * PARTS;
     // key tiles in flight: what leaves room for two CTAs per SM with one query tile, or fills the SM with two
     static constexpr int ST = F32 ? 1 : (NQ == 2 ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1));
+    // Softmax warps of a query tile; with 8, two threads share a row.
+    static constexpr int WPT = NQ == 2 ? ROWS_WPT2 : ROWS_WPT1, SOFT = NQ * WPT * 32;  // and softmax threads in all
+    static constexpr int COLS = 128 * 4 / WPT;                      // scores of a thread
     static constexpr int WORDS = 2 * ST + 2;  // key tiles whose visible keys are kept
     static constexpr uint32_t SQ = 0, SK = NQ * OPER, SV = SK + ST * OPER, SAUX = SV + ST * OPER;
-    static constexpr uint32_t PTRS = SAUX, VALID = PTRS + 4 * 128 * 8, BARS = VALID + WORDS * 16;
+    static constexpr uint32_t VALID = SAUX, MAXS = VALID + WORDS * 16, BARS = MAXS + (WPT == 8 ? 2 * NQ * 2 * 128 * 4 : 0);
     // P beside S in tensor memory, where there is room: the next scores can then be taken as soon as a row is read
     static constexpr bool AHEAD = NQ == 2 && D == 64;
     static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D;
-    static constexpr int N_BARS = 4 * ST + 5 * NQ + 1;
+    static constexpr int N_BARS = 4 * ST + 9 * NQ + 1;
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
-    static constexpr int THREADS = NQ * 128 + kLoaders + 32;
+    static constexpr int THREADS = SOFT + kLoaders + 32;
     static constexpr uint32_t TMEM = NQ == 2 ? 512 : 256;  // S: 128 columns per tile, O: D per tile
     static constexpr int CTAS = NQ == 2 || (F32 && D == 128) ? 1 : 2;
-    static constexpr bool HOLD = NQ == 2;  // a row's scores stay in registers between their maximum and the weights
     static constexpr int LD = D + 4;  // fp32 row of a split's state: D sums, then m, l
     static_assert(NQ * 128 + NQ * D + (AHEAD ? NQ * 64 : 0) <= (int)TMEM, "tensor memory");
     static_assert(128 * LD * 4 <= (int)SAUX || NQ == 2, "a split's state fits over the operands");
@@ -101,28 +112,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// A row's 128 scores (warp-wide), under one wait.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float* v) {
-    uint32_t r[128];
-#define NLLB_TMEM_LD32(T, R)                                                                                  \
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                    \
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "                    \
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"    \
-                 : "=r"(R[0]), "=r"(R[1]), "=r"(R[2]), "=r"(R[3]), "=r"(R[4]), "=r"(R[5]), "=r"(R[6]),        \
-                   "=r"(R[7]), "=r"(R[8]), "=r"(R[9]), "=r"(R[10]), "=r"(R[11]), "=r"(R[12]), "=r"(R[13]),    \
-                   "=r"(R[14]), "=r"(R[15]), "=r"(R[16]), "=r"(R[17]), "=r"(R[18]), "=r"(R[19]), "=r"(R[20]), \
-                   "=r"(R[21]), "=r"(R[22]), "=r"(R[23]), "=r"(R[24]), "=r"(R[25]), "=r"(R[26]), "=r"(R[27]), \
-                   "=r"(R[28]), "=r"(R[29]), "=r"(R[30]), "=r"(R[31])                                         \
-                 : "r"(T))
-    NLLB_TMEM_LD32(taddr, r);
-    NLLB_TMEM_LD32(taddr + 32, (r + 32));
-    NLLB_TMEM_LD32(taddr + 64, (r + 64));
-    NLLB_TMEM_LD32(taddr + 96, (r + 96));
-#undef NLLB_TMEM_LD32
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // D[128 x N] (+)= A . B, A from tensor memory.
 __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -161,7 +150,12 @@ __device__ __forceinline__ float ex2_approx(float x) {  // 2^x, -inf -> +0
     return y;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b, float c) {  // NaN if any is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
     float c;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
     return c;
@@ -211,7 +205,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + C::BARS);
     uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
     uint64_t *s_full = v_empty + ST, *p_full = s_full + NQ, *o_full = p_full + NQ, *q_full = o_full + NQ;
-    uint64_t *s_read = q_full + NQ, *done = s_read + NQ;
+    uint64_t *s_read = q_full + NQ, *pair = s_read + NQ, *done = pair + 4 * NQ;
     uint32_t* slot = reinterpret_cast<uint32_t*>(sm + C::SLOT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::SLOT + 4);
     const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::VALID);
@@ -240,9 +234,10 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             }
             for (int i = 0; i < NQ; ++i) {
                 mbar_init(s_full + i, 1);
-                mbar_init(p_full + i, kTile);
-                mbar_init(q_full + i, kTile);
-                mbar_init(s_read + i, kTile);
+                mbar_init(p_full + i, C::WPT);
+                mbar_init(q_full + i, C::WPT * 32);
+                mbar_init(s_read + i, C::WPT);
+                for (int k = 0; k < 4; ++k) mbar_init(pair + 4 * i + k, 2);
                 mbar_init(o_full + i, 1);
             }
             mbar_init(done, 1);
@@ -278,18 +273,24 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         }
         return true;
     };
+    // One arrival for a whole warp: 32 at one address are taken one after the other.
+    auto warp_arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
     // The same for a whole warp, with one answer.
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         return __all_sync(0xffffffffu, wait_one(bar, parity));
     };
 
-    if (warp < NQ * 4) {
-        // ---- softmax: thread = query row
-        const int t = warp >> 2, lq = warp & 3;  // query tile, TMEM lane quarter
+    if (warp < NQ * C::WPT) {
+        // ---- softmax: a thread, or two, to a query row
+        const int t = warp / C::WPT, lq = warp & 3;                     // query tile, TMEM lane quarter
+        const int half = C::WPT == 8 ? (warp % C::WPT) >> 2 : 0;        // of the row's scores
         if (PAGED && p.k_new && split == 0) {
             const int t0 = (row0 + p.group - 1) / p.group;
             const int t1 = min(sq.qn, (row0 + NQ * kTile + p.group - 1) / p.group);
-            rows_append<T, D>(p, sq, s, g, t0, t1, tid, NQ * 128);
+            rows_append<T, D>(p, sq, s, g, t0, t1, tid, C::SOFT);
         }
         const int row = row0 + t * kTile + lq * 32 + lane;
         const bool there = row < rows;
@@ -300,18 +301,28 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + C::O_COL + (uint32_t)t * D;
         // the weights of 32 keys: 16 columns (and fp32's low parts in the next 16)
         auto p_at = [&](int c) { return C::AHEAD ? tmem + lane_off + C::P_COL + t * 64 + 16 * c : tS + 32 * c; };
+        // x of this thread's row and y of the other thread's, whichever way round: the step'th exchange of the pair
+        auto other = [&](float x, int step, float& y) -> bool {
+            float* at = reinterpret_cast<float*>(sm + C::MAXS) + ((step & 1) * NQ + t) * 256 + lq * 32 + lane;
+            at[half * 128] = x;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pair + t * 4 + lq);
+            const bool ok = wait(pair + t * 4 + lq, step & 1);
+            y = at[(half ^ 1) * 128];
+            return ok;
+        };
         const float sl = p.scale_log2;
         // this tile's queries, 16 bytes (fp32: 32) at a time
         if (n > 0) {
-            const int lt = tid - t * kTile;
-            constexpr int CH = D / 8;
+            constexpr int CH = D / 8, N = C::WPT * 32, TAKE = kTile * CH / N < 8 ? kTile * CH / N : 8;
+            const int lt = tid - t * N;
 #pragma unroll
-            for (int i0 = 0; i0 < CH; i0 += 8) {
-                const T* src[8];
-                float4 a[C::F32 ? 8 : 1], b[C::F32 ? 8 : 1];
+            for (int i0 = 0; i0 < kTile * CH / N; i0 += TAKE) {
+                const T* src[TAKE];
+                float4 a[C::F32 ? TAKE : 1], b[C::F32 ? TAKE : 1];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int x = lt + (i0 + i) * kTile, r = row0 + t * kTile + x / CH, tk = r / p.group;
+                for (int i = 0; i < TAKE; ++i) {
+                    const int x = lt + (i0 + i) * N, r = row0 + t * kTile + x / CH, tk = r / p.group;
                     src[i] = r < rows ? static_cast<const T*>(p.q) + (long long)(sq.q0 + tk) * p.q_row +
                                             (long long)(g * p.group + (r - tk * p.group)) * p.q_head + (x % CH) * 8
                                       : nullptr;
@@ -324,8 +335,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int x = lt + (i0 + i) * kTile;
+                for (int i = 0; i < TAKE; ++i) {
+                    const int x = lt + (i0 + i) * N;
                     const uint32_t at = C::SQ + t * C::OPER + chunk_off(x / CH, x % CH);
                     if constexpr (C::F32) split_store<C::PART>(sm + at, a[i], b[i]);
                     else cp_async16(base + at, src[i] ? src[i] : static_cast<const T*>(p.q), src[i] != nullptr);
@@ -343,42 +354,40 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             if (any) {
                 const uint32_t* vw = valid + (j % C::WORDS) * 4;
                 const int left = lim - (j0 + j) * kTile;  // visible keys of this tile, before the valid bits
-                uint32_t bits[4];
+                constexpr int NC = C::COLS / 32;
+                uint32_t bits[NC], all = 0xffffffffu;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int x = min(max(left - 32 * c, 0), 32);
-                    bits[c] = vw[c] & (x == 32 ? 0xffffffffu : (1u << x) - 1u);
+                for (int c = 0; c < NC; ++c) {
+                    const int x = min(max(left - 32 * (half * NC + c), 0), 32);
+                    bits[c] = vw[half * NC + c] & (x == 32 ? 0xffffffffu : (1u << x) - 1u);
+                    all &= bits[c];
                 }
                 // (one copy of the row's work for whole tiles, one for those with hidden keys)
-                const bool whole = __all_sync(0xffffffffu, (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu);
-                float v[C::HOLD ? 128 : 64];
-                float mx = -INFINITY;
+                const bool whole = __all_sync(0xffffffffu, all == 0xffffffffu);
+                const uint32_t tR = tS + half * C::COLS;
+                float v[C::COLS];  // (a row's scores stay in registers between their maximum and the weights)
                 auto hide = [&](float* x, uint32_t w) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1u ? x[i] : -INFINITY;
                 };
-                if constexpr (C::HOLD) {
-                    tmem_ld128(tS, v);
-                    if constexpr (C::AHEAD) {
-                        tc_fence_before();
-                        mbar_arrive(s_read + t);
-                    }
-                    if (!whole) {
+                float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) hide(v + 32 * c, bits[c]);
-                    }
-                    float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int c = 0; c < NC; c += 2) {
+                    float* x = v + 32 * c;
+                    tmem_ld32x2(tR + 32 * c, tR + 32 * c + 32, x, x + 32);
+                    if (!whole) hide(x, bits[c]), hide(x + 32, bits[c + 1]);
 #pragma unroll
-                    for (int i = 0; i < 128; i += 2) y[(i >> 1) & 3] = max_nan(y[(i >> 1) & 3], max_nan(v[i], v[i + 1]));
-                    mx = max_nan(max_nan(y[0], y[1]), max_nan(y[2], y[3]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; c += 2) {
-                        tmem_ld32x2(tS + 32 * c, tS + 32 * c + 32, v, v + 32);
-                        if (!whole) hide(v, bits[c]), hide(v + 32, bits[c + 1]);
-#pragma unroll
-                        for (int i = 0; i < 64; ++i) mx = max_nan(mx, v[i]);
-                    }
+                    for (int i = 0; i < 64; i += 2) y[(i >> 1) & 3] = max_nan(y[(i >> 1) & 3], x[i], x[i + 1]);
+                }
+                if constexpr (C::AHEAD) {
+                    tc_fence_before();
+                    warp_arrive(s_read + t);
+                }
+                float mx = max_nan(max_nan(y[0], y[1]), max_nan(y[2], y[3]));
+                if constexpr (C::WPT == 8) {
+                    float his;
+                    if (!(ok = other(mx, j, his))) break;
+                    mx = max_nan(mx, his);
                 }
                 if (C::AHEAD && j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;  // P and O are free
                 if (C::AHEAD) tc_fence_after();
@@ -392,7 +401,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     l *= corr;
                     if (j > 0) {
 #pragma unroll
-                        for (int c = 0; c < D; c += 16) {
+                        for (int c = half * (D / 2); c < (C::WPT == 8 ? (half + 1) * (D / 2) : D); c += 16) {
                             uint32_t o[16];
                             tmem_ld16(tO + c, o);
 #pragma unroll
@@ -404,16 +413,10 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 const float off = (m == -INFINITY ? 0.f : m) - kWeightExp;
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float* x = v + (C::HOLD ? 32 * c : 32 * (c & 1));
-                    if constexpr (!C::HOLD) {
-                        // (the second half is still in registers only for c = 2, 3, so all are read again)
-                        if ((c & 1) == 0) {
-                            tmem_ld32x2(tS + 32 * c, tS + 32 * c + 32, v, v + 32);
-                            if (!whole) hide(v, bits[c]), hide(v + 32, bits[c + 1]);
-                        }
-                    }
+                for (int c = 0; c < NC; ++c) {
+                    float* x = v + 32 * c;
                     uint32_t hi[16], lo[C::F32 ? 16 : 1];
+#if ROWS_EXP == 0
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sl, sl), make_float2(-off, -off));
@@ -422,28 +425,69 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         if constexpr (C::F32) split2(e.x, e.y, hi[i], lo[i]);
                         else hi[i] = pack2<T>(e.x, e.y);
                     }
-                    tmem_st16(p_at(c), hi);
-                    if constexpr (C::F32) tmem_st16(p_at(c) + 16, lo);
+#elif ROWS_EXP == 1
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], sl, -off);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        sum[i & 1].x += x[2 * i], sum[i & 1].y += x[2 * i + 1];
+                        if constexpr (C::F32) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+                        else hi[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+                    }
+#elif ROWS_EXP == 2
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        x[2 * i] = ex2_approx(fmaf(x[2 * i], sl, -off));
+                        x[2 * i + 1] = ex2_approx(fmaf(x[2 * i + 1], sl, -off));
+                        sum[i & 1].x += x[2 * i], sum[i & 1].y += x[2 * i + 1];
+                        if constexpr (C::F32) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+                        else hi[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+                    }
+#elif ROWS_EXP == 3
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sl, sl), make_float2(-off, -off));
+                        x[2 * i] = y.x, x[2 * i + 1] = y.y;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        sum[i & 1] = add2(sum[i & 1], make_float2(x[2 * i], x[2 * i + 1]));
+                        if constexpr (C::F32) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+                        else hi[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+                    }
+#endif
+                    tmem_st16(p_at(half * NC + c), hi);
+                    if constexpr (C::F32) tmem_st16(p_at(half * NC + c) + 16, lo);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
             } else if (C::AHEAD) {
-                mbar_arrive(s_read + t);
+                warp_arrive(s_read + t);
                 // not a tile ahead of the other warps, whose arrivals would be taken for this one's
                 if (j > 0 && !(ok = wait(o_full + t, (j - 1) & 1))) break;
             }
             tc_fence_before();
-            mbar_arrive(p_full + t);
+            warp_arrive(p_full + t);
         }
         if (ok && n > 0) ok = wait(o_full + t, (n - 1) & 1);
         tc_fence_after();
+        if constexpr (C::WPT == 8) {  // the row's whole sum
+            float his = 0.f;
+            if (ok && any && n > 0) ok = other(l, n, his);
+            l = half ? his + l : l + his;
+        }
+        const int d0 = half * (D / 2), d1 = C::WPT == 8 ? d0 + D / 2 : D;  // this thread's part of the output
         if (n_split == 1) {
             if (ok && any) {
                 const float inv = 1.0f / l;
                 T* dst = static_cast<T*>(p.out) + (long long)(sq.q0 + tok) * p.o_row +
                          (long long)(g * p.group + row % p.group) * p.o_head;
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
+                for (int c = d0; c < d1; c += 32) {
                     float o[32];
                     if (n > 0) tmem_ld32(tO + c, o);
                     constexpr int VEC = 16 / (int)sizeof(T);
@@ -463,7 +507,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             if (any) {
                 float* st = reinterpret_cast<float*>(sm) + (lq * 32 + lane) * C::LD;
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
+                for (int c = d0; c < d1; c += 32) {
                     float o[32];
                     if (n > 0) tmem_ld32(tO + c, o);
 #pragma unroll
@@ -471,98 +515,92 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         *reinterpret_cast<float4*>(st + c + i) =
                             l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
-                *reinterpret_cast<float4*>(st + D) = make_float4(l == 0.f ? -INFINITY : m, ok ? l : -1.f, 0.f, 0.f);
+                if (half == 0) *reinterpret_cast<float4*>(st + D) = make_float4(l == 0.f ? -INFINITY : m, ok ? l : -1.f, 0.f, 0.f);
             }
         }
-    } else if (warp < NQ * 4 + kLoaders / 32) {
+    } else if (warp < (C::SOFT + kLoaders) / 32) {
         // ---- fetch
-        const int lt = tid - NQ * 128;
-        uint64_t* ptrs = reinterpret_cast<uint64_t*>(sm + C::PTRS);
-        uint32_t* vw = reinterpret_cast<uint32_t*>(sm + C::VALID);
-        // barrier of the fetching threads; true if all of them are still at work
-        auto loaders_sync = [](bool ok) -> bool {
-            uint32_t all;
-            asm volatile(
-                "{\n\t.reg .pred p, q;\n\t"
-                "setp.ne.b32 p, %1, 0;\n\t"
-                "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
-                "selp.u32 %0, 1, 0, q;\n\t}"
-                : "=r"(all)
-                : "r"((uint32_t)ok), "n"(kLoaders)
-                : "memory");
-            return all != 0;
-        };
-        // row addresses of key tile j, a row per thread (the first warp takes two), and which rows are visible
-        auto addresses = [&](int j) {
-            uint64_t* at = ptrs + (j & 1) * 256;
+        // Two lanes to a row, which take its 16-byte chunks in turns (a row's 32-byte sectors are then used whole):
+        // the row's address stays in a register, and a copy costs little beside it.
+        const int lt = tid - C::SOFT, odd = lt & 1;
+        constexpr int CH = D / 8, RP = (2 * kTile + kLoaders - 1) / kLoaders;  // chunks of 8 elements; rows of a lane
+        uint16_t* seen16 = reinterpret_cast<uint16_t*>(sm + C::VALID);
+        int entry[RP];
+        auto look_up = [&](int j) {
 #pragma unroll
-            for (int r = lt; r < kTile; r += kLoaders) {
-                const int key = (j0 + j) * kTile + r;
-                const T *k = nullptr, *v = nullptr;
-                const bool seen = key < longest && rows_key<T, PAGED>(p, sq, s, g, key, k, v);
-                at[r] = seen ? reinterpret_cast<uint64_t>(k) : 0;
-                at[128 + r] = seen ? reinterpret_cast<uint64_t>(v) : 0;
-                const uint32_t word = __ballot_sync(0xffffffffu, seen);
-                if (lane == 0) vw[(j % C::WORDS) * 4 + (r >> 5)] = word;
+            for (int i = 0; i < RP; ++i) {
+                const int r = (lt >> 1) + i * (kLoaders / 2), key = (j0 + j) * kTile + r;
+                entry[i] = r < kTile && key < longest ? rows_entry<PAGED>(p, sq, s, key) : 0;
             }
         };
-        // body(j, the tile's row addresses): both copies of a tile, the next tile's addresses under way
         bool ok = true;
-        auto tiles_of = [&](auto&& body) {
-            if (n > 0) addresses(0);
-            for (int j = 0; j < n; ++j) {
-                if (!(ok = loaders_sync(ok))) break;
-                if (j + 1 < n) addresses(j + 1);
-                body(j, ptrs + (j & 1) * 256);
-            }
-        };
-        constexpr int CH = D / 8, PASSES = (kTile * CH + kLoaders - 1) / kLoaders;  // chunks of 8 elements
-        tiles_of([&](int j, const uint64_t* at) {
+        if (n > 0) look_up(0);
+        for (int j = 0; j < n && ok; ++j) {
             const int st = j % ST;
+            const T *k[RP], *v[RP];
+            // (visible keys of a tile: kept until its weights are formed, at least one tile after V of this slot)
+#pragma unroll
+            for (int i = 0; i < RP; ++i) {
+                const int r = (lt >> 1) + i * (kLoaders / 2), key = (j0 + j) * kTile + r;
+                const bool seen =
+                    r < kTile && key < longest && rows_at<T, PAGED>(p, sq, g, key, entry[i], k[i], v[i]);
+                if (!seen) k[i] = v[i] = nullptr;
+                uint32_t w = __ballot_sync(0xffffffffu, seen) & 0x55555555u;  // a bit for two lanes
+                w = (w | w >> 1) & 0x33333333u;
+                w = (w | w >> 2) & 0x0f0f0f0fu;
+                w = (w | w >> 4) & 0x00ff00ffu;
+                w = (w | w >> 8) & 0x0000ffffu;
+                if (lane == 0 && r < kTile) seen16[(j % C::WORDS) * 8 + (r >> 4)] = (uint16_t)w;
+            }
+            if (j + 1 < n) look_up(j + 1);
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
                 uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
                 const uint32_t dst = (kv ? C::SV : C::SK) + st * C::OPER;
                 if constexpr (!C::F32) {
-                    if (j >= ST) ok = ok && wait(empty, ((j / ST) - 1) & 1);
-                    if (!ok) continue;  // to the next barrier, which all then leave together
+                    if (j >= ST && !(ok = wait(empty, ((j / ST) - 1) & 1))) break;
 #pragma unroll
-                    for (int i = 0; i < PASSES; ++i) {
-                        const int x = lt + i * kLoaders, r = x / CH, c = x % CH;
-                        if (x >= kTile * CH) break;
-                        const T* src = reinterpret_cast<const T*>(at[kv * 128 + r]);
-                        cp_async16(base + dst + chunk_off(r, c), src ? src + c * 8 : static_cast<const T*>(p.q),
-                                   src != nullptr);
+                    for (int i = 0; i < RP; ++i) {
+                        const int r = (lt >> 1) + i * (kLoaders / 2);
+                        const T* src = kv ? v[i] : k[i];
+                        const uint32_t to = base + dst + r * 128;
+                        if (r < kTile) {
+#pragma unroll
+                            for (int c = 0; c < CH; c += 2)
+                                cp_async16(to + (c >> 3) * kBlock + ((((c & 7) + odd) ^ (r & 7)) << 4),
+                                           src ? src + (c + odd) * 8 : static_cast<const T*>(p.q), src != nullptr);
+                        }
                     }
                     cp_arrive(full);
                 } else {
-                    // fp32: 32 bytes of a row per thread become a chunk of each part
-                    constexpr int BATCH = 11;
 #pragma unroll
-                    for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
-                        float4 a[BATCH], b[BATCH];
+                    for (int i = 0; i < RP; ++i) {
+                        const int r = (lt >> 1) + i * (kLoaders / 2);
+                        const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
 #pragma unroll
-                        for (int i = 0; i < BATCH; ++i) {
-                            const int x = lt + (i0 + i) * kLoaders;
-                            const T* src = x < kTile * CH ? reinterpret_cast<const T*>(at[kv * 128 + x / CH]) : nullptr;
-                            a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (src) {
-                                const float4* f = reinterpret_cast<const float4*>(src) + (x % CH) * 2;
-                                a[i] = __ldg(f), b[i] = __ldg(f + 1);
+                        for (int c0 = 0; c0 < CH; c0 += 8) {
+                            float4 a[4], b[4];
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                a[c] = b[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (src) {
+                                    a[c] = __ldg(src + 2 * (c0 + 2 * c + odd));
+                                    b[c] = __ldg(src + 2 * (c0 + 2 * c + odd) + 1);
+                                }
+                            }
+                            if (i == 0 && c0 == 0 && j >= ST) ok = wait(empty, ((j / ST) - 1) & 1);
+                            if (ok && r < kTile) {
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    split_store<C::PART>(sm + dst + chunk_off(r, c0 + 2 * c + odd), a[c], b[c]);
                             }
                         }
-                        if (i0 == 0 && j >= ST) ok = ok && wait(empty, ((j / ST) - 1) & 1);
-                        if (!ok) break;
-#pragma unroll
-                        for (int i = 0; i < BATCH; ++i) {
-                            const int x = lt + (i0 + i) * kLoaders;
-                            if (x < kTile * CH) split_store<C::PART>(sm + dst + chunk_off(x / CH, x % CH), a[i], b[i]);
-                        }
                     }
-                    if (ok) mbar_arrive(full);
+                    if (!ok) break;
+                    mbar_arrive(full);
                 }
             }
-        });
+        }
         if constexpr (!C::F32) cp_wait_all();
     } else if (lane == 0) {
         // ---- products
@@ -613,8 +651,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             auto next = [&](int t) -> bool {
                 if (j + 1 >= n) return true;
                 if (t == 0 && !wait_one(k_full + nx, ((j + 1) / ST) & 1)) return false;
+                if (t == 0) fence_async_smem();  // what the copies wrote
                 if (C::AHEAD && !wait_one(s_read + t, j & 1)) return false;
-                fence_async_smem();
                 tc_fence_after();
                 scores(t, nx);
                 tc_commit(s_full + t);
@@ -626,9 +664,11 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 if (!ok) break;
             }
             for (int t = 0; t < NQ && ok; ++t) {
-                if (t == 0 && !(ok = wait_one(v_full + st, (j / ST) & 1))) break;
+                if (t == 0) {
+                    if (!(ok = wait_one(v_full + st, (j / ST) & 1))) break;
+                    fence_async_smem();
+                }
                 if (!(ok = wait_one(p_full + t, j & 1))) break;
-                fence_async_smem();
                 tc_fence_after();
                 output(t, st, j > 0);
                 tc_commit(o_full + t);
