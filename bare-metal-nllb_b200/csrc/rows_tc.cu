@@ -124,6 +124,12 @@ __device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, 
         : "memory");
 }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // 16 columns of this thread's lane (warp-wide).
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -210,7 +216,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::SLOT + 4);
     const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::VALID);
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (known to be the same in all lanes)
     const int split = blockIdx.x % n_split, tiles = gridDim.x / n_split;
     // a chunk's last tokens see the most keys: they start first
     const int tile = PAGED ? tiles - 1 - blockIdx.x / n_split : blockIdx.x / n_split;
@@ -602,61 +609,73 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             }
         }
         if constexpr (!C::F32) cp_wait_all();
-    } else if (lane == 0) {
-        // ---- products
+    } else {
+        // ---- products.  The whole warp walks the loop and one lane issues, so that descriptors and addresses are the
+        // same in all lanes to the compiler and stay in uniform registers: issued from a branch of one lane, each
+        // product cost about 100 cycles of moves, and the issuing thread was the kernel's bound.
         constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t id_s = umma_idesc_f16(128, 128) | fmt, id_o = umma_idesc_f16(128, D) | fmt | (1u << 16);
         // V's descriptor: the leading byte offset is the distance between 64-element blocks of a row
         constexpr uint64_t lead = ((uint64_t)(kBlock >> 4) << 16) ^ ((uint64_t)1 << 16);
+        const uint64_t q0 = umma_desc_k_sw128(base + C::SQ), k0 = umma_desc_k_sw128(base + C::SK);
+        const uint64_t v0 = umma_desc_k_sw128(base + C::SV) ^ lead;
+        const bool leader = elect_one();
         auto scores = [&](int t, int st) {
-            const uint32_t q = base + C::SQ + t * C::OPER, k = base + C::SK + st * C::OPER;
+            const uint64_t q = q0 + (uint32_t)t * (C::OPER >> 4), k = k0 + (uint32_t)st * (C::OPER >> 4);
+            if (leader) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                const uint32_t o = (uint32_t)(ks >> 2) * kBlock + (ks & 3) * 32;
-                const uint64_t a = umma_desc_k_sw128(q + o), b = umma_desc_k_sw128(k + o);
-                tc_mma_f16(tmem + t * 128, a, b, id_s, ks > 0);
-                if constexpr (C::F32) {
-                    tc_mma_f16(tmem + t * 128, a, umma_desc_k_sw128(k + C::PART + o), id_s, 1);
-                    tc_mma_f16(tmem + t * 128, umma_desc_k_sw128(q + C::PART + o), b, id_s, 1);
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint32_t o = ((uint32_t)(ks >> 2) * kBlock + (ks & 3) * 32) >> 4;
+                    tc_mma_f16(tmem + t * 128, q + o, k + o, id_s, ks > 0);
+                    if constexpr (C::F32) {
+                        tc_mma_f16(tmem + t * 128, q + o, k + (C::PART >> 4) + o, id_s, 1);
+                        tc_mma_f16(tmem + t * 128, q + (C::PART >> 4) + o, k + o, id_s, 1);
+                    }
                 }
+                tc_commit(s_full + t);
+                if (t == NQ - 1) tc_commit(k_empty + st);
             }
+            __syncwarp();
         };
         auto output = [&](int t, int st, bool accumulate) {
-            const uint32_t v = base + C::SV + st * C::OPER, o = tmem + C::O_COL + t * D;
+            const uint64_t v = v0 + (uint32_t)st * (C::OPER >> 4);
+            const uint32_t o = tmem + C::O_COL + t * D;
+            if (leader) {
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                const uint32_t a = C::AHEAD ? tmem + C::P_COL + t * 64 + ks * 8 : tmem + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8;
-                const uint64_t b = umma_desc_k_sw128(v + ks * 2048) ^ lead;
-                tc_mma_f16_ta(o, a, b, id_o, accumulate || ks > 0);
-                if constexpr (C::F32) {
-                    tc_mma_f16_ta(o, a, umma_desc_k_sw128(v + C::PART + ks * 2048) ^ lead, id_o, 1);
-                    tc_mma_f16_ta(o, a + 16, b, id_o, 1);
+                for (int ks = 0; ks < 8; ++ks) {
+                    const uint32_t a = C::AHEAD ? tmem + C::P_COL + t * 64 + ks * 8
+                                                : tmem + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8;
+                    const uint64_t b = v + ks * (2048 >> 4);
+                    tc_mma_f16_ta(o, a, b, id_o, accumulate || ks > 0);
+                    if constexpr (C::F32) {
+                        tc_mma_f16_ta(o, a, b + (C::PART >> 4), id_o, 1);
+                        tc_mma_f16_ta(o, a + 16, b, id_o, 1);
+                    }
                 }
+                tc_commit(o_full + t);
+                if (t == NQ - 1) tc_commit(v_empty + st);
             }
+            __syncwarp();
         };
         bool ok = true;
-        if (n > 0 && (ok = wait_one(k_full, 0))) {
+        if (n > 0 && (ok = wait(k_full, 0))) {
             for (int t = 0; t < NQ && ok; ++t) {
-                if (!(ok = wait_one(q_full + t, 0))) break;
+                if (!(ok = wait(q_full + t, 0))) break;
                 fence_async_smem();  // what the copies wrote
                 tc_fence_after();
                 scores(t, 0);
-                tc_commit(s_full + t);
             }
-            if (ok) tc_commit(k_empty);
         }
         for (int j = 0; j < n && ok; ++j) {
             const int st = j % ST, nx = (j + 1) % ST;
             // scores of the next key tile: K has come and (AHEAD) the row's last ones are read
             auto next = [&](int t) -> bool {
                 if (j + 1 >= n) return true;
-                if (t == 0 && !wait_one(k_full + nx, ((j + 1) / ST) & 1)) return false;
+                if (t == 0 && !wait(k_full + nx, ((j + 1) / ST) & 1)) return false;
                 if (t == 0) fence_async_smem();  // what the copies wrote
-                if (C::AHEAD && !wait_one(s_read + t, j & 1)) return false;
+                if (C::AHEAD && !wait(s_read + t, j & 1)) return false;
                 tc_fence_after();
                 scores(t, nx);
-                tc_commit(s_full + t);
-                if (t == NQ - 1) tc_commit(k_empty + nx);
                 return true;
             };
             if constexpr (C::AHEAD) {
@@ -665,20 +684,21 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             }
             for (int t = 0; t < NQ && ok; ++t) {
                 if (t == 0) {
-                    if (!(ok = wait_one(v_full + st, (j / ST) & 1))) break;
+                    if (!(ok = wait(v_full + st, (j / ST) & 1))) break;
                     fence_async_smem();
                 }
-                if (!(ok = wait_one(p_full + t, j & 1))) break;
+                if (!(ok = wait(p_full + t, j & 1))) break;
                 tc_fence_after();
                 output(t, st, j > 0);
-                tc_commit(o_full + t);
-                if (t == NQ - 1) tc_commit(v_empty + st);
                 if constexpr (!C::AHEAD) ok = next(t);  // P lies over S
             }
         }
         // whatever was issued is over before tensor memory is given back
-        tc_commit(done);
-        (void)mbar_wait_bounded(done, 0);
+        if (leader) {
+            tc_commit(done);
+            (void)mbar_wait_bounded(done, 0);
+        }
+        __syncwarp();
     }
 
     tc_fence_before();
