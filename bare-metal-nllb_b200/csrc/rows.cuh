@@ -39,6 +39,11 @@ __device__ __forceinline__ int rows_page(const RowsParams& p, int j) {
     return (int)((unsigned long long)(uint32_t)j * p.page_mul >> p.page_shr);
 }
 
+// row / group in the same way (rows stay below 2^27).
+__device__ __forceinline__ int rows_token(const RowsParams& p, int row) {
+    return (int)((unsigned long long)(uint32_t)row * p.group_mul >> p.group_shr);
+}
+
 // What has to be looked up to place key `j` of the sequence (j < kvn): its
 // page number, or its byte of the mask.  Apart from rows_at, so that it can be
 // asked for ahead of its use.

@@ -33,6 +33,8 @@ struct RowsParams {
     int table_ld, n_pages, page;
     uint32_t page_mul;  // j / page = j * page_mul >> page_shr
     int page_shr;
+    uint32_t group_mul;  // row / group = row * group_mul >> group_shr
+    int group_shr;
     float scale_log2;  // scale * log2(e)
     int* err;
 };

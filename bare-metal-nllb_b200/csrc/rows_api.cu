@@ -43,10 +43,20 @@ bool rows_ok(const void* base, int dtype, int64_t a, int64_t b, int64_t c = 0) {
     return aligned16(base) && a >= 0 && b >= 0 && c >= 0 && a % unit == 0 && b % unit == 0 && c % unit == 0;
 }
 
+// Division of a j < 2^30 by d: with 2^(b-1) < d <= 2^b the multiplier ceil(2^(30+b) / d) is too large by less than 1, so
+// the quotient by less than 2^30 / 2^(30+b) <= 1 / d: it stays below the next whole number.
+void set_division(int d, uint32_t* mul, int* shr) {
+    int b = 0;
+    while ((1LL << b) < d) ++b;
+    *shr = 30 + b;
+    *mul = (uint32_t)(((1ULL << *shr) + (uint64_t)d - 1) / (uint64_t)d);
+}
+
 int launch(nllb_attn_ctx* c, RowsParams& p, int dtype, int head_dim, bool paged) {
     if (!c) return bad("ctx is NULL");
     if (p.n_seq == 0) return NLLB_ATTN_OK;  // nothing to do
     p.err = c->err;
+    set_division(p.group, &p.group_mul, &p.group_shr);
     cudaError_t e = cudaSetDevice(c->device);
     if (e == cudaSuccess) e = launch_rows(p, static_cast<RowType>(dtype), head_dim, paged, c->num_sms, c->stream);
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("launch_rows: ") + cudaGetErrorString(e));
@@ -90,12 +100,7 @@ int nllb_attn_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a) {
     p.n_seq = a->n_seq, p.kv_heads = a->n_kv_heads, p.group = a->n_heads / a->n_kv_heads;
     p.q_rows = a->q_rows, p.max_q = a->max_q, p.max_kv = a->max_kv;
     p.table_ld = a->page_table_stride, p.n_pages = a->n_pages, p.page = a->page_size;
-    // With 2^(b-1) < page <= 2^b the multiplier ceil(2^(30+b) / page) is too large by less than 1, so the quotient of a
-    // j < 2^30 by less than 2^30 / 2^(30+b) <= 1 / page: it stays below the next whole number.
-    int b = 0;
-    while ((1LL << b) < a->page_size) ++b;
-    p.page_shr = 30 + b;
-    p.page_mul = (uint32_t)(((1ULL << p.page_shr) + (uint64_t)a->page_size - 1) / (uint64_t)a->page_size);
+    set_division(a->page_size, &p.page_mul, &p.page_shr);
     p.scale_log2 = a->scale * kLog2e;
     return launch(c, p, a->dtype, a->head_dim, true);
 }

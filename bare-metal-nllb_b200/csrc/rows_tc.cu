@@ -30,9 +30,6 @@
 
 #include "rows.cuh"
 
-#ifndef ROWS_EXP
-#define ROWS_EXP 0
-#endif
 #ifndef ROWS_WPT1
 #define ROWS_WPT1 8
 #endif
@@ -150,6 +147,26 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 64 or 128 columns of this thread's lane (warp-wide), under one wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float* v) {
+    uint32_t r[N];
+#pragma unroll
+    for (int k = 0; k < N; k += 32)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+            "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=r"(r[k]), "=r"(r[k + 1]), "=r"(r[k + 2]), "=r"(r[k + 3]), "=r"(r[k + 4]), "=r"(r[k + 5]), "=r"(r[k + 6]), "=r"(r[k + 7]),
+              "=r"(r[k + 8]), "=r"(r[k + 9]), "=r"(r[k + 10]), "=r"(r[k + 11]), "=r"(r[k + 12]), "=r"(r[k + 13]), "=r"(r[k + 14]), "=r"(r[k + 15]),
+              "=r"(r[k + 16]), "=r"(r[k + 17]), "=r"(r[k + 18]), "=r"(r[k + 19]), "=r"(r[k + 20]), "=r"(r[k + 21]), "=r"(r[k + 22]), "=r"(r[k + 23]),
+              "=r"(r[k + 24]), "=r"(r[k + 25]), "=r"(r[k + 26]), "=r"(r[k + 27]), "=r"(r[k + 28]), "=r"(r[k + 29]), "=r"(r[k + 30]), "=r"(r[k + 31])
+            : "r"(taddr + k));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 __device__ __forceinline__ float ex2_approx(float x) {  // 2^x, -inf -> +0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -260,7 +277,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     pdl_launch_dependents();
 
     // keys of this CTA: all that its last row sees, in tiles, shared among the splits
-    const int last_tok = (min(rows, row0 + NQ * kTile) - 1) / p.group;
+    const int last_tok = rows_token(p, min(rows, row0 + NQ * kTile) - 1);
     const int longest = PAGED ? sq.kvn - sq.qn + last_tok + 1 : sq.kvn;
     const int all_tiles = (longest + kTile - 1) / kTile;
     const int per = (all_tiles + n_split - 1) / n_split;
@@ -295,14 +312,14 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         const int t = warp / C::WPT, lq = warp & 3;                     // query tile, TMEM lane quarter
         const int half = C::WPT == 8 ? (warp % C::WPT) >> 2 : 0;        // of the row's scores
         if (PAGED && p.k_new && split == 0) {
-            const int t0 = (row0 + p.group - 1) / p.group;
-            const int t1 = min(sq.qn, (row0 + NQ * kTile + p.group - 1) / p.group);
+            const int t0 = rows_token(p, row0 + p.group - 1);
+            const int t1 = min(sq.qn, rows_token(p, row0 + NQ * kTile + p.group - 1));
             rows_append<T, D>(p, sq, s, g, t0, t1, tid, C::SOFT);
         }
         const int row = row0 + t * kTile + lq * 32 + lane;
         const bool there = row < rows;
         const bool any = row0 + t * kTile + lq * 32 < rows;  // the warp has a row
-        const int tok = row / p.group;
+        const int tok = rows_token(p, row);
         const int lim = there ? (PAGED ? sq.kvn - sq.qn + tok + 1 : sq.kvn) : 0;
         const uint32_t lane_off = (uint32_t)(lq * 32) << 16;
         const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + C::O_COL + (uint32_t)t * D;
@@ -329,7 +346,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 float4 a[C::F32 ? TAKE : 1], b[C::F32 ? TAKE : 1];
 #pragma unroll
                 for (int i = 0; i < TAKE; ++i) {
-                    const int x = lt + (i0 + i) * N, r = row0 + t * kTile + x / CH, tk = r / p.group;
+                    const int x = lt + (i0 + i) * N, r = row0 + t * kTile + x / CH, tk = rows_token(p, r);
                     src[i] = r < rows ? static_cast<const T*>(p.q) + (long long)(sq.q0 + tk) * p.q_row +
                                             (long long)(g * p.group + (r - tk * p.group)) * p.q_head + (x % CH) * 8
                                       : nullptr;
@@ -378,14 +395,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1u ? x[i] : -INFINITY;
                 };
                 float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_ld<C::COLS>(tR, v);
+                if (!whole) {
 #pragma unroll
-                for (int c = 0; c < NC; c += 2) {
-                    float* x = v + 32 * c;
-                    tmem_ld32x2(tR + 32 * c, tR + 32 * c + 32, x, x + 32);
-                    if (!whole) hide(x, bits[c]), hide(x + 32, bits[c + 1]);
-#pragma unroll
-                    for (int i = 0; i < 64; i += 2) y[(i >> 1) & 3] = max_nan(y[(i >> 1) & 3], x[i], x[i + 1]);
+                    for (int c = 0; c < NC; ++c) hide(v + 32 * c, bits[c]);
                 }
+#pragma unroll
+                for (int i = 0; i < C::COLS; i += 2) y[(i >> 1) & 3] = max_nan(y[(i >> 1) & 3], v[i], v[i + 1]);
                 if constexpr (C::AHEAD) {
                     tc_fence_before();
                     warp_arrive(s_read + t);
@@ -423,7 +439,6 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 for (int c = 0; c < NC; ++c) {
                     float* x = v + 32 * c;
                     uint32_t hi[16], lo[C::F32 ? 16 : 1];
-#if ROWS_EXP == 0
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sl, sl), make_float2(-off, -off));
@@ -432,41 +447,6 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         if constexpr (C::F32) split2(e.x, e.y, hi[i], lo[i]);
                         else hi[i] = pack2<T>(e.x, e.y);
                     }
-#elif ROWS_EXP == 1
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], sl, -off);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        sum[i & 1].x += x[2 * i], sum[i & 1].y += x[2 * i + 1];
-                        if constexpr (C::F32) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-                        else hi[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-                    }
-#elif ROWS_EXP == 2
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        x[2 * i] = ex2_approx(fmaf(x[2 * i], sl, -off));
-                        x[2 * i + 1] = ex2_approx(fmaf(x[2 * i + 1], sl, -off));
-                        sum[i & 1].x += x[2 * i], sum[i & 1].y += x[2 * i + 1];
-                        if constexpr (C::F32) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-                        else hi[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-                    }
-#elif ROWS_EXP == 3
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sl, sl), make_float2(-off, -off));
-                        x[2 * i] = y.x, x[2 * i + 1] = y.y;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        sum[i & 1] = add2(sum[i & 1], make_float2(x[2 * i], x[2 * i + 1]));
-                        if constexpr (C::F32) split2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-                        else hi[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-                    }
-#endif
                     tmem_st16(p_at(half * NC + c), hi);
                     if constexpr (C::F32) tmem_st16(p_at(half * NC + c) + 16, lo);
                 }
@@ -492,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             if (ok && any) {
                 const float inv = 1.0f / l;
                 T* dst = static_cast<T*>(p.out) + (long long)(sq.q0 + tok) * p.o_row +
-                         (long long)(g * p.group + row % p.group) * p.o_head;
+                         (long long)(g * p.group + (row - tok * p.group)) * p.o_head;
 #pragma unroll
                 for (int c = d0; c < d1; c += 32) {
                     float o[32];
