@@ -75,7 +75,7 @@ struct Shared {
     u64 chunk[kMaxChunks];     // kept weight of each chunk of the slice
     u64 warp_sum[kWarpsS];
     u64 sum;                   // this CTA's kept weight
-    u64 found_before;
+    u64 found_before, border;
     uint32_t found_cnt;
     int found_bin;
     float best;                // this CTA's largest logit
@@ -141,8 +141,7 @@ __device__ __forceinline__ u64 weight(float l, const Weigher& g) {
     const double x = __hiloint2double(hi + (int)((unsigned)(n >> 5) << 20), lo);
     // w < 2^52: adding 2^52 rounds it to a whole number in the low bits
     const u64 w = (u64)__double_as_longlong(fma(x, p, x) + 4503599627370496.0) & 0xfffffffffffffull;
-    const float d = (g.m - l) * g.to_bin;  // past the last step (NaN for two infinities) nothing is left
-    return l == g.m ? 1ull << kWeightBits : d < (float)kBins ? w : 0;
+    return (g.m - l) * g.to_bin < (float)kBins - 0.5f ? w : 0;  // past the last step nothing is left
 }
 
 template <typename T>
@@ -180,6 +179,45 @@ struct alignas(16) Vec {
     T x[16 / sizeof(T)];
 };
 
+// The largest of this thread's elements, NaN if one is.
+template <typename T>
+__device__ __forceinline__ float row_max(const Vec<T>* data, int n) {
+    if constexpr (sizeof(T) == 4) {
+        float a = -INFINITY, b = -INFINITY;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const Vec<T> v = data[i];
+            asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(a) : "f"(v.x[0]), "f"(v.x[1]));
+            asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(b) : "f"(v.x[2]), "f"(v.x[3]));
+        }
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+        return a;
+    } else {
+        uint32_t m[4];
+        m[0] = m[1] = m[2] = m[3] = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const uint4 v = *reinterpret_cast<const uint4*>(data + i);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m[e]) : "r"(w[e]));
+                else asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m[e]) : "r"(w[e]));
+            }
+        }
+        float a = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            T x;
+            const unsigned short h = (unsigned short)(m[e >> 1] >> (16 * (e & 1)));
+            if constexpr (std::is_same<T, __half>::value) x = __ushort_as_half(h);
+            else x = __ushort_as_bfloat16(h);
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(as_float(x)));
+        }
+        return a;
+    }
+}
+
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -216,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     const T* src = static_cast<const T*>(a.logits) + (long long)row * a.ld + first;
 
     // ---- the slice into shared memory, NaN as -inf, and its largest logit
-    float best = -INFINITY;
+    float best;
     const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
     const int n_vec = vec ? n / VEC : 0;  // whole vectors come by one bulk copy
     if (n_vec > 0 && tid == 0) {
@@ -237,20 +275,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         (void)mbar_wait_bounded(&sh.loaded, 0);  // the copy may still be on its way
     }
     __syncthreads();
-#pragma unroll 4
-    for (int i = tid; i < n_chunks * 32; i += kThreads) {
-        Vec<T> v = data[i];
-        bool nan = false;
+    best = row_max<T>(data, n_chunks * 32);
+    if (best != best) {  // a NaN is among them
+        best = -INFINITY;
+        for (int i = tid; i < n_chunks * 32; i += kThreads) {
+            Vec<T> v = data[i];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float l = as_float(v.x[e]);
-            nan |= l != l;
-            best = fmaxf(best, l);  // (fmaxf passes over NaN)
-        }
-        if (nan) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
+            for (int e = 0; e < VEC; ++e) {
                 if (as_float(v.x[e]) != as_float(v.x[e])) v.x[e] = minus_inf<T>();
+                best = fmaxf(best, as_float(v.x[e]));
+            }
             data[i] = v;
         }
     }
@@ -288,6 +322,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         return;
     }
 
+    if (m == INFINITY) {  // the infinite ones share all the weight: as 0 among -inf
+        for (int i = tid; i < n_chunks * 32; i += kThreads) {
+            Vec<T> v = data[i];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v.x[e] = as_float(v.x[e]) == INFINITY ? T(0.0f) : minus_inf<T>();
+            data[i] = v;
+        }
+        m = 0.0f;
+        __syncthreads();
+    }
+
     // f(l, local index) for every element of the slice, a warp's lanes together
     auto each = [&](auto&& f) {
         for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
@@ -319,11 +364,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     const float to_bin = (float)kBins / (kSpan * temp);
     // Place of a logit on the scale of the first histogram, in steps.  Places
     // rise as logits fall, in fp32 as well as in exact arithmetic, since every
-    // operation rounds monotonically; so do the finer places below.
-    auto place = [&](float l) -> float { return l == m ? 0.0f : (m - l) * to_bin; };
+    // operation rounds monotonically; so do the steps (the nearest one, by an
+    // addition: the conversion instruction is four times slower) and the finer
+    // places below.
+    auto place = [&](float l) -> float { return (m - l) * to_bin; };
     auto step_of = [&](float l) -> int {
         const float d = place(l);
-        return d < (float)kBins ? (int)d : kBins;
+        return d < (float)kBins - 0.5f ? (__float_as_int(d + 8388608.0f) & (2 * kBins - 1)) : kBins;
     };
     Weigher weigher;
     weigher.m = m, weigher.to_bin = to_bin;
@@ -472,8 +519,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const float x = (float)(tid * PER + i), w = kSpan / (float)kBins;
-            lo[i] = (double)c[i] * (double)expf(-(x + 1.01f) * w);
-            hi[i] = (double)c[i] * (double)expf(-fmaxf(x - 0.01f, 0.0f) * w);
+            lo[i] = (double)c[i] * (double)expf(-(x + 0.51f) * w);
+            hi[i] = (double)c[i] * (double)expf(-fmaxf(x - 0.51f, 0.0f) * w);
             lo_mine += lo[i], hi_mine += hi[i];
         }
         if (tid == 0) sh.win_lo = sh.win_hi = kBins - 1;
@@ -489,12 +536,91 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         __syncthreads();
     };
 
+    const bool cut_k = k > 0 && k < a.vocab, cut_p = top_p < 1.0f;
+    u64 limit = ~0ull;  // the composite of the last element kept; its logit and its index in this slice
+    float last_l = -INFINITY;
+    int last_i = INT_MAX;
+    auto set_limit = [&](u64 to) {
+        limit = to;
+        last_l = key_logit((uint32_t)(limit >> kIndexBits));
+        last_i = (int)(limit & ((1ull << kIndexBits) - 1ull)) - first;
+    };
+    auto within = [&](float l, int i) { return l > last_l || (l == last_l && i <= last_i); };
+
+    // ---- lists in rank 0's shared memory, in the place of the masses
+    auto gather = [&](auto&& in) {  // the composites of the elements that in(l, i) picks, in any order
+        for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
+            const Vec<T> v = data[ch * 32 + lane];
+            int mine = 0;
+            bool is[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                is[e] = in(as_float(v.x[e]), (ch * 32 + lane) * VEC + e);
+                mine += is[e];
+            }
+            if (__any_sync(0xffffffffu, mine > 0) && mine > 0) {
+                uint32_t at = add_cluster_u32(map_rank(&sh.listed, 0), (uint32_t)mine);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (is[e]) {
+                        if (at < kList)
+                            st_cluster_u64(map_rank(&sh.mass[at], 0),
+                                           composite(as_float(v.x[e]), (ch * 32 + lane) * VEC + e));
+                        ++at;
+                    }
+            }
+        }
+    };
+    auto sort = [&](int n) -> int {  // sh.mass[0 .. n) rising, padded to a power of two, which it returns
+        int n2 = 64;
+        while (n2 < n) n2 *= 2;
+        for (int i = n + tid; i < n2; i += kThreads) sh.mass[i] = ~0ull;
+        for (int size = 2; size <= n2; size *= 2)
+            for (int stride = size / 2; stride > 0; stride /= 2) {
+                __syncthreads();
+                for (int t = tid; t < n2 / 2; t += kThreads) {
+                    const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+                    const u64 x = sh.mass[i], y = sh.mass[j];
+                    if ((x > y) == ((i & size) == 0)) sh.mass[i] = y, sh.mass[j] = x;
+                }
+            }
+        __syncthreads();
+        return n2;
+    };
+
     // The composite of the element at which the sum reaches `want`, among the
     // elements (of composite <= limit) that in(l) picks, `base` before them.
-    auto refine = [&](auto&& in, bool by_mass, bool one, u64 base, u64 want, u64 limit) -> u64 {
+    auto refine = [&](auto&& in, bool by_mass, uint32_t n_in, u64 base, u64 want) -> u64 {
+        if (n_in <= kList) {  // rank 0 sorts them
+            gather([&](float l, int i) { return in(l) && within(l, i); });
+            cluster_sync_all();
+            if (rank == 0) {
+                const int n = (int)n_in, n2 = sort((int)n_in);
+                (void)n2;
+                constexpr int EACH = kList / kThreads;
+                u64 w[EACH], mine = 0, all;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    const int i = tid * EACH + e;
+                    const u64 weighs = by_mass ? wt(key_logit((uint32_t)(sh.mass[i] >> kIndexBits))) : 1;
+                    w[e] = i < n ? weighs : 0;
+                    mine += w[e];
+                }
+                u64 before = base + block_scan(mine, all);
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    if (before < want && want <= before + w[e]) sh.border = sh.mass[tid * EACH + e];
+                    before += w[e];
+                }
+                if (tid == 0) sh.listed = 0;
+            }
+            cluster_sync_all();
+            return ld_cluster_u64(map_rank(&sh.border, 0));
+        }
+        bool one = false;
         uint32_t lo = 0xffffffffu, hi = 0;
         each([&](float l, int i) {
-            if (in(l) && composite(l, i) <= limit) {
+            if (in(l) && within(l, i)) {
                 lo = min(lo, order_key(l));
                 hi = max(hi, order_key(l));
             }
@@ -541,14 +667,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         return min(to, limit);
     };
 
-    const bool cut_k = k > 0 && k < a.vocab, cut_p = top_p < 1.0f;
-    u64 limit = ~0ull;  // the composite of the last element kept
     if (cut_k || cut_p) {
         auto count = [&] {
             clear(false);
             each([&](float l, int i) {
                 const int b = step_of(l);
-                if (b < kBins && composite(l, i) <= limit) atomicAdd(&sh.cnt[b], 1u);
+                if (b < kBins && within(l, i)) atomicAdd(&sh.cnt[b], 1u);
             });
         };
         u64 v[PER];
@@ -583,35 +707,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
                 each([&](float l, int) { z += wt(l); });
                 cluster_sums(z, 0, whole, unused);
             }
-            each([&](float l, int i) {
-                const bool in = step_of(l) <= last;
-                const unsigned who = __ballot_sync(0xffffffffu, in);
-                if (who) {
-                    uint32_t at = 0;
-                    if (lane == 0) at = add_cluster_u32(map_rank(&sh.listed, 0), __popc(who));
-                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-                    if (in && at < kList) st_cluster_u64(map_rank(&sh.mass[at], 0), composite(l, i));
-                }
-            });
+            gather([&](float l, int) { return step_of(l) <= last; });
             cluster_sync_all();
             if (rank != 0) return;  // (nobody reads this CTA's shared memory any more)
             const int n = (int)n_list;
-            int n2 = 64;
-            while (n2 < n) n2 *= 2;
-            auto sort = [&] {  // sh.mass[0 .. n2) rising
-                for (int size = 2; size <= n2; size *= 2)
-                    for (int stride = size / 2; stride > 0; stride /= 2) {
-                        __syncthreads();
-                        for (int t = tid; t < n2 / 2; t += kThreads) {
-                            const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-                            const u64 x = sh.mass[i], y = sh.mass[j];
-                            if ((x > y) == ((i & size) == 0)) sh.mass[i] = y, sh.mass[j] = x;
-                        }
-                    }
-                __syncthreads();
-            };
-            for (int i = n + tid; i < n2; i += kThreads) sh.mass[i] = ~0ull;
-            sort();
+            const int n2 = sort(n);
             // weights in the order, the cuts, then the kept ones in the order of their indices
             constexpr int EACH = kList / kThreads;
             u64 w[EACH], x[EACH], mine = 0, all;
@@ -641,7 +741,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
                 }
             }
             (void)block_scan(mine, all);
-            sort();
+            (void)sort(n2);
             mine = 0;
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
@@ -662,8 +762,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             return;
         }
         if (by_k)
-            limit = refine([&](float l) { return step_of(l) == last; }, false, sh.found_cnt == 1, sh.found_before,
-                           (u64)k, limit);
+            set_limit(refine([&](float l) { return step_of(l) == last; }, false, sh.found_cnt, sh.found_before, (u64)k));
         if (cut_p) {
             if (by_k) {
                 __syncthreads();
@@ -674,13 +773,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             // exact weights: of everything, of what lies above the window, and in 2048 steps within it
             const int lo = sh.win_lo, hi = sh.win_hi;
             const float finer = (float)kBins / (float)(hi - lo + 1);
-            auto fine = [&](float l) { return min(max((int)((place(l) - (float)lo) * finer), 0), kBins - 1); };
+            auto fine = [&](float l) { return min(max((int)((place(l) - ((float)lo - 0.5f)) * finer), 0), kBins - 1); };
             clear(true);
             u64 z = 0, above = 0;
             each([&](float l, int i) {
                 const int b = step_of(l);
                 const u64 w = wt(l);
-                if (b < kBins && composite(l, i) <= limit) {
+                if (b < kBins && within(l, i)) {
                     z += w;
                     if (b < lo) above += w;
                     else if (b <= hi) {
@@ -696,25 +795,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             const u64 want = share_of(all_z);
             find(v, all_above, want);
             const int f = sh.found_bin;
-            limit = refine(
+            set_limit(refine(
                 [&](float l) {
                     const int b = step_of(l);
                     return b >= lo && b <= hi && fine(l) == f;
                 },
-                true, sh.found_cnt == 1, sh.found_before, want, limit);
+                true, sh.found_cnt, sh.found_before, want));
         }
     }
     // ---- the kept weight of each chunk, of this CTA, of the row
-    const bool whole_row = limit == ~0ull;
-    const float last_l = key_logit((uint32_t)(limit >> kIndexBits));
-    const int last_i = (int)(limit & ((1ull << kIndexBits) - 1ull)) - first;
     // the weights of vector `at` of the slice that are kept, and their sum
     auto kept = [&](int at, const Vec<T>& v, u64 (&w)[VEC]) -> u64 {
         bool in[VEC], any = false;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const float l = as_float(v.x[e]);
-            in[e] = whole_row || l > last_l || (l == last_l && at * VEC + e <= last_i);
+            in[e] = within(l, at * VEC + e);
             any |= in[e];
             w[e] = 0;
         }
