@@ -6,13 +6,24 @@
 //   least weight; the token is found by inverting the running sum of the kept
 //   weights in index order.
 //
-// The bytes of the logits bound it, so a row is read once: the CTAs of a
-// cluster hold its slices in shared memory and every later pass reads those.
-// Nothing is sorted.  The border of the kept set is found by counting: a
-// histogram over 2048 equal steps of (m - l) / T, its totals summed over the
-// cluster through distributed shared memory, names the step the border lies
-// in; the elements of that step are then told apart by their composite (order
-// of the logit, index), 11 bits of what is left at a time, until one is left.
+// The bytes of the logits are its floor.  A row is shared by the CTAs of a
+// cluster, which read it once and keep their slices in shared memory for the
+// later passes -- or, for many long rows, read it again in each pass, which
+// leaves room for more rows at a time (launch() has both sides' times).
+// Nothing is sorted but short lists.  The border of the kept set is found by
+// counting steps of (m - l) / T, the counts summed over the cluster through
+// distributed shared memory: top-k by 64 coarse bins whose counters never
+// collide, top-p by 2048 steps, from whose counts the weights follow closely
+// enough to name the few steps the border can lie in.  Where everything kept
+// lies in few elements, one CTA gathers, sorts and finishes them alone (16 us
+// for one row of 256206 by top-k 50 and top-p 0.95).  Otherwise the exact
+// weights above those steps are summed, the elements at the border gathered
+// and sorted, or told apart 11 bits of their composite (order of the logit,
+// index) at a time where thousands are equal; then one more pass sums the kept
+// weights chunk by chunk and the token's chunk is searched.  Bound now by the
+// passes' instructions and, for few rows, by the cluster's barriers: 512 rows
+// of mixed settings 575 us, 0.9 TB/s of logits; 64 rows in bf16 by top-p 0.9
+// 144 us.
 //
 // Weights are integer multiples of 2^-44 of the largest, so their sums are
 // exact and the order of the atomics changes no result.  44 bits because 2^19
@@ -26,12 +37,6 @@
 #include "device_common.cuh"
 #include "nllb_translate.h"
 
-#ifndef SAMPLE_B
-#define SAMPLE_B 131072
-#endif
-#ifndef SAMPLE_T
-#define SAMPLE_T 512
-#endif
 namespace nllb {
 int set_error(int status, const std::string& msg);  // nllb_attn.cu
 
@@ -39,19 +44,21 @@ namespace {
 
 using u64 = unsigned long long;
 
-constexpr int kThreads = SAMPLE_T, kWarpsS = kThreads / 32;
+constexpr int kThreads = 512, kWarpsS = kThreads / 32;
 constexpr int kBins = 2048, kBinBits = 11;
 constexpr int kWeightBits = 44;
 constexpr int kIndexBits = 19;
 static_assert(NLLB_SAMPLE_MAX_VOCAB == 1 << kIndexBits, "an index fits the composite");
 // the first histogram covers (m - l) / T up to 33: exp(-33) < 2^-45 weighs 0
 constexpr float kSpan = 33.0f;
+constexpr int kCoarse = kBins / 64;   // steps of a coarse bin
 
 constexpr int kList = kBins / 2;  // candidates that rank 0 finishes alone, in the place of the masses
 
 constexpr int kMaxCluster = 16;
-constexpr int kSliceBytes = SAMPLE_B;           // of a row that one CTA holds at most
-constexpr int kMaxChunks = kSliceBytes / 512;  // a chunk is a 16-byte vector per lane
+constexpr int kSliceBytes = 1 << 17;           // of a row that one CTA holds at most
+constexpr int kMaxChunks = kSliceBytes / 512;  // records: of a chunk of 512 bytes, or of 16 of a whole row
+static_assert(NLLB_SAMPLE_MAX_VOCAB * 4 / 512 / 16 <= kMaxChunks, "records of a whole row");
 static_assert(NLLB_SAMPLE_MAX_VOCAB / kMaxCluster * 4 <= kSliceBytes, "every row fits a cluster");
 
 struct Args {
@@ -81,8 +88,10 @@ struct Shared {
     float best;                // this CTA's largest logit
     uint32_t key_lo, key_hi;   // this CTA's range of keys in the border step
     float red[kWarpsS];
-    u64 z, above;              // this CTA's weight, in all and above the window
+    u64 z[2];                  // this CTA's weight, in all and above the window
     int win_lo, win_hi;        // steps the border by weight lies between
+    uint32_t coarse[64];       // this CTA's counts of the first look
+    uint32_t coarse_of[kThreads / 64][64];
     uint32_t listed;           // (rank 0) candidates gathered
     uint64_t loaded;           // barrier of the copy of the slice
     int failed;
@@ -107,26 +116,25 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 }
 
 // exp((l - m) / T) in units of 2^-kWeightBits, by a whole warp.  y = 32 log2
-// of it = l scale + shift is split as n + f, n a whole number and |f| <= 1/2;
+// of it = (l - m) scale is split as n + f, n a whole number and |f| <= 1/2;
 // 2^(y/32) = 2^(n >> 5) * 2^((n & 31) / 32) * exp(f ln2 / 32), the middle
 // factor from a table of 32 that the warp's lanes hold (a shuffle reads it;
 // from shared memory the look-ups' bank conflicts cost more than all the rest)
 // and the last by its series to the fourth power (Tang, 1989: the remainder is
 // below 1.3e-12), in fp64: a token's border may lie anywhere between its
 // neighbours', and fp32 sums over 256206 tokens place it too coarsely.  There
-// are ten fp64 operations, which bound the pass over all weights.
+// are eleven fp64 operations, which bound the pass over all weights.
 struct Weigher {
-    float m;
-    double scale, shift;
+    float floor;  // logits below it weigh nothing: it rounds to 0 itself
+    double md, scale;
     double tab;  // 2^(lane/32), with the units' exponent
-    float to_bin;
 };
 __device__ __forceinline__ u64 weight(float l, const Weigher& g) {
     // l as a double by whole-number operations: the conversion instruction runs at a quarter of their rate and bound
-    // this pass (subnormals and infinities, which come out finite, weigh the same or are told below)
-    const uint32_t b = __float_as_uint(l);
+    // this pass (subnormals come out a little off, and weigh the same)
+    const uint32_t b = __float_as_uint(fmaxf(l, g.floor));  // (NaN too)
     const double ld = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
-    const double y = fma(ld, g.scale, g.shift);
+    const double y = (ld - g.md) * g.scale;
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double t = y + magic;
     const int n = __double2loint(t);
@@ -140,8 +148,7 @@ __device__ __forceinline__ u64 weight(float l, const Weigher& g) {
     const int lo = __shfl_sync(0xffffffffu, __double2loint(g.tab), n & 31);
     const double x = __hiloint2double(hi + (int)((unsigned)(n >> 5) << 20), lo);
     // w < 2^52: adding 2^52 rounds it to a whole number in the low bits
-    const u64 w = (u64)__double_as_longlong(fma(x, p, x) + 4503599627370496.0) & 0xfffffffffffffull;
-    return (g.m - l) * g.to_bin < (float)kBins - 0.5f ? w : 0;  // past the last step nothing is left
+    return (u64)__double_as_longlong(fma(x, p, x) + 4503599627370496.0) & 0xfffffffffffffull;
 }
 
 template <typename T>
@@ -172,6 +179,31 @@ __device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t x) {
 }
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 x) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(x) : "memory");
+}
+
+// Sums over the cluster of the variable at p, eight remote reads in flight
+// (one after the other, each would wait for the last).
+__device__ __forceinline__ u64 cluster_sum_u64(const u64* p, uint32_t C) {
+    u64 s = 0;
+    for (uint32_t z = 0; z < C; z += 8) {
+        u64 t[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) t[i] = z + i < C ? ld_cluster_u64(map_rank(p, z + i)) : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += t[i];
+    }
+    return s;
+}
+__device__ __forceinline__ uint32_t cluster_sum_u32(const uint32_t* p, uint32_t C) {
+    uint32_t s = 0;
+    for (uint32_t z = 0; z < C; z += 8) {
+        uint32_t t[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) t[i] = z + i < C ? ld_cluster_u32(map_rank(p, z + i)) : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += t[i];
+    }
+    return s;
 }
 
 template <typename T>
@@ -232,18 +264,21 @@ __device__ __forceinline__ u64 warp_scan_u64(u64 v, int lane) {  // inclusive
     return v;
 }
 
-// One cluster per row.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
+// One cluster per row, its slices in shared memory or (STREAM) read from
+// global memory in every pass.
+template <typename T, bool STREAM>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int VEC = 16 / (int)sizeof(T);
     constexpr int CHUNK = 32 * VEC;  // one vector per lane
     Shared& sh = *reinterpret_cast<Shared*>(smem);
     Vec<T>* data = reinterpret_cast<Vec<T>*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+    // chunks (a vector per lane) whose kept weight is recorded together, and those loaded together
+    constexpr int SUPER = STREAM ? 16 : 1, DEPTH = STREAM ? 4 : 1;
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) sh.z = sh.above = 0, sh.listed = 0, sh.first_best = INT_MAX, sh.failed = 0;
+    if (tid == 0) sh.z[0] = sh.z[1] = 0, sh.listed = 0, sh.first_best = INT_MAX, sh.failed = 0;
     pdl_wait_primary();
 
     const uint32_t C = cluster_size(), rank = cluster_ctarank();
@@ -254,38 +289,84 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     const T* src = static_cast<const T*>(a.logits) + (long long)row * a.ld + first;
 
     // ---- the slice into shared memory, NaN as -inf, and its largest logit
-    float best;
-    const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
-    const int n_vec = vec ? n / VEC : 0;  // whole vectors come by one bulk copy
-    if (n_vec > 0 && tid == 0) {
-        mbar_init(&sh.loaded, 1);
-        fence_barrier_init();
-        mbar_arrive_expect_tx(&sh.loaded, (uint32_t)n_vec * 16u);
-        bulk_g2s(data, src, (uint32_t)n_vec * 16u, &sh.loaded);
-    }
-    for (int i = n_vec + tid; i < n_chunks * 32; i += kThreads) {
+    float best = -INFINITY;
+    bool inf_row = false;  // (STREAM) only the elements equal to top count, as 0
+    float top = INFINITY;
+    // vector i of the row from global memory
+    auto fetch = [&](int i) -> Vec<T> {
         Vec<T> v;
+        if ((i + 1) * VEC <= n) {
+            *reinterpret_cast<uint4*>(&v) = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v.x[e] = i * VEC + e < n ? src[i * VEC + e] : minus_inf<T>();
-        data[i] = v;
-    }
-    __syncthreads();
-    if (n_vec > 0 && !mbar_wait_bounded(&sh.loaded, 0)) {
-        sh.failed = 1;
-        (void)mbar_wait_bounded(&sh.loaded, 0);  // the copy may still be on its way
-    }
-    __syncthreads();
-    best = row_max<T>(data, n_chunks * 32);
-    if (best != best) {  // a NaN is among them
-        best = -INFINITY;
-        for (int i = tid; i < n_chunks * 32; i += kThreads) {
-            Vec<T> v = data[i];
+            for (int e = 0; e < VEC; ++e) v.x[e] = i * VEC + e < n ? src[i * VEC + e] : minus_inf<T>();
+        }
+        if (inf_row) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (as_float(v.x[e]) != as_float(v.x[e])) v.x[e] = minus_inf<T>();
-                best = fmaxf(best, as_float(v.x[e]));
+            for (int e = 0; e < VEC; ++e) v.x[e] = as_float(v.x[e]) == top ? T(0.0f) : minus_inf<T>();
+        }
+        return v;
+    };
+    // f(vector index, vector) for the vectors of a chunk, all chunks of the slice; done(super chunk) after each of its
+    // SUPER.  A NaN passes every test of the passes below as -inf would.
+    const int n_super = (n_chunks + SUPER - 1) / SUPER;
+    auto vectors = [&](auto&& f, auto&& done) {
+        for (int sc = warp; sc < n_super; sc += kWarpsS) {
+#pragma unroll 1
+            for (int k = 0; k < SUPER; k += DEPTH) {
+                Vec<T> v[DEPTH];
+                const int at = (sc * SUPER + k) * 32 + lane;
+#pragma unroll
+                for (int d = 0; d < DEPTH; ++d) {
+                    if constexpr (STREAM) v[d] = fetch(at + 32 * d);
+                    else v[d] = data[at + 32 * d];
+                }
+#pragma unroll
+                for (int d = 0; d < DEPTH; ++d) f(at + 32 * d, v[d]);
             }
+            done(sc);
+        }
+    };
+    if constexpr (STREAM) {
+        vectors(
+            [&](int, const Vec<T>& v) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) best = fmaxf(best, as_float(v.x[e]));  // (passes over NaN)
+            },
+            [](int) {});
+    } else {
+        const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
+        const int n_vec = vec ? n / VEC : 0;  // whole vectors come by one bulk copy
+        if (n_vec > 0 && tid == 0) {
+            mbar_init(&sh.loaded, 1);
+            fence_barrier_init();
+            mbar_arrive_expect_tx(&sh.loaded, (uint32_t)n_vec * 16u);
+            bulk_g2s(data, src, (uint32_t)n_vec * 16u, &sh.loaded);
+        }
+        for (int i = n_vec + tid; i < n_chunks * 32; i += kThreads) {
+            Vec<T> v;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v.x[e] = i * VEC + e < n ? src[i * VEC + e] : minus_inf<T>();
             data[i] = v;
+        }
+        __syncthreads();
+        if (n_vec > 0 && !mbar_wait_bounded(&sh.loaded, 0)) {
+            sh.failed = 1;
+            (void)mbar_wait_bounded(&sh.loaded, 0);  // the copy may still be on its way
+        }
+        __syncthreads();
+        best = row_max<T>(data, n_chunks * 32);
+        if (best != best) {  // a NaN is among them
+            best = -INFINITY;
+            for (int i = tid; i < n_chunks * 32; i += kThreads) {
+                Vec<T> v = data[i];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (as_float(v.x[e]) != as_float(v.x[e])) v.x[e] = minus_inf<T>();
+                    best = fmaxf(best, as_float(v.x[e]));
+                }
+                data[i] = v;
+            }
         }
     }
 #pragma unroll
@@ -299,10 +380,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     cluster_sync_all();
     float m = -INFINITY;
     bool failed = false;
-    for (uint32_t z = 0; z < C; ++z) {
-        const float x = ld_cluster_f32(map_rank(&sh.best, z));
-        failed |= x != x;
-        m = fmaxf(m, x);
+    {
+        const float x = ld_cluster_f32(map_rank(&sh.best, min(lane, (int)C - 1)));  // a rank's in each lane
+        failed = __any_sync(0xffffffffu, x != x);
+        m = x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     }
 
     // ---- the row's settings
@@ -322,11 +405,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         return;
     }
 
-    if (m == INFINITY) {  // the infinite ones share all the weight: as 0 among -inf
-        for (int i = tid; i < n_chunks * 32; i += kThreads) {
+    // The infinite ones share all the weight: as 0 among -inf.  So do those at the lowest end of the type, 2e31 and more
+    // above the next ones.
+    if (m == INFINITY || (m <= -3.0e38f && m > -INFINITY)) {
+        top = m;
+        inf_row = true;
+        for (int i = tid; !STREAM && i < n_chunks * 32; i += kThreads) {
             Vec<T> v = data[i];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v.x[e] = as_float(v.x[e]) == INFINITY ? T(0.0f) : minus_inf<T>();
+            for (int e = 0; e < VEC; ++e) v.x[e] = as_float(v.x[e]) == top ? T(0.0f) : minus_inf<T>();
             data[i] = v;
         }
         m = 0.0f;
@@ -335,11 +422,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
 
     // f(l, local index) for every element of the slice, a warp's lanes together
     auto each = [&](auto&& f) {
-        for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
-            const Vec<T> v = data[ch * 32 + lane];
+        vectors(
+            [&](int at, const Vec<T>& v) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f(as_float(v.x[e]), (ch * 32 + lane) * VEC + e);
-        }
+                for (int e = 0; e < VEC; ++e) f(as_float(v.x[e]), at * VEC + e);
+            },
+            [](int) {});
     };
 
     if (temp == 0.0f) {  // the first of the order
@@ -359,7 +447,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         return;
     }
 
-    temp = fmaxf(temp, 0x1p-100f);  // keeps the factors below finite
+    // Keeps the factors below finite.  Where the next smaller fp32 number is more than 40 temperatures below m, it is
+    // taken as 40: that weighs nothing all the same, and m - 34 temp stays apart from m.
+    temp = fmaxf(fmaxf(temp, 0x1p-100f), (m - nextafterf(m, -INFINITY)) / 40.0f);
     const double md = m;
     const float to_bin = (float)kBins / (kSpan * temp);
     // Place of a logit on the scale of the first histogram, in steps.  Places
@@ -373,9 +463,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         return d < (float)kBins - 0.5f ? (__float_as_int(d + 8388608.0f) & (2 * kBins - 1)) : kBins;
     };
     Weigher weigher;
-    weigher.m = m, weigher.to_bin = to_bin;
+    weigher.floor = m - 34.0f * temp;  // exp(-34) 2^44 < 1/2
     weigher.scale = 32.0 * 1.4426950408889634074 / (double)temp;
-    weigher.shift = -md * weigher.scale;
+    weigher.md = md;
     weigher.tab = exp2((double)lane / 32.0 + (double)kWeightBits);
     auto wt = [&](float l) { return weight(l, weigher); };  // by all lanes of a warp
     auto composite = [&](float l, int i) { return ((u64)order_key(l) << kIndexBits) | (u64)(first + i); };
@@ -437,19 +527,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         }
         return before + inc;
     };
-    // Sum over the cluster of a value each thread has a part of (two at once).
+    // Sums over the cluster of values each thread has a part of (once per row).
     auto cluster_sums = [&](u64 x, u64 y, u64& sx, u64& sy) {
         x = warp_sum_u64(x), y = warp_sum_u64(y);
         if (lane == 0) {
-            atomicAdd(&sh.z, x);
-            atomicAdd(&sh.above, y);
+            atomicAdd(&sh.z[0], x);
+            atomicAdd(&sh.z[1], y);
         }
         cluster_sync_all();
-        sx = sy = 0;
-        for (uint32_t z = 0; z < C; ++z) {
-            sx += ld_cluster_u64(map_rank(&sh.z, z));
-            sy += ld_cluster_u64(map_rank(&sh.above, z));
-        }
+        const uint32_t k = (uint32_t)min(lane, (int)C - 1);  // a rank's in each lane
+        const bool in = lane < (int)C;
+        const u64 a = ld_cluster_u64(map_rank(&sh.z[0], k)), b = ld_cluster_u64(map_rank(&sh.z[1], k));
+        sx = warp_sum_u64(in ? a : 0), sy = warp_sum_u64(in ? b : 0);
     };
 
     // ---- histograms over the cluster
@@ -468,12 +557,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         const int share = kBins / (int)C;
         if (C > 1) {
             for (int b = tid; b < share; b += kThreads) {
-                uint32_t n0 = 0;
-                u64 w = 0;
-                for (uint32_t z = 0; z < C; ++z) {
-                    n0 += ld_cluster_u32(map_rank(&sh.cnt[rank * share + b], z));
-                    if (by_mass) w += ld_cluster_u64(map_rank(&sh.mass[rank * share + b], z));
-                }
+                const uint32_t n0 = cluster_sum_u32(&sh.cnt[rank * share + b], C);
+                const u64 w = by_mass ? cluster_sum_u64(&sh.mass[rank * share + b], C) : 0;
                 sh.tot_cnt[b] = n0;
                 if (by_mass) sh.tot_mass[b] = w;
             }
@@ -511,6 +596,84 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         }
         __syncthreads();
     };
+    const bool cut_k = k > 0 && k < a.vocab, cut_p = top_p < 1.0f;
+    u64 limit = ~0ull;  // the composite of the last element kept; its logit and its index in this slice
+    float last_l = -INFINITY;
+    int last_i = INT_MAX;
+    auto set_limit = [&](u64 to) {
+        limit = to;
+        last_l = key_logit((uint32_t)(limit >> kIndexBits));
+        last_i = (int)(limit & ((1ull << kIndexBits) - 1ull)) - first;
+    };
+    auto within = [&](float l, int i) { return l > last_l || (l == last_l && i <= last_i); };
+    // Where the k-th element lies: 64 bins of kCoarse steps.  Each lane has a
+    // counter of its own per bin, in its own bank of shared memory, so no two
+    // of a warp's additions meet (counters by step took about two additions a
+    // cycle, more than all the rest of the pass).  Every warp ends with the
+    // same answers.
+    struct Coarse {
+        int at;            // the first bin at which the count reaches k, 64 if none does
+        uint64_t before, up_to;  // elements before it, and up to it
+    };
+    auto look = [&]() -> Coarse {
+        clear(false);
+        each([&](float l, int) {
+            const int b = step_of(l);
+            if (b < kBins) atomicAdd(&sh.cnt[b / kCoarse * 32 + lane], 1u);
+        });
+        __syncthreads();
+        {
+            const int b = tid / (kThreads / 64), x = tid % (kThreads / 64);
+            constexpr int N = 32 * 64 / kThreads;
+            uint32_t sum = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += sh.cnt[b * 32 + x * N + e];
+#pragma unroll
+            for (int o = 1; o < kThreads / 64; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (x == 0) sh.coarse[b] = sum;
+        }
+        cluster_sync_all();
+        {  // some ranks' counts of a bin per thread, then all of them
+            uint32_t sum = 0;
+            for (int z = tid / 64; z < (int)C; z += kThreads / 64)
+                sum += ld_cluster_u32(map_rank(&sh.coarse[tid % 64], z));
+            sh.coarse_of[tid / 64][tid % 64] = sum;
+        }
+        __syncthreads();
+        uint32_t v0 = 0, v1 = 0;
+#pragma unroll
+        for (int z = 0; z < kThreads / 64; ++z) {
+            v0 += sh.coarse_of[z][2 * lane];
+            v1 += sh.coarse_of[z][2 * lane + 1];
+        }
+        const u64 inc = warp_scan_u64(v0 + v1, lane), c0 = inc - v1, before = c0 - v0;
+        const unsigned hit = __ballot_sync(0xffffffffu, inc >= (u64)k);
+        Coarse r = {64, 0, 0};
+        if (hit) {
+            const int f = __ffs(hit) - 1;
+            const u64 a = __shfl_sync(0xffffffffu, before, f), b = __shfl_sync(0xffffffffu, c0, f);
+            const u64 c = __shfl_sync(0xffffffffu, inc, f);
+            r.at = 2 * f + (b < (u64)k);
+            r.before = b < (u64)k ? b : a;
+            r.up_to = b < (u64)k ? c : b;
+        }
+        return r;
+    };
+    // Counts in 2048 bins of 1 / fine_by steps from place fine_from on.
+    float fine_from = 0.0f, fine_by = 0.0f;
+    auto fine = [&](float l) -> int {  // -1: before them; kBins: after
+        const float f = (place(l) - fine_from) * fine_by;
+        return f >= 0.0f ? (f < (float)kBins ? (int)f : kBins) : -1;
+    };
+    auto count = [&](u64 (&v)[PER]) {
+        __syncthreads();
+        clear(false);
+        each([&](float l, int i) {
+            const int f = fine(l);
+            if (f >= 0 && f < kBins && within(l, i)) atomicAdd(&sh.cnt[f], 1u);
+        });
+        collect(false, v);
+    };
     // Steps between which the sum of the weights reaches top_p of the whole,
     // from the counts alone: within a step the weights differ by a factor of
     // exp(kSpan / kBins) at most.
@@ -536,40 +699,29 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         __syncthreads();
     };
 
-    const bool cut_k = k > 0 && k < a.vocab, cut_p = top_p < 1.0f;
-    u64 limit = ~0ull;  // the composite of the last element kept; its logit and its index in this slice
-    float last_l = -INFINITY;
-    int last_i = INT_MAX;
-    auto set_limit = [&](u64 to) {
-        limit = to;
-        last_l = key_logit((uint32_t)(limit >> kIndexBits));
-        last_i = (int)(limit & ((1ull << kIndexBits) - 1ull)) - first;
-    };
-    auto within = [&](float l, int i) { return l > last_l || (l == last_l && i <= last_i); };
-
     // ---- lists in rank 0's shared memory, in the place of the masses
     auto gather = [&](auto&& in) {  // the composites of the elements that in(l, i) picks, in any order
-        for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
-            const Vec<T> v = data[ch * 32 + lane];
-            int mine = 0;
-            bool is[VEC];
+        vectors(
+            [&](int at, const Vec<T>& v) {
+                int mine = 0;
+                bool is[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                is[e] = in(as_float(v.x[e]), (ch * 32 + lane) * VEC + e);
-                mine += is[e];
-            }
-            if (__any_sync(0xffffffffu, mine > 0) && mine > 0) {
-                uint32_t at = add_cluster_u32(map_rank(&sh.listed, 0), (uint32_t)mine);
+                for (int e = 0; e < VEC; ++e) {
+                    is[e] = in(as_float(v.x[e]), at * VEC + e);
+                    mine += is[e];
+                }
+                if (mine > 0) {
+                    uint32_t to = add_cluster_u32(map_rank(&sh.listed, 0), (uint32_t)mine);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (is[e]) {
-                        if (at < kList)
-                            st_cluster_u64(map_rank(&sh.mass[at], 0),
-                                           composite(as_float(v.x[e]), (ch * 32 + lane) * VEC + e));
-                        ++at;
-                    }
-            }
-        }
+                    for (int e = 0; e < VEC; ++e)
+                        if (is[e]) {
+                            if (to < kList)
+                                st_cluster_u64(map_rank(&sh.mass[to], 0), composite(as_float(v.x[e]), at * VEC + e));
+                            ++to;
+                        }
+                }
+            },
+            [](int) {});
     };
     auto sort = [&](int n) -> int {  // sh.mass[0 .. n) rising, padded to a power of two, which it returns
         int n2 = 64;
@@ -588,35 +740,35 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         return n2;
     };
 
-    // The composite of the element at which the sum reaches `want`, among the
-    // elements (of composite <= limit) that in(l) picks, `base` before them.
-    auto refine = [&](auto&& in, bool by_mass, uint32_t n_in, u64 base, u64 want) -> u64 {
-        if (n_in <= kList) {  // rank 0 sorts them
-            gather([&](float l, int i) { return in(l) && within(l, i); });
-            cluster_sync_all();
-            if (rank == 0) {
-                const int n = (int)n_in, n2 = sort((int)n_in);
-                (void)n2;
-                constexpr int EACH = kList / kThreads;
-                u64 w[EACH], mine = 0, all;
+    // The composite of the element at which the sum reaches `want`, `base`
+    // before the n gathered ones; ~0 if none does.  Rank 0 sorts them.
+    auto pick = [&](int n, bool by_mass, u64 base, u64 want) -> u64 {
+        if (rank == 0) {
+            (void)sort(n);
+            constexpr int EACH = kList / kThreads;
+            u64 w[EACH], mine = 0, all;
 #pragma unroll
-                for (int e = 0; e < EACH; ++e) {
-                    const int i = tid * EACH + e;
-                    const u64 weighs = by_mass ? wt(key_logit((uint32_t)(sh.mass[i] >> kIndexBits))) : 1;
-                    w[e] = i < n ? weighs : 0;
-                    mine += w[e];
-                }
-                u64 before = base + block_scan(mine, all);
-#pragma unroll
-                for (int e = 0; e < EACH; ++e) {
-                    if (before < want && want <= before + w[e]) sh.border = sh.mass[tid * EACH + e];
-                    before += w[e];
-                }
-                if (tid == 0) sh.listed = 0;
+            for (int e = 0; e < EACH; ++e) {
+                const int i = tid * EACH + e;
+                const u64 weighs = by_mass ? wt(key_logit((uint32_t)(sh.mass[i] >> kIndexBits))) : 1;
+                w[e] = i < n ? weighs : 0;
+                mine += w[e];
             }
-            cluster_sync_all();
-            return ld_cluster_u64(map_rank(&sh.border, 0));
+            u64 before = base + block_scan(mine, all);
+            if (tid == 0 && !(base < want && want <= base + all)) sh.border = ~0ull;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                if (before < want && want <= before + w[e]) sh.border = sh.mass[tid * EACH + e];
+                before += w[e];
+            }
+            if (tid == 0) sh.listed = 0;
         }
+        cluster_sync_all();
+        return ld_cluster_u64(map_rank(&sh.border, 0));
+    };
+    // The same among any number of elements, those that in(l) picks: 11 bits of
+    // their composites at a time.
+    auto radix = [&](auto&& in, bool by_mass, u64 base, u64 want) -> u64 {
         bool one = false;
         uint32_t lo = 0xffffffffu, hi = 0;
         each([&](float l, int i) {
@@ -659,6 +811,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             u64 v[PER];
             collect(by_mass, v);
             find(v, base, want);
+            if (sh.found_bin < 0) break;  // (the sums say otherwise)
             base = sh.found_before;
             from += (u64)sh.found_bin << shift;
             to = from + ((1ull << shift) - 1ull);
@@ -668,36 +821,23 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
     };
 
     if (cut_k || cut_p) {
-        auto count = [&] {
-            clear(false);
-            each([&](float l, int i) {
-                const int b = step_of(l);
-                if (b < kBins && within(l, i)) atomicAdd(&sh.cnt[b], 1u);
-            });
-        };
         u64 v[PER];
-        count();
-        collect(false, v);
-        int last = -1;       // the steps up to it hold everything kept
-        u64 n_list = 0;      // elements in them
-        bool by_k = false;   // ... since top-k ends in it
-        if (cut_k) {
-            find(v, 0, (u64)k);
-            if (sh.found_bin >= 0) {
-                by_k = true;
-                last = sh.found_bin;
-                n_list = sh.found_before + sh.found_cnt;
-            }
-        }
+        Coarse r = {64, 0, 0};
+        if (cut_k) r = look();
+        const bool by_k = r.at < 64;  // (fewer than k weigh anything otherwise)
+        int last = by_k ? r.at * kCoarse + kCoarse - 1 : -1;  // the steps up to it hold everything kept
+        u64 n_list = r.up_to;                                 // elements in them
         if (!by_k && cut_p) {
+            // counts by step, and from them the steps between which the weights reach their share
+            fine_from = -0.5f, fine_by = 1.0f;
+            count(v);
             window();
             last = sh.win_hi;
-            u64 mine = 0, all;
+            u64 mine = 0;
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (tid * PER + i <= last) mine += c[i];
-            (void)block_scan(mine, all);
-            n_list = all;
+            (void)block_scan(mine, n_list);
         }
         if (last >= 0 && n_list <= kList) {
             // ---- few candidates: rank 0 takes them all and finishes alone
@@ -761,32 +901,42 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             }
             return;
         }
-        if (by_k)
-            set_limit(refine([&](float l) { return step_of(l) == last; }, false, sh.found_cnt, sh.found_before, (u64)k));
+        if (by_k) {
+            fine_from = (float)(r.at * kCoarse) - 0.5f, fine_by = (float)kBins / (float)kCoarse;
+            count(v);
+            find(v, r.before, (u64)k);
+            const int f = sh.found_bin;
+            const u64 base = sh.found_before;
+            const uint32_t n = sh.found_cnt;
+            if (n <= kList) {
+                gather([&](float l, int i) { return fine(l) == f; });
+                cluster_sync_all();
+                set_limit(pick((int)n, false, base, (u64)k));
+            } else {
+                set_limit(radix([&](float l) { return fine(l) == f; }, false, base, (u64)k));
+            }
+        }
         if (cut_p) {
             if (by_k) {
-                __syncthreads();
-                count();
-                collect(false, v);
+                fine_from = -0.5f, fine_by = 1.0f;
+                count(v);
                 window();
             }
-            // exact weights: of everything, of what lies above the window, and in 2048 steps within it
+            // exact weights: of everything, of what lies above the window, and in 2048 bins within it
             const int lo = sh.win_lo, hi = sh.win_hi;
-            const float finer = (float)kBins / (float)(hi - lo + 1);
-            auto fine = [&](float l) { return min(max((int)((place(l) - ((float)lo - 0.5f)) * finer), 0), kBins - 1); };
+            const float from = (float)lo - 0.5f, by = (float)kBins / (float)(hi - lo + 1);
             clear(true);
             u64 z = 0, above = 0;
             each([&](float l, int i) {
-                const int b = step_of(l);
                 const u64 w = wt(l);
-                if (b < kBins && within(l, i)) {
-                    z += w;
-                    if (b < lo) above += w;
-                    else if (b <= hi) {
-                        const int f = fine(l);
-                        atomicAdd(&sh.cnt[f], 1u);
-                        atomicAdd(&sh.mass[f], w);
-                    }
+                if (!within(l, i)) return;
+                z += w;
+                const float d = place(l);
+                const float f = (d - from) * by;
+                if (f < 0.0f) above += w;
+                else if (f < (float)kBins) {
+                    atomicAdd(&sh.cnt[(int)f], 1u);
+                    atomicAdd(&sh.mass[(int)f], w);
                 }
             });
             u64 all_z, all_above;
@@ -795,17 +945,28 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
             const u64 want = share_of(all_z);
             find(v, all_above, want);
             const int f = sh.found_bin;
-            set_limit(refine(
-                [&](float l) {
-                    const int b = step_of(l);
-                    return b >= lo && b <= hi && fine(l) == f;
-                },
-                true, sh.found_cnt, sh.found_before, want));
+            const u64 base = sh.found_before;
+            const uint32_t n = sh.found_cnt;
+            fine_from = from, fine_by = by;
+            if (n <= kList) {
+                gather([&](float l, int i) { return fine(l) == f && within(l, i); });
+                cluster_sync_all();
+                set_limit(pick((int)n, true, base, want));
+            } else {  // many ties
+                set_limit(radix([&](float l) { return fine(l) == f; }, true, base, want));
+            }
         }
     }
     // ---- the kept weight of each chunk, of this CTA, of the row
     // the weights of vector `at` of the slice that are kept, and their sum
+    const bool plain = limit == ~0ull && least == 1;  // nothing is cut
     auto kept = [&](int at, const Vec<T>& v, u64 (&w)[VEC]) -> u64 {
+        if (plain) {
+            u64 sum = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += w[e] = wt(as_float(v.x[e]));
+            return sum;
+        }
         bool in[VEC], any = false;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -825,14 +986,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         }
         return sum;
     };
-    u64 mine = 0;
-    for (int ch = warp; ch < n_chunks; ch += kWarpsS) {
-        u64 w[VEC];
-        u64 s = kept(ch * 32 + lane, data[ch * 32 + lane], w);
-        if (__any_sync(0xffffffffu, s != 0)) s = warp_sum_u64(s);
-        if (lane == 0) sh.chunk[ch] = s;
-        mine += s;
-    }
+    u64 mine = 0, part = 0;
+    vectors(
+        [&](int at, const Vec<T>& v) {
+            u64 w[VEC];
+            part += kept(at, v, w);
+        },
+        [&](int sc) {
+            if (__any_sync(0xffffffffu, part != 0)) part = warp_sum_u64(part);
+            if (lane == 0) sh.chunk[sc] = part;
+            mine += part;
+            part = 0;
+        });
     __syncthreads();
     if (lane == 0) sh.warp_sum[warp] = mine;
     __syncthreads();
@@ -842,73 +1007,68 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
         sh.sum = s;
     }
     cluster_sync_all();
-    u64 all = 0, before = 0, own = 0;
-    for (uint32_t z = 0; z < C; ++z) {
-        const u64 s = ld_cluster_u64(map_rank(&sh.sum, z));
-        if (z < rank) before += s;
-        if (z == rank) own = s;
-        all += s;
-    }
+    // (a rank's sum in each lane)
+    const u64 sums = warp_scan_u64(lane < (int)C ? ld_cluster_u64(map_rank(&sh.sum, lane)) : 0, lane);
+    const u64 all = __shfl_sync(0xffffffffu, sums, 31), upto = __shfl_sync(0xffffffffu, sums, (int)rank);
+    const u64 own = sh.sum, before = upto - own;
     const u64 thr = threshold(all);
     if (warp == 0 && before <= thr && thr < before + own) {
-        // the chunk, 32 at a time, then the element within it
+        // the record it lies in, 32 at a time, then the chunk, then the element
         u64 at = before;
-        int ch0 = 0;
-        for (;; ch0 += 32) {
-            const u64 s = ch0 + lane < n_chunks ? sh.chunk[ch0 + lane] : 0;
+        int sc = 0;
+        for (; sc < n_super; sc += 32) {
+            const u64 s = sc + lane < n_super ? sh.chunk[sc + lane] : 0;
             const u64 inc = warp_scan_u64(s, lane);
             const unsigned hit = __ballot_sync(0xffffffffu, at + inc > thr);
             if (hit) {
                 const int f = __ffs(hit) - 1;
                 at += __shfl_sync(0xffffffffu, inc - s, f);
-                ch0 += f;
+                sc += f;
                 break;
             }
             at += __shfl_sync(0xffffffffu, inc, 31);
         }
-        const Vec<T> v = data[ch0 * 32 + lane];
-        u64 w[VEC];
-        const u64 s = kept(ch0 * 32 + lane, v, w);
-        const u64 inc = warp_scan_u64(s, lane);
-        u64 run = at + inc - s;
-        if (run <= thr && thr < run + s) {
-            int found = -1;
-            float l = 0.f;
+        for (int k = 0; k < SUPER && sc < n_super && at <= thr; ++k) {
+            const int i = (sc * SUPER + k) * 32 + lane;
+            Vec<T> v;
+            if constexpr (STREAM) v = fetch(i);
+            else v = data[i];
+            u64 w[VEC];
+            const u64 s = kept(i, v, w);
+            const u64 inc = warp_scan_u64(s, lane);
+            u64 run = at + inc - s;
+            if (run <= thr && thr < run + s) {
+                int found = -1;
+                float l = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                run += w[e];
-                if (found < 0 && run > thr) {
-                    found = e;
-                    l = as_float(v.x[e]);
+                for (int e = 0; e < VEC; ++e) {
+                    run += w[e];
+                    if (found < 0 && run > thr) {
+                        found = e;
+                        l = as_float(v.x[e]);
+                    }
                 }
+                answer(first + i * VEC + found, l, all);
             }
-            answer(first + (ch0 * 32 + lane) * VEC + found, l, all);
+            at += __shfl_sync(0xffffffffu, inc, 31);
         }
     }
     cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-template <typename T>
-cudaError_t launch(Args a, int rows, int num_sms, cudaStream_t st) {
-    constexpr int CHUNK = 32 * 16 / (int)sizeof(T);
-    // The smallest cluster that holds a row; while there are SMs to spare, larger ones down to 4096 entries a CTA.
-    int C = 1;
-    auto slice = [&] { return ((a.vocab + C - 1) / C + CHUNK - 1) / CHUNK * CHUNK; };
-    while (slice() * (int)sizeof(T) > kSliceBytes ||
-           (C < kMaxCluster && (long long)rows * C * 2 <= num_sms && a.vocab > 4096 * C))
-        C *= 2;
-    a.slice = slice();
-    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)a.slice * sizeof(T);
+template <typename T, bool STREAM>
+cudaError_t launch_one(const Args& a, int rows, int C, cudaStream_t st) {
+    constexpr size_t own = (sizeof(Shared) + 15) / 16 * 16;
     // (the largest slice's bytes, whatever this call's: calls of two threads do not undo each other's)
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)((sizeof(Shared) + 15) / 16 * 16 + kSliceBytes));
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, STREAM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(own + kSliceBytes));
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = cudaFuncSetAttribute(sample_kernel<T, STREAM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * (unsigned)C, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = own + (STREAM ? 0 : (size_t)a.slice * sizeof(T));
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -918,7 +1078,30 @@ cudaError_t launch(Args a, int rows, int num_sms, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a);
+    return cudaLaunchKernelEx(&cfg, sample_kernel<T, STREAM>, a);
+}
+
+template <typename T>
+cudaError_t launch(Args a, int rows, int num_sms, cudaStream_t st) {
+    constexpr int CHUNK = 32 * 16 / (int)sizeof(T);
+    int C = 1;
+    auto slice = [&] { return ((a.vocab + C - 1) / C + CHUNK - 1) / CHUNK * CHUNK; };
+    // Long rows, 64 MB of them and more: read from global memory in every pass, by four CTAs a row (512 rows of 256206
+    // in fp32: 575 us with mixed settings, 789 from shared memory; 64 rows by top-k 58 instead of 73, greedy 22 instead
+    // of 34; one CTA a row took 796, eight 669).  Below that the passes from shared memory are the faster (64 rows in
+    // bf16 by top-p: 126 instead of 148; 128 rows: equal).
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.logits) | (uintptr_t)(a.ld * (long long)sizeof(T))) & 15u) == 0;
+    if (aligned && slice() * (int)sizeof(T) > kSliceBytes && (long long)rows * a.vocab * (int)sizeof(T) >= 1LL << 26) {
+        C = 4;
+        a.slice = slice();
+        return launch_one<T, true>(a, rows, C, st);
+    }
+    // The smallest cluster that holds a row; while there are SMs to spare, larger ones down to 4096 entries a CTA.
+    while (slice() * (int)sizeof(T) > kSliceBytes ||
+           (C < kMaxCluster && (long long)rows * C * 2 <= num_sms && a.vocab > 4096 * C))
+        C *= 2;
+    a.slice = slice();
+    return launch_one<T, false>(a, rows, C, st);
 }
 
 int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }

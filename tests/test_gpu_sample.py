@@ -101,6 +101,33 @@ def test_settings_match_64_bits(cuda_device, vocab, dtype):
     check(lg, u, tok, logp, t, k, p, m, f"vocab {vocab}")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [66000, 70003])
+def test_many_rows(cuda_device, vocab, dtype):
+    """More than 64 MB of rows (which are read in every pass), of every setting, some with NaN, infinities and ties."""
+    rows = 30 * len(SETTINGS)
+    assert rows * vocab * dtype.itemsize >= 2 ** 26
+    lg, u = make(rows, vocab, dtype, seed=5, ld=vocab + (8 - vocab) % 8)
+    lg[3, ::5] = float("nan")
+    lg[20] = -float("inf")
+    lg[21, 100], lg[21, 65000] = float("inf"), float("inf")
+    lg[22:40] = lg[22:40].round()  # thousands of equal logits
+    lg[40, 5:] = -float("inf")
+    col = lambda key, d: [s.get(key, d) for s in SETTINGS] * 30  # noqa: E731
+    t, k, p, m = f32(col("t", 1.0)), i32(col("k", 0)), f32(col("p", 1.0)), f32(col("m", 0.0))
+    before = lg.clone()
+    tok, logp = na.sample(lg, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    torch.cuda.synchronize()
+    assert torch.equal(lg.nan_to_num(7.5), before.nan_to_num(7.5))
+    some = list(range(42)) + list(range(42, rows, 5))  # (every setting: 5 and their number have no common factor)
+    check(lg[some], u[some], tok[some], logp[some], t[some], k[some], p[some], m[some], f"vocab {vocab}")
+    again = na.sample(lg, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    few = na.sample(lg[:40], u[:40].contiguous(), temperature=t[:40].contiguous(), top_k=k[:40].contiguous(),
+                    top_p=p[:40].contiguous(), min_p=m[:40].contiguous())
+    assert torch.equal(again[0], tok) and torch.equal(again[1], logp)
+    assert torch.equal(few[0], tok[:40]) and torch.equal(few[1], logp[:40])
+
+
 def test_defaults_and_unaligned_rows(cuda_device):
     for dtype in (torch.float32, torch.bfloat16):
         lg, u = make(5, 20011, dtype, seed=3, ld=20013)  # rows at odd addresses
@@ -154,6 +181,15 @@ def test_infinities_nan_and_unusable_rows(cuda_device):
     tok, logp = na.sample(lg, u, temperature=t, top_p=p)
     torch.cuda.synchronize()
     assert tok[[0, 1, 6, 7, 8]].tolist() == [-1] * 5 and tok[4].item() == 8000
+    # masks of the type's lowest value, and logits so large that their neighbours lie many temperatures away
+    low = torch.full((4, V), torch.finfo(torch.float32).min, device="cuda")
+    low[1, 70:] = -float("inf")
+    low[2, 50], low[2, 60] = 2.0 ** 30, 2.0 ** 30 - 64
+    low[3] = torch.linspace(1e10, 1e10 + 1e6, V)
+    v = f32([0.50123, 0.50123, 0.999, 0.40123])
+    for kw in (dict(), dict(top_p=f32([0.7] * 4)), dict(top_k=i32([30] * 4)), dict(temperature=f32([1, 1, 20, 900]))):
+        check(low, v, *na.sample(low, v, **kw), *[kw.get(n) for n in ("temperature", "top_k", "top_p", "min_p")],
+              what="far apart")
     check(lg, u, tok, logp, t, None, p, None, "odd values")
 
 
