@@ -63,7 +63,9 @@ struct Cfg {
     // P beside S in tensor memory, where there is room: the next scores can then be taken as soon as a row is read
     static constexpr bool AHEAD = NQ == 2 && D == 64;
     static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D;
-    static constexpr int N_BARS = 4 * ST + 9 * NQ + 1;
+    // fp32: the softmax threads also fetch the first key tile, with all of its loads in flight at once
+    static constexpr bool FIRST = F32;  // (one slot: the first tile's phase is simply not counted)
+    static constexpr int N_BARS = 4 * ST + 9 * NQ + 2;
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
     static constexpr int THREADS = SOFT + kLoaders + 32;
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sm + C::BARS);
     uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
     uint64_t *s_full = v_empty + ST, *p_full = s_full + NQ, *o_full = p_full + NQ, *q_full = o_full + NQ;
-    uint64_t *s_read = q_full + NQ, *pair = s_read + NQ, *done = pair + 4 * NQ;
+    uint64_t *s_read = q_full + NQ, *pair = s_read + NQ, *done = pair + 4 * NQ, *v_first = done + 1;
     uint32_t* slot = reinterpret_cast<uint32_t*>(sm + C::SLOT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::SLOT + 4);
     const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::VALID);
@@ -259,12 +261,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             for (int i = 0; i < NQ; ++i) {
                 mbar_init(s_full + i, 1);
                 mbar_init(p_full + i, C::WPT);
-                mbar_init(q_full + i, C::WPT * 32);
+                mbar_init(q_full + i, C::WPT * 32 + (C::FIRST ? kLoaders : 0));
                 mbar_init(s_read + i, C::WPT);
                 for (int k = 0; k < 4; ++k) mbar_init(pair + 4 * i + k, 2);
                 mbar_init(o_full + i, 1);
             }
             mbar_init(done, 1);
+            mbar_init(v_first, C::SOFT);
             fence_barrier_init();
             *abort_flag = 0;
         }
@@ -366,8 +369,38 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     else cp_async16(base + at, src[i] ? src[i] : static_cast<const T*>(p.q), src[i] != nullptr);
                 }
             }
-            if constexpr (C::F32) mbar_arrive(q_full + t);
-            else cp_arrive(q_full + t);
+            if constexpr (C::FIRST) {
+                const T *k[TAKE], *v[TAKE];
+#pragma unroll
+                for (int i0 = 0; i0 < kTile * CH / N; i0 += TAKE) {
+#pragma unroll
+                    for (int i = 0; i < TAKE; ++i) {
+                        const int r = (lt + (i0 + i) * N) / CH, key = j0 * kTile + r;
+                        if (!(key < longest && rows_key<T, PAGED>(p, sq, s, g, key, k[i], v[i]))) k[i] = v[i] = nullptr;
+                    }
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        float4 a[TAKE], b[TAKE];
+#pragma unroll
+                        for (int i = 0; i < TAKE; ++i) {
+                            const int c = (lt + (i0 + i) * N) % CH;
+                            const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
+                            a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (src) a[i] = __ldg(src + 2 * c), b[i] = __ldg(src + 2 * c + 1);
+                        }
+#pragma unroll
+                        for (int i = 0; i < TAKE; ++i) {
+                            const int x = lt + (i0 + i) * N;
+                            split_store<C::PART>(sm + (kv ? C::SV : C::SK) + chunk_off(x / CH, x % CH), a[i], b[i]);
+                        }
+                        if (i0 + TAKE >= kTile * CH / N) mbar_arrive(kv ? v_first : q_full + t);
+                    }
+                }
+            } else if constexpr (C::F32) {
+                mbar_arrive(q_full + t);
+            } else {
+                cp_arrive(q_full + t);
+            }
         }
         float m = -INFINITY, l = 0.f;  // m: the maximum in use, in units of the scaled score
         bool ok = true;
@@ -540,6 +573,10 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 if (lane == 0 && r < kTile) seen16[(j % C::WORDS) * 8 + (r >> 4)] = (uint16_t)w;
             }
             if (j + 1 < n) look_up(j + 1);
+            if (C::FIRST && j == 0) {  // fetched by the softmax threads
+                mbar_arrive(q_full);
+                continue;
+            }
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
                 uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
@@ -638,7 +675,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             __syncwarp();
         };
         bool ok = true;
-        if (n > 0 && (ok = wait(k_full, 0))) {
+        if (n > 0 && (C::FIRST || (ok = wait(k_full, 0)))) {
             for (int t = 0; t < NQ && ok; ++t) {
                 if (!(ok = wait(q_full + t, 0))) break;
                 fence_async_smem();  // what the copies wrote
@@ -651,7 +688,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             // scores of the next key tile: K has come and (AHEAD) the row's last ones are read
             auto next = [&](int t) -> bool {
                 if (j + 1 >= n) return true;
-                if (t == 0 && !wait(k_full + nx, ((j + 1) / ST) & 1)) return false;
+                if (t == 0 && !wait(k_full + nx, ((j + 1) / ST - C::FIRST) & 1)) return false;
                 if (t == 0) fence_async_smem();  // what the copies wrote
                 if (C::AHEAD && !wait(s_read + t, j & 1)) return false;
                 tc_fence_after();
@@ -664,7 +701,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             }
             for (int t = 0; t < NQ && ok; ++t) {
                 if (t == 0) {
-                    if (!(ok = wait(v_full + st, (j / ST) & 1))) break;
+                    // (a slot's k_full and v_full do not count the first tile where the softmax threads fetched it)
+                    if (!(ok = C::FIRST && j == 0 ? wait(v_first, 0) : wait(v_full + st, (j / ST - C::FIRST) & 1))) break;
                     fence_async_smem();
                 }
                 if (!(ok = wait(p_full + t, j & 1))) break;
