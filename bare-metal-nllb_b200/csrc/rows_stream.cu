@@ -22,6 +22,12 @@
 // and, when few CTAs would be at work, across a cluster of CTAs that share the
 // keys of one (sequence, key head) through distributed shared memory: no
 // workspace, and always in the same order.
+//
+// Measured: 64 sequences of one token and four query heads to a key head over
+// 200..8191 keys (bf16, heads of 128) 106 us = 5.4 TB/s; 256 tokens over
+// memories of 18..512 rows (bf16) 56 us = 5.1 TB/s; one fp32 token after 99
+// keys 4.5 us, latency; one token over 99990 keys with two key heads 31 us,
+// bound by the 32 CTAs that two clusters of 16 make.
 #include <algorithm>
 #include <type_traits>
 
@@ -469,8 +475,10 @@ cudaError_t launch_one(const RowsParams& p, int n_split, cudaStream_t st) {
 template <typename T, int D, int R, bool PAGED>
 cudaError_t launch_by_units(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long units = ((long long)p.max_q * p.group + R - 1) / R * p.kv_heads * p.n_seq;
-    // A warp alone per unit where that already fills the SMs and the keys are few; else four warps, and as many
-    // splits as give every SM work, none with less than a block per warp, one cluster at most.
+    // A warp alone per unit where that already fills the SMs and the keys are few (256 sequences of 16 heads over
+    // 18..512 keys: 56 us, with four warps 75); else many warps, and as many splits as give every SM work (four CTAs
+    // per SM instead of two cost 134 us against 113 over 200..8191 keys), none with less than a block per warp, one
+    // cluster at most.
     if (units >= 8LL * num_sms && p.max_kv <= 1024) return launch_one<T, D, R, PAGED, 1>(p, 1, st);
     constexpr int MANY = Cfg<T, D, R, 0>::MANY, step = MANY * Cfg<T, D, R, 0>::BLK;
     int n_split = 1;

@@ -7,35 +7,40 @@
 // row's sums are only rescaled when a maximum has grown by more than 2^8, so
 // the accumulator in tensor memory is rarely touched between products.
 //
-// Roles of a CTA's warps: 4 per query tile for the softmax (a thread owns a
-// row = a TMEM lane), 3 that fetch, 1 that issues the products.  Key rows are
-// fetched row by row (cp.async of 16 bytes, or loads and a split for fp32):
-// each row's address is worked out once by one thread, so pages of any size,
+// Roles of a CTA's warps: 4 or 8 per query tile for the softmax (one thread, or
+// two, to a row = a TMEM lane), 3 that fetch, 1 that issues the products.  Key
+// rows are fetched row by row (cp.async of 16 bytes, or loads and a split for
+// fp32): two lanes keep a row's address in registers, so pages of any size,
 // strides of any order and masks need no copy, and a hidden row becomes zeros
 // without being read.  K lies K-major and V as it comes (an MN-major operand),
-// both in the 128-byte swizzle; P goes back over S in tensor memory, 32 keys
-// in the columns of the same 32 scores, and is the A operand from there.
+// both in the 128-byte swizzle; P goes back to tensor memory and is the A
+// operand from there: over S, or, with two tiles of heads of 64, beside it, so
+// that the next scores can be taken as soon as a row's last ones are read.
 // With two query tiles per CTA the tensor cores work on one while the other's
 // softmax runs, and a key tile is fetched once for 256 rows; with one tile two
-// CTAs share an SM to the same end.
+// CTAs share an SM to the same end.  Few CTAs over many keys share the keys in
+// a cluster and join their states through distributed shared memory.
 //
 // Types: 16-bit inputs are the operands as they come, the weights are rounded
 // to the type (half a step each, unbiased; the sum that divides them stays
 // fp32).  fp32 inputs and weights are split into two fp16 parts, hi + lo, and
-// a product is taken as hi hi' + hi lo' + lo hi' (22 bits).  Weights are held
-// times 2^7, so fp16 keeps them normal down to 2^-21 of the largest while
-// 2^7 * 2^8 stays in its range.
+// a product is taken as hi hi' + hi lo' + lo hi' (22 bits, and an absolute
+// 2^-25 where lo leaves fp16's normal range).  Weights are held times 2^7, so
+// fp16 keeps them normal down to 2^-21 of the largest while 2^7 * 2^8 stays in
+// its range.
+//
+// Measured: documents of 1500..2048 over 3500..4096 rows, heads of 128, bf16,
+// a tenth of the keys hidden 302 us (696 TFLOP/s); chunks of 500..1024 tokens
+// behind up to 7000, heads of 64, 337 us (502 TFLOP/s of visible pairs); 128
+// sentences of fp32 89 us.  Bound by the softmax warps' instructions (without
+// exponentials the chunks take 287 us, without the softmax 216); a share of
+// the exponentials on the fp32 multipliers, or turns between the two tiles'
+// exponentials, made it slower (a quarter of them 366 us, turns 361 us).
 #include <algorithm>
 #include <type_traits>
 
 #include "rows.cuh"
 
-#ifndef ROWS_WPT1
-#define ROWS_WPT1 8
-#endif
-#ifndef ROWS_WPT2
-#define ROWS_WPT2 4
-#endif
 namespace nllb {
 namespace {
 
@@ -54,8 +59,9 @@ struct Cfg {
     static constexpr uint32_t OPER = PART * PARTS;
     // key tiles in flight: what leaves room for two CTAs per SM with one query tile, or fills the SM with two
     static constexpr int ST = F32 ? 1 : (NQ == 2 ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1));
-    // Softmax warps of a query tile; with 8, two threads share a row.
-    static constexpr int WPT = NQ == 2 ? ROWS_WPT2 : ROWS_WPT1, SOFT = NQ * WPT * 32;  // and softmax threads in all
+    // Softmax warps of a query tile; with 8, two threads share a row.  Two tiles: 4 (long chunks 343 us, with 8 355);
+    // one, where the time to the first result counts: 8 (64 prefixes 70 us, with 4 88).
+    static constexpr int WPT = NQ == 2 ? 4 : 8, SOFT = NQ * WPT * 32;  // and softmax threads in all
     static constexpr int COLS = 128 * 4 / WPT;                      // scores of a thread
     static constexpr int WORDS = 2 * ST + 2;  // key tiles whose visible keys are kept
     static constexpr uint32_t SQ = 0, SK = NQ * OPER, SV = SK + ST * OPER, SAUX = SV + ST * OPER;
@@ -794,9 +800,12 @@ cudaError_t launch_by_tiles(const RowsParams& p, int num_sms, cudaStream_t st) {
             return launch_tc<T, D, 2, PAGED>(p, 1, st);
     }
     const long long units = (rows + kTile - 1) / kTile * heads;
-    // splits: until two CTAs per SM are at work, none below two key tiles, one cluster at most
+    // Splits, while they leave two CTAs or fewer per SM: two from 257 keys on (one sequence of 16 heads, 21 fp32 rows
+    // over 500 keys: 12.0 us instead of 17.4), more where each keeps four key tiles (128 rows over 1500 keys: 20 us
+    // with four, 36 with eight), one cluster at most.
     int n_split = 1;
-    while (n_split < 8 && units * n_split * 2 <= 2LL * num_sms && p.max_kv >= 512 * n_split) n_split *= 2;
+    while (n_split < 8 && units * n_split * 2 <= 2LL * num_sms && p.max_kv > (n_split == 1 ? 256 : 512 * n_split))
+        n_split *= 2;
     return launch_tc<T, D, 1, PAGED>(p, n_split, st);
 }
 

@@ -558,8 +558,10 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     rows, vocab = logits.shape
     if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("the rows of logits must be contiguous")
+    import torch
+    if not logits.is_cuda:
+        raise ValueError("logits must be on a GPU")
     if out_tok is None or out_logp is None:
-        import torch
         out_tok = torch.empty(rows, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
         out_logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
     f = "torch.float32"
@@ -568,7 +570,11 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
                    _ints(top_p, "top_p", rows, logits, f), _ints(min_p, "min_p", rows, logits, f),
                    _ints(u, "u", rows, logits, f), _ints(out_tok, "out_tok", rows, logits),
                    _ints(out_logp, "out_logp", rows, logits, f))
-    _check(lib, lib.nllb_sample(ctypes.byref(a), stream), "nllb_sample")
+    if logits.device.index != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            _check(lib, lib.nllb_sample(ctypes.byref(a), stream), "nllb_sample")
+    else:
+        _check(lib, lib.nllb_sample(ctypes.byref(a), stream), "nllb_sample")
     return out_tok, out_logp
 
 

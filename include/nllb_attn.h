@@ -207,7 +207,10 @@ NLLB_ATTN_API int nllb_attn_cross_host(nllb_attn_ctx* ctx, int layer, int n_sent
  * sums and outputs are accumulated in fp32 and an output is rounded once.
  * The weights of 16-bit calls of many rows are rounded to the type before
  * their product with V; fp32 calls of many rows split q, k and v into two
- * fp16 parts, which keeps fp32 accuracy for |q|, |k|, |v| < 65504.
+ * fp16 parts, which keeps fp32 accuracy (22 bits, and an absolute 2^-25 for
+ * small values) for |q|, |k|, |v| < 65504.  At most 8 rows of a key head
+ * (max_q times the query heads that share it; 16-bit types: 16) count as few.
+ * All pointers are of the context's device.
  * n_heads is a multiple of n_kv_heads: query head h reads key head
  * h / (n_heads / n_kv_heads).  head_dim is 64 or 128.
  * Sequence s has q_len[s] query rows from row q_start[s] of q and out
