@@ -68,17 +68,20 @@ struct Cfg {
     static constexpr uint32_t VALID = SAUX, MAXS = VALID + WORDS * 16, BARS = MAXS + (WPT == 8 ? 2 * NQ * 2 * 128 * 4 : 0);
     // P beside S in tensor memory, where there is room: the next scores can then be taken as soon as a row is read
     static constexpr bool AHEAD = NQ == 2 && D == 64;
-    static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D;
+    // fp32: the outputs' sum over the tiles.  The tensor cores cut what they accumulate, so a sum over many tiles would
+    // drift (20000 keys: an error of 1e-5); they sum one tile, the softmax threads add the tiles.
+    static constexpr bool TOTAL = F32;
+    static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D, T_COL = P_COL;
     // fp32: the softmax threads also fetch the first key tile, with all of its loads in flight at once
     static constexpr bool FIRST = F32;  // (one slot: the first tile's phase is simply not counted)
     static constexpr int N_BARS = 4 * ST + 9 * NQ + 2;
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
     static constexpr int THREADS = SOFT + kLoaders + 32;
-    static constexpr uint32_t TMEM = NQ == 2 ? 512 : 256;  // S: 128 columns per tile, O: D per tile
+    static constexpr uint32_t TMEM = NQ == 2 || (F32 && D == 128) ? 512 : 256;  // S: 128 columns per tile, O: D per tile
     static constexpr int CTAS = NQ == 2 || (F32 && D == 128) ? 1 : 2;
     static constexpr int LD = D + 4;  // fp32 row of a split's state: D sums, then m, l
-    static_assert(NQ * 128 + NQ * D + (AHEAD ? NQ * 64 : 0) <= (int)TMEM, "tensor memory");
+    static_assert(NQ * 128 + NQ * D + (AHEAD ? NQ * 64 : 0) + (TOTAL ? D : 0) <= (int)TMEM, "tensor memory");
     static_assert(128 * LD * 4 <= (int)SAUX || NQ == 2, "a split's state fits over the operands");
 };
 
@@ -152,6 +155,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// 8 columns, the load to be waited for.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -332,6 +347,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         const int lim = there ? (PAGED ? sq.kvn - sq.qn + tok + 1 : sq.kvn) : 0;
         const uint32_t lane_off = (uint32_t)(lq * 32) << 16;
         const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + C::O_COL + (uint32_t)t * D;
+        const uint32_t tT = tmem + lane_off + C::T_COL;  // (TOTAL) the tiles before the last
         // the weights of 32 keys: 16 columns (and fp32's low parts in the next 16)
         auto p_at = [&](int c) { return C::AHEAD ? tmem + lane_off + C::P_COL + t * 64 + 16 * c : tS + 32 * c; };
         // x of this thread's row and y of the other thread's, whichever way round: the step'th exchange of the pair
@@ -455,7 +471,28 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 if (C::AHEAD) tc_fence_after();
                 const float mn = mx * sl;
                 const bool grown = !(mn <= m + kGrow);  // a NaN makes the whole row NaN
-                if (__any_sync(0xffffffffu, grown)) {
+                if constexpr (C::TOTAL) {
+                    const float to = grown ? max_nan(m, mn) : m;
+                    const float corr = m == to ? 1.f : m == -INFINITY ? 0.f : ex2_approx(m - to);
+                    m = to;
+                    l *= corr;
+                    if (j > 0) {
+#pragma unroll
+                        for (int c = half * (D / 2); c < (C::WPT == 8 ? (half + 1) * (D / 2) : D); c += 8) {
+                            uint32_t o[8], x[8];
+                            tmem_ld8(tO + c, o);
+                            if (j > 1) tmem_ld8(tT + c, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                float y = __uint_as_float(o[i]);
+                                if (j > 1) y += __uint_as_float(x[i]);
+                                o[i] = __float_as_uint(y * corr);
+                            }
+                            tmem_st8(tT + c, o);
+                        }
+                    }
+                } else if (__any_sync(0xffffffffu, grown)) {
                     // (a row's own affair: what its neighbours hold changes none of its roundings)
                     const float to = grown ? max_nan(m, mn) : m;
                     const float corr = m == to ? 1.f : m == -INFINITY ? 0.f : ex2_approx(m - to);
@@ -506,6 +543,15 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             if (ok && any && n > 0) ok = other(l, n, his);
             l = half ? his + l : l + his;
         }
+        auto last_output = [&](int c, float* o) {
+            tmem_ld32(tO + c, o);
+            if (C::TOTAL && n > 1) {
+                float x[32];
+                tmem_ld32(tT + c, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] += x[i];
+            }
+        };
         const int d0 = half * (D / 2), d1 = C::WPT == 8 ? d0 + D / 2 : D;  // this thread's part of the output
         if (n_split == 1) {
             if (ok && any) {
@@ -515,7 +561,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
 #pragma unroll
                 for (int c = d0; c < d1; c += 32) {
                     float o[32];
-                    if (n > 0) tmem_ld32(tO + c, o);
+                    if (n > 0) last_output(c, o);
                     constexpr int VEC = 16 / (int)sizeof(T);
                     if (there) {
 #pragma unroll
@@ -535,7 +581,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
 #pragma unroll
                 for (int c = d0; c < d1; c += 32) {
                     float o[32];
-                    if (n > 0) tmem_ld32(tO + c, o);
+                    if (n > 0) last_output(c, o);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<float4*>(st + c + i) =
@@ -649,11 +695,17 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     const uint32_t o = ((uint32_t)(ks >> 2) * kBlock + (ks & 3) * 32) >> 4;
-                    tc_mma_f16(tmem + t * 128, q + o, k + o, id_s, ks > 0);
-                    if constexpr (C::F32) {
-                        tc_mma_f16(tmem + t * 128, q + o, k + (C::PART >> 4) + o, id_s, 1);
+                    if constexpr (C::F32) {  // (the small products first, while little is cut off their sum)
+                        tc_mma_f16(tmem + t * 128, q + o, k + (C::PART >> 4) + o, id_s, ks > 0);
                         tc_mma_f16(tmem + t * 128, q + (C::PART >> 4) + o, k + o, id_s, 1);
+                    } else {
+                        tc_mma_f16(tmem + t * 128, q + o, k + o, id_s, ks > 0);
                     }
+                }
+#pragma unroll
+                for (int ks = 0; C::F32 && ks < D / 16; ++ks) {
+                    const uint32_t o = ((uint32_t)(ks >> 2) * kBlock + (ks & 3) * 32) >> 4;
+                    tc_mma_f16(tmem + t * 128, q + o, k + o, id_s, 1);
                 }
                 tc_commit(s_full + t);
                 if (t == NQ - 1) tc_commit(k_empty + st);
@@ -669,12 +721,16 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     const uint32_t a = C::AHEAD ? tmem + C::P_COL + t * 64 + ks * 8
                                                 : tmem + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8;
                     const uint64_t b = v + ks * (2048 >> 4);
-                    tc_mma_f16_ta(o, a, b, id_o, accumulate || ks > 0);
                     if constexpr (C::F32) {
-                        tc_mma_f16_ta(o, a, b + (C::PART >> 4), id_o, 1);
+                        tc_mma_f16_ta(o, a, b + (C::PART >> 4), id_o, ks > 0);
                         tc_mma_f16_ta(o, a + 16, b, id_o, 1);
+                    } else {
+                        tc_mma_f16_ta(o, a, b, id_o, accumulate || ks > 0);
                     }
                 }
+#pragma unroll
+                for (int ks = 0; C::F32 && ks < 8; ++ks)
+                    tc_mma_f16_ta(o, tmem + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8, v + ks * (2048 >> 4), id_o, 1);
                 tc_commit(o_full + t);
                 if (t == NQ - 1) tc_commit(v_empty + st);
             }
