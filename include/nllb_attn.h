@@ -237,7 +237,9 @@ NLLB_ATTN_API int nllb_attn_cross_host(nllb_attn_ctx* ctx, int layer, int n_sent
  * the chunk's keys and values into their slots; without, they are there
  * already.  The slots written belong to one sequence each: a page that two
  * sequences of a call share may only hold keys from before both chunks.
- * Entries of page_table past a sequence's last page are not read. */
+ * Entries of page_table past a sequence's last page are not read.  A value
+ * that is not finite in a chunk's keys or values may also reach the rows of
+ * earlier tokens of the same chunk (a weight of 0 times it is no number). */
 typedef struct {
     const void* q;
     const void* k_new;
