@@ -1096,8 +1096,10 @@ cudaError_t launch(Args a, int rows, int num_sms, cudaStream_t st) {
         a.slice = slice();
         return launch_one<T, true>(a, rows, C, st);
     }
-    // The smallest cluster that holds a row; while there are SMs to spare, larger ones down to 4096 entries a CTA.
-    while (slice() * (int)sizeof(T) > kSliceBytes ||
+    // Up to eight CTAs a row while they hold more than 64 KB each, so that two share an SM (64 rows in bf16 by top-p:
+    // 125 us, with four CTAs of 128 KB 144), more where they could not hold it; while there are SMs to spare, larger
+    // clusters down to 4096 entries a CTA.
+    while (slice() * (int)sizeof(T) > (C < 8 ? kSliceBytes / 2 : kSliceBytes) ||
            (C < kMaxCluster && (long long)rows * C * 2 <= num_sms && a.vocab > 4096 * C))
         C *= 2;
     a.slice = slice();
