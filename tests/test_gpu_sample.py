@@ -128,6 +128,22 @@ def test_many_rows(cuda_device, vocab, dtype):
     assert torch.equal(few[0], tok[:40]) and torch.equal(few[1], logp[:40])
 
 
+@pytest.mark.parametrize("rows,dtype", [(1, torch.float32), (3, torch.bfloat16), (34, torch.float32)],
+                         ids=["one", "few", "many"])
+def test_largest_vocabulary(cuda_device, rows, dtype):
+    V = 524288
+    lg, u = make(rows, V, dtype, seed=rows)
+    k = i32([(0, 50, 3000)[r % 3] for r in range(rows)])
+    p = f32([(0.9, 1.0)[r % 2] for r in range(rows)])
+    tok, logp = na.sample(lg, u, top_k=k, top_p=p)
+    torch.cuda.synchronize()
+    check(lg, u, tok, logp, None, k, p, None, "largest")
+    flat = torch.zeros(rows, V, dtype=dtype, device="cuda")  # the largest sum of weights
+    tok, logp = na.sample(flat, u)
+    assert tok.tolist() == [int(x * V) for x in u.double().tolist()]
+    assert (logp.double() + np.log(V)).abs().max() < 1e-6
+
+
 def test_defaults_and_unaligned_rows(cuda_device):
     for dtype in (torch.float32, torch.bfloat16):
         lg, u = make(5, 20011, dtype, seed=3, ld=20013)  # rows at odd addresses
