@@ -37,6 +37,7 @@ struct RowsParams {
     int group_shr;
     float scale_log2;  // scale * log2(e)
     int* err;
+    bool expire;  // test: a wait of the tensor-core form runs out
 };
 
 enum class RowType { f32 = 0, f16 = 1, bf16 = 2 };

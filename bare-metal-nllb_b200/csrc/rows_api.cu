@@ -58,6 +58,8 @@ int launch(nllb_attn_ctx* c, RowsParams& p, int dtype, int head_dim, bool paged)
     p.err = c->err;
     set_division(p.group, &p.group_mul, &p.group_shr);
     cudaError_t e = cudaSetDevice(c->device);
+    p.expire = c->expire_next_rows;
+    c->expire_next_rows = false;
     if (e == cudaSuccess) e = launch_rows(p, static_cast<RowType>(dtype), head_dim, paged, c->num_sms, c->stream);
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("launch_rows: ") + cudaGetErrorString(e));
     return NLLB_ATTN_OK;
@@ -66,6 +68,12 @@ int launch(nllb_attn_ctx* c, RowsParams& p, int dtype, int head_dim, bool paged)
 }  // namespace
 
 extern "C" {
+
+int nllb_attn_test_expire_next_rows_wait(nllb_attn_ctx* c) {
+    if (!c) return bad("ctx is NULL");
+    c->expire_next_rows = true;
+    return NLLB_ATTN_OK;
+}
 
 int nllb_attn_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a) {
     if (!a) return bad("args is NULL");

@@ -308,12 +308,12 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     const int j0 = split * per, n = max(0, min(all_tiles, j0 + per) - j0);
 
     // Bounded wait; false (and the CTA gives up) once any wait has run out.
-    auto wait_one = [&](uint64_t* bar, uint32_t parity) -> bool {
+    auto wait_one = [&](uint64_t* bar, uint32_t parity, long long budget = kWaitBudgetCycles) -> bool {
         if (mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
         while (!mbar_try_wait(bar, parity)) {
             if (*abort_flag) return false;
-            if (clock64() - t0 > kWaitBudgetCycles) {
+            if (clock64() - t0 > budget) {
                 *abort_flag = 1;
                 atomicOr(p.err, NLLB_DEV_ERR_TIMEOUT);
                 return false;
@@ -737,7 +737,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             __syncwarp();
         };
         bool ok = true;
-        if (n > 0 && (C::FIRST || (ok = wait(k_full, 0)))) {
+        if (p.expire) ok = __all_sync(0xffffffffu, wait_one(done, 0, kTestWaitBudgetCycles));  // nothing arrives there
+        if (ok && n > 0 && (C::FIRST || (ok = wait(k_full, 0)))) {
             for (int t = 0; t < NQ && ok; ++t) {
                 if (!(ok = wait(q_full + t, 0))) break;
                 fence_async_smem();  // what the copies wrote

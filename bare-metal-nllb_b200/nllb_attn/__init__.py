@@ -113,6 +113,7 @@ SIGNATURES = {
     "nllb_attn_cross": (_c_int, [_c_void_p, _c_int, _c_int, _fp, _fp]),
     "nllb_attn_cross_host": (_c_int, [_c_void_p, _c_int, _c_int, _fp, _fp]),
     "nllb_attn_paged": (_c_int, [_c_void_p, ctypes.POINTER(PagedArgs)]),
+    "nllb_attn_test_expire_next_rows_wait": (_c_int, [_c_void_p]),
     "nllb_attn_cross_rows": (_c_int, [_c_void_p, ctypes.POINTER(CrossRowsArgs)]),
     "nllb_attention_head": (None, [_fp, _fp, _fp, _fp, _fp, _fp, _c_int, _c_int]),
     "nllb_attention_head_flash": (None, [_fp, _fp, _fp, _fp, _fp, _c_int, _c_int]),
@@ -399,6 +400,11 @@ class Context:
             q_stride_row=q.stride(0), q_stride_head=q.stride(1), k_stride_row=k.stride(0), k_stride_head=k.stride(1),
             v_stride_row=v.stride(0), v_stride_head=v.stride(1), out_stride_row=out.stride(0),
             out_stride_head=out.stride(1))
+
+    def test_expire_next_rows_wait(self) -> None:
+        """nllb_attn_test_expire_next_rows_wait: a bounded wait of the next
+        call of many rows runs out."""
+        _check(self.lib, self.lib.nllb_attn_test_expire_next_rows_wait(self.handle), "test_expire_next_rows_wait")
 
     def cross_rows(self, args: CrossRowsArgs) -> None:
         """nllb_attn_cross_rows: target rows over encoder states of another length."""

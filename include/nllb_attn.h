@@ -291,6 +291,13 @@ typedef struct {
 
 NLLB_ATTN_API int nllb_attn_cross_rows(nllb_attn_ctx* ctx, const nllb_attn_cross_rows_args* args);
 
+/* Test of the bounded device waits: if the next nllb_attn_paged or
+ * nllb_attn_cross_rows of this context counts as many rows, a wait of its
+ * launch runs out after about 1 ms; it writes no output (paged: the chunk's
+ * keys and values may be written) and the next nllb_attn_sync returns
+ * NLLB_ATTN_ETIMEOUT.  The context stays usable. */
+NLLB_ATTN_API int nllb_attn_test_expire_next_rows_wait(nllb_attn_ctx* ctx);
+
 /* ---- drop-ins for the declared single-head API (pico.h:85-92) -----------
  * Same signatures and meaning as the reference's attention_head
  * (tensor.c:255-282) and attention_head_flash (tensor.c:286-332): host

@@ -453,6 +453,21 @@ def test_cross_rows_padded_batch_and_extreme_scores(ctx):
                 check(out[b * n:(b + 1) * n], ref, tol, f"{dtype} batch {b}")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens,kv_heads", [([(40, 900)], 2), (MANY, 12)], ids=["cluster", "two-tiles"])
+def test_bounded_wait_runs_out_and_context_recovers(ctx, lens, kv_heads, dtype):
+    c = Paged(lens, kv_heads, kv_heads, 64, 16, dtype, seed=3)
+    ctx.test_expire_next_rows_wait()
+    c.run(ctx)
+    with pytest.raises(na.NllbAttnError) as e:
+        ctx.sync()
+    assert e.value.status == na.ETIMEOUT
+    assert (c.out == 7.0).all()
+    c.run(ctx)
+    ctx.sync()
+    c.verify("after the timeout")
+
+
 def test_cross_rows_on_another_stream(ctx):
     c = Cross(CROSS["rows"], 4, 4, 64, torch.float32)
     st = torch.cuda.Stream()
