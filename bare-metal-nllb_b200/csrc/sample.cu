@@ -454,13 +454,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     const float to_bin = (float)kBins / (kSpan * temp);
     // Place of a logit on the scale of the first histogram, in steps.  Places
     // rise as logits fall, in fp32 as well as in exact arithmetic, since every
-    // operation rounds monotonically; so do the steps (the nearest one, by an
-    // addition: the conversion instruction is four times slower) and the finer
-    // places below.
-    auto place = [&](float l) -> float { return (m - l) * to_bin; };
+    // operation rounds monotonically; so does the step (the nearest whole
+    // number, by an addition: the conversion instruction is four times slower).
+    // Every pass asks this one function which step a logit belongs to, and its
+    // operations are spelled out so that no pass's are contracted into others:
+    // what one pass counts in a step is what the next one gathers from it.
+    constexpr float kWhole = 8388608.0f;  // 2^23: adding it rounds to a whole number
+    auto place = [&](float l) -> float { return __fmul_rn(__fsub_rn(m, l), to_bin); };
     auto step_of = [&](float l) -> int {
         const float d = place(l);
-        return d < (float)kBins - 0.5f ? (__float_as_int(d + 8388608.0f) & (2 * kBins - 1)) : kBins;
+        return d < (float)kBins - 0.5f ? (__float_as_int(__fadd_rn(d, kWhole)) & (2 * kBins - 1)) : kBins;
     };
     Weigher weigher;
     weigher.floor = m - 34.0f * temp;  // exp(-34) 2^44 < 1/2
@@ -584,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) mine += v[i];
         u64 before = base + block_scan(mine, all);
-        if (tid == 0 && !(base < want && want <= base + all)) sh.found_bin = -1;
+        if (tid == 0 && !(base < want && want <= base + all)) sh.found_bin = -1, sh.found_cnt = 0, sh.found_before = base;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (before < want && want <= before + v[i]) {
@@ -601,6 +604,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     float last_l = -INFINITY;
     int last_i = INT_MAX;
     auto set_limit = [&](u64 to) {
+        if (to == ~0ull) return;  // nothing is cut
         limit = to;
         last_l = key_logit((uint32_t)(limit >> kIndexBits));
         last_i = (int)(limit & ((1ull << kIndexBits) - 1ull)) - first;
@@ -659,24 +663,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         }
         return r;
     };
-    // Counts in 2048 bins of 1 / fine_by steps from place fine_from on.
-    float fine_from = 0.0f, fine_by = 0.0f;
+    // Steps fine_lo to fine_hi in fine_per bins each, at most 2048 in all: the
+    // step decides, then the place within it, held inside the step.
+    int fine_lo = 0, fine_hi = 0, fine_per = 0;
+    auto set_fine = [&](int lo, int hi) { fine_lo = lo, fine_hi = hi, fine_per = kBins / (hi - lo + 1); };
     auto fine = [&](float l) -> int {  // -1: before them; kBins: after
-        const float f = (place(l) - fine_from) * fine_by;
-        return f >= 0.0f ? (f < (float)kBins ? (int)f : kBins) : -1;
+        const int s = step_of(l);
+        if (s < fine_lo) return -1;
+        if (s > fine_hi) return kBins;
+        const float d = place(l), nearest = __fsub_rn(__fadd_rn(d, kWhole), kWhole);  // s
+        const float within = __fadd_rn(__fsub_rn(d, nearest), 0.5f);                  // 0 to 1
+        const float x = fmaxf(__fsub_rn(__fmul_rn(within, (float)fine_per), 0.5f), 0.0f);
+        return (s - fine_lo) * fine_per + min(__float_as_int(__fadd_rn(x, kWhole)) & (2 * kBins - 1), fine_per - 1);
     };
-    auto count = [&](u64 (&v)[PER]) {
+    auto count = [&](auto&& bin, u64 (&v)[PER]) {  // what `bin` puts into [0, kBins)
         __syncthreads();
         clear(false);
         each([&](float l, int i) {
-            const int f = fine(l);
+            const int f = bin(l);
             if (f >= 0 && f < kBins && within(l, i)) atomicAdd(&sh.cnt[f], 1u);
         });
         collect(false, v);
     };
     // Steps between which the sum of the weights reaches top_p of the whole,
     // from the counts alone: within a step the weights differ by a factor of
-    // exp(kSpan / kBins) at most.
+    // exp(kSpan / kBins) at most.  The exact sums reach it there too: the slack
+    // of 1e-5 is far above what the bounds here and the weights' units round off
+    // (2^19 halves of 2^-44 of the largest weight, fp32's exponentials), and
+    // steps past the last weigh nothing.
     auto window = [&] {
         double lo[PER], hi[PER], lo_mine = 0.0, hi_mine = 0.0, lo_all, hi_all;
 #pragma unroll
@@ -741,9 +755,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     };
 
     // The composite of the element at which the sum reaches `want`, `base`
-    // before the n gathered ones; ~0 if none does.  Rank 0 sorts them.
-    auto pick = [&](int n, bool by_mass, u64 base, u64 want) -> u64 {
+    // before the gathered ones; ~0 if none does.  Rank 0 sorts them.
+    auto pick = [&](bool by_mass, u64 base, u64 want) -> u64 {
         if (rank == 0) {
+            const int n = min((int)sh.listed, kList);
             (void)sort(n);
             constexpr int EACH = kList / kThreads;
             u64 w[EACH], mine = 0, all;
@@ -829,8 +844,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         u64 n_list = r.up_to;                                 // elements in them
         if (!by_k && cut_p) {
             // counts by step, and from them the steps between which the weights reach their share
-            fine_from = -0.5f, fine_by = 1.0f;
-            count(v);
+            count(step_of, v);
             window();
             last = sh.win_hi;
             u64 mine = 0;
@@ -850,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
             gather([&](float l, int) { return step_of(l) <= last; });
             cluster_sync_all();
             if (rank != 0) return;  // (nobody reads this CTA's shared memory any more)
-            const int n = (int)n_list;
+            const int n = min((int)sh.listed, kList);  // (n_list: the same function counted and gathered)
             const int n2 = sort(n);
             // weights in the order, the cuts, then the kept ones in the order of their indices
             constexpr int EACH = kList / kThreads;
@@ -902,8 +916,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
             return;
         }
         if (by_k) {
-            fine_from = (float)(r.at * kCoarse) - 0.5f, fine_by = (float)kBins / (float)kCoarse;
-            count(v);
+            set_fine(r.at * kCoarse, r.at * kCoarse + kCoarse - 1);
+            count(fine, v);
             find(v, r.before, (u64)k);
             const int f = sh.found_bin;
             const u64 base = sh.found_before;
@@ -911,32 +925,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
             if (n <= kList) {
                 gather([&](float l, int i) { return fine(l) == f; });
                 cluster_sync_all();
-                set_limit(pick((int)n, false, base, (u64)k));
+                set_limit(pick(false, base, (u64)k));
             } else {
                 set_limit(radix([&](float l) { return fine(l) == f; }, false, base, (u64)k));
             }
         }
         if (cut_p) {
             if (by_k) {
-                fine_from = -0.5f, fine_by = 1.0f;
-                count(v);
+                count(step_of, v);
                 window();
             }
             // exact weights: of everything, of what lies above the window, and in 2048 bins within it
-            const int lo = sh.win_lo, hi = sh.win_hi;
-            const float from = (float)lo - 0.5f, by = (float)kBins / (float)(hi - lo + 1);
+            set_fine(sh.win_lo, sh.win_hi);
             clear(true);
             u64 z = 0, above = 0;
             each([&](float l, int i) {
                 const u64 w = wt(l);
                 if (!within(l, i)) return;
                 z += w;
-                const float d = place(l);
-                const float f = (d - from) * by;
-                if (f < 0.0f) above += w;
-                else if (f < (float)kBins) {
-                    atomicAdd(&sh.cnt[(int)f], 1u);
-                    atomicAdd(&sh.mass[(int)f], w);
+                const int f = fine(l);
+                if (f < 0) above += w;
+                else if (f < kBins) {
+                    atomicAdd(&sh.cnt[f], 1u);
+                    atomicAdd(&sh.mass[f], w);
                 }
             });
             u64 all_z, all_above;
@@ -947,11 +958,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
             const int f = sh.found_bin;
             const u64 base = sh.found_before;
             const uint32_t n = sh.found_cnt;
-            fine_from = from, fine_by = by;
             if (n <= kList) {
                 gather([&](float l, int i) { return fine(l) == f && within(l, i); });
                 cluster_sync_all();
-                set_limit(pick((int)n, true, base, want));
+                set_limit(pick(true, base, want));
             } else {  // many ties
                 set_limit(radix([&](float l) { return fine(l) == f; }, true, base, want));
             }
