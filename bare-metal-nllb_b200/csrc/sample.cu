@@ -405,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         return;
     }
 
-    // The infinite ones share all the weight: as 0 among -inf.  So do those at the lowest end of the type, 2e31 and more
-    // above the next ones.
+    // The infinite ones share all the weight: as 0 among -inf.  So do those at the lowest end of the type, 2^104 and more
+    // above the next ones, which is more than 34 of the largest temperature.
     if (m == INFINITY || (m <= -3.0e38f && m > -INFINITY)) {
         top = m;
         inf_row = true;
@@ -447,9 +447,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         return;
     }
 
-    // Keeps the factors below finite.  Where the next smaller fp32 number is more than 40 temperatures below m, it is
-    // taken as 40: that weighs nothing all the same, and m - 34 temp stays apart from m.
-    temp = fmaxf(fmaxf(temp, 0x1p-100f), (m - nextafterf(m, -INFINITY)) / 40.0f);
+    // Keeps the factors below finite, and m - 34 temp above fp32's lowest number.  Where the next smaller fp32 number is
+    // more than 40 temperatures below m, it is taken as 40: that weighs nothing all the same.
+    temp = fmaxf(fminf(fmaxf(temp, 0x1p-100f), 0x1p96f), (m - nextafterf(m, -INFINITY)) / 40.0f);
     const double md = m;
     const float to_bin = (float)kBins / (kSpan * temp);
     // Place of a logit on the scale of the first histogram, in steps.  Places
@@ -466,7 +466,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         return d < (float)kBins - 0.5f ? (__float_as_int(__fadd_rn(d, kWhole)) & (2 * kBins - 1)) : kBins;
     };
     Weigher weigher;
-    weigher.floor = m - 34.0f * temp;  // exp(-34) 2^44 < 1/2
+    // exp(-34) 2^44 < 1/2.  Rounded away from m: half of fp32's step at m may be many temperatures.
+    weigher.floor = __fsub_rd(m, 34.0f * temp);
     weigher.scale = 32.0 * 1.4426950408889634074 / (double)temp;
     weigher.md = md;
     weigher.tab = exp2((double)lane / 32.0 + (double)kWeightBits);

@@ -210,7 +210,7 @@ NLLB_ATTN_API int nllb_logsoftmax_topk(const float* logits, long long ld, int vo
  * out_logp (may be NULL): its log-probability among the remaining tokens.
  * temperature, top_k, top_p, min_p: device arrays of one entry per row, or
  * NULL for 1, 0, 1, 0.  T = 0 takes the first token of the order (logp 0),
- * T below 2^-100 counts as 2^-100;
+ * T below 2^-100 counts as 2^-100 and above 2^96 as 2^96;
  * top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 cut nothing, top_p <= 0
  * keeps one token, min_p above 1 counts as 1; NaN in top_p or min_p cuts
  * nothing, u is clamped into [0, 1) and NaN counts as 0.  A NaN logit counts

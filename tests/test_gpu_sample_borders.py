@@ -57,8 +57,10 @@ def run(rows, u, **kw):
     names = dict(t="temperature", k="top_k", p="top_p", m="min_p")
     s = {names[n]: (i32 if n == "k" else f32)(v) for n, v in kw.items()}
     a = na.sample(lg, f32(u), **s)
+    if "t" in kw:
+        s["temperature"] = s["temperature"].clamp(max=2.0 ** 96)  # as the header says
     for _ in range(2):
-        b = na.sample(lg, f32(u), **s)
+        b = na.sample(lg, f32(u), **{**s, **({"temperature": f32(kw["t"])} if "t" in kw else {})})
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     check(lg, f32(u), *a, *[s.get(n) for n in ("temperature", "top_k", "top_p", "min_p")], what="borders")
 
@@ -124,3 +126,53 @@ def test_logits_on_every_edge(cuda_device, t, vocab):
                 cache[key] = share(rows[r], float(np.float32(t)), k[r], p[r])
             p[r] = cache[key]
     run(rows, u, t=[t] * n, k=k, p=p)
+
+
+def extreme_rows(vocab):
+    """(logits, temperature) with masked tokens (-inf, NaN) at the lowest indices, and the weights of the others far
+    above 0 whatever their size."""
+    rng = np.random.default_rng(5)
+    lowest, top = np.finfo(np.float32).min, np.finfo(np.float32).max
+    sets = [
+        (100.0, np.nextafter(np.float32(100), np.float32(0)), 1e-6),
+        (20.0, np.nextafter(np.float32(20), np.float32(0)), 8e-8),
+        (1.0, -4.0, 2e37),
+        (1.0, -4.0, 1e38),
+        (1.0e30, -1.0e30, 1e38),
+        (top, lowest, 3.0e38),
+        (2.0 ** 100, -2.0 ** 98, 9e36),
+        (-2.0 ** 99, -2.0 ** 100, 2.0 ** 96),
+        (-2.9e38, -3.0e38, 1e37),
+        (np.nextafter(lowest, np.float32(0)), lowest, 1e32),
+        (lowest, lowest, 1.0),
+        (lowest, lowest, 1e38),
+    ]
+    rows, t = [], []
+    for hi, lo, temp in sets:
+        row = np.full(vocab, -np.inf, np.float32)
+        row[1:300:3] = np.nan
+        at = rng.permutation(np.arange(301, vocab))[:400]
+        row[300], row[at[:150]], row[at[150:]] = hi, hi, lo
+        rows.append(row)
+        t.append(float(np.float32(temp)))
+    return rows, t
+
+
+@pytest.mark.parametrize("copies,vocab", [(1, 20011), (8, 3001), (16, 90003)], ids=["cluster", "cta", "streamed"])
+def test_masked_tokens_weigh_nothing_at_any_temperature(cuda_device, copies, vocab):
+    base, temps = extreme_rows(vocab)
+    if copies == 1:
+        for i, (row, t) in enumerate(zip(base, temps)):
+            for kw in (dict(), dict(p=[0.77]), dict(k=[170], p=[0.9]), dict(m=[1e-3])):
+                run(row[None], [[0.0, 0.999, 0.4][i % 3]], t=[t], **kw)
+        return
+    rows, t, u, k, p, m = [], [], [], [], [], []
+    for c in range(copies):
+        for row, temp in zip(base, temps):
+            rows.append(row)
+            t.append(temp)
+            u.append([0.0, 0.9999, 0.37, 0.61][c % 4])
+            k.append([0, 0, 170, 0][(c // 4) % 4])
+            p.append([1.0, 0.77, 0.9, 1.0][(c // 4) % 4])
+            m.append([0.0, 0.0, 0.0, 1e-3][(c // 4) % 4])
+    run(np.stack(rows), u, t=t, k=k, p=p, m=m)
