@@ -126,15 +126,18 @@ __device__ __forceinline__ uint32_t order_key(float l) {
 // are eleven fp64 operations, which bound the pass over all weights.
 struct Weigher {
     float floor;  // logits below it weigh nothing: it rounds to 0 itself
-    double md, scale;
+    double md, scale;  // widened(m); 32 log2(e) / T
     double tab;  // 2^(lane/32), with the units' exponent
 };
+// l as a double by whole-number operations: the conversion instruction runs at a quarter of their rate and bound the
+// pass over all weights.  Zeros and subnormals come out up to 2^-126 off; the largest logit is taken the same way, so it
+// weighs 1 exactly, and 2^-126 is nothing beside a temperature of 2^-100.
+__device__ __forceinline__ double widened(float l) {
+    const uint32_t b = __float_as_uint(l);
+    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
 __device__ __forceinline__ u64 weight(float l, const Weigher& g) {
-    // l as a double by whole-number operations: the conversion instruction runs at a quarter of their rate and bound
-    // this pass (subnormals come out a little off, and weigh the same)
-    const uint32_t b = __float_as_uint(fmaxf(l, g.floor));  // (NaN too)
-    const double ld = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
-    const double y = (ld - g.md) * g.scale;
+    const double y = (widened(fmaxf(l, g.floor)) - g.md) * g.scale;  // (NaN as the floor)
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double t = y + magic;
     const int n = __double2loint(t);
@@ -450,7 +453,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     // Keeps the factors below finite, and m - 34 temp above fp32's lowest number.  Where the next smaller fp32 number is
     // more than 40 temperatures below m, it is taken as 40: that weighs nothing all the same.
     temp = fmaxf(fminf(fmaxf(temp, 0x1p-100f), 0x1p96f), (m - nextafterf(m, -INFINITY)) / 40.0f);
-    const double md = m;
     const float to_bin = (float)kBins / (kSpan * temp);
     // Place of a logit on the scale of the first histogram, in steps.  Places
     // rise as logits fall, in fp32 as well as in exact arithmetic, since every
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     // exp(-34) 2^44 < 1/2.  Rounded away from m: half of fp32's step at m may be many temperatures.
     weigher.floor = __fsub_rd(m, 34.0f * temp);
     weigher.scale = 32.0 * 1.4426950408889634074 / (double)temp;
-    weigher.md = md;
+    weigher.md = widened(m);
     weigher.tab = exp2((double)lane / 32.0 + (double)kWeightBits);
     auto wt = [&](float l) { return weight(l, weigher); };  // by all lanes of a warp
     auto composite = [&](float l, int i) { return ((u64)order_key(l) << kIndexBits) | (u64)(first + i); };
@@ -490,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     auto answer = [&](int token, float l, u64 whole) {
         a.out_tok[row] = token;
         if (a.out_logp) {
-            const double x = l == m ? 0.0 : ((double)l - md) / (double)temp;
+            const double x = l == m ? 0.0 : ((double)l - (double)m) / (double)temp;
             a.out_logp[row] = (float)(x - log((double)whole * (1.0 / (double)(1ull << kWeightBits))));
         }
     };

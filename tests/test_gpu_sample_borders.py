@@ -176,3 +176,12 @@ def test_masked_tokens_weigh_nothing_at_any_temperature(cuda_device, copies, voc
             p.append([1.0, 0.77, 0.9, 1.0][(c // 4) % 4])
             m.append([0.0, 0.0, 0.0, 1e-3][(c // 4) % 4])
     run(np.stack(rows), u, t=t, k=k, p=p, m=m)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 20011), (9, 3001), (200, 90003)], ids=["cluster", "cta", "streamed"])
+def test_min_p_of_one_keeps_the_largest_subnormal(cuda_device, rows, vocab):
+    """The largest logit weighs 1 whatever its size, so a least weight of 1 keeps it and its equals."""
+    for best, t in ((-1e-40, 2.0 ** -100), (-1e-45, 0.0009765625 * 2.0 ** -90), (0.0, 2.0 ** -100), (1e-40, 1e-30)):
+        lg = np.full((rows, vocab), -1.0, np.float32)
+        lg[:, 17::400] = best
+        run(lg, [US[r % 7] for r in range(rows)], t=[t] * rows, m=[1.0] * rows)
