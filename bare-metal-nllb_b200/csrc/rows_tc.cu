@@ -25,7 +25,12 @@
 // to the type (half a step each, unbiased; the sum that divides them stays
 // fp32).  fp32 inputs and weights are split into two fp16 parts, hi + lo, and
 // a product is taken as hi hi' + hi lo' + lo hi' (22 bits, and an absolute
-// 2^-25 where lo leaves fp16's normal range).  Weights are held times 2^7, so
+// 2^-25 where lo leaves fp16's normal range).  So that this holds at any size,
+// rows whose largest size lies outside [2^-3, 65504) are divided by a power of
+// two first: queries and keys 16 rows alike, which a warp settles for itself
+// and the scores undo; values a tile alike, which the sum over the tiles
+// undoes.  (Ordinary sizes pay for the look: 64 prefixes 71 us instead of 67,
+// 128 scored sentences 96 instead of 91.)  Weights are held times 2^7, so
 // fp16 keeps them normal down to 2^-21 of the largest while 2^7 * 2^8 stays in
 // its range.
 //
@@ -37,6 +42,7 @@
 // the exponentials on the fp32 multipliers, or turns between the two tiles'
 // exponentials, made it slower (a quarter of them 366 us, turns 361 us).
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -65,7 +71,13 @@ struct Cfg {
     static constexpr int COLS = 128 * 4 / WPT;                      // scores of a thread
     static constexpr int WORDS = 2 * ST + 2;  // key tiles whose visible keys are kept
     static constexpr uint32_t SQ = 0, SK = NQ * OPER, SV = SK + ST * OPER, SAUX = SV + ST * OPER;
-    static constexpr uint32_t VALID = SAUX, MAXS = VALID + WORDS * 16, BARS = MAXS + (WPT == 8 ? 2 * NQ * 2 * 128 * 4 : 0);
+    static constexpr uint32_t VALID = SAUX, MAXS = VALID + WORDS * 16;
+    // fp32: what rows of the queries and of the K tiles (the first one last), and V tiles, were divided by; a byte per
+    // warp that tells of divisors other than 1; largest sizes of V: of the first tile, by softmax warp, and of others
+    static constexpr uint32_t QS = MAXS + (WPT == 8 ? 2 * NQ * 2 * 128 * 4 : 0), KS = QS + (F32 ? kTile * 4 : 0);
+    static constexpr uint32_t VS = KS + (F32 ? (WORDS + 1) * kTile * 4 : 0), TOPS = VS + (F32 ? (WORDS + 1) * 4 : 0);
+    static constexpr uint32_t ODD = (TOPS + (F32 ? (8 + 2 * kLoaders / 32) * 4 : 0) + 7) / 8 * 8;  // queries, V's first, K tiles
+    static constexpr uint32_t BARS = ODD + (F32 ? (WORDS + 3) * 8 : 0);
     // P beside S in tensor memory, where there is room: the next scores can then be taken as soon as a row is read
     static constexpr bool AHEAD = NQ == 2 && D == 64;
     // fp32: the outputs' sum over the tiles.  The tensor cores cut what they accumulate, so a sum over many tiles would
@@ -74,7 +86,7 @@ struct Cfg {
     static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D, T_COL = P_COL;
     // fp32: the softmax threads also fetch the first key tile, with all of its loads in flight at once
     static constexpr bool FIRST = F32;  // (one slot: the first tile's phase is simply not counted)
-    static constexpr int N_BARS = 4 * ST + 9 * NQ + 2;
+    static constexpr int N_BARS = 4 * ST + 9 * NQ + 3;
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
     static constexpr int THREADS = SOFT + kLoaders + 32;
@@ -240,6 +252,46 @@ __device__ __forceinline__ void split_store(unsigned char* to, const float4& a, 
     *reinterpret_cast<uint4*>(to + PART) = lo;
 }
 
+constexpr float kLeastSize = 0x1p-3f, kMostSize = 65504.0f;
+
+// The larger of `top` and the sizes of 8 values (passes over NaN).
+__device__ __forceinline__ float larger(float top, const float4& a, const float4& b) {
+    top = fmaxf(fmaxf(top, fabsf(a.x)), fabsf(a.y));
+    top = fmaxf(fmaxf(top, fabsf(a.z)), fabsf(a.w));
+    top = fmaxf(fmaxf(top, fabsf(b.x)), fabsf(b.y));
+    return fmaxf(fmaxf(top, fabsf(b.z)), fabsf(b.w));
+}
+// What values of up to `top` in size are divided by before they are split: 1 where the largest keeps 22 bits in two fp16
+// parts as it is, else the power of two that takes it to 2^14 or more (values down to 2^-17 of it keep 22 bits, smaller
+// ones 2^-39 of it).  Not finite: 1.
+__device__ __forceinline__ float divisor(float top) {
+    const uint32_t b = __float_as_uint(top);
+    if ((top >= kLeastSize && top < kMostSize) || b == 0u || b >= 0x7f800000u) return 1.0f;
+    return __uint_as_float((max(b >> 23, 15u) - 14u) << 23);
+}
+__device__ __forceinline__ float power_inverse(float x) {  // of a power of two, 2^-126 to 2^113
+    return __uint_as_float((254u << 23) - __float_as_uint(x));
+}
+__device__ __forceinline__ float warp_top(float top) {  // the largest of a warp's sizes
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+}
+__device__ __forceinline__ void times(float4& a, float by) { a.x *= by, a.y *= by, a.z *= by, a.w *= by; }
+// Divides what a warp holds by a power of two, where its largest size asks for that.
+template <int N>
+__device__ __forceinline__ float divide(float4 (&a)[N], float4 (&b)[N]) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = larger(top, a[i], b[i]);
+    const float div = divisor(warp_top(top));
+    if (div != 1.0f) {
+        const float by = power_inverse(div);
+#pragma unroll
+        for (int i = 0; i < N; ++i) times(a[i], by), times(b[i], by);
+    }
+    return div;
+}
+__device__ __forceinline__ void loaders_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory"); }
+
 template <typename T, int D, int NQ, bool PAGED>
 __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     rows_tc_kernel(const RowsParams p, int n_split) {
@@ -252,9 +304,15 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     uint64_t *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
     uint64_t *s_full = v_empty + ST, *p_full = s_full + NQ, *o_full = p_full + NQ, *q_full = o_full + NQ;
     uint64_t *s_read = q_full + NQ, *pair = s_read + NQ, *done = pair + 4 * NQ, *v_first = done + 1;
+    uint64_t* again = v_first + 1;  // (fp32) the first tile of V, split once more
     uint32_t* slot = reinterpret_cast<uint32_t*>(sm + C::SLOT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::SLOT + 4);
     const uint32_t* valid = reinterpret_cast<const uint32_t*>(sm + C::VALID);
+    // (fp32) divisors, largest sizes, and the bytes of what is divided
+    float *q_div = reinterpret_cast<float*>(sm + C::QS), *k_div = reinterpret_cast<float*>(sm + C::KS);
+    float *v_div = reinterpret_cast<float*>(sm + C::VS), *tops = reinterpret_cast<float*>(sm + C::TOPS);
+    uint64_t *q_odd = reinterpret_cast<uint64_t*>(sm + C::ODD), *v_kinds = q_odd + 1, *k_odd = q_odd + 2;
+    auto place = [](int j) { return j == 0 ? C::WORDS : j % C::WORDS; };  // of tile j among the divisors
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (known to be the same in all lanes)
@@ -289,6 +347,11 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
             }
             mbar_init(done, 1);
             mbar_init(v_first, C::SOFT);
+            if constexpr (C::F32) {
+                mbar_init(again, kLoaders);
+                for (int i = 0; i < C::WORDS + 3; ++i) q_odd[i] = 0;
+                v_div[C::WORDS] = 1.0f;
+            }
             fence_barrier_init();
             *abort_flag = 0;
         }
@@ -307,11 +370,19 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     const int per = (all_tiles + n_split - 1) / n_split;
     const int j0 = split * per, n = max(0, min(all_tiles, j0 + per) - j0);
 
+    // (fp32) Whether the first tile of V has to be split again, by the softmax warps' bytes (1: a size of 2^-3, 2: too large).
+    auto v_first_odd = [&]() -> bool {
+        static_assert(!C::F32 || C::SOFT == 256, "a byte of each softmax warp");
+        const uint64_t f = *v_kinds, bytes = 0x0101010101010101ull;
+        return (f & bytes) == 0 || (f & bytes * 2) != 0;
+    };
+
     // Bounded wait; false (and the CTA gives up) once any wait has run out.
-    auto wait_one = [&](uint64_t* bar, uint32_t parity, long long budget = kWaitBudgetCycles) -> bool {
+    auto wait_one = [&](uint64_t* bar, uint32_t parity, long long budget = kWaitBudgetCycles, int pause = 0) -> bool {
         if (mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
         while (!mbar_try_wait(bar, parity)) {
+            if (pause) __nanosleep(pause);
             if (*abort_flag) return false;
             if (clock64() - t0 > budget) {
                 *abort_flag = 1;
@@ -383,6 +454,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         }
                     }
                 }
+                if constexpr (C::F32) {
+                    const float div = divide(a, b);
+                    if (lane == 0) reinterpret_cast<uint8_t*>(q_odd)[warp] = div != 1.0f;
+#pragma unroll
+                    for (int i = 0; i < TAKE; ++i)
+                        if ((lt + i * N) % CH == 0) q_div[(lt + i * N) / CH] = div;
+                }
 #pragma unroll
                 for (int i = 0; i < TAKE; ++i) {
                     const int x = lt + (i0 + i) * N;
@@ -392,31 +470,45 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 }
             }
             if constexpr (C::FIRST) {
+                static_assert(kTile * CH == TAKE * N && NQ == 1, "a tile in registers");
                 const T *k[TAKE], *v[TAKE];
 #pragma unroll
-                for (int i0 = 0; i0 < kTile * CH / N; i0 += TAKE) {
+                for (int i = 0; i < TAKE; ++i) {
+                    const int r = (lt + i * N) / CH, key = j0 * kTile + r;
+                    if (!(key < longest && rows_key<T, PAGED>(p, sq, s, g, key, k[i], v[i]))) k[i] = v[i] = nullptr;
+                }
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    float4 a[TAKE], b[TAKE];
 #pragma unroll
                     for (int i = 0; i < TAKE; ++i) {
-                        const int r = (lt + (i0 + i) * N) / CH, key = j0 * kTile + r;
-                        if (!(key < longest && rows_key<T, PAGED>(p, sq, s, g, key, k[i], v[i]))) k[i] = v[i] = nullptr;
+                        const int c = (lt + i * N) % CH;
+                        const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
+                        a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (src) a[i] = __ldg(src + 2 * c), b[i] = __ldg(src + 2 * c + 1);
                     }
+                    if (kv == 0) {
+                        const float div = divide(a, b);
+                        if (lane == 0) reinterpret_cast<uint8_t*>(k_odd + C::WORDS)[warp] = div != 1.0f;
 #pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
-                        float4 a[TAKE], b[TAKE];
-#pragma unroll
-                        for (int i = 0; i < TAKE; ++i) {
-                            const int c = (lt + (i0 + i) * N) % CH;
-                            const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
-                            a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (src) a[i] = __ldg(src + 2 * c), b[i] = __ldg(src + 2 * c + 1);
-                        }
-#pragma unroll
-                        for (int i = 0; i < TAKE; ++i) {
-                            const int x = lt + (i0 + i) * N;
-                            split_store<C::PART>(sm + (kv ? C::SV : C::SK) + chunk_off(x / CH, x % CH), a[i], b[i]);
-                        }
-                        if (i0 + TAKE >= kTile * CH / N) mbar_arrive(kv ? v_first : q_full + t);
+                        for (int i = 0; i < TAKE; ++i)
+                            if ((lt + i * N) % CH == 0) k_div[C::WORDS * kTile + (lt + i * N) / CH] = div;
                     }
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < TAKE; ++i) {
+                        const int x = lt + i * N;
+                        split_store<C::PART>(sm + (kv ? C::SV : C::SK) + chunk_off(x / CH, x % CH), a[i], b[i]);
+                        if (kv) top = larger(top, a[i], b[i]);
+                    }
+                    if (kv) {  // (the fetching warps see whether the tile has to be split again)
+                        top = warp_top(top);
+                        if (lane == 0) {
+                            reinterpret_cast<uint8_t*>(v_kinds)[warp] = (top >= kLeastSize ? 1 : 0) | (top >= kMostSize ? 2 : 0);
+                            tops[warp] = top;
+                        }
+                    }
+                    mbar_arrive(kv ? v_first : q_full + t);
                 }
             } else if constexpr (C::F32) {
                 mbar_arrive(q_full + t);
@@ -451,6 +543,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 };
                 float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 tmem_ld<C::COLS>(tR, v);
+                if constexpr (C::F32) {
+                    if ((*q_odd | k_odd[place(j)]) != 0) {
+                        const float qd = q_div[lq * 32 + lane], *kd = k_div + place(j) * kTile + half * C::COLS;
+#pragma unroll
+                        for (int i = 0; i < C::COLS; ++i) v[i] *= fminf(qd * kd[i], FLT_MAX);  // (no 0 times infinity)
+                    }
+                }
                 if (!whole) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c) hide(v + 32 * c, bits[c]);
@@ -477,6 +576,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     m = to;
                     l *= corr;
                     if (j > 0) {
+                        const float vd = v_div[place(j - 1)];
 #pragma unroll
                         for (int c = half * (D / 2); c < (C::WPT == 8 ? (half + 1) * (D / 2) : D); c += 8) {
                             uint32_t o[8], x[8];
@@ -485,8 +585,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                float y = __uint_as_float(o[i]);
-                                if (j > 1) y += __uint_as_float(x[i]);
+                                const float y = fmaf(__uint_as_float(o[i]), vd, j > 1 ? __uint_as_float(x[i]) : 0.f);
                                 o[i] = __float_as_uint(y * corr);
                             }
                             tmem_st8(tT + c, o);
@@ -545,11 +644,18 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         }
         auto last_output = [&](int c, float* o) {
             tmem_ld32(tO + c, o);
-            if (C::TOTAL && n > 1) {
-                float x[32];
-                tmem_ld32(tT + c, x);
+            if constexpr (C::TOTAL) {
+                const float vd = v_div[place(n - 1)];
+                if (vd != 1.0f) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] += x[i];
+                    for (int i = 0; i < 32; ++i) o[i] *= vd;
+                }
+                if (n > 1) {
+                    float x[32];
+                    tmem_ld32(tT + c, x);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] += x[i];
+                }
             }
         };
         const int d0 = half * (D / 2), d1 = C::WPT == 8 ? d0 + D / 2 : D;  // this thread's part of the output
@@ -607,7 +713,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         };
         bool ok = true;
         if (n > 0) look_up(0);
-        for (int j = 0; j < n && ok; ++j) {
+        for (int j = 0; j < n && (ok || C::F32); ++j) {  // (fp32: the warps give up together)
             const int st = j % ST;
             const T *k[RP], *v[RP];
             // (visible keys of a tile: kept until its weights are formed, at least one tile after V of this slot)
@@ -625,10 +731,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 if (lane == 0 && r < kTile) seen16[(j % C::WORDS) * 8 + (r >> 4)] = (uint16_t)w;
             }
             if (j + 1 < n) look_up(j + 1);
-            if (C::FIRST && j == 0) {  // fetched by the softmax threads
-                mbar_arrive(q_full);
-                continue;
-            }
+            if (C::FIRST && j == 0) mbar_arrive(q_full);  // fetched by the softmax threads
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
                 uint64_t *full = (kv ? v_full : k_full) + st, *empty = (kv ? v_empty : k_empty) + st;
@@ -649,33 +752,72 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     }
                     cp_arrive(full);
                 } else {
+                    // K: 16 rows divided alike.  V: the tile alike, since its sums are: split as it is (the first tile by the
+                    // softmax threads) and, where the tile's largest size asks for a divisor, read and split once more.
+                    if (j == 0 && kv == 0) continue;
+                    float div = 1.0f;
+                    if (j == 0) {
+                        if (ok) ok = __all_sync(0xffffffffu, wait_one(v_first, 0, kWaitBudgetCycles, 200));
+                        if (!ok || !v_first_odd()) continue;
+                        float top = 0.f;
+                        for (int w = 0; w < 8; ++w) top = fmaxf(top, tops[w]);
+                        div = divisor(top);
+                    }
+                    for (int pass = j == 0; pass < 2; ++pass) {
+                        const float by = power_inverse(div);
+                        float top = 0.f;
+                        bool odd = false;
 #pragma unroll
-                    for (int i = 0; i < RP; ++i) {
-                        const int r = (lt >> 1) + i * (kLoaders / 2);
-                        const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
+                        for (int i = 0; i < RP; ++i) {
+                            const int r = (lt >> 1) + i * (kLoaders / 2);
+                            const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
+                            float4 a[CH / 2], b[CH / 2];
 #pragma unroll
-                        for (int c0 = 0; c0 < CH; c0 += 8) {
-                            float4 a[4], b[4];
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
+                            for (int c = 0; c < CH / 2; ++c) {
                                 a[c] = b[c] = make_float4(0.f, 0.f, 0.f, 0.f);
                                 if (src) {
-                                    a[c] = __ldg(src + 2 * (c0 + 2 * c + odd));
-                                    b[c] = __ldg(src + 2 * (c0 + 2 * c + odd) + 1);
+                                    a[c] = __ldg(src + 2 * (2 * c + (lt & 1)));
+                                    b[c] = __ldg(src + 2 * (2 * c + (lt & 1)) + 1);
                                 }
                             }
-                            if (i == 0 && c0 == 0 && j >= ST) ok = wait(empty, ((j / ST) - 1) & 1);
+                            if (kv == 0) {
+                                const float d = divide(a, b);
+                                odd = odd || d != 1.0f;
+                                if ((lt & 1) == 0 && r < kTile) k_div[place(j) * kTile + r] = d;
+                            } else if (pass == 1) {
+#pragma unroll
+                                for (int c = 0; c < CH / 2; ++c) times(a[c], by), times(b[c], by);
+                            }
+                            if (i == 0 && pass == 0 && ok) ok = wait(empty, (j - 1) & 1);
                             if (ok && r < kTile) {
 #pragma unroll
-                                for (int c = 0; c < 4; ++c)
-                                    split_store<C::PART>(sm + dst + chunk_off(r, c0 + 2 * c + odd), a[c], b[c]);
+                                for (int c = 0; c < CH / 2; ++c) {
+                                    if (kv) top = larger(top, a[c], b[c]);
+                                    split_store<C::PART>(sm + dst + chunk_off(r, 2 * c + (lt & 1)), a[c], b[c]);
+                                }
                             }
                         }
+                        if (kv == 0 && lane == 0) reinterpret_cast<uint8_t*>(k_odd + place(j))[warp - C::SOFT / 32] = odd;
+                        if (kv == 0 || pass == 1) break;
+                        // A warp that gave up says so, and all leave together: nobody waits here for one that left.  (Two
+                        // sets of words: the next tile's are not written where a slower warp still reads this one's.)
+                        float* all = tops + 8 + (j & 1) * (kLoaders / 32);
+                        top = warp_top(top);
+                        if (lane == 0) all[warp - C::SOFT / 32] = ok ? top : -1.0f;
+                        loaders_meet();
+#pragma unroll
+                        for (int w = 0; w < kLoaders / 32; ++w) {
+                            ok = ok && all[w] >= 0.f;
+                            top = fmaxf(top, all[w]);
+                        }
+                        div = divisor(top);
+                        if (!ok || div == 1.0f) break;
                     }
-                    if (!ok) break;
-                    mbar_arrive(full);
+                    if (kv && lt == 0) v_div[place(j)] = div;
+                    if (ok) mbar_arrive(j == 0 ? again : full);
                 }
             }
+            if (!ok && (j > 0 || !C::F32)) break;  // (fp32: after the warps have met)
         }
         if constexpr (!C::F32) cp_wait_all();
     } else {
@@ -766,6 +908,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 if (t == 0) {
                     // (a slot's k_full and v_full do not count the first tile where the softmax threads fetched it)
                     if (!(ok = C::FIRST && j == 0 ? wait(v_first, 0) : wait(v_full + st, (j / ST - C::FIRST) & 1))) break;
+                    if (C::FIRST && j == 0 && v_first_odd() && !(ok = wait(again, 0))) break;
                     fence_async_smem();
                 }
                 if (!(ok = wait(p_full + t, j & 1))) break;
