@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         tmem_alloc(slot, C::TMEM);
         if (lane == 0) {
             for (int i = 0; i < ST; ++i) {
-                mbar_init(k_full + i, kLoaders);
+                mbar_init(k_full + i, kLoaders + (C::F32 ? 0 : kLoaders / 32));
                 mbar_init(v_full + i, kLoaders);
                 mbar_init(k_empty + i, 1);
                 mbar_init(v_empty + i, 1);
@@ -738,6 +738,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 const uint32_t dst = (kv ? C::SV : C::SK) + st * C::OPER;
                 if constexpr (!C::F32) {
                     if (j >= ST && !(ok = wait(empty, ((j / ST) - 1) & 1))) break;
+                    // (an ordinary arrival, for the words of visible keys: that of the copies vouches for the copies alone)
+                    if (kv == 0) warp_arrive(full);
 #pragma unroll
                     for (int i = 0; i < RP; ++i) {
                         const int r = (lt >> 1) + i * (kLoaders / 2);
