@@ -1,6 +1,5 @@
 // rows_api.cu -- nllb_attn_paged and nllb_attn_cross_rows: argument checks and
 // launch parameters.
-#include <climits>
 #include <cmath>
 #include <string>
 
@@ -30,8 +29,8 @@ int check_common(int dtype, int head_dim, int n_heads, int n_kv_heads, int n_seq
     if (n_heads > 1024) return bad("at most 1024 heads");
     if (n_seq < 0 || q_rows < 0 || max_q < 0 || max_kv < 0) return bad("negative size");
     if (n_seq > 65535) return set_error(NLLB_ATTN_ECAPACITY, "at most 65535 sequences per call");
-    if ((long long)n_seq * max_q > INT_MAX || (long long)max_q * (n_heads / n_kv_heads) > (1 << 26) ||
-        (long long)n_seq * max_kv > INT_MAX || max_kv > (1 << 30))
+    // (n_seq * max_q and n_seq * max_kv number rows only where starts are NULL: they are held against q_rows and kv_rows)
+    if ((long long)max_q * (n_heads / n_kv_heads) > (1 << 26) || max_kv > (1 << 30))
         return set_error(NLLB_ATTN_ECAPACITY, "more rows than a call takes");
     if (!(scale > 0.0f) || !std::isfinite(scale)) return bad("scale must be positive");
     return NLLB_ATTN_OK;

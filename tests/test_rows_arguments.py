@@ -1,0 +1,42 @@
+"""Arguments of nllb_attn_paged, nllb_attn_cross_rows and nllb_sample that are taken, or refused, before touching a GPU;
+beside test_rows_sample_refusals.py."""
+import ctypes
+
+import pytest
+
+import nllb_attn as na
+from test_rows_sample_refusals import P, cross_args, paged_args
+
+
+def status(fn, a):
+    lib = na.load()
+    rc = getattr(lib, fn)(None, ctypes.byref(a))
+    return rc, lib.nllb_attn_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_seq=4096, max_kv=1 << 20, page_table_stride=1 << 16),  # 2^32 places in the tables, of which few are used
+    dict(n_seq=65535, max_q=1 << 16, q_start=P, q_len=P, q_rows=70000),  # one long chunk among single tokens
+    dict(n_seq=65535, max_kv=1 << 30, page_size=1 << 20, page_table_stride=1 << 10),
+])
+def test_paged_takes_wide_bounds(kw):
+    """Bounds of single sequences: their products number nothing where the starts are given."""
+    rc, text = status("nllb_attn_paged", paged_args(**dict(dict(q_rows=65535 * 2), **kw)))
+    assert rc == na.EINVAL and "ctx" in text  # all that is left to refuse
+
+
+def test_cross_rows_takes_wide_bounds_with_starts():
+    kw = dict(n_seq=40000, max_q=1 << 16, max_kv=1 << 18, q_start=P, q_len=P, kv_start=P, q_rows=90000, kv_rows=1 << 19)
+    rc, text = status("nllb_attn_cross_rows", cross_args(**kw))
+    assert rc == na.EINVAL and "ctx" in text
+
+
+@pytest.mark.parametrize("fn,kw,needle", [
+    ("nllb_attn_paged", dict(n_seq=65535, max_q=1 << 16, q_rows=2 ** 31 - 1), "q_rows"),
+    ("nllb_attn_cross_rows", dict(n_seq=65535, max_q=1 << 16, q_rows=2 ** 31 - 1, max_kv=1), "q_rows"),
+    ("nllb_attn_cross_rows", dict(n_seq=65535, max_q=1, q_rows=70000, max_kv=1 << 16, kv_rows=2 ** 31 - 1), "kv_rows"),
+])
+def test_rows_without_starts_have_to_exist(fn, kw, needle):
+    a = paged_args(**kw) if fn.endswith("paged") else cross_args(**kw)
+    rc, text = status(fn, a)
+    assert rc == na.EINVAL and needle in text
