@@ -42,6 +42,9 @@ bool rows_ok(const void* base, int dtype, int64_t a, int64_t b, int64_t c = 0) {
     return aligned16(base) && a >= 0 && b >= 0 && c >= 0 && a % unit == 0 && b % unit == 0 && c % unit == 0;
 }
 
+// Rows that are written may not lie in one another: `n` of them `stride` apart.
+bool apart(int64_t n, int64_t stride, int head_dim) { return n <= 1 || stride >= head_dim; }
+
 // Division of a j < 2^30 by d: with 2^(b-1) < d <= 2^b the multiplier ceil(2^(30+b) / d) is too large by less than 1, so
 // the quotient by less than 2^30 / 2^(30+b) <= 1 / d: it stays below the next whole number.
 void set_division(int d, uint32_t* mul, int* shr) {
@@ -96,6 +99,15 @@ int nllb_attn_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a) {
         (a->k_new && (!rows_ok(a->k_new, a->dtype, a->k_new_stride_row, a->k_new_stride_head) ||
                       !rows_ok(a->v_new, a->dtype, a->v_new_stride_row, a->v_new_stride_head))))
         return bad("rows must be 16-byte aligned, strides non-negative multiples of 16 bytes");
+    if (!apart(a->q_rows, a->out_stride_row, a->head_dim) || !apart(a->n_heads, a->out_stride_head, a->head_dim))
+        return bad("out: strides below head_dim, its rows would overlap");
+    auto pages_apart = [&](int64_t page, int64_t slot, int64_t head) {
+        return apart(a->n_pages, page, a->head_dim) && apart(a->page_size, slot, a->head_dim) &&
+               apart(a->n_kv_heads, head, a->head_dim);
+    };
+    if (a->k_new && !(pages_apart(a->k_stride_page, a->k_stride_slot, a->k_stride_head) &&
+                      pages_apart(a->v_stride_page, a->v_stride_slot, a->v_stride_head)))
+        return bad("k_pages, v_pages: strides below head_dim, the rows written would overlap");
     p.q = a->q, p.k = a->k_pages, p.v = a->v_pages, p.k_new = a->k_new, p.v_new = a->v_new;
     p.k_w = a->k_pages, p.v_w = a->v_pages, p.out = a->out;
     p.q_row = a->q_stride_row, p.q_head = a->q_stride_head, p.o_row = a->out_stride_row, p.o_head = a->out_stride_head;
@@ -129,6 +141,8 @@ int nllb_attn_cross_rows(nllb_attn_ctx* c, const nllb_attn_cross_rows_args* a) {
         !rows_ok(a->k, a->dtype, a->k_stride_row, a->k_stride_head) ||
         !rows_ok(a->v, a->dtype, a->v_stride_row, a->v_stride_head))
         return bad("rows must be 16-byte aligned, strides non-negative multiples of 16 bytes");
+    if (!apart(a->q_rows, a->out_stride_row, a->head_dim) || !apart(a->n_heads, a->out_stride_head, a->head_dim))
+        return bad("out: strides below head_dim, its rows would overlap");
     p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out;
     p.q_row = a->q_stride_row, p.q_head = a->q_stride_head, p.o_row = a->out_stride_row, p.o_head = a->out_stride_head;
     p.k_row = a->k_stride_row, p.k_head = a->k_stride_head, p.v_row = a->v_stride_row, p.v_head = a->v_stride_head;

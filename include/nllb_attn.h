@@ -220,7 +220,7 @@ NLLB_ATTN_API int nllb_attn_cross_host(nllb_attn_ctx* ctx, int layer, int n_sent
  * (device arrays; q_len NULL: max_q rows each, q_start NULL: s * max_q).
  * Rows of q and out that belong to no sequence are neither read nor written.
  * Strides count elements; every row must start on 16 bytes (out may not
- * overlap an input).  max_q and max_kv bound the lengths: they size the
+ * overlap an input, nor rows that the call writes one another).  max_q and max_kv bound the lengths: they size the
  * launch, larger lengths on the device are refused there.  A length, start
  * or page number outside its bound or buffer sets the device error word
  * (nllb_attn_sync then returns NLLB_ATTN_EINVAL): a sequence with a bad

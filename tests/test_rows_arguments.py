@@ -40,3 +40,25 @@ def test_rows_without_starts_have_to_exist(fn, kw, needle):
     a = paged_args(**kw) if fn.endswith("paged") else cross_args(**kw)
     rc, text = status(fn, a)
     assert rc == na.EINVAL and needle in text
+
+
+@pytest.mark.parametrize("kw", [dict(out_stride_row=0), dict(out_stride_head=0), dict(out_stride_head=32)])
+def test_overlapping_outputs_are_refused(kw):
+    for fn, a in (("nllb_attn_paged", paged_args(**kw)), ("nllb_attn_cross_rows", cross_args(**kw))):
+        rc, text = status(fn, a)
+        assert rc == na.EINVAL and "overlap" in text
+
+
+@pytest.mark.parametrize("kw", [dict(k_stride_page=0), dict(v_stride_slot=0), dict(k_stride_head=0), dict(v_stride_page=32)])
+def test_overlapping_pages_are_refused_where_they_are_written(kw):
+    new = dict(k_new=P, v_new=P, k_new_stride_row=128, k_new_stride_head=64, v_new_stride_row=128, v_new_stride_head=64)
+    rc, text = status("nllb_attn_paged", paged_args(**new, **kw))
+    assert rc == na.EINVAL and "overlap" in text
+    for read in (paged_args(**kw), paged_args(**new)):  # read only, or apart
+        rc, text = status("nllb_attn_paged", read)
+        assert rc == na.EINVAL and "ctx" in text
+
+
+def test_single_rows_take_any_output_stride():
+    rc, text = status("nllb_attn_paged", paged_args(n_seq=1, q_rows=1, max_q=1, out_stride_row=0))
+    assert rc == na.EINVAL and "ctx" in text
