@@ -230,6 +230,7 @@ class Context:
         _check(self.lib, self.lib.nllb_attn_create(device, ctypes.byref(self.dims), ctypes.byref(h)),
                "nllb_attn_create")
         self.handle = h
+        self.device = device
         self.n_beams, self.n_heads = n_beams, n_heads
 
     def close(self) -> None:
@@ -369,10 +370,19 @@ class Context:
             a.k_new, a.v_new = _rows(k_new, "k_new", q, 3), _rows(v_new, "v_new", q, 3)
             a.k_new_stride_row, a.k_new_stride_head = k_new.stride(0), k_new.stride(1)
             a.v_new_stride_row, a.v_new_stride_head = v_new.stride(0), v_new.stride(1)
+        a.tensors_on = q.device
         return a
+
+    def _same_device(self, args) -> None:
+        """The tensors the arguments were built from lie on the context's GPU
+        (a structure filled by hand is the caller's to get right)."""
+        on = getattr(args, "tensors_on", None)
+        if on is not None and (on.type != "cuda" or on.index != self.device):
+            raise ValueError(f"the tensors are on {on}, the context on cuda:{self.device}")
 
     def paged(self, args: PagedArgs) -> None:
         """nllb_attn_paged: a chunk of new tokens over a paged cache."""
+        self._same_device(args)
         _check(self.lib, self.lib.nllb_attn_paged(self.handle, ctypes.byref(args)), "nllb_attn_paged")
 
     @staticmethod
@@ -390,7 +400,7 @@ class Context:
             max_q = rows if q_len is not None else rows // max(n_seq, 1)
         if max_kv is None:
             max_kv = kv_rows if kv_start is not None else kv_rows // max(n_seq, 1)
-        return CrossRowsArgs(
+        a = CrossRowsArgs(
             q=_rows(q, "q", q, 3), k=_rows(k, "k", q, 3), v=_rows(v, "v", q, 3), out=_rows(out, "out", q, 3),
             q_start=_ints(q_start, "q_start", n_seq, q), q_len=_ints(q_len, "q_len", n_seq, q),
             kv_start=_ints(kv_start, "kv_start", n_seq, q), kv_len=_ints(kv_len, "kv_len", n_seq, q),
@@ -400,6 +410,8 @@ class Context:
             q_stride_row=q.stride(0), q_stride_head=q.stride(1), k_stride_row=k.stride(0), k_stride_head=k.stride(1),
             v_stride_row=v.stride(0), v_stride_head=v.stride(1), out_stride_row=out.stride(0),
             out_stride_head=out.stride(1))
+        a.tensors_on = q.device
+        return a
 
     def test_expire_next_rows_wait(self) -> None:
         """nllb_attn_test_expire_next_rows_wait: a bounded wait of the next
@@ -408,6 +420,7 @@ class Context:
 
     def cross_rows(self, args: CrossRowsArgs) -> None:
         """nllb_attn_cross_rows: target rows over encoder states of another length."""
+        self._same_device(args)
         _check(self.lib, self.lib.nllb_attn_cross_rows(self.handle, ctypes.byref(args)), "nllb_attn_cross_rows")
 
 

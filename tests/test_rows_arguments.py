@@ -62,3 +62,39 @@ def test_overlapping_pages_are_refused_where_they_are_written(kw):
 def test_single_rows_take_any_output_stride():
     rc, text = status("nllb_attn_paged", paged_args(n_seq=1, q_rows=1, max_q=1, out_stride_row=0))
     assert rc == na.EINVAL and "ctx" in text
+
+
+class FakeDevice:
+    def __init__(self, type, index):
+        self.type, self.index = type, index
+
+
+def test_binding_refuses_tensors_of_another_device():
+    """Arguments built from CPU tensors, or those of another GPU, never reach the library."""
+    import torch
+    q, lens = torch.zeros(4, 2, 64), torch.ones(2, dtype=torch.int32)
+    pages, table = torch.zeros(3, 16, 2, 64), torch.zeros(2, 2, dtype=torch.int32)
+    c = object.__new__(na.Context)  # a context without a GPU: the library refuses its handle
+    c.lib, c.handle, c.device = na.load(), None, 1
+    for call, args in ((c.paged, na.Context.paged_args(q, pages, pages, table, lens, q)),
+                       (c.cross_rows, na.Context.cross_rows_args(q, q, q, q, lens))):
+        with pytest.raises(ValueError, match="cpu"):
+            call(args)
+        args.tensors_on = FakeDevice("cuda", 0)
+        with pytest.raises(ValueError, match="cuda:1"):
+            call(args)
+        args.tensors_on = FakeDevice("cuda", 1)
+        with pytest.raises(na.NllbAttnError, match="ctx"):
+            call(args)
+    with pytest.raises(na.NllbAttnError):
+        c.paged(paged_args())  # filled by hand
+
+
+@pytest.mark.gpu
+def test_binding_refuses_cpu_tensors_on_a_gpu(cuda_device):
+    import torch
+    q, lens = torch.zeros(4, 2, 64), torch.ones(2, dtype=torch.int32)
+    with na.Context(0, n_layers=0, max_sentences=0) as ctx:
+        with pytest.raises(ValueError, match="cpu"):
+            ctx.cross_rows(na.Context.cross_rows_args(q, q, q, q, lens))
+        ctx.sync()
