@@ -571,8 +571,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
            stream=None):
     """nllb_sample on torch CUDA tensors: logits [rows][vocab] (rows may be
     strided), u [rows] fp32; temperature, top_p, min_p [rows] fp32 and top_k
-    [rows] int32 or None.  Returns (tokens [rows] int32, log-probabilities
-    [rows] fp32)."""
+    [rows] int32 or None.  Runs on torch's current stream of the logits'
+    device unless `stream` names another.  Returns (tokens [rows] int32,
+    log-probabilities [rows] fp32)."""
     lib = load()
     rows, vocab = logits.shape
     if vocab > 1 and logits.stride(1) != 1:
@@ -580,6 +581,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     import torch
     if not logits.is_cuda:
         raise ValueError("logits must be on a GPU")
+    if stream is None:
+        stream = torch.cuda.current_stream(logits.device).cuda_stream
     if out_tok is None or out_logp is None:
         out_tok = torch.empty(rows, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
         out_logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
