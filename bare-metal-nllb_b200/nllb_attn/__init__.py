@@ -567,6 +567,14 @@ def logsoftmax_topk(logits, k=8, vocab=None, stream=None):
     return tok, lp
 
 
+def current_stream(device: int = 0) -> int:
+    """Handle of torch's current stream of a GPU, as Context.set_stream and the
+    stream arguments take it: the legacy default stream, which torch calls 0,
+    is CUDA's handle 1."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device) or 1
+
+
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_tok=None, out_logp=None,
            stream=None):
     """nllb_sample on torch CUDA tensors: logits [rows][vocab] (rows may be
@@ -582,7 +590,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     if not logits.is_cuda:
         raise ValueError("logits must be on a GPU")
     if stream is None:
-        stream = torch.cuda.current_stream(logits.device).cuda_stream
+        stream = current_stream(logits.device.index)
     if out_tok is None or out_logp is None:
         out_tok = torch.empty(rows, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
         out_logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
