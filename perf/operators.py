@@ -25,17 +25,25 @@ _state = {}
 
 
 def _library():
-    """The binding, and one context for the process that works on torch's current stream."""
     if "na" not in _state:
         pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bare-metal-nllb_b200")
         if pkg not in sys.path:
             sys.path.insert(0, pkg)
         import nllb_attn
         _state["na"] = nllb_attn
-        _state["ctx"] = nllb_attn.Context(torch.cuda.current_device(), n_layers=0, max_sentences=0)
-        # 1 is CUDA's handle of the legacy default stream, which torch calls 0
-        _state["ctx"].set_stream(torch.cuda.current_stream().cuda_stream or 1)
-    return _state["na"], _state["ctx"]
+    return _state["na"]
+
+
+def _context(device):
+    """The context of a GPU, on torch's current stream there."""
+    na = _library()
+    if device not in _state:
+        _state[device] = [na.Context(device, n_layers=0, max_sentences=0), None]
+    held, stream = _state[device], na.current_stream(device)
+    if held[1] != stream:
+        held[0].set_stream(stream)
+        held[1] = stream
+    return held[0]
 
 
 # ---- cases ---------------------------------------------------------------------------------------------------
@@ -164,7 +172,7 @@ def prepare(case, seed):
     def ints(v):
         return torch.tensor(v, dtype=torch.int32, device=dev)
 
-    s = dict(case=case)
+    s = dict(case=case, device=dev.index)
     if case["op"] == "sample":
         rows, vocab = case["rows"], case["vocab"]
         ld = -(-vocab // 8) * 8  # rows start on 16 bytes, as the engine's logits do
@@ -218,7 +226,7 @@ def prepare(case, seed):
         if case["mask"]:
             s["mask"] = (torch.rand((keys,), device=dev, generator=gen) >= case["mask"]).to(torch.uint8)
     if own:
-        _, ctx = _library()
+        ctx = _context(dev.index)
         s["out"] = torch.empty_like(s["q"])
         if case["op"] == "paged":
             s["args"] = ctx.paged_args(s["q"], s["k_pages"], s["v_pages"], s["table"], s["kv_len"], s["out"],
@@ -237,15 +245,14 @@ def prepare(case, seed):
 def run(s):
     op = s["case"]["op"]
     if own:
-        na, ctx = _library()
         if op == "paged":
-            ctx.paged(s["args"])
+            _context(s["device"]).paged(s["args"])
             return {"out": s["out"], "k_pages": s["k_pages"], "v_pages": s["v_pages"]}
         if op == "cross":
-            ctx.cross_rows(s["args"])
+            _context(s["device"]).cross_rows(s["args"])
             return {"out": s["out"]}
-        na.sample(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
-                  min_p=s["min_p"], out_tok=s["tokens"], out_logp=s["logp"])
+        _library().sample(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"], top_p=s["top_p"],
+                          min_p=s["min_p"], out_tok=s["tokens"], out_logp=s["logp"])
         return {"tokens": s["tokens"], "logp": s["logp"]}
     return {"paged": _paged, "cross": _cross, "sample": _sample}[op](s)
 
