@@ -72,6 +72,7 @@ struct Args {
     const float* u;
     int* out_tok;
     float* out_logp;
+    bool expire;  // test: a wait of each row's last CTA runs out
 };
 
 struct Shared {
@@ -94,6 +95,7 @@ struct Shared {
     uint32_t coarse_of[kThreads / 64][64];
     uint32_t listed;           // (rank 0) candidates gathered
     uint64_t loaded;           // barrier of the copy of the slice
+    uint64_t never;            // test: a barrier that nothing arrives at
     int failed;
     int first_best;            // this CTA's lowest index of the largest logit
 };
@@ -357,6 +359,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
             sh.failed = 1;
             (void)mbar_wait_bounded(&sh.loaded, 0);  // the copy may still be on its way
         }
+        if (a.expire && rank == C - 1) {
+            if (tid == 0) {
+                mbar_init(&sh.never, 1);
+                fence_barrier_init();
+            }
+            __syncthreads();
+            if (!mbar_wait_bounded(&sh.never, 0, kTestWaitBudgetCycles)) sh.failed = 1;
+        }
         __syncthreads();
         best = row_max<T>(data, n_chunks * 32);
         if (best != best) {  // a NaN is among them
@@ -401,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     const bool usable = !failed && m > -INFINITY && temp >= 0.0f && temp < INFINITY;
     if (!usable) {  // (uniform over the cluster)
         if (rank == 0 && tid == 0) {
-            a.out_tok[row] = -1;
+            a.out_tok[row] = failed ? NLLB_SAMPLE_TIMEOUT : -1;
             if (a.out_logp) a.out_logp[row] = -INFINITY;
         }
         cluster_sync_all();
@@ -1121,8 +1131,15 @@ cudaError_t launch(Args a, int rows, int num_sms, cudaStream_t st) {
 
 int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
 
+thread_local bool t_expire_next = false;
+
 }  // namespace
 }  // namespace nllb
+
+extern "C" int nllb_sample_test_expire_next_wait(void) {
+    nllb::t_expire_next = true;
+    return NLLB_ATTN_OK;
+}
 
 extern "C" int nllb_sample(const nllb_sample_args* s, void* stream) {
     using namespace nllb;
@@ -1141,6 +1158,8 @@ extern "C" int nllb_sample(const nllb_sample_args* s, void* stream) {
     a.logits = s->logits, a.ld = s->ld, a.vocab = s->vocab;
     a.temperature = s->temperature, a.top_k = s->top_k, a.top_p = s->top_p, a.min_p = s->min_p, a.u = s->u;
     a.out_tok = s->out_tok, a.out_logp = s->out_logp;
+    a.expire = t_expire_next;
+    t_expire_next = false;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int device = 0, num_sms = 0;
     cudaError_t e = cudaGetDevice(&device);

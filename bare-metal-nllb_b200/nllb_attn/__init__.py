@@ -56,6 +56,7 @@ class KernelProfile(ctypes.Structure):
 
 
 F32, F16, BF16 = range(3)
+SAMPLE_TIMEOUT = -2
 
 
 class PagedArgs(ctypes.Structure):
@@ -142,6 +143,7 @@ SIGNATURES = {
     "nllb_logsoftmax_topk_ws_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
     "nllb_logsoftmax_topk": (_c_int, [_fp, ctypes.c_longlong, _c_int, _c_int, _c_int, _fp, _fp, _fp, _c_void_p]),
     "nllb_sample": (_c_int, [ctypes.POINTER(SampleArgs), _c_void_p]),
+    "nllb_sample_test_expire_next_wait": (_c_int, []),
 }
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -606,6 +608,13 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     else:
         _check(lib, lib.nllb_sample(ctypes.byref(a), stream), "nllb_sample")
     return out_tok, out_logp
+
+
+def sample_test_expire_next_wait() -> None:
+    """nllb_sample_test_expire_next_wait: a bounded wait of every row of this
+    thread's next sample runs out (tokens SAMPLE_TIMEOUT)."""
+    lib = load()
+    _check(lib, lib.nllb_sample_test_expire_next_wait(), "sample_test_expire_next_wait")
 
 
 class PreparedLinear:

@@ -216,13 +216,15 @@ NLLB_ATTN_API int nllb_logsoftmax_topk(const float* logits, long long ld, int vo
  * nothing, u is clamped into [0, 1) and NaN counts as 0.  A NaN logit counts
  * as -inf; logits of +inf share all the weight.  A row with no logit above
  * -inf, or with a temperature that is negative, infinite or NaN, gives token
- * -1 and logp -inf (so does a row whose bounded device wait gave up).
+ * -1 and logp -inf; a row whose bounded device wait gave up gives token
+ * NLLB_SAMPLE_TIMEOUT and logp -inf.
  * Weights are summed as integer multiples of 2^-44, so a result does not
  * depend on the order of the additions.  Device pointers; asynchronous on
  * `stream` (a cudaStream_t, NULL = default); nothing is allocated, the logits
  * are not modified.  At most NLLB_SAMPLE_MAX_VOCAB entries a row (more:
  * NLLB_ATTN_ECAPACITY). */
 #define NLLB_SAMPLE_MAX_VOCAB 524288
+#define NLLB_SAMPLE_TIMEOUT (-2)
 typedef struct {
     const void*  logits;
     long long    ld;
@@ -236,6 +238,12 @@ typedef struct {
     float*       out_logp;
 } nllb_sample_args;
 NLLB_ATTN_API int nllb_sample(const nllb_sample_args* args, void* stream);
+
+/* Test of the bounded device waits: in the calling thread's next nllb_sample,
+ * if it copies its rows to shared memory (it does below 64 MB of logits), a
+ * wait of every row runs out after about 1 ms, and every token is
+ * NLLB_SAMPLE_TIMEOUT.  Later calls are as ever. */
+NLLB_ATTN_API int nllb_sample_test_expire_next_wait(void);
 
 #ifdef __cplusplus
 }
