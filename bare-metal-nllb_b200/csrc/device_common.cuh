@@ -87,6 +87,14 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     return true;
 }
 
+// A coherent load.  A launch that may start before its predecessor has ended (programmatic dependent launch) must not read
+// what that one writes through the read-only path: such a load asks for data that nobody writes while the kernel lives, and
+// the compiler may move it above the wait for the predecessor.
+template <typename T>
+__device__ __forceinline__ T ld_coherent(const T* p) {
+    return *p;
+}
+
 __device__ __forceinline__ float4 f4_scale(float4 a, float s) {
     return make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
 }

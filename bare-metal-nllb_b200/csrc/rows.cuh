@@ -18,15 +18,15 @@ struct RowsSeq {
 
 template <bool PAGED>
 __device__ __forceinline__ bool rows_sequence(const RowsParams& p, int s, RowsSeq& q) {
-    q.q0 = p.q_start ? __ldg(p.q_start + s) : s * p.max_q;
-    q.qn = p.q_len ? __ldg(p.q_len + s) : p.max_q;
-    q.kvn = __ldg(p.kv_len + s);
+    q.q0 = p.q_start ? ld_coherent(p.q_start + s) : s * p.max_q;
+    q.qn = p.q_len ? ld_coherent(p.q_len + s) : p.max_q;
+    q.kvn = ld_coherent(p.kv_len + s);
     q.kv0 = 0;
     bool ok = q.q0 >= 0 && q.qn >= 0 && q.qn <= p.max_q && q.q0 <= p.q_rows - q.qn && q.kvn >= 0 && q.kvn <= p.max_kv;
     if (PAGED) {
         ok = ok && q.kvn >= q.qn;
     } else {
-        q.kv0 = p.kv_start ? __ldg(p.kv_start + s) : s * p.max_kv;
+        q.kv0 = p.kv_start ? ld_coherent(p.kv_start + s) : s * p.max_kv;
         ok = ok && q.kv0 >= 0 && q.kv0 <= p.kv_rows - q.kvn;
     }
     if (!ok && threadIdx.x == 0) atomicOr(p.err, NLLB_DEV_ERR_BAD_LENGTH);
@@ -51,9 +51,9 @@ template <bool PAGED>
 __device__ __forceinline__ int rows_entry(const RowsParams& p, const RowsSeq& q, int s, int j) {
     if (PAGED) {
         if (p.k_new && j >= q.kvn - q.qn) return 0;
-        return __ldg(p.table + (long long)s * p.table_ld + rows_page(p, j));
+        return ld_coherent(p.table + (long long)s * p.table_ld + rows_page(p, j));
     }
-    return p.mask ? __ldg(p.mask + q.kv0 + j) : 1;
+    return p.mask ? ld_coherent(p.mask + q.kv0 + j) : 1;
 }
 
 // Where key `j` lies, for K and for V.  False: its page number is outside the
@@ -98,15 +98,15 @@ __device__ __forceinline__ void rows_append(const RowsParams& p, const RowsSeq& 
     constexpr int CH = D * (int)sizeof(T) / 16;
     for (int i = tid; i < (t1 - t0) * CH; i += n_threads) {
         const int t = t0 + i / CH, c = i % CH, j = q.kvn - q.qn + t;
-        const int at = rows_page(p, j), pg = __ldg(p.table + (long long)s * p.table_ld + at);
+        const int at = rows_page(p, j), pg = ld_coherent(p.table + (long long)s * p.table_ld + at);
         if ((unsigned)pg >= (unsigned)p.n_pages) {
             atomicOr(p.err, NLLB_DEV_ERR_BAD_PAGE);
             continue;
         }
         const long long r = q.q0 + t, slot = j - at * p.page;
-        const uint4 kv = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + r * p.kn_row +
+        const uint4 kv = ld_coherent(reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_new) + r * p.kn_row +
                                                                (long long)g * p.kn_head) + c);
-        const uint4 vv = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + r * p.vn_row +
+        const uint4 vv = ld_coherent(reinterpret_cast<const uint4*>(static_cast<const T*>(p.v_new) + r * p.vn_row +
                                                                (long long)g * p.vn_head) + c);
         reinterpret_cast<uint4*>(static_cast<T*>(p.k_w) + pg * p.k_page + slot * p.k_row + (long long)g * p.k_head)[c] = kv;
         reinterpret_cast<uint4*>(static_cast<T*>(p.v_w) + pg * p.v_page + slot * p.v_row + (long long)g * p.v_head)[c] = vv;

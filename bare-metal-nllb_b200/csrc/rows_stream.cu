@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
             const T* src = there ? q_at(lr + 8 * h) : nullptr;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                qf[k][h] = there ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 2 * lc)) : 0u;
-                qf[k][h + 2] = there ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * lc)) : 0u;
+                qf[k][h] = there ? ld_coherent(reinterpret_cast<const uint32_t*>(src + k * 16 + 2 * lc)) : 0u;
+                qf[k][h + 2] = there ? ld_coherent(reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * lc)) : 0u;
             }
         }
         const int lim[2] = {sees(lr), HALVES == 2 ? sees(lr + 8) : 0};
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
 #pragma unroll
             for (int i = 0; i < VEC; ++i) q[r][i] = acc[r][i] = 0.f;
             if (row0 + r < rows) {
-                rows_unpack<T>(__ldg(reinterpret_cast<const uint4*>(q_at(r)) + c), q[r]);
+                rows_unpack<T>(ld_coherent(reinterpret_cast<const uint4*>(q_at(r)) + c), q[r]);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) q[r][i] *= p.scale_log2;
             }

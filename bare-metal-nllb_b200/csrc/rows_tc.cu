@@ -436,6 +436,14 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         if (n > 0) {
             constexpr int CH = D / 8, N = C::WPT * 32, TAKE = kTile * CH / N < 8 ? kTile * CH / N : 8;
             const int lt = tid - t * N;
+            int entry[C::FIRST ? TAKE : 1];  // (fp32) of the first tile's keys, asked for ahead of their use
+            if constexpr (C::FIRST) {
+#pragma unroll
+                for (int i = 0; i < TAKE; ++i) {
+                    const int key = j0 * kTile + (lt + i * N) / CH;
+                    entry[i] = key < longest ? rows_entry<PAGED>(p, sq, s, key) : 0;
+                }
+            }
 #pragma unroll
             for (int i0 = 0; i0 < kTile * CH / N; i0 += TAKE) {
                 const T* src[TAKE];
@@ -449,8 +457,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                     if constexpr (C::F32) {
                         a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (src[i]) {
-                            a[i] = __ldg(reinterpret_cast<const float4*>(src[i]));
-                            b[i] = __ldg(reinterpret_cast<const float4*>(src[i]) + 1);
+                            a[i] = ld_coherent(reinterpret_cast<const float4*>(src[i]));
+                            b[i] = ld_coherent(reinterpret_cast<const float4*>(src[i]) + 1);
                         }
                     }
                 }
@@ -475,7 +483,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
 #pragma unroll
                 for (int i = 0; i < TAKE; ++i) {
                     const int r = (lt + i * N) / CH, key = j0 * kTile + r;
-                    if (!(key < longest && rows_key<T, PAGED>(p, sq, s, g, key, k[i], v[i]))) k[i] = v[i] = nullptr;
+                    if (!(key < longest && rows_at<T, PAGED>(p, sq, g, key, entry[i], k[i], v[i]))) k[i] = v[i] = nullptr;
                 }
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
@@ -485,7 +493,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                         const int c = (lt + i * N) % CH;
                         const float4* src = reinterpret_cast<const float4*>(kv ? v[i] : k[i]);
                         a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (src) a[i] = __ldg(src + 2 * c), b[i] = __ldg(src + 2 * c + 1);
+                        if (src) a[i] = ld_coherent(src + 2 * c), b[i] = ld_coherent(src + 2 * c + 1);
                     }
                     if (kv == 0) {
                         const float div = divide(a, b);
@@ -778,8 +786,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                             for (int c = 0; c < CH / 2; ++c) {
                                 a[c] = b[c] = make_float4(0.f, 0.f, 0.f, 0.f);
                                 if (src) {
-                                    a[c] = __ldg(src + 2 * (2 * c + (lt & 1)));
-                                    b[c] = __ldg(src + 2 * (2 * c + (lt & 1)) + 1);
+                                    a[c] = ld_coherent(src + 2 * (2 * c + (lt & 1)));
+                                    b[c] = ld_coherent(src + 2 * (2 * c + (lt & 1)) + 1);
                                 }
                             }
                             if (kv == 0) {

@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     auto fetch = [&](int i) -> Vec<T> {
         Vec<T> v;
         if ((i + 1) * VEC <= n) {
-            *reinterpret_cast<uint4*>(&v) = __ldg(reinterpret_cast<const uint4*>(src) + i);
+            *reinterpret_cast<uint4*>(&v) = ld_coherent(reinterpret_cast<const uint4*>(src) + i);
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v.x[e] = i * VEC + e < n ? src[i * VEC + e] : minus_inf<T>();
@@ -402,11 +402,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
     }
 
     // ---- the row's settings
-    float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
-    const int k = a.top_k ? __ldg(a.top_k + row) : 0;
-    const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
-    const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
-    float u = __ldg(a.u + row);
+    float temp = a.temperature ? ld_coherent(a.temperature + row) : 1.0f;
+    const int k = a.top_k ? ld_coherent(a.top_k + row) : 0;
+    const float top_p = a.top_p ? ld_coherent(a.top_p + row) : 1.0f;
+    const float min_p = a.min_p ? ld_coherent(a.min_p + row) : 0.0f;
+    float u = ld_coherent(a.u + row);
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;  // (NaN too)
     const bool usable = !failed && m > -INFINITY && temp >= 0.0f && temp < INFINITY;
     if (!usable) {  // (uniform over the cluster)
