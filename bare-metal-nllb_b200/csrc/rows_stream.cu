@@ -29,6 +29,7 @@
 // keys 4.5 us, latency; one token over 99990 keys with two key heads 31 us,
 // bound by the 32 CTAs that two clusters of 16 make.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -43,6 +44,7 @@ constexpr int kRing = 2;      // key blocks in a warp's ring
 // 106 us, 6 x 2 113, 5 x 2 148, 4 x 3 145; one over 99990 keys, 8 rows of 64: 14 x 2 blocks of 8 KB 31.5 us, 12 x 2
 // 36.2, 8 x 3 37.6, 6 x 4 48.1).
 constexpr int kWarps8 = 14, kWarps16 = 7;
+constexpr int kWarpKeys = 32768;
 constexpr float kWeightExp = 7.0f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
@@ -481,8 +483,11 @@ cudaError_t launch_by_units(const RowsParams& p, int num_sms, cudaStream_t st) {
     // cluster at most.
     if (units >= 8LL * num_sms && p.max_kv <= 1024) return launch_one<T, D, R, PAGED, 1>(p, 1, st);
     constexpr int MANY = Cfg<T, D, R, 0>::MANY, step = MANY * Cfg<T, D, R, 0>::BLK;
+    // The matrix products' sums lose up to a step of fp32 with every 16 keys, so a warp of them takes 32768 at most.
+    const int most = Cfg<T, D, R, 0>::MMA ? MANY * kWarpKeys : INT_MAX;
     int n_split = 1;
-    while (n_split < 16 && units * n_split < 2LL * num_sms && p.max_kv > step * n_split) n_split *= 2;
+    while (n_split < 16 && ((units * n_split < 2LL * num_sms && p.max_kv > step * n_split) || p.max_kv / n_split > most))
+        n_split *= 2;
     return launch_one<T, D, R, PAGED, MANY>(p, n_split, st);
 }
 
@@ -550,9 +555,12 @@ cudaError_t configure_rows_kernels() {
 }
 
 cudaError_t launch_rows(const RowsParams& p, RowType type, int head_dim, bool paged, int num_sms, cudaStream_t st) {
-    // more rows than one CTA of this kernel takes would read the keys again
+    // more rows than one CTA of this kernel takes would read the keys again; and keys that a cluster of the fewest warps
+    // cannot share (kWarpKeys)
     const long long rows = (long long)p.max_q * p.group;
-    if (rows > (type == RowType::f32 ? 8 : kRowsMax)) return launch_rows_tc(p, type, head_dim, paged, num_sms, st);
+    if (rows > (type == RowType::f32 ? 8 : kRowsMax) ||
+        (type != RowType::f32 && rows > 1 && p.max_kv > 16 * kWarps16 * kWarpKeys))
+        return launch_rows_tc(p, type, head_dim, paged, num_sms, st);
     switch (type) {
         case RowType::f32: return launch_by_dim<float>(p, head_dim, paged, num_sms, st);
         case RowType::f16: return launch_by_dim<__half>(p, head_dim, paged, num_sms, st);

@@ -23,7 +23,13 @@
 //
 // Types: 16-bit inputs are the operands as they come, the weights are rounded
 // to the type (half a step each, unbiased; the sum that divides them stays
-// fp32).  fp32 inputs and weights are split into two fp16 parts, hi + lo, and
+// fp32).  The tensor cores cut what they add to a sum: n keys lose up to n/16
+// steps of fp32, n 2^-27 of an output (measured 6.4e-9 n).  Up to 32768 keys
+// that is half of what fp16 rounds an output by, and a CTA's tiles are added
+// there.  Calls of more keys move the sums of 16 tiles on to a total that the
+// softmax threads add to, and fp32 ones every tile (1024 rows of 32 heads over
+// 100000 keys: heads of 64 2.04 ms, 1.86 without; of 128, where two tiles leave
+// no room for the total, 2.87 and 2.40).  fp32 inputs and weights are split into two fp16 parts, hi + lo, and
 // a product is taken as hi hi' + hi lo' + lo hi' (22 bits, and an absolute
 // 2^-25 where lo leaves fp16's normal range).  So that this holds at any size,
 // rows whose largest size lies outside [2^-3, 65504) are divided by a power of
@@ -52,11 +58,13 @@ namespace {
 
 constexpr int kTile = 128;              // query rows of a tile, keys of a tile
 constexpr int kLoaders = 96;            // fetching threads: 8 or 12 warps in all, so registers divide evenly
+constexpr int kLongKeys = 32768;        // of 16 bits: from there on a CTA's tiles are added outside the tensor cores
+constexpr int kTilesTogether = 16;       // there: tiles that the tensor cores add
 constexpr float kGrow = 8.0f;           // a maximum may lag by 2^8
 constexpr float kWeightExp = 7.0f;      // weights are held times 2^7
 constexpr uint32_t kBlock = 128 * 128;  // bytes of [128 rows][64 16-bit elements]
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, bool LONG>
 struct Cfg {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int PARTS = F32 ? 2 : 1;
@@ -64,7 +72,7 @@ struct Cfg {
     static constexpr uint32_t PART = kBlock * KB;     // one part of a [128][D] operand
     static constexpr uint32_t OPER = PART * PARTS;
     // key tiles in flight: what leaves room for two CTAs per SM with one query tile, or fills the SM with two
-    static constexpr int ST = F32 ? 1 : (NQ == 2 ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1));
+    static constexpr int ST = F32 ? 1 : (NQ == 2 ? (D == 64 ? 4 : 2) : (D == 64 || LONG ? 2 : 1));
     // Softmax warps of a query tile; with 8, two threads share a row.  Two tiles: 4 (long chunks 343 us, with 8 355);
     // one, where the time to the first result counts: 8 (64 prefixes 70 us, with 4 88).
     static constexpr int WPT = NQ == 2 ? 4 : 8, SOFT = NQ * WPT * 32;  // and softmax threads in all
@@ -79,10 +87,10 @@ struct Cfg {
     static constexpr uint32_t ODD = (TOPS + (F32 ? (8 + 2 * kLoaders / 32) * 4 : 0) + 7) / 8 * 8;  // queries, V's first, K tiles
     static constexpr uint32_t BARS = ODD + (F32 ? (WORDS + 3) * 8 : 0);
     // P beside S in tensor memory, where there is room: the next scores can then be taken as soon as a row is read
-    static constexpr bool AHEAD = NQ == 2 && D == 64;
-    // fp32: the outputs' sum over the tiles.  The tensor cores cut what they accumulate, so a sum over many tiles would
-    // drift (20000 keys: an error of 1e-5); they sum one tile, the softmax threads add the tiles.
-    static constexpr bool TOTAL = F32;
+    static constexpr bool AHEAD = NQ == 2 && D == 64 && !LONG;
+    // fp32, and 16 bits over many keys: the outputs' total.  The tensor cores cut what they accumulate, so a sum over many
+    // tiles would drift; they sum one tile, or kTilesTogether, and the softmax threads add those.
+    static constexpr bool TOTAL = F32 || LONG;
     static constexpr uint32_t O_COL = NQ * 128, P_COL = O_COL + NQ * D, T_COL = P_COL;
     // fp32: the softmax threads also fetch the first key tile, with all of its loads in flight at once
     static constexpr bool FIRST = F32;  // (one slot: the first tile's phase is simply not counted)
@@ -90,10 +98,11 @@ struct Cfg {
     static constexpr uint32_t SLOT = BARS + N_BARS * 8, BYTES = SLOT + 16;
     static constexpr uint32_t SMEM = BYTES + 1024;  // + alignment slack
     static constexpr int THREADS = SOFT + kLoaders + 32;
-    static constexpr uint32_t TMEM = NQ == 2 || (F32 && D == 128) ? 512 : 256;  // S: 128 columns per tile, O: D per tile
-    static constexpr int CTAS = NQ == 2 || (F32 && D == 128) ? 1 : 2;
+    static constexpr uint32_t TMEM = NQ == 2 || (TOTAL && D == 128) ? 512 : 256;  // S: 128 columns per tile, O: D per tile
+    static constexpr int CTAS = NQ == 2 || (TOTAL && D == 128) ? 1 : 2;
     static constexpr int LD = D + 4;  // fp32 row of a split's state: D sums, then m, l
-    static_assert(NQ * 128 + NQ * D + (AHEAD ? NQ * 64 : 0) + (TOTAL ? D : 0) <= (int)TMEM, "tensor memory");
+    static_assert(NQ * 128 + NQ * D + (AHEAD ? NQ * 64 : 0) + (TOTAL ? NQ * D : 0) <= (int)TMEM, "tensor memory");
+    static_assert(!(F32 && LONG), "fp32 adds every tile");
     static_assert(128 * LD * 4 <= (int)SAUX || NQ == 2, "a split's state fits over the operands");
 };
 
@@ -292,10 +301,10 @@ __device__ __forceinline__ float divide(float4 (&a)[N], float4 (&b)[N]) {
 }
 __device__ __forceinline__ void loaders_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory"); }
 
-template <typename T, int D, int NQ, bool PAGED>
-__global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
+template <typename T, int D, int NQ, bool PAGED, bool LONG>
+__global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LONG>::CTAS)
     rows_tc_kernel(const RowsParams p, int n_split) {
-    using C = Cfg<T, D, NQ>;
+    using C = Cfg<T, D, NQ, LONG>;
     constexpr int ST = C::ST;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -418,7 +427,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         const int lim = there ? (PAGED ? sq.kvn - sq.qn + tok + 1 : sq.kvn) : 0;
         const uint32_t lane_off = (uint32_t)(lq * 32) << 16;
         const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + C::O_COL + (uint32_t)t * D;
-        const uint32_t tT = tmem + lane_off + C::T_COL;  // (TOTAL) the tiles before the last
+        const uint32_t tT = tmem + lane_off + C::T_COL + (uint32_t)t * D;  // (TOTAL) the tiles before those in O
         // the weights of 32 keys: 16 columns (and fp32's low parts in the next 16)
         auto p_at = [&](int c) { return C::AHEAD ? tmem + lane_off + C::P_COL + t * 64 + 16 * c : tS + 32 * c; };
         // x of this thread's row and y of the other thread's, whichever way round: the step'th exchange of the pair
@@ -578,7 +587,32 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 if (C::AHEAD) tc_fence_after();
                 const float mn = mx * sl;
                 const bool grown = !(mn <= m + kGrow);  // a NaN makes the whole row NaN
-                if constexpr (C::TOTAL) {
+                if constexpr (LONG) {
+                    const bool full = j % kTilesTogether == 0;  // the sums in O move on to the total
+                    if (j > 0 && (full || __any_sync(0xffffffffu, grown))) {
+                        const float to = grown ? max_nan(m, mn) : m;
+                        const float corr = m == to ? 1.f : m == -INFINITY ? 0.f : ex2_approx(m - to);
+                        m = to;
+                        l *= corr;
+#pragma unroll
+                        for (int c = half * (D / 2); c < (C::WPT == 8 ? (half + 1) * (D / 2) : D); c += 8) {
+                            uint32_t o[8], x[8];
+                            tmem_ld8(tO + c, o);
+                            if (j > kTilesTogether) tmem_ld8(tT + c, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float y = __uint_as_float(o[i]), z = j > kTilesTogether ? __uint_as_float(x[i]) : 0.f;
+                                o[i] = __float_as_uint(y * corr);
+                                x[i] = __float_as_uint((full ? y + z : z) * corr);
+                            }
+                            if (!full) tmem_st8(tO + c, o);
+                            if (full || j > kTilesTogether) tmem_st8(tT + c, x);
+                        }
+                    } else if (j == 0 && grown) {
+                        m = max_nan(m, mn);
+                    }
+                } else if constexpr (C::TOTAL) {
                     const float to = grown ? max_nan(m, mn) : m;
                     const float corr = m == to ? 1.f : m == -INFINITY ? 0.f : ex2_approx(m - to);
                     m = to;
@@ -653,12 +687,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
         auto last_output = [&](int c, float* o) {
             tmem_ld32(tO + c, o);
             if constexpr (C::TOTAL) {
-                const float vd = v_div[place(n - 1)];
+                const float vd = C::F32 ? v_div[place(n - 1)] : 1.0f;
+                constexpr int before = LONG ? kTilesTogether : 1;  // tiles that the total may be behind O
                 if (vd != 1.0f) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] *= vd;
                 }
-                if (n > 1) {
+                if (n > before) {
                     float x[32];
                     tmem_ld32(tT + c, x);
 #pragma unroll
@@ -923,7 +958,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
                 }
                 if (!(ok = wait(p_full + t, j & 1))) break;
                 tc_fence_after();
-                output(t, st, j > 0);
+                output(t, st, LONG ? j % kTilesTogether != 0 : j > 0 && !C::TOTAL);
                 if constexpr (!C::AHEAD) ok = next(t);  // P lies over S
             }
         }
@@ -981,9 +1016,9 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ>::THREADS, Cfg<T, D, NQ>::CTAS)
     }
 }
 
-template <typename T, int D, int NQ, bool PAGED>
+template <typename T, int D, int NQ, bool PAGED, bool LONG>
 cudaError_t launch_tc(const RowsParams& p, int n_split, cudaStream_t st) {
-    using C = Cfg<T, D, NQ>;
+    using C = Cfg<T, D, NQ, LONG>;
     const long long tiles = ((long long)p.max_q * p.group + NQ * kTile - 1) / (NQ * kTile);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * n_split), (unsigned)p.kv_heads, (unsigned)p.n_seq);
@@ -998,16 +1033,20 @@ cudaError_t launch_tc(const RowsParams& p, int n_split, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = n_split > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, rows_tc_kernel<T, D, NQ, PAGED>, p, n_split);
+    return cudaLaunchKernelEx(&cfg, rows_tc_kernel<T, D, NQ, PAGED, LONG>, p, n_split);
 }
 
 template <typename T, int D, bool PAGED>
 cudaError_t launch_by_tiles(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long rows = (long long)p.max_q * p.group, heads = (long long)p.kv_heads * p.n_seq;
+    const bool is_long = sizeof(T) == 2 && p.max_kv > kLongKeys;
     if constexpr (sizeof(T) == 2) {
         // two query tiles per CTA where they still give every SM one
-        if (rows > kTile && (rows + 2 * kTile - 1) / (2 * kTile) * heads >= num_sms)
-            return launch_tc<T, D, 2, PAGED>(p, 1, st);
+        if (rows > kTile && (rows + 2 * kTile - 1) / (2 * kTile) * heads >= num_sms) {
+            if (!is_long) return launch_tc<T, D, 2, PAGED, false>(p, 1, st);
+            // (two tiles of heads of 128 fill the tensor memory)
+            if constexpr (D == 64) return launch_tc<T, D, 2, PAGED, true>(p, 1, st);
+        }
     }
     const long long units = (rows + kTile - 1) / kTile * heads;
     // Splits, while they leave two CTAs or fewer per SM: two from 257 keys on (one sequence of 16 heads, 21 fp32 rows
@@ -1016,7 +1055,10 @@ cudaError_t launch_by_tiles(const RowsParams& p, int num_sms, cudaStream_t st) {
     int n_split = 1;
     while (n_split < 8 && units * n_split * 2 <= 2LL * num_sms && p.max_kv > (n_split == 1 ? 256 : 512 * n_split))
         n_split *= 2;
-    return launch_tc<T, D, 1, PAGED>(p, n_split, st);
+    if constexpr (sizeof(T) == 2) {
+        if (is_long) return launch_tc<T, D, 1, PAGED, true>(p, n_split, st);
+    }
+    return launch_tc<T, D, 1, PAGED, false>(p, n_split, st);
 }
 
 template <typename T>
@@ -1026,13 +1068,13 @@ cudaError_t launch_by_dim(const RowsParams& p, int head_dim, bool paged, int num
     return paged ? launch_by_tiles<T, 128, true>(p, num_sms, st) : launch_by_tiles<T, 128, false>(p, num_sms, st);
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, bool LONG = false>
 cudaError_t configure_one() {
-    cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Cfg<T, D, NQ>::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, true, LONG>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<T, D, NQ, LONG>::SMEM);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)Cfg<T, D, NQ>::SMEM);
+        e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, false, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)Cfg<T, D, NQ, LONG>::SMEM);
     return e;
 }
 
@@ -1043,12 +1085,18 @@ cudaError_t configure_rows_tc() {
     if (e == cudaSuccess) e = configure_one<float, 128, 1>();
     if (e == cudaSuccess) e = configure_one<__half, 64, 1>();
     if (e == cudaSuccess) e = configure_one<__half, 64, 2>();
+    if (e == cudaSuccess) e = configure_one<__half, 64, 1, true>();
+    if (e == cudaSuccess) e = configure_one<__half, 64, 2, true>();
     if (e == cudaSuccess) e = configure_one<__half, 128, 1>();
     if (e == cudaSuccess) e = configure_one<__half, 128, 2>();
+    if (e == cudaSuccess) e = configure_one<__half, 128, 1, true>();
     if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 64, 1>();
     if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 64, 2>();
+    if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 64, 1, true>();
+    if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 64, 2, true>();
     if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 128, 1>();
     if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 128, 2>();
+    if (e == cudaSuccess) e = configure_one<__nv_bfloat16, 128, 1, true>();
     return e;
 }
 
