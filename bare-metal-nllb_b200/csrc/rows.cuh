@@ -133,6 +133,23 @@ __device__ __forceinline__ void rows_unpack(uint4 u, float (&x)[16 / sizeof(T)])
     }
 }
 
+// 16 bytes into shared memory, asynchronously; zeros, without a read, if they are not `there`.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Two fp32 values rounded to a 16-bit type.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
 // fp32 values rounded once to the output's type.
 template <typename T>
 __device__ __forceinline__ uint4 rows_pack(const float (&x)[16 / sizeof(T)]) {

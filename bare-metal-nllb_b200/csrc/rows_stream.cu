@@ -47,9 +47,6 @@ constexpr int kWarps8 = 14, kWarps16 = 7;
 constexpr int kWarpKeys = 32768;
 constexpr float kWeightExp = 7.0f;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
@@ -76,17 +73,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
-
 template <typename T, int D, int R, int NW>
 struct Cfg {
     static constexpr int ROW = D * (int)sizeof(T);      // bytes of a key row

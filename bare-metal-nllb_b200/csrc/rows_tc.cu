@@ -111,9 +111,6 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
     return (uint32_t)((c >> 3) * (int)kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0));
-}
 // Arrives on `bar` (one of its expected arrivals) once this thread's copies so far have landed.  Their writes are
 // plain ones: who waits on the barrier fences before the tensor cores read them.
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
@@ -226,17 +223,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     float c;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
     return c;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
 }
 
 // x rounded to 11 significant bits, exact in fp16's normal range.
