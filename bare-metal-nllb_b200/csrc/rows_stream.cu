@@ -100,21 +100,19 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     pdl_launch_dependents();
     pdl_wait_primary();
 
-    const int split = blockIdx.x % n_split, tile = blockIdx.x / n_split;
+    const int split = blockIdx.x;
     const int g = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int sub = lane / CH, c = lane % CH;
     RowsSeq sq;
-    // (uniform over the cluster: its CTAs share tile, key head and sequence)
+    // (uniform over the cluster: its CTAs share key head and sequence)
     if (!rows_sequence<PAGED>(p, s, sq)) return;
-    const int rows = sq.qn * p.group, row0 = tile * R;
-    if (row0 >= rows) return;
+    const int rows = sq.qn * p.group;  // R at most
+    if (rows == 0) return;
     const int past = sq.kvn - sq.qn;  // (paged) keys before the chunk
 
-    // keys of this CTA: what its last row sees, in blocks, shared among the splits; a warp takes every NW-th
-    const int last_tok = (min(rows, row0 + R) - 1) / p.group;
-    const int longest = PAGED ? past + last_tok + 1 : sq.kvn;
-    const int blocks = (longest + BLK - 1) / BLK, per = (blocks + n_split - 1) / n_split;
+    // the keys in blocks, shared among the splits; a warp takes every NW-th
+    const int blocks = (sq.kvn + BLK - 1) / BLK, per = (blocks + n_split - 1) / n_split;
     const int b_end = min(blocks, (split + 1) * per);
     int b_next = split * per + warp;  // the next block to locate
 
@@ -122,7 +120,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     const T *kp = nullptr, *vp = nullptr;
     auto locate = [&] {  // this lane's row of the next block
         const int key = b_next * BLK + lane;
-        if (!(lane < BLK && b_next < b_end && key < longest && rows_key<T, PAGED>(p, sq, s, g, key, kp, vp)))
+        if (!(lane < BLK && b_next < b_end && key < sq.kvn && rows_key<T, PAGED>(p, sq, s, g, key, kp, vp)))
             kp = vp = nullptr;
         b_next += NW;
     };
@@ -154,20 +152,16 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     }
     locate();
 
-    if (PAGED && p.k_new && split == 0) {
-        // a token belongs to the tile that holds its first row
-        const int t0 = (row0 + p.group - 1) / p.group, t1 = min(sq.qn, (row0 + R + p.group - 1) / p.group);
-        rows_append<T, D>(p, sq, s, g, t0, t1, tid, NW * 32);
-    }
+    if (PAGED && p.k_new && split == 0) rows_append<T, D>(p, sq, s, g, 0, sq.qn, tid, NW * 32);
 
     float* state = reinterpret_cast<float*>(smem) + warp * R * C::LD;
-    auto q_at = [&](int r) {  // query row r of the tile (there)
-        const int t = (row0 + r) / p.group, h = g * p.group + (row0 + r) % p.group;
+    auto q_at = [&](int r) {  // query row r (there)
+        const int t = r / p.group, h = g * p.group + r % p.group;
         return static_cast<const T*>(p.q) + (long long)(sq.q0 + t) * p.q_row + (long long)h * p.q_head;
     };
     auto sees = [&](int r) {  // keys query row r sees
-        if (row0 + r >= rows) return 0;
-        return PAGED ? past + (row0 + r) / p.group + 1 : sq.kvn;
+        if (r >= rows) return 0;
+        return PAGED ? past + r / p.group + 1 : sq.kvn;
     };
     // body(block index, its visible keys, its K in the ring) for every block of the warp
     auto run = [&](auto&& body) {
@@ -195,7 +189,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
         uint32_t qf[D / 16][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const bool there = h < HALVES && row0 + lr + 8 * h < rows;
+            const bool there = h < HALVES && lr + 8 * h < rows;
             const T* src = there ? q_at(lr + 8 * h) : nullptr;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
@@ -293,7 +287,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
             lim[r] = sees(r);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) q[r][i] = acc[r][i] = 0.f;
-            if (row0 + r < rows) {
+            if (r < rows) {
                 rows_unpack<T>(ld_coherent(reinterpret_cast<const uint4*>(q_at(r)) + c), q[r]);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) q[r][i] *= p.scale_log2;
@@ -406,8 +400,8 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     // join the splits (rank by rank, so the order is fixed): rank z finishes
     // the 16-byte pieces z, z + n_split, ...
     for (int i = split + n_split * tid; i < R * CH; i += n_split * NW * 32) {
-        const int r = i / CH, cc = i % CH, row = row0 + r;
-        if (row >= rows) continue;
+        const int r = i / CH, cc = i % CH;
+        if (r >= rows) continue;
         const float* st = part + r * C::LD;
         float x[VEC], sum = 0.f;
         if (n_split == 1) {
@@ -434,7 +428,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
         const float inv = 1.f / sum;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) x[e] = sum == 0.f ? 0.f : x[e] * inv;  // no visible key: zeros
-        const int t = row / p.group, h = g * p.group + row % p.group;
+        const int t = r / p.group, h = g * p.group + r % p.group;
         T* dst = static_cast<T*>(p.out) + (long long)(sq.q0 + t) * p.o_row + (long long)h * p.o_head;
         reinterpret_cast<uint4*>(dst)[cc] = rows_pack<T>(x);
     }
@@ -443,9 +437,8 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
 
 template <typename T, int D, int R, bool PAGED, int NW>
 cudaError_t launch_one(const RowsParams& p, int n_split, cudaStream_t st) {
-    const long long tiles = ((long long)p.max_q * p.group + R - 1) / R;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * n_split), (unsigned)p.kv_heads, (unsigned)p.n_seq);
+    cfg.gridDim = dim3((unsigned)n_split, (unsigned)p.kv_heads, (unsigned)p.n_seq);
     cfg.blockDim = dim3(NW * 32, 1, 1);
     cfg.dynamicSmemBytes = Cfg<T, D, R, NW>::SMEM;
     cfg.stream = st;
@@ -462,7 +455,7 @@ cudaError_t launch_one(const RowsParams& p, int n_split, cudaStream_t st) {
 
 template <typename T, int D, int R, bool PAGED>
 cudaError_t launch_by_units(const RowsParams& p, int num_sms, cudaStream_t st) {
-    const long long units = ((long long)p.max_q * p.group + R - 1) / R * p.kv_heads * p.n_seq;
+    const long long units = (long long)p.kv_heads * p.n_seq;
     // A warp alone per unit where that already fills the SMs and the keys are few (256 sequences of 16 heads over
     // 18..512 keys: 56 us, with four warps 75); else many warps, and as many splits as give every SM work (four CTAs
     // per SM instead of two cost 134 us against 113 over 200..8191 keys), none with less than a block per warp, one
