@@ -32,10 +32,10 @@
 // no room for the total, 2.87 and 2.40).  fp32 inputs and weights are split into two fp16 parts, hi + lo, and
 // a product is taken as hi hi' + hi lo' + lo hi' (22 bits, and an absolute
 // 2^-25 where lo leaves fp16's normal range).  So that this holds at any size,
-// rows whose largest size lies outside [2^-3, 65504) are divided by a power of
-// two first: queries and keys 16 rows alike, which a warp settles for itself
-// and the scores undo; values a tile alike, which the sum over the tiles
-// undoes.  (Ordinary sizes pay for the look: 64 prefixes 71 us instead of 67,
+// rows are divided by powers of two first where the largest size lies outside
+// [2^-3, 65504): of 16 query or key rows, which a warp settles for itself, each
+// row by its own size, and the scores undo it; of a tile of values, alike,
+// which the sum over the tiles undoes.  (Ordinary sizes pay for the look: 64 prefixes 71 us instead of 67,
 // 128 scored sentences 96 instead of 91.)  Weights are held times 2^7, so
 // fp16 keeps them normal down to 2^-21 of the largest while 2^7 * 2^8 stays in
 // its range.
@@ -271,19 +271,28 @@ __device__ __forceinline__ float warp_top(float top) {  // the largest of a warp
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
 }
 __device__ __forceinline__ void times(float4& a, float by) { a.x *= by, a.y *= by, a.z *= by, a.w *= by; }
-// Divides what a warp holds by a power of two, where its largest size asks for that.
-template <int N>
-__device__ __forceinline__ float divide(float4 (&a)[N], float4 (&b)[N]) {
+// A warp's rows, each divided by a power of two of its own where the largest size of all asks for a look at each (a row
+// that is huge, or garbage that nobody reads, leaves its neighbours as they are).  a[i], b[i]: 8 values, LANES neighbouring
+// lanes to a row for each i (ONE: for all i together); put(i, divisor) then takes row i's.  False: nothing is divided.
+template <int LANES, bool ONE, int N, typename Put>
+__device__ __forceinline__ bool divide(float4 (&a)[N], float4 (&b)[N], Put&& put) {
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) top = larger(top, a[i], b[i]);
-    const float div = divisor(warp_top(top));
-    if (div != 1.0f) {
-        const float by = power_inverse(div);
+    if (divisor(warp_top(top)) == 1.0f) return false;
+    float div = 1.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) times(a[i], by), times(b[i], by);
+    for (int i = 0; i < N; ++i) {
+        if (i == 0 || !ONE) {
+            float t = ONE ? top : larger(0.f, a[i], b[i]);
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            div = divisor(t);
+            put(i, div);
+        }
+        times(a[i], power_inverse(div)), times(b[i], power_inverse(div));
     }
-    return div;
+    return true;
 }
 __device__ __forceinline__ void loaders_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory"); }
 
@@ -458,11 +467,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
                     }
                 }
                 if constexpr (C::F32) {
-                    const float div = divide(a, b);
-                    if (lane == 0) reinterpret_cast<uint8_t*>(q_odd)[warp] = div != 1.0f;
-#pragma unroll
-                    for (int i = 0; i < TAKE; ++i)
+                    auto put = [&](int i, float div) {
                         if ((lt + i * N) % CH == 0) q_div[(lt + i * N) / CH] = div;
+                    };
+#pragma unroll
+                    for (int i = 0; i < TAKE; ++i) put(i, 1.0f);
+                    const bool odd = divide<CH, false>(a, b, put);
+                    if (lane == 0) reinterpret_cast<uint8_t*>(q_odd)[warp] = odd;
                 }
 #pragma unroll
                 for (int i = 0; i < TAKE; ++i) {
@@ -491,11 +502,13 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
                         if (src) a[i] = ld_coherent(src + 2 * c), b[i] = ld_coherent(src + 2 * c + 1);
                     }
                     if (kv == 0) {
-                        const float div = divide(a, b);
-                        if (lane == 0) reinterpret_cast<uint8_t*>(k_odd + C::WORDS)[warp] = div != 1.0f;
-#pragma unroll
-                        for (int i = 0; i < TAKE; ++i)
+                        auto put = [&](int i, float div) {
                             if ((lt + i * N) % CH == 0) k_div[C::WORDS * kTile + (lt + i * N) / CH] = div;
+                        };
+#pragma unroll
+                        for (int i = 0; i < TAKE; ++i) put(i, 1.0f);
+                        const bool odd = divide<CH, false>(a, b, put);
+                        if (lane == 0) reinterpret_cast<uint8_t*>(k_odd + C::WORDS)[warp] = odd;
                     }
                     float top = 0.f;
 #pragma unroll
@@ -783,7 +796,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
                     }
                     cp_arrive(full);
                 } else {
-                    // K: 16 rows divided alike.  V: the tile alike, since its sums are: split as it is (the first tile by the
+                    // K: a row by itself.  V: the tile alike, since its sums are: split as it is (the first tile by the
                     // softmax threads) and, where the tile's largest size asks for a divisor, read and split once more.
                     if (j == 0 && kv == 0) continue;
                     float div = 1.0f;
@@ -812,9 +825,11 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
                                 }
                             }
                             if (kv == 0) {
-                                const float d = divide(a, b);
-                                odd = odd || d != 1.0f;
-                                if ((lt & 1) == 0 && r < kTile) k_div[place(j) * kTile + r] = d;
+                                auto put = [&](int, float d) {
+                                    if ((lt & 1) == 0 && r < kTile) k_div[place(j) * kTile + r] = d;
+                                };
+                                put(0, 1.0f);
+                                odd = divide<2, true>(a, b, put) || odd;
                             } else if (pass == 1) {
 #pragma unroll
                                 for (int c = 0; c < CH / 2; ++c) times(a[c], by), times(b[c], by);

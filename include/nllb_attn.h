@@ -208,13 +208,14 @@ NLLB_ATTN_API int nllb_attn_cross_host(nllb_attn_ctx* ctx, int layer, int n_sent
  * The weights of 16-bit calls of several rows are rounded to the type before
  * their product with V, and their sums over n keys may come out up to n 2^-27
  * short (relative), over more than 32768 no more than over 32768: 2^-12, where
- * half a step of fp16 is 2^-11.  fp32 calls of many rows split q, k and v into two fp16
- * parts, after a division by a power of two where sizes ask for it: 22 bits
- * down to 2^-17 of the largest value of 16 rows of q, of 16 rows of k, of 128
- * rows of v, less below that (an absolute 2^-39 of the largest; of 1 where the
- * largest lies in [2^-3, 65504): 2^-25).  Finite values below 2^100 are meant;
- * scores have to be finite in fp32.  At most 8 rows of a key head (max_q times
- * the query heads that share it; 16-bit types: 16) count as few.
+ * half a step of fp16 is 2^-11.  fp32 calls of many rows split q, k and v into
+ * two fp16 parts, after a division by a power of two where sizes ask for it:
+ * 22 bits down to 2^-17 of the largest value of a row of q or k, or of 128 rows
+ * of v (a chunk's later tokens among them); below that an absolute 2^-39 of the
+ * largest, or 2^-25 where the largest of 16 rows of q or k, or of the 128 of v,
+ * lies in [2^-3, 65504).  Finite values below 2^100 are meant; scores have to
+ * be finite in fp32.  At most 8 rows of a key head (max_q times the query heads
+ * that share it; 16-bit types: 16) count as few.
  * All pointers are of the context's device.
  * n_heads is a multiple of n_kv_heads: query head h reads key head
  * h / (n_heads / n_kv_heads).  head_dim is 64 or 128.

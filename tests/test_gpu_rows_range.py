@@ -81,3 +81,31 @@ def test_zeros(ctx, dim):  # noqa: F811
     assert (c.out[:170] == 0).all()
     ref, tol = reference(c.q[:150], c.k[:500], c.v[:500], torch.ones(150, 500, dtype=torch.bool), c.scale)
     check(c.out[:150], ref, tol, "zero values")
+
+
+@pytest.mark.parametrize("huge", [1e6, 1e18, 1e30])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_huge_rows_leave_their_neighbours_alone(ctx, dim, huge):  # noqa: F811
+    """Query rows of finite garbage (padding that nobody reads), and keys of a chunk's later tokens, change nothing in the
+    rows beside and before them."""
+    c = Paged([(150, 300), (33, 0)], 2, 2, dim, 16, torch.float32, seed=dim)
+    c.run(ctx)
+    ctx.sync()
+    plain = c.out.clone()
+    bad = [5, 16, 17, 100, 149]
+    c.q[bad] = huge
+    c.k_new[149] = huge  # (row 149's own token sees it)
+    c.out.fill_(7.0)
+    c.run(ctx)
+    ctx.sync()
+    others = [i for i in range(183) if i not in bad]
+    ref, tol = [], []
+    for i, (n, p) in enumerate(c.lens):
+        k, v = c.keys(i, c.k_pages, c.k_new), c.keys(i, c.v_pages, c.v_new)
+        seen = torch.arange(n + p)[None, :] <= (p + torch.arange(n))[:, None]
+        a = c.starts[i]
+        r, t = reference(c.q[a:a + n], k, v, seen, c.scale)
+        ref.append(r), tol.append(t)
+    ref, tol = torch.cat(ref), torch.cat(tol)
+    check(c.out[others], ref[others], tol[others], "beside huge rows")
+    assert torch.equal(c.out[others], plain[others])  # bit for bit: each of them is of ordinary size
