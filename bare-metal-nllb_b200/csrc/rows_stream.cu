@@ -24,8 +24,8 @@
 // workspace, and always in the same order.
 //
 // Measured: 64 sequences of one token and four query heads to a key head over
-// 200..8191 keys (bf16, heads of 128) 106 us = 5.4 TB/s; 256 tokens over
-// memories of 18..512 rows (bf16) 56 us = 5.1 TB/s; one fp32 token after 99
+// 200..8191 keys (bf16, heads of 128) 107 us = 5.4 TB/s; 256 tokens over
+// memories of 18..512 rows (bf16) 57 us = 5.0 TB/s; one fp32 token after 99
 // keys 4.5 us, latency; one token over 99990 keys with two key heads 31 us,
 // bound by the 32 CTAs that two clusters of 16 make.
 #include <algorithm>

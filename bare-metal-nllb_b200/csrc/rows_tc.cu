@@ -36,14 +36,14 @@
 // [2^-3, 65504): of 16 query or key rows, which a warp settles for itself, each
 // row by its own size, and the scores undo it; of a tile of values, alike,
 // which the sum over the tiles undoes.  (Ordinary sizes pay for the look: 64 prefixes 71 us instead of 67,
-// 128 scored sentences 96 instead of 91.)  Weights are held times 2^7, so
+// 128 scored sentences 95 instead of 91.)  Weights are held times 2^7, so
 // fp16 keeps them normal down to 2^-21 of the largest while 2^7 * 2^8 stays in
 // its range.
 //
 // Measured: documents of 1500..2048 over 3500..4096 rows, heads of 128, bf16,
-// a tenth of the keys hidden 302 us (696 TFLOP/s); chunks of 500..1024 tokens
-// behind up to 7000, heads of 64, 337 us (502 TFLOP/s of visible pairs); 128
-// sentences of fp32 89 us.  Bound by the softmax warps' instructions (without
+// a tenth of the keys hidden 306 us (687 TFLOP/s); chunks of 500..1024 tokens
+// behind up to 7000, heads of 64, 340 us (496 TFLOP/s of visible pairs); 128
+// sentences of fp32 95 us.  Bound by the softmax warps' instructions (without
 // exponentials the chunks take 287 us, without the softmax 216); a share of
 // the exponentials on the fp32 multipliers, or turns between the two tiles'
 // exponentials, made it slower (a quarter of them 366 us, turns 361 us).

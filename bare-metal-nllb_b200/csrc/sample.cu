@@ -15,15 +15,15 @@
 // distributed shared memory: top-k by 64 coarse bins whose counters never
 // collide, top-p by 2048 steps, from whose counts the weights follow closely
 // enough to name the few steps the border can lie in.  Where everything kept
-// lies in few elements, one CTA gathers, sorts and finishes them alone (16 us
+// lies in few elements, one CTA gathers, sorts and finishes them alone (17 us
 // for one row of 256206 by top-k 50 and top-p 0.95).  Otherwise the exact
 // weights above those steps are summed, the elements at the border gathered
 // and sorted, or told apart 11 bits of their composite (order of the logit,
 // index) at a time where thousands are equal; then one more pass sums the kept
 // weights chunk by chunk and the token's chunk is searched.  Bound now by the
 // passes' instructions and, for few rows, by the cluster's barriers: 512 rows
-// of mixed settings 575 us, 0.9 TB/s of logits; 64 rows in bf16 by top-p 0.9
-// 125 us.
+// of mixed settings 575 to 600 us, 0.9 TB/s of logits; 64 rows in bf16 by top-p
+// 0.9 133 us.
 //
 // Weights are integer multiples of 2^-44 of the largest, so their sums are
 // exact and the order of the atomics changes no result.  44 bits because 2^19

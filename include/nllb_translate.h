@@ -222,7 +222,10 @@ NLLB_ATTN_API int nllb_logsoftmax_topk(const float* logits, long long ld, int vo
  * depend on the order of the additions.  Device pointers; asynchronous on
  * `stream` (a cudaStream_t, NULL = default); nothing is allocated, the logits
  * are not modified.  At most NLLB_SAMPLE_MAX_VOCAB entries a row (more:
- * NLLB_ATTN_ECAPACITY). */
+ * NLLB_ATTN_ECAPACITY).  Rows that all start on 16 bytes are read fastest; a
+ * contiguous matrix whose rows do not (256206 columns) takes up to twice as
+ * long for hundreds of rows: pad ld to a multiple of 16 bytes where that is
+ * yours to choose. */
 #define NLLB_SAMPLE_MAX_VOCAB 524288
 #define NLLB_SAMPLE_TIMEOUT (-2)
 typedef struct {
