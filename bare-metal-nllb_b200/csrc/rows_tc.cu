@@ -29,16 +29,16 @@
 // there.  Calls of more keys move the sums of 16 tiles on to a total that the
 // softmax threads add to, and fp32 ones every tile (1024 rows of 32 heads over
 // 100000 keys: heads of 64 2.04 ms, 1.86 without; of 128, where two tiles leave
-// no room for the total, 2.87 and 2.40).  fp32 inputs and weights are split into two fp16 parts, hi + lo, and
-// a product is taken as hi hi' + hi lo' + lo hi' (22 bits, and an absolute
-// 2^-25 where lo leaves fp16's normal range).  So that this holds at any size,
-// rows are divided by powers of two first where the largest size lies outside
-// [2^-3, 65504): of 16 query or key rows, which a warp settles for itself, each
-// row by its own size, and the scores undo it; of a tile of values, alike,
-// which the sum over the tiles undoes.  (Ordinary sizes pay for the look: 64 prefixes 71 us instead of 67,
-// 128 scored sentences 95 instead of 91.)  Weights are held times 2^7, so
-// fp16 keeps them normal down to 2^-21 of the largest while 2^7 * 2^8 stays in
-// its range.
+// no room for the total, 2.87 and 2.40).  fp32 inputs and weights are split
+// into two fp16 parts, hi + lo, and a product is taken as hi hi' + hi lo' +
+// lo hi' (22 bits, and an absolute 2^-25 where lo leaves fp16's normal range).
+// So that this holds at any size, rows are divided by powers of two first where
+// the largest size lies outside [2^-3, 65504): of 16 query or key rows, which a
+// warp settles for itself, each row by its own size, and the scores undo it; of
+// a tile of values, alike, which the sum over the tiles undoes.  (Ordinary
+// sizes pay for the look: 64 prefixes 71 us instead of 67, 128 scored sentences
+// 95 instead of 91.)  Weights are held times 2^7, so fp16 keeps them normal
+// down to 2^-21 of the largest while 2^7 * 2^8 stays in its range.
 //
 // Measured: documents of 1500..2048 over 3500..4096 rows, heads of 128, bf16,
 // a tenth of the keys hidden 306 us (687 TFLOP/s); chunks of 500..1024 tokens

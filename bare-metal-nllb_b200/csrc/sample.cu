@@ -685,8 +685,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Args a) {
         if (s < fine_lo) return -1;
         if (s > fine_hi) return kBins;
         const float d = place(l), nearest = __fsub_rn(__fadd_rn(d, kWhole), kWhole);  // s
-        const float within = __fadd_rn(__fsub_rn(d, nearest), 0.5f);                  // 0 to 1
-        const float x = fmaxf(__fsub_rn(__fmul_rn(within, (float)fine_per), 0.5f), 0.0f);
+        const float along = __fadd_rn(__fsub_rn(d, nearest), 0.5f);                   // 0 to 1
+        const float x = fmaxf(__fsub_rn(__fmul_rn(along, (float)fine_per), 0.5f), 0.0f);
         return (s - fine_lo) * fine_per + min(__float_as_int(__fadd_rn(x, kWhole)) & (2 * kBins - 1), fine_per - 1);
     };
     auto count = [&](auto&& bin, u64 (&v)[PER]) {  // what `bin` puts into [0, kBins)
