@@ -1,0 +1,449 @@
+// logprobs.cu -- log-probabilities of given tokens, the entropy of each row of
+// logits and its likeliest tokens (nllb_logprobs, sm_100a).
+//
+// With y_i = l_i log2(e) - M, M the largest l_i log2(e) rounded (the same for
+// every token, so that its rounding cancels):
+//   Z = sum_i 2^y_i,   S = sum_i 2^y_i y_i,
+//   log p_t = ln2 (y_t - log2 Z),   H = ln2 (log2 Z - S / Z).
+//
+// The bytes of the logits bound it: they are read once, each thread keeping a
+// running M, Z and S of its stripe of 16-byte vectors, which are joined in a
+// fixed order: across the warp, the CTA and the cluster that shares the row.
+//
+// The likeliest tokens cost the stream nothing: a thread notes, where its
+// running maximum grows anyway, which vector it came from.  Of n tokens in the
+// order (falling logit, rising index) each lies in one of the n stripes whose
+// maxima come first in that order -- n of them are ahead of any other stripe's
+// -- so those stripes alone are read again, a warp to a stripe, and what is not
+// behind the n-th maximum goes through sorted lists of 32 in registers.  A row
+// with many equal or rising logits takes more batches of 32, never another way.
+#include <cmath>
+#include <string>
+
+#include "nllb_translate.h"
+#include "rows.cuh"
+
+namespace nllb {
+int set_error(int status, const std::string& msg);  // nllb_attn.cu
+
+namespace {
+
+using u64 = unsigned long long;
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kUnroll = 4;         // 16-byte vectors of a thread in flight
+constexpr int kMaxCluster = 16;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNoWeight = -200.0f;  // 2^-200 is 0 in fp32
+// A largest scaled logit of this size and more: what M was rounded by could be more than an exponent holds, and different
+// logits are at least 32 apart.
+constexpr float kFar = 0x1.8p28f;
+
+struct Args {
+    const void* logits;
+    long long ld;
+    int vocab, top_n;
+    const int* target;
+    float *out_logp, *out_entropy;
+    int* out_top_tok;
+    float* out_top_logp;
+};
+
+struct State {  // of a set of tokens: sums of 2^(y - m) and 2^(y - m) (y - m), y = l log2(e)
+    float m, z, s;
+};
+
+struct Shared {
+    State warp[kWarps];
+    State cta;
+    u64 list[kWarps][32];
+    uint32_t top, n_top;  // beyond kFar: the largest logit's order, and how many there are
+};
+
+// Weight 2^y, y <= 0 (or what infinities and NaN make of it): below kNoWeight, and for NaN, none.
+__device__ __forceinline__ float weigh(float& y) {
+    y = fmaxf(y, kNoWeight);  // (NaN: kNoWeight)
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+    return e;
+}
+
+// The state's sums with its maximum moved to m >= st.m.
+__device__ __forceinline__ void move_to(State& st, float m) {
+    if (st.m == m) return;
+    float d = st.m - m;
+    if (!(d > kNoWeight)) {  // (sums beside a maximum beyond kFar may be infinite)
+        st.z = st.s = 0.f;
+    } else {
+        const float f = weigh(d);
+        st.s = f * fmaf(st.z, d, st.s);
+        st.z *= f;
+    }
+    st.m = m;
+}
+
+__device__ __forceinline__ State join(State a, State b) {
+    const float m = fmaxf(a.m, b.m);
+    move_to(a, m);
+    move_to(b, m);
+    return {m, a.z + b.z, a.s + b.s};
+}
+
+// Bits that order like the logits (-0 as +0, NaN as -inf).
+__device__ __forceinline__ uint32_t order_of(float l) {
+    const uint32_t b = __float_as_uint(isnan(l) ? -INFINITY : l + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+// The order of falling logits, then rising indices.
+__device__ __forceinline__ u64 order_key(float l, uint32_t index) { return (u64)order_of(l) << 32 | (~index); }
+__device__ __forceinline__ uint32_t key_index(u64 key) { return ~(uint32_t)key; }
+constexpr uint32_t kLeastOrder = 0x007fffffu;                           // -inf
+constexpr u64 kNothing = (u64)kLeastOrder << 32 | 0xffffffffull;        // the keys up to it are not listed
+
+// A warp's 32 keys in falling order.
+__device__ __forceinline__ u64 clean(u64 x, int lane, int from, int up) {
+#pragma unroll
+    for (int j = from; j > 0; j >>= 1) {
+        const u64 y = __shfl_xor_sync(0xffffffffu, x, j);
+        const bool first = ((lane & j) == 0) == ((lane & up) == 0);
+        x = (x > y) == first ? x : y;
+    }
+    return x;
+}
+__device__ __forceinline__ u64 sort32(u64 x, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1) x = clean(x, lane, k / 2, k);
+    return x;
+}
+// The first 32 of two sorted lists.
+__device__ __forceinline__ u64 merge32(u64 a, u64 b, int lane) {
+    const u64 r = __shfl_sync(0xffffffffu, b, 31 - lane);
+    return clean(a > r ? a : r, lane, 16, 32);
+}
+// The first 32 of the sorted lists of `n` warps (a power of two), in warp 0.
+__device__ __forceinline__ u64 merge_warps(Shared& sh, u64 x, int n, int warp, int lane) {
+    for (int half = n / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (warp >= half && warp < 2 * half) sh.list[warp][lane] = x;
+        __syncthreads();
+        if (warp < half) x = merge32(x, sh.list[warp + half][lane], lane);
+    }
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x) {
+    if constexpr (std::is_same<T, float>::value) return x;
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(x);
+    else return __bfloat162float(x);
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int C) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    __shared__ Shared sh;
+    pdl_launch_dependents();
+    pdl_wait_primary();
+
+    const int rank = blockIdx.x % C, row = blockIdx.x / C;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int target = a.target ? ld_coherent(a.target + row) : 0;
+    if (target < 0) {  // (the same in the whole cluster)
+        if (rank == 0) {
+            if (tid == 0) {
+                if (a.out_logp) a.out_logp[row] = 0.f;
+                if (a.out_entropy) a.out_entropy[row] = 0.f;
+            }
+            if (TOP && tid < a.top_n) {
+                a.out_top_tok[(long long)row * a.top_n + tid] = -1;
+                a.out_top_logp[(long long)row * a.top_n + tid] = -INFINITY;
+            }
+        }
+        return;
+    }
+    const T* src = static_cast<const T*>(a.logits) + row * a.ld;
+    // single elements up to the first 16-byte boundary and behind the last one, vectors between them
+    const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / (int)sizeof(T));
+    const int n_vec = (a.vocab - head) / VEC, tail = head + n_vec * VEC;
+    const int n_single = rank == 0 ? head + a.vocab - tail : 0;  // rank 0's
+    auto single = [&](int i) { return i < head ? i : tail + i - head; };
+    const uint4* vec = reinterpret_cast<const uint4*>(src + head);
+    const int per = (n_vec + C - 1) / C, v_end = min(n_vec, (rank + 1) * per), v_begin = min(n_vec, rank * per) + tid;
+
+    State st = {-INFINITY, 0.f, 0.f};
+    float best = -INFINITY;
+    uint32_t best_at = 0xffffffffu;  // the stripe's first vector that holds its maximum
+    auto batch = [&](const uint4 (&u)[kUnroll], int at) {
+        float x[kUnroll][VEC], top[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            rows_unpack<T>(u[k], x[k]);
+            top[k] = x[k][0];
+#pragma unroll
+            for (int e = 1; e < VEC; ++e) top[k] = fmaxf(top[k], x[k][e]);
+        }
+        float t = top[0];
+#pragma unroll
+        for (int k = 1; k < kUnroll; ++k) t = fmaxf(t, top[k]);
+        if (t > best) {
+            best = t;
+#pragma unroll
+            for (int k = kUnroll - 1; k >= 0; --k)
+                if (top[k] == t) best_at = at + k * kThreads;
+            move_to(st, t * kLog2e);
+        }
+        const float off = -st.m;
+        float z[2] = {0.f, 0.f}, s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float y = fmaf(x[k][e], kLog2e, off);
+                const float w = weigh(y);
+                z[e & 1] += w;
+                s[e & 1] = fmaf(w, y, s[e & 1]);
+            }
+        st.z += z[0] + z[1];
+        st.s += s[0] + s[1];
+    };
+    int v = v_begin;
+    for (; v + (kUnroll - 1) * kThreads < v_end; v += kUnroll * kThreads) {
+        uint4 u[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) u[k] = ld_coherent(vec + v + k * kThreads);
+        batch(u, v);
+    }
+    if (v < v_end) {
+        // (-inf in every element: no weight, no maximum)
+        const uint32_t none = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        uint4 u[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+            u[k] = v + k * kThreads < v_end ? ld_coherent(vec + v + k * kThreads) : make_uint4(none, none, none, none);
+        batch(u, v);
+    }
+    for (int i = tid; i < n_single; i += kThreads) {
+        const float l = to_float(ld_coherent(src + single(i)));
+        if (l * kLog2e > st.m) move_to(st, l * kLog2e);
+        float y = fmaf(l, kLog2e, -st.m);
+        const float w = weigh(y);
+        st.z += w;
+        st.s = fmaf(w, y, st.s);
+    }
+
+    // ---- the row's M, Z and S
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        State b;
+        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+        b.z = __shfl_xor_sync(0xffffffffu, st.z, o);
+        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+        st = join(st, b);
+    }
+    if (lane == 0) sh.warp[warp] = st;
+    if (tid == 0) sh.top = sh.n_top = 0;
+    u64 list = 0;
+    if constexpr (TOP) {
+        // the stripes whose maxima come first, by the index of the vector's first element
+        u64 key = best_at == 0xffffffffu ? 0 : order_key(best, (uint32_t)head + best_at * VEC);
+        key = merge_warps(sh, sort32(key, lane), kWarps, warp, lane);
+        __syncthreads();
+        if (warp == 0) sh.list[0][lane] = key;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        State w = lane < kWarps ? sh.warp[lane] : State{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) {
+            State b;
+            b.m = __shfl_xor_sync(0xffffffffu, w.m, o);
+            b.z = __shfl_xor_sync(0xffffffffu, w.z, o);
+            b.s = __shfl_xor_sync(0xffffffffu, w.s, o);
+            w = join(w, b);
+        }
+        if (lane == 0) sh.cta = w;
+    }
+    if constexpr (TOP) {
+        const u64 bar = sh.list[0][a.top_n - 1];  // nothing behind it is among the first (0: fewer stripes)
+        auto take = [&](u64 key, int further, bool there) {
+            const bool in = there && key >= bar && key > kNothing;
+            if (__any_sync(0xffffffffu, in)) list = merge32(list, sort32(in ? key - further : 0, lane), lane);
+        };
+        for (int i = warp; i < a.top_n; i += kWarps) {
+            const u64 stripe = sh.list[0][i];
+            if (stripe <= kNothing) break;
+            const int t = ((int)(key_index(stripe) - head) / VEC - min(n_vec, rank * per)) % kThreads;  // whose
+            const int first = v_begin - tid + t, n = (v_end - first + kThreads - 1) / kThreads;
+            for (int k0 = 0; k0 < n; k0 += 32 * kUnroll) {
+                uint4 u[kUnroll];
+#pragma unroll
+                for (int j = 0; j < kUnroll; ++j) {
+                    const int k = k0 + 32 * j + lane;
+                    u[j] = ld_coherent(vec + first + min(k, n - 1) * kThreads);
+                }
+#pragma unroll
+                for (int j = 0; j < kUnroll; ++j) {
+                    const int k = k0 + 32 * j + lane;
+                    const uint32_t at = (uint32_t)head + (first + k * kThreads) * VEC;
+                    float x[VEC];
+                    rows_unpack<T>(u[j], x);
+                    // (an element stands behind the bar's vector, as its own vector does)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) take(order_key(x[e], at), e, k < n);
+                }
+            }
+        }
+        if (warp == kWarps - 1 && n_single > 0)
+            take(lane < n_single ? order_key(to_float(ld_coherent(src + single(lane))), single(lane)) : 0, 0, lane < n_single);
+        list = merge_warps(sh, list, kWarps, warp, lane);
+        if (C > 1) {
+            __syncthreads();
+            if (warp == 0) sh.list[0][lane] = list;
+        }
+    }
+    if (C > 1) cluster_sync_all();
+    else __syncthreads();
+    State all = sh.cta;
+    if (C > 1) {  // (the same order in every CTA)
+        all = {-INFINITY, 0.f, 0.f};
+        for (int r = 0; r < C; ++r) {
+            const uint32_t at = map_rank(&sh.cta, r);
+            all = join(all, State{ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)});
+        }
+        if constexpr (TOP) {
+            if (rank == 0) {
+                list = 0;
+                if (warp < C) {
+                    const uint32_t at = map_rank(&sh.list[0][lane], warp);
+                    list = (u64)(uint32_t)ld_cluster_s32(at + 4) << 32 | (uint32_t)ld_cluster_s32(at);
+                }
+                __syncthreads();
+                list = merge_warps(sh, list, C, warp, lane);
+            }
+        }
+    }
+    // A largest logit that is infinite or far out: the logits equal to it share all the weight.
+    const bool far = !(fabsf(all.m) < kFar);
+    float most = 0.f;
+    if (far) {
+        auto each = [&](auto&& f) {
+            for (int i = v_begin; i < v_end; i += kThreads) {
+                float x[VEC];
+                rows_unpack<T>(ld_coherent(vec + i), x);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f(order_of(x[e]));
+            }
+            for (int i = tid; i < n_single; i += kThreads) f(order_of(to_float(ld_coherent(src + single(i)))));
+        };
+        uint32_t top = 0, n = 0;
+        each([&](uint32_t o) { top = max(top, o); });
+        if (top) atomicMax(&sh.top, top);
+        if (C > 1) cluster_sync_all();
+        else __syncthreads();
+        for (int r = 0; r < C; ++r)
+            top = max(top, C > 1 ? (uint32_t)ld_cluster_s32(map_rank(&sh.top, r)) : *(volatile uint32_t*)&sh.top);
+        each([&](uint32_t o) { n += o == top; });
+        if (n) atomicAdd(&sh.n_top, n);
+        if (C > 1) cluster_sync_all();
+        else __syncthreads();
+        n = 0;
+        for (int r = 0; r < C; ++r)
+            n += C > 1 ? (uint32_t)ld_cluster_s32(map_rank(&sh.n_top, r)) : *(volatile uint32_t*)&sh.n_top;
+        most = logit_of(top);
+        all.z = (float)n;
+        all.s = 0.f;
+    }
+    if (rank == 0 && warp == 0) {
+        const bool none = far && most == -INFINITY;
+        const float log_z = log2f(all.z);
+        auto logp = [&](float l) {
+            if (none || !(l > -INFINITY)) return -INFINITY;
+            if (far) return (l == most ? 0.f : l - most) - kLn2 * log_z;
+            // (a token far behind, whose scaled difference may leave fp32: M's rounding is nothing beside it)
+            const float y = fmaf(l, kLog2e, -all.m);
+            return y > -1e6f ? kLn2 * (y - log_z) : (l - kLn2 * all.m) - kLn2 * log_z;
+        };
+        if (lane == 0) {
+            if (a.out_logp) a.out_logp[row] = target < a.vocab ? logp(to_float(ld_coherent(src + target))) : -INFINITY;
+            if (a.out_entropy) a.out_entropy[row] = none ? 0.f : kLn2 * (log_z - all.s / all.z);
+        }
+        if (TOP && lane < a.top_n) {
+            const bool there = list > kNothing;
+            a.out_top_tok[(long long)row * a.top_n + lane] = there ? (int)key_index(list) : -1;
+            a.out_top_logp[(long long)row * a.top_n + lane] = there ? logp(logit_of((uint32_t)(list >> 32))) : -INFINITY;
+        }
+    }
+    if (C > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
+}
+
+template <typename T, bool TOP>
+cudaError_t launch_one(const Args& a, int rows, int C, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * (unsigned)C, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = kPdlLaunch;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)C;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = C > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, a, C);
+}
+
+template <typename T>
+cudaError_t launch(const Args& a, int rows, int num_sms, cudaStream_t st) {
+    // CTAs of a row: what lets the last of them end first, at 22 bytes a nanosecond each and 2 us for what follows the stream
+    const double bytes = (double)a.vocab * sizeof(T);
+    int C = 1;
+    double least = 1e300;
+    for (int c = 1; c <= kMaxCluster; c *= 2) {
+        const long long turns = ((long long)rows * c + 2 * num_sms - 1) / (2 * num_sms);
+        const double t = (double)turns * (bytes / c / 22.0 + 2000.0);
+        if (t < least) least = t, C = c;
+    }
+    return a.top_n ? launch_one<T, true>(a, rows, C, st) : launch_one<T, false>(a, rows, C, st);
+}
+
+int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
+
+}  // namespace
+}  // namespace nllb
+
+extern "C" int nllb_logprobs(const nllb_logprobs_args* s, void* stream) {
+    using namespace nllb;
+    if (!s) return bad("args is NULL");
+    if (s->dtype != NLLB_F32 && s->dtype != NLLB_F16 && s->dtype != NLLB_BF16)
+        return bad("dtype must be NLLB_F32, NLLB_F16 or NLLB_BF16");
+    if (s->rows < 0 || s->vocab < 1) return bad("rows >= 0 and vocab >= 1 required");
+    if (s->vocab > (1 << 30) || s->rows > (1 << 26)) return set_error(NLLB_ATTN_ECAPACITY, "more logits than a call takes");
+    if (s->top_n < 0) return bad("top_n must not be negative");
+    if (s->top_n > NLLB_LOGPROBS_MAX_TOP) return set_error(NLLB_ATTN_ECAPACITY, "top_n above NLLB_LOGPROBS_MAX_TOP");
+    if (s->rows == 0) return NLLB_ATTN_OK;
+    if (!s->logits) return bad("logits is required");
+    if (s->out_logp && !s->target) return bad("out_logp needs target");
+    if (s->top_n > 0 && (!s->out_top_tok || !s->out_top_logp)) return bad("top_n needs out_top_tok and out_top_logp");
+    if (!s->out_logp && !s->out_entropy && s->top_n == 0) return bad("no output is asked for");
+    if (s->ld < s->vocab) return bad("ld must be at least vocab");
+    const uintptr_t size = s->dtype == NLLB_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(s->logits) % size) return bad("logits must be aligned to their type");
+    Args a = {};
+    a.logits = s->logits, a.ld = s->ld, a.vocab = s->vocab, a.top_n = s->top_n, a.target = s->target;
+    a.out_logp = s->out_logp, a.out_entropy = s->out_entropy;
+    a.out_top_tok = s->out_top_tok, a.out_top_logp = s->out_top_logp;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int device = 0, num_sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess)
+        e = s->dtype == NLLB_F32   ? launch<float>(a, s->rows, num_sms, st)
+            : s->dtype == NLLB_F16 ? launch<__half>(a, s->rows, num_sms, st)
+                                   : launch<__nv_bfloat16>(a, s->rows, num_sms, st);
+    if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_logprobs: ") + cudaGetErrorString(e));
+    return NLLB_ATTN_OK;
+}

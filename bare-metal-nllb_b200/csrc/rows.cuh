@@ -44,6 +44,23 @@ __device__ __forceinline__ int rows_token(const RowsParams& p, int row) {
     return (int)((unsigned long long)(uint32_t)row * p.group_mul >> p.group_shr);
 }
 
+// The keys that some row of a CTA sees through a sliding window, counted without the gap between the first keys and the
+// windows: number i stands for key `key(i)` of the sequence.  Without a window (WIN false) they are the keys.
+template <bool WIN>
+struct RowsWindow {
+    int skip, sinks, window, past;
+
+    // first_tok: the first token of the CTA's rows, whose window starts first
+    __device__ __forceinline__ RowsWindow(const RowsParams& p, const RowsSeq& q, int first_tok)
+        : skip(0), sinks(p.sinks), window(p.window), past(q.kvn - q.qn) {
+        if (WIN) skip = max(0, past + first_tok - window + 1 - sinks);
+    }
+    __device__ __forceinline__ int key(int i) const { return WIN && i >= sinks ? i + skip : i; }
+    // Token `tok` sees the numbers below end(tok) except those in [sinks, gap(tok)).
+    __device__ __forceinline__ int end(int tok) const { return past + tok + 1 - skip; }
+    __device__ __forceinline__ int gap(int tok) const { return max(sinks, past + tok - window + 1 - skip); }
+};
+
 // What has to be looked up to place key `j` of the sequence (j < kvn): its
 // page number, or its byte of the mask.  Apart from rows_at, so that it can be
 // asked for ahead of its use.

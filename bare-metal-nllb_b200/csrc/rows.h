@@ -1,6 +1,7 @@
 // rows.h -- parameters and launchers of the attention over many query rows
 // against keys of another length: a chunk of new tokens over a paged cache
-// (nllb_attn_paged) and target rows over encoder states (nllb_attn_cross_rows).
+// (nllb_attn_paged, and nllb_attn_window with a sliding window) and target rows
+// over encoder states (nllb_attn_cross_rows).
 #pragma once
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -30,6 +31,8 @@ struct RowsParams {
     const uint8_t* mask; // packed keys: one byte per key row, 0 hides it (null: all visible)
     int n_seq, kv_heads, group;
     int q_rows, kv_rows, max_q, max_kv;
+    int max_seen;  // keys that the rows of one CTA see, at most
+    int window, sinks;  // paged: a token sees the last `window` positions and the first `sinks`; window 0: all
     int table_ld, n_pages, page;
     uint32_t page_mul;  // j / page = j * page_mul >> page_shr
     int page_shr;
@@ -41,6 +44,16 @@ struct RowsParams {
 };
 
 enum class RowType { f32 = 0, f16 = 1, bf16 = 2 };
+
+// nllb_attn_append: of `rows`, q, out (the turned queries), the chunk's rows, the pages, their lengths and tables.
+struct AppendParams {
+    RowsParams rows;
+    const int* position;    // of each row of q (null: its place in the sequence)
+    const float* inv_freq;  // [half]
+    int half;               // pairs that are turned; 0: none
+    bool neighbours;        // pairs (2i, 2i + 1), else (i, i + half)
+};
+cudaError_t launch_append(const AppendParams& p, RowType type, int head_dim, int num_sms, cudaStream_t st);
 
 // Per-device kernel attributes; call once per device.
 cudaError_t configure_rows_kernels();

@@ -91,7 +91,7 @@ struct Cfg {
     static constexpr uint32_t SMEM = NW * RING > STATES ? NW * RING : STATES;
 };
 
-template <typename T, int D, int R, bool PAGED, int NW>
+template <typename T, int D, int R, bool PAGED, int NW, bool WIN>
 __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p, int n_split) {
     using C = Cfg<T, D, R, NW>;
     constexpr int VEC = 16 / (int)sizeof(T), CH = C::CH, KPW = C::KPW, BLK = C::BLK;
@@ -109,10 +109,12 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     if (!rows_sequence<PAGED>(p, s, sq)) return;
     const int rows = sq.qn * p.group;  // R at most
     if (rows == 0) return;
-    const int past = sq.kvn - sq.qn;  // (paged) keys before the chunk
+    const RowsWindow<WIN> win(p, sq, 0);
+    const int past = sq.kvn - sq.qn - win.skip;  // (paged) keys before the chunk
+    const int n_keys = sq.kvn - win.skip;
 
     // the keys in blocks, shared among the splits; a warp takes every NW-th
-    const int blocks = (sq.kvn + BLK - 1) / BLK, per = (blocks + n_split - 1) / n_split;
+    const int blocks = (n_keys + BLK - 1) / BLK, per = (blocks + n_split - 1) / n_split;
     const int b_end = min(blocks, (split + 1) * per);
     int b_next = split * per + warp;  // the next block to locate
 
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     const T *kp = nullptr, *vp = nullptr;
     auto locate = [&] {  // this lane's row of the next block
         const int key = b_next * BLK + lane;
-        if (!(lane < BLK && b_next < b_end && key < sq.kvn && rows_key<T, PAGED>(p, sq, s, g, key, kp, vp)))
+        if (!(lane < BLK && b_next < b_end && key < n_keys && rows_key<T, PAGED>(p, sq, s, g, win.key(key), kp, vp)))
             kp = vp = nullptr;
         b_next += NW;
     };
@@ -163,6 +165,9 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
         if (r >= rows) return 0;
         return PAGED ? past + r / p.group + 1 : sq.kvn;
     };
+    // (WIN) of the keys before a row's window, number `end` is the first that it sees again
+    auto gap_of = [&](int r) { return WIN ? win.gap(r / p.group) : 0; };
+    const int gap_last = WIN ? win.gap(sq.qn - 1) : 0;
     // body(block index, its visible keys, its K in the ring) for every block of the warp
     auto run = [&](auto&& body) {
         int b = split * per + warp, buf = 0;
@@ -198,6 +203,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
             }
         }
         const int lim[2] = {sees(lr), HALVES == 2 ? sees(lr + 8) : 0};
+        const int gap[2] = {gap_of(lr), HALVES == 2 ? gap_of(lr + 8) : 0};
         float m[HALVES], l[HALVES], o[D / 8][4];
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) m[h] = -INFINITY, l[h] = 0.f;
@@ -219,7 +225,8 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
                 }
             }
             const int j0 = b * BLK;
-            const bool whole = seen == (BLK == 32 ? 0xffffffffu : 0xffffu) && (!PAGED || j0 + BLK <= past);
+            const bool whole = seen == (BLK == 32 ? 0xffffffffu : 0xffffu) && (!PAGED || j0 + BLK <= past) &&
+                               (!WIN || j0 >= gap_last || j0 + BLK <= win.sinks);
             uint32_t pf[BLK / 16][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -237,6 +244,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
                         x *= p.scale_log2;
                         const int i = n * 8 + 2 * lc + e;
                         if (!whole && !(((seen >> i) & 1u) && j0 + i < lim[h])) x = -INFINITY;
+                        if (WIN && !whole && j0 + i >= win.sinks && j0 + i < gap[h]) x = -INFINITY;
                         mx = fmaxf(mx, x);
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -280,11 +288,12 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     } else {
         constexpr int U = BLK / KPW < 4 ? BLK / KPW : 4;  // keys of a lane taken together
         float q[R][VEC], m[R], l[R], acc[R][VEC];
-        int lim[R];
+        int lim[R], gap[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             m[r] = -INFINITY, l[r] = 0.f;
             lim[r] = sees(r);
+            gap[r] = gap_of(r);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) q[r][i] = acc[r][i] = 0.f;
             if (r < rows) {
@@ -313,6 +322,8 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
 #pragma unroll
                         for (int o = CH / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
                         sc[x][u] = there && j0 + r < lim[x] ? d : -INFINITY;
+                        // (one row: its window starts where the gap ends)
+                        if (WIN && R > 1 && j0 + r >= win.sinks && j0 + r < gap[x]) sc[x][u] = -INFINITY;
                     }
                 }
 #pragma unroll
@@ -435,7 +446,7 @@ __global__ void __launch_bounds__(NW * 32) rows_stream_kernel(const RowsParams p
     if (n_split > 1) cluster_sync_all();  // no CTA leaves while another reads its state
 }
 
-template <typename T, int D, int R, bool PAGED, int NW>
+template <typename T, int D, int R, bool PAGED, int NW, bool WIN>
 cudaError_t launch_one(const RowsParams& p, int n_split, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n_split, (unsigned)p.kv_heads, (unsigned)p.n_seq);
@@ -450,52 +461,55 @@ cudaError_t launch_one(const RowsParams& p, int n_split, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = n_split > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, rows_stream_kernel<T, D, R, PAGED, NW>, p, n_split);
+    return cudaLaunchKernelEx(&cfg, rows_stream_kernel<T, D, R, PAGED, NW, WIN>, p, n_split);
 }
 
-template <typename T, int D, int R, bool PAGED>
+template <typename T, int D, int R, bool PAGED, bool WIN>
 cudaError_t launch_by_units(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long units = (long long)p.kv_heads * p.n_seq;
     // A warp alone per unit where that already fills the SMs and the keys are few (256 sequences of 16 heads over
     // 18..512 keys: 56 us, with four warps 75); else many warps, and as many splits as give every SM work (four CTAs
     // per SM instead of two cost 134 us against 113 over 200..8191 keys), none with less than a block per warp, one
     // cluster at most.
-    if (units >= 8LL * num_sms && p.max_kv <= 1024) return launch_one<T, D, R, PAGED, 1>(p, 1, st);
+    if (units >= 8LL * num_sms && p.max_seen <= 1024) return launch_one<T, D, R, PAGED, 1, WIN>(p, 1, st);
     constexpr int MANY = Cfg<T, D, R, 0>::MANY, step = MANY * Cfg<T, D, R, 0>::BLK;
     // The matrix products' sums lose up to a step of fp32 with every 16 keys, so a warp of them takes 32768 at most.
     const int most = Cfg<T, D, R, 0>::MMA ? MANY * kWarpKeys : INT_MAX;
     int n_split = 1;
-    while (n_split < 16 && ((units * n_split < 2LL * num_sms && p.max_kv > step * n_split) || p.max_kv / n_split > most))
+    while (n_split < 16 && ((units * n_split < 2LL * num_sms && p.max_seen > step * n_split) || p.max_seen / n_split > most))
         n_split *= 2;
-    return launch_one<T, D, R, PAGED, MANY>(p, n_split, st);
+    return launch_one<T, D, R, PAGED, MANY, WIN>(p, n_split, st);
 }
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool WIN>
 cudaError_t launch_by_rows(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long rows = (long long)p.max_q * p.group;
-    if (rows == 1) return launch_by_units<T, D, 1, PAGED>(p, num_sms, st);
+    if (rows == 1) return launch_by_units<T, D, 1, PAGED, WIN>(p, num_sms, st);
     if constexpr (sizeof(T) == 2) {
-        if (rows > 8) return launch_by_units<T, D, 16, PAGED>(p, num_sms, st);
+        if (rows > 8) return launch_by_units<T, D, 16, PAGED, WIN>(p, num_sms, st);
     } else {
-        if (rows <= 4) return launch_by_units<T, D, 4, PAGED>(p, num_sms, st);
+        if (rows <= 4) return launch_by_units<T, D, 4, PAGED, WIN>(p, num_sms, st);
     }
-    return launch_by_units<T, D, 8, PAGED>(p, num_sms, st);
+    return launch_by_units<T, D, 8, PAGED, WIN>(p, num_sms, st);
 }
 
 template <typename T>
 cudaError_t launch_by_dim(const RowsParams& p, int head_dim, bool paged, int num_sms, cudaStream_t st) {
+    if (p.window)
+        return head_dim == 64 ? launch_by_rows<T, 64, true, true>(p, num_sms, st)
+                              : launch_by_rows<T, 128, true, true>(p, num_sms, st);
     if (head_dim == 64)
-        return paged ? launch_by_rows<T, 64, true>(p, num_sms, st) : launch_by_rows<T, 64, false>(p, num_sms, st);
-    return paged ? launch_by_rows<T, 128, true>(p, num_sms, st) : launch_by_rows<T, 128, false>(p, num_sms, st);
+        return paged ? launch_by_rows<T, 64, true, false>(p, num_sms, st) : launch_by_rows<T, 64, false, false>(p, num_sms, st);
+    return paged ? launch_by_rows<T, 128, true, false>(p, num_sms, st) : launch_by_rows<T, 128, false, false>(p, num_sms, st);
 }
 
-template <typename T, int D, int R, bool PAGED, int NW>
+template <typename T, int D, int R, bool PAGED, int NW, bool WIN = false>
 cudaError_t configure_one() {
     // clusters of 16 CTAs are beyond the portable size
-    cudaError_t e = cudaFuncSetAttribute(rows_stream_kernel<T, D, R, PAGED, NW>,
+    cudaError_t e = cudaFuncSetAttribute(rows_stream_kernel<T, D, R, PAGED, NW, WIN>,
                                          cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(rows_stream_kernel<T, D, R, PAGED, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(rows_stream_kernel<T, D, R, PAGED, NW, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)Cfg<T, D, R, NW>::SMEM);
 }
 
@@ -505,6 +519,8 @@ cudaError_t configure_rows() {
     if (e == cudaSuccess) e = configure_one<T, D, R, true, 1>();
     if (e == cudaSuccess) e = configure_one<T, D, R, false, Cfg<T, D, R, 0>::MANY>();
     if (e == cudaSuccess) e = configure_one<T, D, R, true, Cfg<T, D, R, 0>::MANY>();
+    if (e == cudaSuccess) e = configure_one<T, D, R, true, 1, true>();
+    if (e == cudaSuccess) e = configure_one<T, D, R, true, Cfg<T, D, R, 0>::MANY, true>();
     return e;
 }
 
@@ -538,7 +554,7 @@ cudaError_t launch_rows(const RowsParams& p, RowType type, int head_dim, bool pa
     // cannot share (kWarpKeys)
     const long long rows = (long long)p.max_q * p.group;
     if (rows > (type == RowType::f32 ? 8 : kRowsMax) ||
-        (type != RowType::f32 && rows > 1 && p.max_kv > 16 * kWarps16 * kWarpKeys))
+        (type != RowType::f32 && rows > 1 && p.max_seen > 16 * kWarps16 * kWarpKeys))
         return launch_rows_tc(p, type, head_dim, paged, num_sms, st);
     switch (type) {
         case RowType::f32: return launch_by_dim<float>(p, head_dim, paged, num_sms, st);

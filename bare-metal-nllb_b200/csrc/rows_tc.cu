@@ -106,6 +106,13 @@ struct Cfg {
     static_assert(128 * LD * 4 <= (int)SAUX || NQ == 2, "a split's state fits over the operands");
 };
 
+// Of the 32 numbers from `base` on, a bit for each outside [from, to).
+__device__ __forceinline__ uint32_t outside(int base, int from, int to) {
+    const int a = min(max(from - base, 0), 32), b = min(max(to - base, 0), 32);
+    const uint32_t below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u, below_b = b == 32 ? 0xffffffffu : (1u << b) - 1u;
+    return below_a | ~below_b;
+}
+
 // byte offset of 16-byte chunk c of row r in an operand part
 __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
     return (uint32_t)((c >> 3) * (int)kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -296,7 +303,7 @@ __device__ __forceinline__ bool divide(float4 (&a)[N], float4 (&b)[N], Put&& put
 }
 __device__ __forceinline__ void loaders_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory"); }
 
-template <typename T, int D, int NQ, bool PAGED, bool LONG>
+template <typename T, int D, int NQ, bool PAGED, bool LONG, bool WIN>
 __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LONG>::CTAS)
     rows_tc_kernel(const RowsParams p, int n_split) {
     using C = Cfg<T, D, NQ, LONG>;
@@ -369,7 +376,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
 
     // keys of this CTA: all that its last row sees, in tiles, shared among the splits
     const int last_tok = rows_token(p, min(rows, row0 + NQ * kTile) - 1);
-    const int longest = PAGED ? sq.kvn - sq.qn + last_tok + 1 : sq.kvn;
+    const RowsWindow<WIN> win(p, sq, WIN ? rows_token(p, row0) : 0);  // (from here on keys are its numbers)
+    const int longest = PAGED ? win.end(last_tok) : sq.kvn;
     const int all_tiles = (longest + kTile - 1) / kTile;
     const int per = (all_tiles + n_split - 1) / n_split;
     const int j0 = split * per, n = max(0, min(all_tiles, j0 + per) - j0);
@@ -419,7 +427,8 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
         const bool there = row < rows;
         const bool any = row0 + t * kTile + lq * 32 < rows;  // the warp has a row
         const int tok = rows_token(p, row);
-        const int lim = there ? (PAGED ? sq.kvn - sq.qn + tok + 1 : sq.kvn) : 0;
+        const int lim = there ? (PAGED ? win.end(tok) : sq.kvn) : 0;
+        const int gap = WIN && there ? win.gap(tok) : 0;
         const uint32_t lane_off = (uint32_t)(lq * 32) << 16;
         const uint32_t tS = tmem + lane_off + (uint32_t)t * 128, tO = tmem + lane_off + C::O_COL + (uint32_t)t * D;
         const uint32_t tT = tmem + lane_off + C::T_COL + (uint32_t)t * D;  // (TOTAL) the tiles before those in O
@@ -445,7 +454,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
 #pragma unroll
                 for (int i = 0; i < TAKE; ++i) {
                     const int key = j0 * kTile + (lt + i * N) / CH;
-                    entry[i] = key < longest ? rows_entry<PAGED>(p, sq, s, key) : 0;
+                    entry[i] = key < longest ? rows_entry<PAGED>(p, sq, s, win.key(key)) : 0;
                 }
             }
 #pragma unroll
@@ -489,7 +498,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
 #pragma unroll
                 for (int i = 0; i < TAKE; ++i) {
                     const int r = (lt + i * N) / CH, key = j0 * kTile + r;
-                    if (!(key < longest && rows_at<T, PAGED>(p, sq, g, key, entry[i], k[i], v[i]))) k[i] = v[i] = nullptr;
+                    if (!(key < longest && rows_at<T, PAGED>(p, sq, g, win.key(key), entry[i], k[i], v[i]))) k[i] = v[i] = nullptr;
                 }
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
@@ -547,6 +556,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
                 for (int c = 0; c < NC; ++c) {
                     const int x = min(max(left - 32 * (half * NC + c), 0), 32);
                     bits[c] = vw[half * NC + c] & (x == 32 ? 0xffffffffu : (1u << x) - 1u);
+                    if constexpr (WIN) bits[c] &= outside((j0 + j) * kTile + 32 * (half * NC + c), p.sinks, gap);
                     all &= bits[c];
                 }
                 // (one copy of the row's work for whole tiles, one for those with hidden keys)
@@ -750,7 +760,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
 #pragma unroll
             for (int i = 0; i < RP; ++i) {
                 const int r = (lt >> 1) + i * (kLoaders / 2), key = (j0 + j) * kTile + r;
-                entry[i] = r < kTile && key < longest ? rows_entry<PAGED>(p, sq, s, key) : 0;
+                entry[i] = r < kTile && key < longest ? rows_entry<PAGED>(p, sq, s, win.key(key)) : 0;
             }
         };
         bool ok = true;
@@ -763,7 +773,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
             for (int i = 0; i < RP; ++i) {
                 const int r = (lt >> 1) + i * (kLoaders / 2), key = (j0 + j) * kTile + r;
                 const bool seen =
-                    r < kTile && key < longest && rows_at<T, PAGED>(p, sq, g, key, entry[i], k[i], v[i]);
+                    r < kTile && key < longest && rows_at<T, PAGED>(p, sq, g, win.key(key), entry[i], k[i], v[i]);
                 if (!seen) k[i] = v[i] = nullptr;
                 uint32_t w = __ballot_sync(0xffffffffu, seen) & 0x55555555u;  // a bit for two lanes
                 w = (w | w >> 1) & 0x33333333u;
@@ -1017,7 +1027,7 @@ __global__ void __launch_bounds__(Cfg<T, D, NQ, LONG>::THREADS, Cfg<T, D, NQ, LO
     }
 }
 
-template <typename T, int D, int NQ, bool PAGED, bool LONG>
+template <typename T, int D, int NQ, bool PAGED, bool LONG, bool WIN>
 cudaError_t launch_tc(const RowsParams& p, int n_split, cudaStream_t st) {
     using C = Cfg<T, D, NQ, LONG>;
     const long long tiles = ((long long)p.max_q * p.group + NQ * kTile - 1) / (NQ * kTile);
@@ -1034,19 +1044,19 @@ cudaError_t launch_tc(const RowsParams& p, int n_split, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = n_split > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, rows_tc_kernel<T, D, NQ, PAGED, LONG>, p, n_split);
+    return cudaLaunchKernelEx(&cfg, rows_tc_kernel<T, D, NQ, PAGED, LONG, WIN>, p, n_split);
 }
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool WIN>
 cudaError_t launch_by_tiles(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long rows = (long long)p.max_q * p.group, heads = (long long)p.kv_heads * p.n_seq;
-    const bool is_long = sizeof(T) == 2 && p.max_kv > kLongKeys;
+    const bool is_long = sizeof(T) == 2 && p.max_seen > kLongKeys;
     if constexpr (sizeof(T) == 2) {
         // two query tiles per CTA where they still give every SM one
         if (rows > kTile && (rows + 2 * kTile - 1) / (2 * kTile) * heads >= num_sms) {
-            if (!is_long) return launch_tc<T, D, 2, PAGED, false>(p, 1, st);
+            if (!is_long) return launch_tc<T, D, 2, PAGED, false, WIN>(p, 1, st);
             // (two tiles of heads of 128 fill the tensor memory)
-            if constexpr (D == 64) return launch_tc<T, D, 2, PAGED, true>(p, 1, st);
+            if constexpr (D == 64) return launch_tc<T, D, 2, PAGED, true, WIN>(p, 1, st);
         }
     }
     const long long units = (rows + kTile - 1) / kTile * heads;
@@ -1054,28 +1064,35 @@ cudaError_t launch_by_tiles(const RowsParams& p, int num_sms, cudaStream_t st) {
     // over 500 keys: 12.0 us instead of 17.4), more where each keeps four key tiles (128 rows over 1500 keys: 20 us
     // with four, 36 with eight), one cluster at most.
     int n_split = 1;
-    while (n_split < 8 && units * n_split * 2 <= 2LL * num_sms && p.max_kv > (n_split == 1 ? 256 : 512 * n_split))
+    while (n_split < 8 && units * n_split * 2 <= 2LL * num_sms && p.max_seen > (n_split == 1 ? 256 : 512 * n_split))
         n_split *= 2;
     if constexpr (sizeof(T) == 2) {
-        if (is_long) return launch_tc<T, D, 1, PAGED, true>(p, n_split, st);
+        if (is_long) return launch_tc<T, D, 1, PAGED, true, WIN>(p, n_split, st);
     }
-    return launch_tc<T, D, 1, PAGED, false>(p, n_split, st);
+    return launch_tc<T, D, 1, PAGED, false, WIN>(p, n_split, st);
 }
 
 template <typename T>
 cudaError_t launch_by_dim(const RowsParams& p, int head_dim, bool paged, int num_sms, cudaStream_t st) {
+    if (p.window)
+        return head_dim == 64 ? launch_by_tiles<T, 64, true, true>(p, num_sms, st)
+                              : launch_by_tiles<T, 128, true, true>(p, num_sms, st);
     if (head_dim == 64)
-        return paged ? launch_by_tiles<T, 64, true>(p, num_sms, st) : launch_by_tiles<T, 64, false>(p, num_sms, st);
-    return paged ? launch_by_tiles<T, 128, true>(p, num_sms, st) : launch_by_tiles<T, 128, false>(p, num_sms, st);
+        return paged ? launch_by_tiles<T, 64, true, false>(p, num_sms, st) : launch_by_tiles<T, 64, false, false>(p, num_sms, st);
+    return paged ? launch_by_tiles<T, 128, true, false>(p, num_sms, st) : launch_by_tiles<T, 128, false, false>(p, num_sms, st);
 }
 
 template <typename T, int D, int NQ, bool LONG = false>
 cudaError_t configure_one() {
-    cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, true, LONG>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<T, D, NQ, LONG>::SMEM);
+    constexpr int bytes = (int)Cfg<T, D, NQ, LONG>::SMEM;
+    cudaError_t e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, true, LONG, false>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, false, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)Cfg<T, D, NQ, LONG>::SMEM);
+        e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, false, LONG, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 bytes);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(rows_tc_kernel<T, D, NQ, true, LONG, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 bytes);
     return e;
 }
 

@@ -71,6 +71,10 @@ class PagedArgs(ctypes.Structure):
                     "k_stride_head", "v_stride_page", "v_stride_slot", "v_stride_head")])
 
 
+class WindowArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedArgs), ("window", ctypes.c_int), ("sinks", ctypes.c_int)]
+
+
 class CrossRowsArgs(ctypes.Structure):
     _fields_ = ([(n, _fp) for n in ("q", "k", "v", "out", "q_start", "q_len", "kv_start", "kv_len", "key_mask")]
                 + [(n, ctypes.c_int) for n in ("dtype", "head_dim", "n_heads", "n_kv_heads", "n_seq", "q_rows",
@@ -81,12 +85,34 @@ class CrossRowsArgs(ctypes.Structure):
                     "v_stride_head", "out_stride_row", "out_stride_head")])
 
 
+ROT_HALVES, ROT_NEIGHBOURS = range(2)
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = ([(n, _fp) for n in ("q", "q_out", "k_new", "v_new", "k_pages", "v_pages", "q_start", "q_len", "kv_len",
+                                    "page_table", "position", "inv_freq")]
+                + [(n, ctypes.c_int) for n in ("dtype", "head_dim", "n_heads", "n_kv_heads", "n_seq", "q_rows", "max_q",
+                                               "max_kv", "n_pages", "page_size", "page_table_stride", "rot_dim",
+                                               "rot_pairs")]
+                + [(n, ctypes.c_int64) for n in (
+                    "q_stride_row", "q_stride_head", "q_out_stride_row", "q_out_stride_head", "k_new_stride_row",
+                    "k_new_stride_head", "v_new_stride_row", "v_new_stride_head", "k_stride_page", "k_stride_slot",
+                    "k_stride_head", "v_stride_page", "v_stride_slot", "v_stride_head")])
+
+
 class SampleArgs(ctypes.Structure):
     _fields_ = [("logits", _fp), ("ld", ctypes.c_longlong), ("dtype", ctypes.c_int), ("vocab", ctypes.c_int),
                 ("rows", ctypes.c_int), ("temperature", _fp), ("top_k", _fp), ("top_p", _fp), ("min_p", _fp),
                 ("u", _fp), ("out_tok", _fp), ("out_logp", _fp)]
 
 
+class LogprobsArgs(ctypes.Structure):
+    _fields_ = [("logits", _fp), ("ld", ctypes.c_longlong), ("dtype", ctypes.c_int), ("vocab", ctypes.c_int),
+                ("rows", ctypes.c_int), ("top_n", ctypes.c_int), ("target", _fp), ("out_logp", _fp),
+                ("out_entropy", _fp), ("out_top_tok", _fp), ("out_top_logp", _fp)]
+
+
+LOGPROBS_MAX_TOP = 32
 PROF_CLASSES = 14
 
 SIGNATURES = {
@@ -114,6 +140,8 @@ SIGNATURES = {
     "nllb_attn_cross": (_c_int, [_c_void_p, _c_int, _c_int, _fp, _fp]),
     "nllb_attn_cross_host": (_c_int, [_c_void_p, _c_int, _c_int, _fp, _fp]),
     "nllb_attn_paged": (_c_int, [_c_void_p, ctypes.POINTER(PagedArgs)]),
+    "nllb_attn_window": (_c_int, [_c_void_p, ctypes.POINTER(WindowArgs)]),
+    "nllb_attn_append": (_c_int, [_c_void_p, ctypes.POINTER(AppendArgs)]),
     "nllb_attn_test_expire_next_rows_wait": (_c_int, [_c_void_p]),
     "nllb_attn_cross_rows": (_c_int, [_c_void_p, ctypes.POINTER(CrossRowsArgs)]),
     "nllb_attention_head": (None, [_fp, _fp, _fp, _fp, _fp, _fp, _c_int, _c_int]),
@@ -144,6 +172,7 @@ SIGNATURES = {
     "nllb_logsoftmax_topk": (_c_int, [_fp, ctypes.c_longlong, _c_int, _c_int, _c_int, _fp, _fp, _fp, _c_void_p]),
     "nllb_sample": (_c_int, [ctypes.POINTER(SampleArgs), _c_void_p]),
     "nllb_sample_test_expire_next_wait": (_c_int, []),
+    "nllb_logprobs": (_c_int, [ctypes.POINTER(LogprobsArgs), _c_void_p]),
 }
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -218,6 +247,26 @@ def _ints(x, name, n, like, dtype="torch.int32"):
     if str(x.dtype) != dtype or x.numel() != n or not x.is_contiguous() or x.device != like.device:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} entries on q's device")
     return x.data_ptr()
+
+
+def _page_table(x, n_seq, like):
+    """Entries from one sequence's row of a page table to the next."""
+    if x.dim() != 2 or str(x.dtype) != "torch.int32" or x.shape[0] != n_seq or (x.numel() and x.stride(1) != 1) \
+            or x.device != like.device:
+        raise ValueError("page_table must be an int32 tensor [n_seq][entries] on q's device")
+    # (a one-row table's stride may be anything: its entries bound it)
+    return x.stride(0) if n_seq > 1 else x.shape[1]
+
+
+def _bounds(max_q, max_kv, rows, n_seq, q_len, page_table, page):
+    """max_q and max_kv, or their defaults, which the page table has to reach."""
+    if max_q is None:
+        max_q = rows if q_len is not None else rows // max(n_seq, 1)
+    if max_kv is None:
+        max_kv = page_table.shape[1] * page
+    if max_kv > page_table.shape[1] * page:
+        raise ValueError("page_table has too few entries for max_kv")
+    return max_q, max_kv
 
 
 class Context:
@@ -344,17 +393,8 @@ class Context:
             raise ValueError("out must have q's shape, v_pages k_pages's")
         if (k_new is None) != (v_new is None):
             raise ValueError("k_new and v_new go together")
-        if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32" or page_table.shape[0] != n_seq \
-                or (page_table.numel() and page_table.stride(1) != 1) or page_table.device != q.device:
-            raise ValueError("page_table must be an int32 tensor [n_seq][entries] on q's device")
-        # (a one-row table's stride may be anything: its entries bound it)
-        table_ld = page_table.stride(0) if n_seq > 1 else page_table.shape[1]
-        if max_q is None:
-            max_q = rows if q_len is not None else rows // max(n_seq, 1)
-        if max_kv is None:
-            max_kv = page_table.shape[1] * page
-        if max_kv > page_table.shape[1] * page:
-            raise ValueError("page_table has too few entries for max_kv")
+        table_ld = _page_table(page_table, n_seq, q)
+        max_q, max_kv = _bounds(max_q, max_kv, rows, n_seq, q_len, page_table, page)
         a = PagedArgs(q=_rows(q, "q", q, 3), out=_rows(out, "out", q, 3), k_pages=_rows(k_pages, "k_pages", q, 4),
                       v_pages=_rows(v_pages, "v_pages", q, 4), q_start=_ints(q_start, "q_start", n_seq, q),
                       q_len=_ints(q_len, "q_len", n_seq, q), kv_len=_ints(kv_len, "kv_len", n_seq, q),
@@ -386,6 +426,72 @@ class Context:
         """nllb_attn_paged: a chunk of new tokens over a paged cache."""
         self._same_device(args)
         _check(self.lib, self.lib.nllb_attn_paged(self.handle, ctypes.byref(args)), "nllb_attn_paged")
+
+    @classmethod
+    def window_args(cls, q, k_pages, v_pages, page_table, kv_len, out, window, sinks=0, **kw) -> WindowArgs:
+        """Arguments of :meth:`window`: those of :meth:`paged_args`, and the
+        positions that a token sees up to its own and from the first one on."""
+        a = WindowArgs(cls.paged_args(q, k_pages, v_pages, page_table, kv_len, out, **kw), window, sinks)
+        a.tensors_on = q.device
+        return a
+
+    def window(self, args: WindowArgs) -> None:
+        """nllb_attn_window: a chunk of new tokens over a paged cache, each of
+        which sees a sliding window and the first tokens."""
+        self._same_device(args)
+        _check(self.lib, self.lib.nllb_attn_window(self.handle, ctypes.byref(args)), "nllb_attn_window")
+
+    @staticmethod
+    def append_args(k_new, v_new, k_pages, v_pages, page_table, kv_len, q=None, q_out=None, inv_freq=None,
+                    pairs="halves", position=None, q_start=None, q_len=None, max_q=None, max_kv=None) -> AppendArgs:
+        """Arguments of :meth:`append` from torch CUDA tensors, which the caller
+        keeps alive: k_new, v_new [rows][kv_heads][dim], pages
+        [n_pages][page_size][kv_heads][dim], q, q_out [rows][heads][dim] or
+        None (any strides, the last axis contiguous), page_table
+        [n_seq][entries] int32, inv_freq fp32 of half as many entries as a
+        head's values are turned (None: none are), pairs "halves" or
+        "neighbours", position [rows] int32.  max_q and max_kv default as in
+        :meth:`paged_args`."""
+        n_seq, (rows, kv_heads, dim) = kv_len.numel(), k_new.shape
+        n_pages, page = k_pages.shape[:2]
+        if v_new.shape != k_new.shape or v_pages.shape != k_pages.shape or k_pages.shape[2] != kv_heads:
+            raise ValueError("v_new must have k_new's shape, v_pages k_pages's, and both their key heads")
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out go together")
+        if q is not None and (q.shape[0] != rows or q_out.shape != q.shape):
+            raise ValueError("q and q_out must be [k_new rows][heads][dim]")
+        if pairs not in ("halves", "neighbours"):
+            raise ValueError('pairs must be "halves" or "neighbours"')
+        table_ld = _page_table(page_table, n_seq, k_new)
+        max_q, max_kv = _bounds(max_q, max_kv, rows, n_seq, q_len, page_table, page)
+        rot = 0 if inv_freq is None else inv_freq.numel()
+        a = AppendArgs(k_new=_rows(k_new, "k_new", k_new, 3), v_new=_rows(v_new, "v_new", k_new, 3),
+                       k_pages=_rows(k_pages, "k_pages", k_new, 4), v_pages=_rows(v_pages, "v_pages", k_new, 4),
+                       q_start=_ints(q_start, "q_start", n_seq, k_new), q_len=_ints(q_len, "q_len", n_seq, k_new),
+                       kv_len=_ints(kv_len, "kv_len", n_seq, k_new), page_table=page_table.data_ptr(),
+                       position=_ints(position, "position", rows, k_new),
+                       inv_freq=_ints(inv_freq, "inv_freq", rot, k_new, "torch.float32"), dtype=_dtype_code(k_new),
+                       head_dim=dim, n_heads=kv_heads if q is None else q.shape[1], n_kv_heads=kv_heads, n_seq=n_seq,
+                       q_rows=rows, max_q=max_q, max_kv=max_kv, n_pages=n_pages, page_size=page,
+                       page_table_stride=table_ld, rot_dim=2 * rot,
+                       rot_pairs=ROT_HALVES if pairs == "halves" else ROT_NEIGHBOURS,
+                       k_new_stride_row=k_new.stride(0), k_new_stride_head=k_new.stride(1),
+                       v_new_stride_row=v_new.stride(0), v_new_stride_head=v_new.stride(1),
+                       k_stride_page=k_pages.stride(0), k_stride_slot=k_pages.stride(1),
+                       k_stride_head=k_pages.stride(2), v_stride_page=v_pages.stride(0),
+                       v_stride_slot=v_pages.stride(1), v_stride_head=v_pages.stride(2))
+        if q is not None:
+            a.q, a.q_out = _rows(q, "q", k_new, 3), _rows(q_out, "q_out", k_new, 3)
+            a.q_stride_row, a.q_stride_head = q.stride(0), q.stride(1)
+            a.q_out_stride_row, a.q_out_stride_head = q_out.stride(0), q_out.stride(1)
+        a.tensors_on = k_new.device
+        return a
+
+    def append(self, args: AppendArgs) -> None:
+        """nllb_attn_append: new tokens into a paged cache, queries and keys
+        turned by their positions."""
+        self._same_device(args)
+        _check(self.lib, self.lib.nllb_attn_append(self.handle, ctypes.byref(args)), "nllb_attn_append")
 
     @staticmethod
     def cross_rows_args(q, k, v, out, kv_len, q_start=None, q_len=None, kv_start=None, max_q=None, max_kv=None,
@@ -608,6 +714,53 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     else:
         _check(lib, lib.nllb_sample(ctypes.byref(a), stream), "nllb_sample")
     return out_tok, out_logp
+
+
+def _on_device(device, call):
+    """call(), with the tensors' GPU the current one."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return call()
+    with torch.cuda.device(device):
+        return call()
+
+
+def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entropy=None, out_top_tok=None,
+             out_top_logp=None, stream=None):
+    """nllb_logprobs on torch CUDA tensors: logits [rows][vocab] (rows may be
+    strided), target [rows] int32 or None.  Runs on torch's current stream of
+    the logits' device unless `stream` names another.  Returns
+    (log-probabilities of the targets [rows] fp32 or None, entropies [rows]
+    fp32 or None, likeliest tokens [rows][top_n] int32 and their
+    log-probabilities fp32, or None and None for top_n 0)."""
+    lib = load()
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("the rows of logits must be contiguous")
+    if target is None and out_logp is not None:
+        raise ValueError("out_logp needs target")
+    if not 0 <= top_n <= LOGPROBS_MAX_TOP:
+        raise ValueError(f"top_n must lie in [0, {LOGPROBS_MAX_TOP}]")
+    import torch
+    if not logits.is_cuda:
+        raise ValueError("logits must be on a GPU")
+    if stream is None:
+        stream = current_stream(logits.device.index)
+
+    def buffer(given, wanted, *shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device=logits.device) if given is None and wanted else given
+
+    out_logp, out_entropy = buffer(out_logp, target is not None, rows), buffer(out_entropy, entropy, rows)
+    out_top_tok = buffer(out_top_tok, top_n > 0, rows, top_n, dtype=torch.int32)
+    out_top_logp = buffer(out_top_logp, top_n > 0, rows, top_n)
+    f = "torch.float32"
+    a = LogprobsArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _dtype_code(logits), vocab, rows, top_n,
+                     _ints(target, "target", rows, logits), _ints(out_logp, "out_logp", rows, logits, f),
+                     _ints(out_entropy, "out_entropy", rows, logits, f),
+                     _ints(out_top_tok, "out_top_tok", rows * top_n, logits),
+                     _ints(out_top_logp, "out_top_logp", rows * top_n, logits, f))
+    _on_device(logits.device, lambda: _check(lib, lib.nllb_logprobs(ctypes.byref(a), stream), "nllb_logprobs"))
+    return out_logp, out_entropy, out_top_tok, out_top_logp
 
 
 def sample_test_expire_next_wait() -> None:

@@ -271,6 +271,25 @@ typedef struct {
 
 NLLB_ATTN_API int nllb_attn_paged(nllb_attn_ctx* ctx, const nllb_attn_paged_args* args);
 
+/* The same where a token sees the last `window` positions, its own among them,
+ * and the first `sinks` ones (of a running translation: the tokens that name the
+ * languages), so that a cache need not grow with what was said:
+ *    out_i = softmax over the keys j <= its position p with j > p - window or
+ *    j < sinks.
+ * Keys that no token of the call sees are not read, nor are the entries of
+ * page_table that hold nothing else and no new token: their pages may be given
+ * back, or be the same as later entries' (a ring), as long as no slot that the
+ * call writes holds a key that a token of the call sees.  max_kv bounds kv_len,
+ * the whole length.  What nllb_attn_paged says holds for the rest; a value that
+ * is not finite, in a key or value that one token of the call sees, may also
+ * reach the call's other tokens of its sequence. */
+typedef struct {
+    nllb_attn_paged_args cache;
+    int window, sinks;      /* window >= 1, sinks >= 0 */
+} nllb_attn_window_args;
+
+NLLB_ATTN_API int nllb_attn_window(nllb_attn_ctx* ctx, const nllb_attn_window_args* args);
+
 /* Target rows over encoder states of another length: every query row of
  * sequence s attends to its kv_len[s] key rows from row kv_start[s] of k and v
  * (kv_start NULL: s * max_kv), except those whose byte of key_mask (indexed
@@ -297,8 +316,55 @@ typedef struct {
 
 NLLB_ATTN_API int nllb_attn_cross_rows(nllb_attn_ctx* ctx, const nllb_attn_cross_rows_args* args);
 
-/* Test of the bounded device waits: if the next nllb_attn_paged or
- * nllb_attn_cross_rows of this context counts as many rows, a wait of its
+/* New tokens into a paged cache without attention, queries and keys turned by
+ * their positions on the way: what a decoder with rotary positions makes of its
+ * projections before nllb_attn_paged or nllb_attn_window (called without k_new)
+ * reads the cache.  Sequences, rows, lengths, pages, types and errors are those of
+ * nllb_attn_paged: token i of sequence s, row q_start[s] + i, goes to position
+ * kv_len[s] - q_len[s] + i.  A head's first rot_dim values (a multiple of 16;
+ * 0: nothing is turned) are rot_dim / 2 pairs: value i with value
+ * i + rot_dim / 2 (NLLB_ROT_HALVES), or 2i with 2i + 1 (NLLB_ROT_NEIGHBOURS).
+ * Pair i of every query and key head becomes
+ *    (a cos x - b sin x, b cos x + a sin x),  x = p * inv_freq[i],
+ * with p the token's position, or position[row] where that is given; x is
+ * taken in 64 bits.  Values are left as they are.  q and q_out (both or
+ * neither) may be one buffer, turned in its place; otherwise outputs may not
+ * overlap inputs, nor one another.  Rows that belong to no sequence are
+ * neither read nor written, of page_table only the entries of written slots
+ * are read; a token whose page number is bad is turned but not stored (nor are
+ * its neighbours hurt), and the error word is set.  Nothing is allocated; the
+ * call may be captured into a graph. */
+#define NLLB_ROT_HALVES 0
+#define NLLB_ROT_NEIGHBOURS 1
+typedef struct {
+    const void* q;
+    void*       q_out;
+    const void* k_new;
+    const void* v_new;
+    void*       k_pages;
+    void*       v_pages;
+    const int*  q_start;
+    const int*  q_len;
+    const int*  kv_len;
+    const int*  page_table;
+    const int*  position;
+    const float* inv_freq;
+    int dtype, head_dim, n_heads, n_kv_heads;
+    int n_seq, q_rows, max_q, max_kv;
+    int n_pages, page_size, page_table_stride;
+    int rot_dim, rot_pairs;
+    int64_t q_stride_row, q_stride_head;
+    int64_t q_out_stride_row, q_out_stride_head;
+    int64_t k_new_stride_row, k_new_stride_head;
+    int64_t v_new_stride_row, v_new_stride_head;
+    int64_t k_stride_page, k_stride_slot, k_stride_head;
+    int64_t v_stride_page, v_stride_slot, v_stride_head;
+} nllb_attn_append_args;
+
+NLLB_ATTN_API int nllb_attn_append(nllb_attn_ctx* ctx, const nllb_attn_append_args* args);
+
+/* Test of the bounded device waits: if the next nllb_attn_paged, _window or
+ * _cross_rows of this context counts as many rows, a wait of its
  * launch runs out after about 1 ms; it writes no output (paged: the chunk's
  * keys and values may be written) and the next nllb_attn_sync returns
  * NLLB_ATTN_ETIMEOUT.  The context stays usable. */

@@ -248,6 +248,38 @@ NLLB_ATTN_API int nllb_sample(const nllb_sample_args* args, void* stream);
  * NLLB_SAMPLE_TIMEOUT.  Later calls are as ever. */
 NLLB_ATTN_API int nllb_sample_test_expire_next_wait(void);
 
+/* ---- log-probabilities of given tokens --------------------------------------
+ * For each row of logits (row r at logits + r*ld, `vocab` entries of `dtype`
+ * NLLB_F32, NLLB_F16 or NLLB_BF16), with p the row's softmax:
+ *   out_logp[r]     log p of token target[r]
+ *   out_entropy[r]  -sum p log p
+ *   out_top_tok[r*top_n + j], out_top_logp[...]: the top_n likeliest tokens by
+ *                   falling logit and then rising index, and their log p
+ * Any of the outputs may be left out (NULL; top_n 0).  No counterpart in the
+ * reference, which only searches.  A row whose target is negative is padding:
+ * its logits are not read, and it gives logp 0, entropy 0, tokens -1 and their
+ * logp -inf.  A target of vocab or above has logp -inf.  A NaN logit counts as
+ * -inf; logits of +inf share all the weight, and so do equal largest ones of
+ * 2^28 and more in size (the others lie 32 lower at least).  Tokens of -inf have
+ * logp -inf and are not listed; a row with nothing above -inf has entropy 0, and places without a
+ * token give -1 and -inf.  target: one entry per row, or NULL (then out_logp
+ * is NULL too and no row is padding).  The logits are read once, rows may start
+ * anywhere; sums are fp32 and their order is fixed.  Device pointers;
+ * asynchronous on `stream` (a cudaStream_t, NULL = default); nothing is
+ * allocated, the logits are not modified. */
+#define NLLB_LOGPROBS_MAX_TOP 32
+typedef struct {
+    const void* logits;
+    long long   ld;
+    int         dtype, vocab, rows, top_n;
+    const int*  target;
+    float*      out_logp;
+    float*      out_entropy;
+    int*        out_top_tok;
+    float*      out_top_logp;
+} nllb_logprobs_args;
+NLLB_ATTN_API int nllb_logprobs(const nllb_logprobs_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
