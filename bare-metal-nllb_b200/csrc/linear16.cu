@@ -1,0 +1,630 @@
+// linear16.cu -- a linear layer in 16 bits with its epilogue (nllb_linear16,
+// sm_100a):  out = act(x w^T + bias) + residual, fp32 sums, one rounding.
+//
+// The weights are the A operand in every form, the tokens the B operand: a
+// lane then holds one output column, so that bias is one register, residual
+// and output rows are read and written 32 columns at a time whatever their
+// alignment, and a few tokens make a narrow tile rather than a mostly empty one.
+//
+// Few tokens (linear16_few): the weights' bytes bound it.  A warp multiplies 16
+// weight rows by 8 tokens at a time (warp-level products); the order of the
+// summands is the same permutation for both operands, so that each lane's
+// operands are 16 contiguous bytes of a row, straight from global memory.
+//
+// More (linear16_tc): tcgen05 products of 128 weight rows by a tile of up to
+// 256 tokens, operands by TMA into a ring of stages (64 wide, 128-byte swizzle),
+// persistent CTAs with two accumulators in tensor memory, so that one is drained
+// while the other is filled.  Pairs of CTAs (cta_group::2) take 256 weight rows
+// and load half of the tokens' tile each.  Where tiles are few, a cluster shares
+// the sum over k of one tile and joins it through distributed shared memory.
+#include <cuda.h>
+
+#include <algorithm>
+#include <string>
+
+#include "engine_kernels.h"
+#include "nllb_translate.h"
+#include "rows.cuh"
+
+namespace nllb {
+int set_error(int status, const std::string& msg);  // nllb_attn.cu
+
+namespace {
+
+__device__ int g_linear16_err;  // a bounded wait gave up (nllb_linear16_status)
+
+struct Args {
+    const void *x, *w, *bias, *residual;
+    void* out;
+    long long ldx, ldw, ldr, ldo;
+    int M, N, K, act;
+    bool expire;  // test: a wait runs out
+};
+
+template <typename T>
+__device__ __forceinline__ float as_float(T x) {
+    if constexpr (std::is_same<T, float>::value) return x;
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(x);
+    else return __bfloat162float(x);
+}
+template <typename T>
+__device__ __forceinline__ T rounded(float x) {
+    if constexpr (std::is_same<T, float>::value) return x;
+    else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+    else return __float2bfloat16_rn(x);
+}
+
+// The activations, each in a form whose small results keep their relative accuracy.
+template <int ACT>
+__device__ __forceinline__ float activate(float y) {
+    if constexpr (ACT == NLLB_ACT_RELU) return y < 0.f ? 0.f : y;  // (NaN stays)
+    if constexpr (ACT == NLLB_ACT_GELU) return 0.5f * y * erfcf(-0.70710678f * y);
+    // y (1 + tanh u) / 2 = y / (1 + e^-2u)
+    if constexpr (ACT == NLLB_ACT_GELU_TANH) return y / (1.0f + expf(-1.5957691f * (y + 0.044715f * y * y * y)));
+    if constexpr (ACT == NLLB_ACT_SILU) return y / (1.0f + expf(-y));
+    return y;
+}
+template <typename F>
+__device__ __forceinline__ void by_activation(int act, F&& f) {
+    switch (act) {
+        case NLLB_ACT_RELU: f(std::integral_constant<int, NLLB_ACT_RELU>()); break;
+        case NLLB_ACT_GELU: f(std::integral_constant<int, NLLB_ACT_GELU>()); break;
+        case NLLB_ACT_GELU_TANH: f(std::integral_constant<int, NLLB_ACT_GELU_TANH>()); break;
+        case NLLB_ACT_SILU: f(std::integral_constant<int, NLLB_ACT_SILU>()); break;
+        default: f(std::integral_constant<int, NLLB_ACT_NONE>());
+    }
+}
+
+// ---- few tokens ------------------------------------------------------------------------------------------------
+
+constexpr int kFewWarps = 8, kFewRows = 16;  // warps of a CTA, which share k; weight rows of a CTA
+constexpr int kFewBlocks = 4;                // blocks of 32 k that a warp takes together
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Elements [k, k + 8) of a row of K, zeros past its end.
+template <typename T>
+__device__ __forceinline__ uint4 row_chunk(const T* row, int k, int K) {
+    if (k + 8 <= K) return ld_coherent(reinterpret_cast<const uint4*>(row + k));
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(row + k) + 2 * i;
+        u[i] = (k + 2 * i < K ? ld_coherent(p) : 0u) | (k + 2 * i + 1 < K ? (uint32_t)ld_coherent(p + 1) : 0u) << 16;
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+template <typename T, typename O, int NT>
+__global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int n_split) {
+    __shared__ float sums[kFewWarps][8 * NT][kFewRows];
+    pdl_launch_dependents();
+    pdl_wait_primary();
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lr = lane >> 2, lc = lane & 3;
+    const int split = blockIdx.x % n_split;
+    const long long n0 = (long long)(blockIdx.x / n_split) * kFewRows;
+    const T* w = static_cast<const T*>(a.w);
+    // (a row past the last one: the last one's, whose sums nobody uses)
+    const T* w0 = w + min(n0 + lr, (long long)a.N - 1) * a.ldw + 8 * lc;
+    const T* w1 = w + min(n0 + lr + 8, (long long)a.N - 1) * a.ldw + 8 * lc;
+    for (int m0 = blockIdx.y * 8 * NT; m0 < a.M; m0 += gridDim.y * 8 * NT) {
+        const T* x[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            x[t] = m0 + t * 8 + lr < a.M ? static_cast<const T*>(a.x) + (m0 + t * 8 + lr) * a.ldx + 8 * lc : nullptr;
+
+        float c[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0.f;
+        constexpr int STEP = 32 * kFewBlocks;
+        for (int k = (split * kFewWarps + warp) * STEP; k < a.K; k += n_split * kFewWarps * STEP) {
+            uint4 u[kFewBlocks], v[kFewBlocks], b[NT][kFewBlocks];
+#pragma unroll
+            for (int i = 0; i < kFewBlocks; ++i) {
+                // (chunks count from this lane's own)
+                u[i] = row_chunk(w0, k + 32 * i, a.K - 8 * lc);
+                v[i] = row_chunk(w1, k + 32 * i, a.K - 8 * lc);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < kFewBlocks; ++i)
+                    b[t][i] = x[t] ? row_chunk(x[t], k + 32 * i, a.K - 8 * lc) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int i = 0; i < kFewBlocks; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    mma<T>(c[t], u[i].x, v[i].x, u[i].y, v[i].y, b[t][i].x, b[t][i].y);
+                    mma<T>(c[t], u[i].z, v[i].z, u[i].w, v[i].w, b[t][i].z, b[t][i].w);
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[warp][t * 8 + 2 * lc + (e & 1)][lr + 8 * (e >> 1)] = c[t][e];
+        __syncthreads();
+        // the warps' sums, then the splits', always in the same order
+        if (n_split > 1) {
+            for (int i = tid; i < 8 * NT * kFewRows; i += kFewWarps * 32) {
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < kFewWarps; ++j) s += sums[j][i / kFewRows][i % kFewRows];
+                sums[0][i / kFewRows][i % kFewRows] = s;
+            }
+            cluster_sync_all();
+        }
+        for (int i = split * kFewWarps * 32 + tid; i < 8 * NT * kFewRows; i += n_split * kFewWarps * 32) {
+            const int m = m0 + i / kFewRows;
+            const long long n = n0 + i % kFewRows;
+            if (m >= a.M || n >= a.N) continue;
+            float y = 0.f;
+            if (n_split > 1) {
+                for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(&sums[0][i / kFewRows][i % kFewRows], r));
+            } else {
+#pragma unroll
+                for (int j = 0; j < kFewWarps; ++j) y += sums[j][i / kFewRows][i % kFewRows];
+            }
+            if (a.bias) y += as_float(ld_coherent(static_cast<const T*>(a.bias) + n));
+            by_activation(a.act, [&](auto act) { y = activate<decltype(act)::value>(y); });
+            if (a.residual) y += as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n));
+            static_cast<O*>(a.out)[m * a.ldo + n] = rounded<O>(y);
+        }
+        // the sums are free again, and no CTA leaves while another reads them
+        if (n_split > 1) cluster_sync_all();
+        else __syncthreads();
+    }
+}
+
+// ---- tensor cores ----------------------------------------------------------------------------------------------
+
+constexpr int kRows = 128, kChunk = 64;                 // weight rows of a CTA's tile; k of a stage
+constexpr uint32_t kRowsBytes = kRows * kChunk * 2;     // 16 KB
+constexpr int kDrain = 8, kThreads = (kDrain + 2) * 32; // warps that drain accumulators; 1 that fetches, 1 that multiplies
+constexpr int kMaxStages = 10;
+constexpr uint32_t kRing = 221184;                      // bytes of all stages at most (216 KB)
+constexpr uint32_t kBars = (2 * kMaxStages + 6) * 8 + 16;
+
+enum { kSingle = 0, kPair = 1, kSplit = 2 };
+
+struct Tiling {
+    int bn;           // tokens of a tile, a multiple of 32 up to 256
+    int stages;
+    int tiles_n, tiles_m;
+    bool tokens_first;  // tiles of the same weights follow one another (else: of the same tokens)
+};
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+// Into this CTA's shared memory, complete on the pair's first CTA's barrier.
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// One arrival on `bar` of each CTA of the pair.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <typename T, typename O, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear16_tc(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const Args a, const Tiling g,
+                int n_split) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    unsigned char* sm = smem_raw + (base - raw);
+    const int stages = g.stages;
+    const uint32_t x_rows = MODE == kPair ? g.bn / 2 : g.bn, stage_bytes = kRowsBytes + x_rows * (kChunk * 2);
+    const uint32_t ring = stages * stage_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + ring);
+    uint64_t *empty = full + kMaxStages, *ready = empty + kMaxStages, *drained = ready + 2, *done = drained + 2, *never = done + 1;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(never + 1);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(slot + 1);
+
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int rank = MODE == kSingle ? 0 : (int)cluster_ctarank();
+    const int width = MODE == kPair ? 2 * kRows : kRows;  // weight rows of a tile
+    const int tiles = g.tiles_n * g.tiles_m;
+    // this CTA's (pair's, cluster's) tiles: first, first + step, ...
+    const int ctas = MODE == kSingle ? 1 : MODE == kPair ? 2 : n_split;
+    const int first = blockIdx.x / ctas, step = gridDim.x / ctas;
+    const int chunks = (a.K + kChunk - 1) / kChunk;
+    const int c0 = MODE == kSplit ? (int)((long long)rank * chunks / n_split) : 0;
+    const int c1 = MODE == kSplit ? (int)((long long)(rank + 1) * chunks / n_split) : chunks;
+    auto rows_at = [&](int t) { return (g.tokens_first ? t / g.tiles_m : t % g.tiles_n) * width; };
+    auto tokens_at = [&](int t) { return (g.tokens_first ? t % g.tiles_m : t / g.tiles_n) * g.bn; };
+    constexpr uint32_t TMEM = MODE == kSplit ? 256 : 512;  // two accumulators of up to 256 columns, or one of up to 256
+
+    if (warp == kDrain) {
+        if constexpr (MODE == kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(TMEM)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(slot, TMEM);
+        }
+    }
+    if (tid == 0) {
+        for (int i = 0; i < stages; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(ready + i, 1);
+            mbar_init(drained + i, MODE == kPair ? 2 * kDrain : kDrain);
+        }
+        mbar_init(done, 1);
+        mbar_init(never, 1);
+        fence_barrier_init();
+        *gave_up = 0;
+    }
+    tc_fence_before();
+    if constexpr (MODE == kPair) cluster_sync_all();  // the partner's barriers exist
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    pdl_wait_primary();
+    pdl_launch_dependents();
+
+    auto give_up = [&] {
+        *gave_up = 1;
+        if constexpr (MODE == kPair)
+            asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(map_rank(const_cast<int*>(gave_up), rank ^ 1)) : "memory");
+        atomicOr(&g_linear16_err, NLLB_DEV_ERR_TIMEOUT);
+    };
+    // Bounded wait; false (and the CTA, or pair, gives up) once any has run out.
+    auto wait_one = [&](uint64_t* bar, uint32_t parity, long long budget = kWaitBudgetCycles) -> bool {
+        if (mbar_try_wait(bar, parity)) return true;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, parity)) {
+            if (*gave_up) return false;
+            if (clock64() - t0 > budget) {
+                give_up();
+                return false;
+            }
+        }
+        return true;
+    };
+
+    if (warp == kDrain) {
+        // ---- fetch
+        if (lane == 0) {
+            const uint32_t full0 = MODE == kPair ? map_rank(full, 0) : 0u;
+            uint32_t i = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step) {
+                const int n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0);
+                const int m0 = tokens_at(t) + (MODE == kPair ? rank * (int)x_rows : 0);
+                for (int c = c0; c < c1; ++c, ++i) {
+                    const uint32_t s = i % stages;
+                    if (i >= (uint32_t)stages && !(ok = wait_one(empty + s, (i / stages - 1) & 1))) break;
+                    const uint32_t at = base + s * stage_bytes;
+                    if constexpr (MODE == kPair) {
+                        if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * stage_bytes);
+                        tma_2d_pair(at, &tw, c * kChunk, n0, full0 + 8 * s);
+                        tma_2d_pair(at + kRowsBytes, &tx, c * kChunk, m0, full0 + 8 * s);
+                    } else {
+                        mbar_arrive_expect_tx(full + s, stage_bytes);
+                        tma_2d(at, &tw, c * kChunk, n0, full + s);
+                        tma_2d(at + kRowsBytes, &tx, c * kChunk, m0, full + s);
+                    }
+                }
+            }
+            // (given up: what is in flight lands before the CTA ends)
+            if (*gave_up && rank == 0)
+                for (uint32_t j = i > (uint32_t)stages ? i - stages : 0; j < i; ++j)
+                    (void)mbar_wait_bounded(full + j % stages, (j / stages) & 1, kTestWaitBudgetCycles);
+        }
+        __syncwarp();
+    } else if (warp == kDrain + 1) {
+        // ---- products (of both CTAs of a pair: by the first one's)
+        if (MODE != kPair || rank == 0) {
+            const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            const uint32_t idesc = umma_idesc_f16(width, g.bn) | fmt;
+            bool ok = true;
+            if (a.expire) ok = __all_sync(0xffffffffu, wait_one(never, 0, kTestWaitBudgetCycles));  // nothing arrives there
+            uint32_t leader;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+            uint32_t i = 0, n = 0;
+            for (int t = first; t < tiles && ok; t += step, ++n) {
+                const uint32_t acc = n & 1;
+                if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait_one(drained + acc, (n / 2 - 1) & 1)))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * 256;
+                for (int c = c0; c < c1; ++c, ++i) {
+                    const uint32_t s = i % stages;
+                    if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, (i / stages) & 1)))) break;
+                    tc_fence_after();
+                    const uint64_t da = umma_desc_k_sw128(base + s * stage_bytes);
+                    const uint64_t db = umma_desc_k_sw128(base + s * stage_bytes + kRowsBytes);
+                    if (leader) {
+#pragma unroll
+                        for (int k = 0; k < kChunk / 16; ++k) {
+                            if constexpr (MODE == kPair) mma_pair(d, da + 2 * k, db + 2 * k, idesc, c > c0 || k > 0);
+                            else tc_mma_f16(d, da + 2 * k, db + 2 * k, idesc, c > c0 || k > 0);
+                        }
+                        if constexpr (MODE == kPair) commit_pair(empty + s);
+                        else tc_commit(empty + s);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (leader) {
+                    if constexpr (MODE == kPair) commit_pair(ready + acc);
+                    else tc_commit(ready + acc);
+                }
+                __syncwarp();
+            }
+            // what was issued is over before tensor memory is given back
+            if (leader) {
+                if constexpr (MODE == kPair) commit_pair(done);
+                else tc_commit(done);
+                (void)mbar_wait_bounded(done, 0);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---- drain: lane quarter warp % 4; the tile's 32-column pieces in turns between the two halves
+        const int quarter = warp & 3, half = warp >> 2;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        uint32_t n = 0;
+        for (int t = first; t < tiles; t += step, ++n) {
+            const uint32_t acc = n & 1;
+            if (!__all_sync(0xffffffffu, wait_one(ready + acc, (n / 2) & 1))) break;
+            tc_fence_after();
+            if constexpr (MODE == kSplit) {
+                // over the ring, which is done with and larger (a partial sum takes 64 KB at most)
+                float* part = reinterpret_cast<float*>(sm) + quarter * 32 + lane;
+                for (int col = half * 32; col < g.bn; col += 64) {
+                    float v[32];
+                    tmem_ld32(tmem + lanes + acc * 256 + col, v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) part[(col + j) * kRows] = v[j];
+                }
+                break;  // (one tile)
+            } else {
+                const int col_n = rows_at(t) + (MODE == kPair ? rank * kRows : 0) + quarter * 32 + lane, m0 = tokens_at(t);
+                const bool there = col_n < a.N;
+                const float bias = a.bias && there ? as_float(ld_coherent(static_cast<const T*>(a.bias) + col_n)) : 0.f;
+                for (int col = half * 32; col < g.bn; col += 64) {
+                    float v[32];
+                    tmem_ld32(tmem + lanes + acc * 256 + col, v);
+                    const int rows = min(32, a.M - m0 - col);
+                    O res[32];
+                    const O* from = static_cast<const O*>(a.residual) + (long long)(m0 + col) * a.ldr + col_n;
+                    if (a.residual && there) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (j < rows) res[j] = ld_coherent(from + j * a.ldr);
+                    }
+                    O* to = static_cast<O*>(a.out) + (long long)(m0 + col) * a.ldo + col_n;
+                    by_activation(a.act, [&](auto act) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j] + bias);
+                    });
+                    if (there) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (j < rows) to[j * a.ldo] = rounded<O>(a.residual ? v[j] + as_float(res[j]) : v[j]);
+                    }
+                    __syncwarp();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (MODE == kPair) arrive_at(map_rank(drained + acc, 0));
+                    else mbar_arrive(drained + acc);
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    if constexpr (MODE != kSingle) cluster_sync_all();  // neither leaves while the other uses its barriers, or reads its sums
+    else __syncthreads();
+    if constexpr (MODE == kSplit) {
+        // rank z finishes the columns z, z + n_split, ...; the sums in the order of the ranks
+        bool ok = true;
+        for (int r = 0; r < n_split; ++r) ok = ok && ld_cluster_s32(map_rank(const_cast<int*>(gave_up), r)) == 0;
+        const int n = rows_at(first) + (tid & (kRows - 1)), m0 = tokens_at(first);
+        if (ok && tid < kDrain * 32 && n < a.N) {
+            const float bias = a.bias ? as_float(ld_coherent(static_cast<const T*>(a.bias) + n)) : 0.f;
+            const float* part = reinterpret_cast<const float*>(sm) + (tid & (kRows - 1));
+            for (int col = rank + n_split * (tid / kRows); col < g.bn && m0 + col < a.M; col += n_split * (kDrain * 32 / kRows)) {
+                float y = 0.f;
+                for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(part + col * kRows, r));
+                y += bias;
+                by_activation(a.act, [&](auto act) { y = activate<decltype(act)::value>(y); });
+                if (a.residual) y += as_float(ld_coherent(static_cast<const O*>(a.residual) + (long long)(m0 + col) * a.ldr + n));
+                static_cast<O*>(a.out)[(long long)(m0 + col) * a.ldo + n] = rounded<O>(y);
+            }
+        }
+        cluster_sync_all();
+    }
+    if (warp == kDrain) {
+        tc_fence_after();
+        if constexpr (MODE == kPair)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM) : "memory");
+        else
+            tmem_dealloc(tmem, TMEM);
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------
+
+void with_cluster(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int ctas, cudaStream_t st) {
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = kPdlLaunch;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctas > 1 ? 2 : 1;
+}
+
+template <typename T, typename O, int NT>
+cudaError_t launch_few(const Args& a, int num_sms, cudaStream_t st) {
+    const long long rows = (a.N + kFewRows - 1) / kFewRows, tokens = (a.M + 8 * NT - 1) / (8 * NT);
+    // CTAs that share k, while that leaves two or fewer per SM and each warp something to do
+    int n_split = 1;
+    while (n_split < 8 && rows * tokens * n_split * 2 <= 2LL * num_sms && a.K > n_split * kFewWarps * 32 * kFewBlocks) n_split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = dim3((unsigned)(rows * n_split), (unsigned)std::min(tokens, 65535LL), 1);
+    cfg.blockDim = dim3(kFewWarps * 32, 1, 1);
+    with_cluster(cfg, attr, n_split, st);
+    return cudaLaunchKernelEx(&cfg, linear16_few<T, O, NT>, a, n_split);
+}
+
+template <typename T, typename O, int MODE>
+cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStream_t st) {
+    const int width = MODE == kPair ? 2 * kRows : kRows, x_rows = MODE == kPair ? g.bn / 2 : g.bn;
+    const int stage = (int)kRowsBytes + x_rows * kChunk * 2;
+    g.stages = std::min(kMaxStages, (int)kRing / stage);
+    g.tiles_n = (a.N + width - 1) / width, g.tiles_m = (a.M + g.bn - 1) / g.bn;
+    g.tokens_first = (long long)a.N >= a.M;  // the larger operand is read once, while its tile is in use
+    CUtensorMap tw, tx;
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    cudaError_t e = encode_rows16_map(&tw, a.w, bf16, a.K, a.N, a.ldw, kChunk, kRows);
+    if (e == cudaSuccess) e = encode_rows16_map(&tx, a.x, bf16, a.K, a.M, a.ldx, kChunk, x_rows);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(linear16_tc<T, O, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kRing + kBars + 1024));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = dim3((unsigned)(groups * ctas), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)g.stages * stage + kBars + 1024;
+    with_cluster(cfg, attr, ctas, st);
+    return cudaLaunchKernelEx(&cfg, linear16_tc<T, O, MODE>, tw, tx, a, g, ctas);
+}
+
+template <typename T, typename O>
+cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
+    if (a.M <= 8) return launch_few<T, O, 1>(a, num_sms, st);
+    if (a.M <= 16 || a.K < kChunk) return launch_few<T, O, 2>(a, num_sms, st);
+    auto up = [](long long x, long long to) { return (x + to - 1) / to; };
+    Tiling g = {};
+    // the tile of tokens whose rounds over the SMs take the least, by the wider of products and operands
+    auto best = [&](int width, int groups, bool pair) {
+        double least = 1e300;
+        for (int bn = 32; bn <= 256; bn += 32) {
+            const double rounds = (double)up(up(a.N, width) * up(a.M, bn), groups);
+            const double t = rounds * std::max(2.0 * bn, (16384.0 + bn * (pair ? 64 : 128)) / 64.0);
+            if (t < least * 0.999) least = t, g.bn = bn;
+        }
+        return least;
+    };
+    const long long few_tiles = up(a.N, kRows) * up(a.M, 128);
+    if (few_tiles * 2 <= num_sms) {
+        int split = 1;
+        while (split < 8 && few_tiles * split * 2 <= num_sms && a.K >= split * 4 * kChunk) split *= 2;
+        g.bn = (int)std::min<long long>(128, up(a.M, 32) * 32);
+        if (split > 1) return launch_mode<T, O, kSplit>(a, g, split, (int)few_tiles, st);
+    }
+    const double pair = best(2 * kRows, num_sms / 2, true);
+    const int pair_bn = g.bn;
+    const double single = best(kRows, num_sms, false);
+    if (pair < single) {
+        g.bn = pair_bn;
+        const long long tiles = up(a.N, 2 * kRows) * up(a.M, g.bn);
+        return launch_mode<T, O, kPair>(a, g, 2, (int)std::min<long long>(tiles, num_sms / 2), st);
+    }
+    const long long tiles = up(a.N, kRows) * up(a.M, g.bn);
+    return launch_mode<T, O, kSingle>(a, g, 1, (int)std::min<long long>(tiles, num_sms), st);
+}
+
+int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
+
+thread_local bool t_expire_next = false;
+
+}  // namespace
+}  // namespace nllb
+
+extern "C" int nllb_linear16_test_expire_next_wait(void) {
+    nllb::t_expire_next = true;
+    return NLLB_ATTN_OK;
+}
+
+extern "C" int nllb_linear16_status(void* stream) {
+    using namespace nllb;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int err = 0;
+    const int none = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&err, g_linear16_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && err) e = cudaMemcpyToSymbolAsync(g_linear16_err, &none, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess && err) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_linear16_status: ") + cudaGetErrorString(e));
+    if (err) return set_error(NLLB_ATTN_ETIMEOUT, "a bounded device wait of nllb_linear16 gave up");
+    return NLLB_ATTN_OK;
+}
+
+extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
+    using namespace nllb;
+    if (!s) return bad("args is NULL");
+    if (s->dtype != NLLB_F16 && s->dtype != NLLB_BF16) return bad("dtype must be NLLB_F16 or NLLB_BF16");
+    if (s->out_dtype != s->dtype && s->out_dtype != NLLB_F32) return bad("out_dtype must be dtype or NLLB_F32");
+    if (s->act < NLLB_ACT_NONE || s->act > NLLB_ACT_SILU) return bad("act must be one of NLLB_ACT_*");
+    if (s->M < 0 || s->N < 1 || s->K < 1) return bad("M >= 0, N >= 1 and K >= 1 required");
+    if (s->M > (1 << 24) || s->N > (1 << 24) || s->K > (1 << 24)) return set_error(NLLB_ATTN_ECAPACITY, "a size above 2^24");
+    if (s->M == 0) return NLLB_ATTN_OK;
+    if (!s->x || !s->w || !s->out) return bad("x, w and out are required");
+    if (s->ldx < s->K || s->ldw < s->K || s->ldo < s->N || (s->residual && s->ldr < s->N))
+        return bad("ldx and ldw must be at least K, ldo and ldr at least N");
+    if (((reinterpret_cast<uintptr_t>(s->x) | reinterpret_cast<uintptr_t>(s->w)) & 15u) || ((s->ldx | s->ldw) & 7))
+        return bad("rows of x and w must be 16-byte aligned, ldx and ldw multiples of 8");
+    if (s->ldx > (1LL << 36) || s->ldw > (1LL << 36)) return set_error(NLLB_ATTN_ECAPACITY, "ldx or ldw above 2^36");
+    const uintptr_t size = s->out_dtype == NLLB_F32 ? 4 : 2;
+    if ((reinterpret_cast<uintptr_t>(s->out) | reinterpret_cast<uintptr_t>(s->residual)) % size ||
+        reinterpret_cast<uintptr_t>(s->bias) % 2)
+        return bad("out, residual and bias must be aligned to their types");
+    Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, s->act, t_expire_next};
+    t_expire_next = false;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int device = 0, num_sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) {
+        const bool wide = s->out_dtype == NLLB_F32;
+        if (s->dtype == NLLB_F16) e = wide ? launch<__half, float>(a, num_sms, st) : launch<__half, __half>(a, num_sms, st);
+        else e = wide ? launch<__nv_bfloat16, float>(a, num_sms, st) : launch<__nv_bfloat16, __nv_bfloat16>(a, num_sms, st);
+    }
+    if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_linear16: ") + cudaGetErrorString(e));
+    return NLLB_ATTN_OK;
+}

@@ -112,6 +112,13 @@ class LogprobsArgs(ctypes.Structure):
                 ("out_entropy", _fp), ("out_top_tok", _fp), ("out_top_logp", _fp)]
 
 
+class Linear16Args(ctypes.Structure):
+    _fields_ = ([(n, _fp) for n in ("x", "w", "bias", "residual", "out")]
+                + [(n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldr", "ldo")]
+                + [(n, ctypes.c_int) for n in ("dtype", "out_dtype", "act", "M", "N", "K")])
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 LOGPROBS_MAX_TOP = 32
 PROF_CLASSES = 14
 
@@ -166,6 +173,9 @@ SIGNATURES = {
     "nllb_linear_status": (_c_int, [_c_void_p]),
     "nllb_linear_test_expire_next_wait": (_c_int, [_c_void_p]),
     "nllb_linear_free": (None, [_c_void_p]),
+    "nllb_linear16": (_c_int, [ctypes.POINTER(Linear16Args), _c_void_p]),
+    "nllb_linear16_status": (_c_int, [_c_void_p]),
+    "nllb_linear16_test_expire_next_wait": (_c_int, []),
     "nllb_apply_penalties": (_c_int, [_fp, ctypes.c_longlong, _c_int, _fp, _c_int, _fp, ctypes.c_float, _c_int,
                                       _c_void_p]),
     "nllb_logsoftmax_topk_ws_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
@@ -647,6 +657,64 @@ def linear_int8_noalloc_status(stream=None) -> int:
     """nllb_linear_int8_noalloc_status: waits for `stream`, reads and clears
     the no-alloc entry point's error word (returns the status, does not raise)."""
     return load().nllb_linear_int8_noalloc_status(stream)
+
+
+def _matrix(x, name, shape, like, dtype):
+    """Address of a matrix whose rows are contiguous, and the elements from one to the next."""
+    if tuple(x.shape) != shape or x.dtype != dtype or x.device != like.device:
+        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on x's device")
+    if x.numel() and shape[1] > 1 and x.stride(1) != 1:
+        raise ValueError(f"the rows of {name} must be contiguous")
+    # (a single row's stride may be anything)
+    return x.data_ptr(), x.stride(0) if shape[0] > 1 else shape[1]
+
+
+def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=None, stream=None):
+    """nllb_linear16 on torch CUDA tensors: act(x w^T + bias) + residual, x
+    [M][K], w [N][K], bias [N] of one 16-bit type, residual and out [M][N] of
+    it or fp32 (rows may be strided).  Runs on torch's current stream of x's
+    device unless `stream` names another."""
+    import torch
+    lib = load()
+    (M, K), N = x.shape, w.shape[0]
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"x must be float16 or bfloat16, not {x.dtype}")
+    kind = out.dtype if out is not None else out_dtype or x.dtype
+    if kind not in (x.dtype, torch.float32) or (out_dtype is not None and kind != out_dtype):
+        raise ValueError("out must have x's type or float32")
+    if not x.is_cuda:
+        raise ValueError("x must be on a GPU")
+    if out is None:
+        out = torch.empty((M, N), dtype=kind, device=x.device)
+    if stream is None:
+        stream = current_stream(x.device.index)
+    a = Linear16Args(bias=_ints(bias, "bias", N, x, str(x.dtype)), dtype=_dtype_code(x), out_dtype=_dtype_code(out),
+                     act=ACTIVATIONS[act], M=M, N=N, K=K)
+    (a.x, a.ldx), (a.w, a.ldw) = _matrix(x, "x", (M, K), x, x.dtype), _matrix(w, "w", (N, K), x, x.dtype)
+    if M == 1:
+        a.ldx = -(-K // 8) * 8
+    if N == 1:
+        a.ldw = -(-K // 8) * 8
+    a.out, a.ldo = _matrix(out, "out", (M, N), x, kind)
+    if residual is not None:
+        a.residual, a.ldr = _matrix(residual, "residual", (M, N), x, kind)
+    _on_device(x.device, lambda: _check(lib, lib.nllb_linear16(ctypes.byref(a), stream), "nllb_linear16"))
+    return out
+
+
+def linear16_status(stream=None) -> int:
+    """nllb_linear16_status: waits for `stream`, reads and clears the current
+    device's error word (returns the status, does not raise)."""
+    return load().nllb_linear16_status(stream)
+
+
+def linear16_test_expire_next_wait() -> None:
+    """nllb_linear16_test_expire_next_wait: a bounded wait of this thread's
+    next linear16 of more than 16 rows runs out."""
+    lib = load()
+    _check(lib, lib.nllb_linear16_test_expire_next_wait(), "linear16_test_expire_next_wait")
 
 
 def apply_penalties(logits, tokens, n_tokens, penalty=1.2, no_repeat_ngram=2, stream=None):

@@ -169,6 +169,45 @@ NLLB_ATTN_API int nllb_linear_status(nllb_linear* layer);
 NLLB_ATTN_API int nllb_linear_test_expire_next_wait(nllb_linear* layer);
 NLLB_ATTN_API void nllb_linear_free(nllb_linear* layer);
 
+/* ---- linear layer in 16 bits ------------------------------------------------
+ * out = act(x w^T + bias) + residual: the projections of a decoder whose rows
+ * and cache are 16 bits wide (nllb_attn_paged, nllb_attn_window, nllb_attn_append
+ * in NLLB_F16 or NLLB_BF16).  No counterpart in the reference, whose layers take
+ * fp32 rows and int8 weights (nllb_linear_int8 and its prepared form here).
+ * x [M][K], w [N][K] and bias [N] (NULL: none) are of `dtype`, out [M][N] and
+ * residual [M][N] (NULL: none; may be out itself) of `out_dtype`: dtype, or
+ * NLLB_F32.  Rows lie ldx, ldw, ldo, ldr elements apart; those of x and w start
+ * on 16 bytes, the others anywhere.  Sums are fp32, from their start to the
+ * residual, and rounded once; over K summands they may come out up to K 2^-27
+ * short (relative to the sum of their sizes).  act: NONE, RELU, GELU (by erf),
+ * GELU_TANH (its tanh form) or SILU.  Device pointers; asynchronous on `stream`
+ * (a cudaStream_t, NULL = default); nothing is allocated and no workspace is
+ * kept, so calls may overlap and be captured.  A bounded device wait that gives
+ * up leaves the outputs invalid and sets a per-device error word, which
+ * nllb_linear16_status (waits for `stream`) reads and clears:
+ * NLLB_ATTN_ETIMEOUT if set. */
+#define NLLB_ACT_NONE 0
+#define NLLB_ACT_RELU 1
+#define NLLB_ACT_GELU 2
+#define NLLB_ACT_GELU_TANH 3
+#define NLLB_ACT_SILU 4
+typedef struct {
+    const void* x;
+    const void* w;
+    const void* bias;
+    const void* residual;
+    void*       out;
+    long long   ldx, ldw, ldr, ldo;
+    int         dtype, out_dtype, act;
+    int         M, N, K;
+} nllb_linear16_args;
+NLLB_ATTN_API int nllb_linear16(const nllb_linear16_args* args, void* stream);
+NLLB_ATTN_API int nllb_linear16_status(void* stream);
+/* Test of the bounded device waits: if the calling thread's next nllb_linear16
+ * runs on the tensor-core kernel (more than 16 rows), a wait of its runs out
+ * after about 1 ms and nllb_linear16_status reports it.  Later calls are as ever. */
+NLLB_ATTN_API int nllb_linear16_test_expire_next_wait(void);
+
 /* ---- per-step vocabulary operations of the beam search --------------------
  * nllb_apply_penalties: for each of `rows` rows of logits (row r at
  * logits + r*ld) and its token history (tokens + r*tokens_ld, n_tokens[r]
