@@ -20,6 +20,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "engine_kernels.h"
@@ -37,7 +38,9 @@ struct Args {
     const void *x, *w, *bias, *residual;
     void* out;
     long long ldx, ldw, ldr, ldo;
-    int M, N, K, act;
+    int M, N, K, kind;
+    float c1, c2;  // of the activation
+    bool out_whole, res_whole;  // (there and) the rows start on 16 bytes
     bool expire;  // test: a wait runs out
 };
 
@@ -54,30 +57,64 @@ __device__ __forceinline__ T rounded(float x) {
     else return __float2bfloat16_rn(x);
 }
 
-// The activations, each in a form whose small results keep their relative accuracy.
-template <int ACT>
-__device__ __forceinline__ float activate(float y) {
-    if constexpr (ACT == NLLB_ACT_RELU) return y < 0.f ? 0.f : y;  // (NaN stays)
-    if constexpr (ACT == NLLB_ACT_GELU) return 0.5f * y * erfcf(-0.70710678f * y);
-    // y (1 + tanh u) / 2 = y / (1 + e^-2u)
-    if constexpr (ACT == NLLB_ACT_GELU_TANH) return y / (1.0f + expf(-1.5957691f * (y + 0.044715f * y * y * y)));
-    if constexpr (ACT == NLLB_ACT_SILU) return y / (1.0f + expf(-y));
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-template <typename F>
-__device__ __forceinline__ void by_activation(int act, F&& f) {
-    switch (act) {
-        case NLLB_ACT_RELU: f(std::integral_constant<int, NLLB_ACT_RELU>()); break;
-        case NLLB_ACT_GELU: f(std::integral_constant<int, NLLB_ACT_GELU>()); break;
-        case NLLB_ACT_GELU_TANH: f(std::integral_constant<int, NLLB_ACT_GELU_TANH>()); break;
-        case NLLB_ACT_SILU: f(std::integral_constant<int, NLLB_ACT_SILU>()); break;
-        default: f(std::integral_constant<int, NLLB_ACT_NONE>());
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+
+// |y| erfc(|y| / sqrt 2) / 2, what y max 0 exceeds gelu(y) by.  With z = |y| / sqrt 2 and t = 1 / (1 + z / 2), erfc z =
+// t 2^(P(t) - z^2 log2 e); P of degree 9 is fitted to log2 (e^(z^2) erfc z / t) over z in [0, 10.2], where its largest error
+// is 4.6e-8, and 2.1e-7 when it is evaluated in fp32 (the library's erfcf takes several times as long: 471 rows of 40012
+// over k = 155 71 us).
+__device__ __forceinline__ float gelu_gap(float y) {
+    const float x = fminf(fabsf(y), 30.0f), t = rcp(fmaf(x, 0.35355339f, 1.0f));  // (0 from 15 on; finite for infinities)
+    float p = 0.20728277f;
+    p = fmaf(p, t, -0.97266638f);
+    p = fmaf(p, t, 1.6471334f);
+    p = fmaf(p, t, -0.97694308f);
+    p = fmaf(p, t, -0.13727684f);
+    p = fmaf(p, t, 0.012391086f);
+    p = fmaf(p, t, 0.046664748f);
+    p = fmaf(p, t, 0.55840427f);
+    p = fmaf(p, t, 1.4406633f);
+    p = fmaf(p, t, -1.8256532f);
+    return 0.5f * x * t * ex2(fmaf(-0.72134752f * x, x, p));
+}
+
+// The activations, each in a form whose small results keep their relative accuracy, in three kinds of code:
+//   kClamp  max(y, c1): none (c1 = -inf) and RELU (0); NaN stays
+//   kSwish  y / (1 + 2^-(y (c1 + c2 y^2))): SILU, and GELU_TANH, since (1 + tanh u) / 2 = 1 / (1 + e^-2u); nothing is left at
+//           -100 (where a smaller y stops, so that infinity does not meet infinity)
+//   kGelu
+enum { kClamp = 0, kSwish = 1, kGelu = 2 };
+template <int KIND>
+__device__ __forceinline__ float activate(const Args& a, float y) {
+    if constexpr (KIND == kClamp) return max_nan(y, a.c1);
+    if constexpr (KIND == kSwish) {
+        y = max_nan(y, -100.f);
+        return __fdividef(y, 1.0f + ex2(-y * fmaf(a.c2 * y, y, a.c1)));
     }
+    return max_nan(y, 0.f) - gelu_gap(y);
+}
+__device__ __forceinline__ float activate(const Args& a, float y) {
+    return a.kind == kClamp ? activate<kClamp>(a, y) : a.kind == kSwish ? activate<kSwish>(a, y) : activate<kGelu>(a, y);
 }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------
 
-constexpr int kFewWarps = 8, kFewRows = 16;  // warps of a CTA, which share k; weight rows of a CTA
+constexpr int kFewWarps = 8, kFewRows = 16;  // warps of a CTA; weight rows of a warp
 constexpr int kFewBlocks = 4;                // blocks of 32 k that a warp takes together
 
 template <typename T>
@@ -107,19 +144,22 @@ __device__ __forceinline__ uint4 row_chunk(const T* row, int k, int K) {
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-template <typename T, typename O, int NT>
+// KG warps share k for the same 16 rows, KG = 8, or fewer where k is short; 8 / KG groups of rows to a CTA.
+template <typename T, typename O, int NT, int KG>
 __global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int n_split) {
-    __shared__ float sums[kFewWarps][8 * NT][kFewRows];
+    constexpr int ROWS = kFewRows * kFewWarps / KG;
+    __shared__ float sums[KG][8 * NT][ROWS];
     pdl_launch_dependents();
     pdl_wait_primary();
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lr = lane >> 2, lc = lane & 3;
+    const int kg = warp % KG, rg = warp / KG * kFewRows;
     const int split = blockIdx.x % n_split;
-    const long long n0 = (long long)(blockIdx.x / n_split) * kFewRows;
+    const long long n0 = (long long)(blockIdx.x / n_split) * ROWS;
     const T* w = static_cast<const T*>(a.w);
     // (a row past the last one: the last one's, whose sums nobody uses)
-    const T* w0 = w + min(n0 + lr, (long long)a.N - 1) * a.ldw + 8 * lc;
-    const T* w1 = w + min(n0 + lr + 8, (long long)a.N - 1) * a.ldw + 8 * lc;
+    const T* w0 = w + min(n0 + rg + lr, (long long)a.N - 1) * a.ldw + 8 * lc;
+    const T* w1 = w + min(n0 + rg + lr + 8, (long long)a.N - 1) * a.ldw + 8 * lc;
     for (int m0 = blockIdx.y * 8 * NT; m0 < a.M; m0 += gridDim.y * 8 * NT) {
         const T* x[NT];
 #pragma unroll
@@ -130,7 +170,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int
 #pragma unroll
         for (int t = 0; t < NT; ++t) c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0.f;
         constexpr int STEP = 32 * kFewBlocks;
-        for (int k = (split * kFewWarps + warp) * STEP; k < a.K; k += n_split * kFewWarps * STEP) {
+        for (int k = (split * KG + kg) * STEP; k < a.K; k += n_split * KG * STEP) {
             uint4 u[kFewBlocks], v[kFewBlocks], b[NT][kFewBlocks];
 #pragma unroll
             for (int i = 0; i < kFewBlocks; ++i) {
@@ -154,31 +194,31 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[warp][t * 8 + 2 * lc + (e & 1)][lr + 8 * (e >> 1)] = c[t][e];
+            for (int e = 0; e < 4; ++e) sums[kg][t * 8 + 2 * lc + (e & 1)][rg + lr + 8 * (e >> 1)] = c[t][e];
         __syncthreads();
         // the warps' sums, then the splits', always in the same order
         if (n_split > 1) {
-            for (int i = tid; i < 8 * NT * kFewRows; i += kFewWarps * 32) {
+            for (int i = tid; i < 8 * NT * ROWS; i += kFewWarps * 32) {
                 float s = 0.f;
 #pragma unroll
-                for (int j = 0; j < kFewWarps; ++j) s += sums[j][i / kFewRows][i % kFewRows];
-                sums[0][i / kFewRows][i % kFewRows] = s;
+                for (int j = 0; j < KG; ++j) s += sums[j][i / ROWS][i % ROWS];
+                sums[0][i / ROWS][i % ROWS] = s;
             }
             cluster_sync_all();
         }
-        for (int i = split * kFewWarps * 32 + tid; i < 8 * NT * kFewRows; i += n_split * kFewWarps * 32) {
-            const int m = m0 + i / kFewRows;
-            const long long n = n0 + i % kFewRows;
+        for (int i = split * kFewWarps * 32 + tid; i < 8 * NT * ROWS; i += n_split * kFewWarps * 32) {
+            const int m = m0 + i / ROWS;
+            const long long n = n0 + i % ROWS;
             if (m >= a.M || n >= a.N) continue;
             float y = 0.f;
             if (n_split > 1) {
-                for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(&sums[0][i / kFewRows][i % kFewRows], r));
+                for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(&sums[0][i / ROWS][i % ROWS], r));
             } else {
 #pragma unroll
-                for (int j = 0; j < kFewWarps; ++j) y += sums[j][i / kFewRows][i % kFewRows];
+                for (int j = 0; j < KG; ++j) y += sums[j][i / ROWS][i % ROWS];
             }
             if (a.bias) y += as_float(ld_coherent(static_cast<const T*>(a.bias) + n));
-            by_activation(a.act, [&](auto act) { y = activate<decltype(act)::value>(y); });
+            y = activate(a, y);
             if (a.residual) y += as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n));
             static_cast<O*>(a.out)[m * a.ldo + n] = rounded<O>(y);
         }
@@ -194,8 +234,10 @@ constexpr int kRows = 128, kChunk = 64;                 // weight rows of a CTA'
 constexpr uint32_t kRowsBytes = kRows * kChunk * 2;     // 16 KB
 constexpr int kDrain = 8, kThreads = (kDrain + 2) * 32; // warps that drain accumulators; 1 that fetches, 1 that multiplies
 constexpr int kMaxStages = 10;
-constexpr uint32_t kRing = 221184;                      // bytes of all stages at most (216 KB)
+constexpr int kPiece = 16, kPieceLd = 36;               // tokens that a warp drains together; floats of their rows of 32
+constexpr uint32_t kPieces = kDrain * kPiece * kPieceLd * 4;
 constexpr uint32_t kBars = (2 * kMaxStages + 6) * 8 + 16;
+constexpr uint32_t kRing = 232448 - 1024 - kBars - kPieces;  // bytes of all stages at most
 
 enum { kSingle = 0, kPair = 1, kSplit = 2 };
 
@@ -235,11 +277,33 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
         "h"((uint16_t)3)
         : "memory");
 }
+// (relaxed: what has to be over before is a read of tensor memory, which has been waited for; a release would wait for the
+// drained rows on their way to memory as well, 8000 cycles a tile of 64 rows of logits)
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_here(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-template <typename T, typename O, int MODE>
+// 16 columns of this thread's lane (warp-wide), there after tmem_wait on the same registers.
+__device__ __forceinline__ void tmem_ask16(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :
+                 : "memory");
+}
+
+template <typename T, typename O, int MODE, int KIND>
 __global__ void __launch_bounds__(kThreads, 1)
     linear16_tc(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const Args a, const Tiling g,
                 int n_split) {
@@ -253,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *empty = full + kMaxStages, *ready = empty + kMaxStages, *drained = ready + 2, *done = drained + 2, *never = done + 1;
     uint32_t* slot = reinterpret_cast<uint32_t*>(never + 1);
     volatile int* gave_up = reinterpret_cast<volatile int*>(slot + 1);
+    float* pieces = reinterpret_cast<float*>(sm + ring + kBars);
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -398,56 +463,146 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else {
-        // ---- drain: lane quarter warp % 4; the tile's 32-column pieces in turns between the two halves
+        // ---- drain: lane quarter warp % 4; the tile's pieces of 16 tokens in turns between the two halves
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        // A piece goes through shared memory, from a lane to a column to 16 bytes of a row to a lane: `per` lanes to a row of
+        // the warp's 32 columns.  (Straight from the lanes' columns each value took an instruction and an address of its own:
+        // 238 rows of 60608 over k = 320 49 us.)
+        constexpr int VEC = 16 / (int)sizeof(O), PER = 32 / VEC, AT_ONCE = 32 / PER, PASSES = kPiece / AT_ONCE;
+        // Residual rows that start on 16 bytes are asked for AHEAD pieces before their use, across tiles (238 rows of 60608
+        // over k = 320 in fp32: one piece ahead 49 us), others a piece before.
+        constexpr int AHEAD = sizeof(O) == 4 ? 4 : 6;
+        float* piece = pieces + warp * kPiece * kPieceLd;
+        const int pr = lane / PER, pc = lane % PER * VEC;
+        struct Place { int n0, m0, count; };  // this warp's first column, the tile's first token, its pieces with tokens
+        auto place_of = [&](int t) {
+            Place p = {0, 0, 0};
+            if (t < tiles) {
+                p.n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0) + quarter * 32, p.m0 = tokens_at(t);
+                p.count = (min(g.bn, a.M - p.m0) + kPiece - 1) / kPiece;
+            }
+            return p;
+        };
+        uint4 res[AHEAD][PASSES];
+        // piece `half` + 2 j of a tile
+        auto residual = [&](const Place& at, int j, uint4 (&to)[PASSES]) {
+            const int i = half + 2 * j, m0 = at.m0 + i * kPiece + pr;
+            if (!(i < at.count && at.n0 + 32 <= a.N)) return;
+            const O* p = static_cast<const O*>(a.residual) + m0 * a.ldr + at.n0 + pc;
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i)
+                if (m0 + i * AT_ONCE < a.M) to[i] = ld_coherent(reinterpret_cast<const uint4*>(p + i * AT_ONCE * a.ldr));
+        };
+        Place here = place_of(first);
         uint32_t n = 0;
+        int asked = 0;  // slots that the tile before this one has filled
         for (int t = first; t < tiles; t += step, ++n) {
             const uint32_t acc = n & 1;
+            const Place there = place_of(t + step);  // the next tile
+            const int n0 = here.n0, m0 = here.m0, count = here.count;
+            const bool mine = n0 + lane < a.N, out_whole = a.out_whole && n0 + 32 <= a.N;
+            const bool res_whole = a.res_whole && n0 + 32 <= a.N, res_lanes = a.residual && !res_whole && mine;
+            O old[kPiece];
+            auto residual_lanes = [&](int col) {
+                const int rows = min(kPiece, a.M - m0 - col);
+                const O* p = static_cast<const O*>(a.residual) + (long long)(m0 + col) * a.ldr + n0 + lane;
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j, p += a.ldr)
+                    if (j < rows) old[j] = ld_coherent(p);
+            };
+            if (MODE != kSplit && a.residual) {
+                if (a.res_whole) {
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k)
+                        if (k >= asked) residual(here, k, res[k]);
+                }
+                if (res_lanes && half < count) residual_lanes(half * kPiece);
+            }
             if (!__all_sync(0xffffffffu, wait_one(ready + acc, (n / 2) & 1))) break;
             tc_fence_after();
+            const uint32_t from = tmem + lanes + acc * 256;
             if constexpr (MODE == kSplit) {
                 // over the ring, which is done with and larger (a partial sum takes 64 KB at most)
                 float* part = reinterpret_cast<float*>(sm) + quarter * 32 + lane;
-                for (int col = half * 32; col < g.bn; col += 64) {
-                    float v[32];
-                    tmem_ld32(tmem + lanes + acc * 256 + col, v);
+                for (int col = half * kPiece; col < g.bn; col += 2 * kPiece) {
+                    float v[kPiece];
+                    tmem_ask16(from + col, v);
+                    tmem_wait(v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) part[(col + j) * kRows] = v[j];
+                    for (int j = 0; j < kPiece; ++j) part[(col + j) * kRows] = v[j];
                 }
                 break;  // (one tile)
             } else {
-                const int col_n = rows_at(t) + (MODE == kPair ? rank * kRows : 0) + quarter * 32 + lane, m0 = tokens_at(t);
-                const bool there = col_n < a.N;
-                const float bias = a.bias && there ? as_float(ld_coherent(static_cast<const T*>(a.bias) + col_n)) : 0.f;
-                for (int col = half * 32; col < g.bn; col += 64) {
-                    float v[32];
-                    tmem_ld32(tmem + lanes + acc * 256 + col, v);
-                    const int rows = min(32, a.M - m0 - col);
-                    O res[32];
-                    const O* from = static_cast<const O*>(a.residual) + (long long)(m0 + col) * a.ldr + col_n;
-                    if (a.residual && there) {
+                const float bias = a.bias && mine ? as_float(ld_coherent(static_cast<const T*>(a.bias) + n0 + lane)) : 0.f;
+                float next[kPiece];
+                if (half < count) tmem_ask16(from + half * kPiece, next);
+                for (int j0 = 0; half + 2 * j0 < count; j0 += AHEAD) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < rows) res[j] = ld_coherent(from + j * a.ldr);
+                    for (int k = 0; k < AHEAD; ++k) {  // (each with registers of its own for the residual)
+                        const int i = half + 2 * (j0 + k), col = i * kPiece;
+                        if (i >= count) break;
+                        float v[kPiece];
+                        tmem_wait(next);
+#pragma unroll
+                        for (int j = 0; j < kPiece; ++j) v[j] = activate<KIND>(a, next[j] + bias);
+                        if (i + 2 < count) tmem_ask16(from + col + 2 * kPiece, next);
+                        if (res_lanes) {
+#pragma unroll
+                            for (int j = 0; j < kPiece; ++j) v[j] += as_float(old[j]);  // (rows past the last one: unused)
+                            if (i + 2 < count) residual_lanes(col + 2 * kPiece);
+                        }
+                        if (out_whole || res_whole) {
+#pragma unroll
+                            for (int j = 0; j < kPiece; ++j) piece[j * kPieceLd + lane] = v[j];
+                            __syncwarp();
+#pragma unroll
+                            for (int r0 = 0; r0 < PASSES; ++r0) {
+                                const int r = r0 * AT_ONCE + pr, m = m0 + col + r;
+                                float y[VEC];
+#pragma unroll
+                                for (int e = 0; e < VEC; e += 4) {
+                                    const float4 f = *reinterpret_cast<const float4*>(piece + r * kPieceLd + pc + e);
+                                    y[e] = f.x, y[e + 1] = f.y, y[e + 2] = f.z, y[e + 3] = f.w;
+                                }
+                                if (res_whole) {
+                                    float z[VEC];
+                                    rows_unpack<O>(res[k][r0], z);
+#pragma unroll
+                                    for (int e = 0; e < VEC; ++e) y[e] += z[e];
+                                }
+                                O* to = static_cast<O*>(a.out) + m * a.ldo + n0 + pc;
+                                if (m < a.M) {
+                                    if (out_whole) {
+                                        *reinterpret_cast<uint4*>(to) = rows_pack<O>(y);
+                                    } else {
+#pragma unroll
+                                        for (int e = 0; e < VEC; ++e) to[e] = rounded<O>(y[e]);
+                                    }
+                                }
+                            }
+                        } else if (mine) {
+                            const int rows = min(kPiece, a.M - m0 - col);
+                            O* p = static_cast<O*>(a.out) + (long long)(m0 + col) * a.ldo + n0 + lane;
+#pragma unroll
+                            for (int j = 0; j < kPiece; ++j, p += a.ldo)
+                                if (j < rows) *p = rounded<O>(v[j]);
+                        }
+                        if (a.res_whole) {
+                            if (half + 2 * (j0 + k + AHEAD) < count) residual(here, j0 + k + AHEAD, res[k]);
+                            else residual(there, k, res[k]);
+                        }
+                        __syncwarp();
                     }
-                    O* to = static_cast<O*>(a.out) + (long long)(m0 + col) * a.ldo + col_n;
-                    by_activation(a.act, [&](auto act) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = activate<decltype(act)::value>(v[j] + bias);
-                    });
-                    if (there) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < rows) to[j * a.ldo] = rounded<O>(a.residual ? v[j] + as_float(res[j]) : v[j]);
-                    }
-                    __syncwarp();
                 }
+                asked = half < count ? min(AHEAD, (count - half + 1) / 2) : 0;
+                here = there;
+                tmem_wait(next);  // (what was asked for and not used)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     if constexpr (MODE == kPair) arrive_at(map_rank(drained + acc, 0));
-                    else mbar_arrive(drained + acc);
+                    else arrive_here(drained + acc);
                 }
             }
         }
@@ -457,20 +612,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (MODE != kSingle) cluster_sync_all();  // neither leaves while the other uses its barriers, or reads its sums
     else __syncthreads();
     if constexpr (MODE == kSplit) {
-        // rank z finishes the columns z, z + n_split, ...; the sums in the order of the ranks
+        // rank z finishes the tokens z, z + n_split, ...: a warp to each, 4 columns to a lane; the sums in the order of the ranks
         bool ok = true;
         for (int r = 0; r < n_split; ++r) ok = ok && ld_cluster_s32(map_rank(const_cast<int*>(gave_up), r)) == 0;
-        const int n = rows_at(first) + (tid & (kRows - 1)), m0 = tokens_at(first);
-        if (ok && tid < kDrain * 32 && n < a.N) {
-            const float bias = a.bias ? as_float(ld_coherent(static_cast<const T*>(a.bias) + n)) : 0.f;
-            const float* part = reinterpret_cast<const float*>(sm) + (tid & (kRows - 1));
-            for (int col = rank + n_split * (tid / kRows); col < g.bn && m0 + col < a.M; col += n_split * (kDrain * 32 / kRows)) {
-                float y = 0.f;
-                for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(part + col * kRows, r));
-                y += bias;
-                by_activation(a.act, [&](auto act) { y = activate<decltype(act)::value>(y); });
-                if (a.residual) y += as_float(ld_coherent(static_cast<const O*>(a.residual) + (long long)(m0 + col) * a.ldr + n));
-                static_cast<O*>(a.out)[(long long)(m0 + col) * a.ldo + n] = rounded<O>(y);
+        const int n = rows_at(first) + 4 * lane, m0 = tokens_at(first);
+        if (ok && warp < kDrain) {
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if (a.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) bias[e] = as_float(ld_coherent(static_cast<const T*>(a.bias) + n + e));
+            }
+            const float* part = reinterpret_cast<const float*>(sm) + 4 * lane;
+            for (int col = rank + n_split * warp; col < g.bn && m0 + col < a.M; col += n_split * kDrain) {
+                const long long m = m0 + col;
+                float old[4] = {0.f, 0.f, 0.f, 0.f};
+                if (a.residual) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < a.N) old[e] = as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n + e));
+                }
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int r = 0; r < n_split; r += 2) {  // (an even number of them)
+                    const float4 f = ld_cluster_f4(map_rank(part + col * kRows, r)), h = ld_cluster_f4(map_rank(part + col * kRows, r + 1));
+                    y[0] += f.x, y[1] += f.y, y[2] += f.z, y[3] += f.w;
+                    y[0] += h.x, y[1] += h.y, y[2] += h.z, y[3] += h.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = activate<KIND>(a, y[e] + bias[e]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) static_cast<O*>(a.out)[m * a.ldo + n + e] = rounded<O>(a.residual ? y[e] + old[e] : y[e]);
             }
         }
         cluster_sync_all();
@@ -497,21 +669,33 @@ void with_cluster(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int c
     cfg.numAttrs = ctas > 1 ? 2 : 1;
 }
 
-template <typename T, typename O, int NT>
-cudaError_t launch_few(const Args& a, int num_sms, cudaStream_t st) {
-    const long long rows = (a.N + kFewRows - 1) / kFewRows, tokens = (a.M + 8 * NT - 1) / (8 * NT);
+template <typename T, typename O, int NT, int KG>
+cudaError_t launch_few_by(const Args& a, int num_sms, cudaStream_t st) {
+    constexpr int ROWS = kFewRows * kFewWarps / KG;
+    const long long rows = (a.N + ROWS - 1) / ROWS, tokens = (a.M + 8 * NT - 1) / (8 * NT);
     // CTAs that share k, while that leaves two or fewer per SM and each warp something to do
     int n_split = 1;
-    while (n_split < 8 && rows * tokens * n_split * 2 <= 2LL * num_sms && a.K > n_split * kFewWarps * 32 * kFewBlocks) n_split *= 2;
+    while (KG == kFewWarps && n_split < 8 && rows * tokens * n_split * 2 <= 2LL * num_sms &&
+           a.K > n_split * kFewWarps * 32 * kFewBlocks)
+        n_split *= 2;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)(rows * n_split), (unsigned)std::min(tokens, 65535LL), 1);
     cfg.blockDim = dim3(kFewWarps * 32, 1, 1);
     with_cluster(cfg, attr, n_split, st);
-    return cudaLaunchKernelEx(&cfg, linear16_few<T, O, NT>, a, n_split);
+    return cudaLaunchKernelEx(&cfg, linear16_few<T, O, NT, KG>, a, n_split);
 }
 
-template <typename T, typename O, int MODE>
+template <typename T, typename O, int NT>
+cudaError_t launch_few(const Args& a, int num_sms, cudaStream_t st) {
+    // warps that share k where it is long enough for them (one row of 241856 over k = 64: 95 us with eight warps on k)
+    constexpr int STEP = 32 * kFewBlocks;
+    if (a.K <= STEP) return launch_few_by<T, O, NT, 1>(a, num_sms, st);
+    if (a.K <= 4 * STEP) return launch_few_by<T, O, NT, 4>(a, num_sms, st);
+    return launch_few_by<T, O, NT, 8>(a, num_sms, st);
+}
+
+template <typename T, typename O, int MODE, int KIND>
 cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStream_t st) {
     const int width = MODE == kPair ? 2 * kRows : kRows, x_rows = MODE == kPair ? g.bn / 2 : g.bn;
     const int stage = (int)kRowsBytes + x_rows * kChunk * 2;
@@ -523,15 +707,22 @@ cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStrea
     cudaError_t e = encode_rows16_map(&tw, a.w, bf16, a.K, a.N, a.ldw, kChunk, kRows);
     if (e == cudaSuccess) e = encode_rows16_map(&tx, a.x, bf16, a.K, a.M, a.ldx, kChunk, x_rows);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(linear16_tc<T, O, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kRing + kBars + 1024));
+    e = cudaFuncSetAttribute(linear16_tc<T, O, MODE, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kRing + kBars + kPieces + 1024));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)(groups * ctas), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)g.stages * stage + kBars + 1024;
+    cfg.dynamicSmemBytes = (size_t)g.stages * stage + kBars + kPieces + 1024;
     with_cluster(cfg, attr, ctas, st);
-    return cudaLaunchKernelEx(&cfg, linear16_tc<T, O, MODE>, tw, tx, a, g, ctas);
+    return cudaLaunchKernelEx(&cfg, linear16_tc<T, O, MODE, KIND>, tw, tx, a, g, ctas);
+}
+
+template <typename T, typename O, int MODE>
+cudaError_t launch_kind(const Args& a, const Tiling& g, int ctas, int groups, cudaStream_t st) {
+    if (a.kind == kClamp) return launch_mode<T, O, MODE, kClamp>(a, g, ctas, groups, st);
+    if (a.kind == kSwish) return launch_mode<T, O, MODE, kSwish>(a, g, ctas, groups, st);
+    return launch_mode<T, O, MODE, kGelu>(a, g, ctas, groups, st);
 }
 
 template <typename T, typename O>
@@ -555,7 +746,7 @@ cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
         int split = 1;
         while (split < 8 && few_tiles * split * 2 <= num_sms && a.K >= split * 4 * kChunk) split *= 2;
         g.bn = (int)std::min<long long>(128, up(a.M, 32) * 32);
-        if (split > 1) return launch_mode<T, O, kSplit>(a, g, split, (int)few_tiles, st);
+        if (split > 1) return launch_kind<T, O, kSplit>(a, g, split, (int)few_tiles, st);
     }
     const double pair = best(2 * kRows, num_sms / 2, true);
     const int pair_bn = g.bn;
@@ -563,10 +754,10 @@ cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
     if (pair < single) {
         g.bn = pair_bn;
         const long long tiles = up(a.N, 2 * kRows) * up(a.M, g.bn);
-        return launch_mode<T, O, kPair>(a, g, 2, (int)std::min<long long>(tiles, num_sms / 2), st);
+        return launch_kind<T, O, kPair>(a, g, 2, (int)std::min<long long>(tiles, num_sms / 2), st);
     }
     const long long tiles = up(a.N, kRows) * up(a.M, g.bn);
-    return launch_mode<T, O, kSingle>(a, g, 1, (int)std::min<long long>(tiles, num_sms), st);
+    return launch_kind<T, O, kSingle>(a, g, 1, (int)std::min<long long>(tiles, num_sms), st);
 }
 
 int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
@@ -614,7 +805,18 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
     if ((reinterpret_cast<uintptr_t>(s->out) | reinterpret_cast<uintptr_t>(s->residual)) % size ||
         reinterpret_cast<uintptr_t>(s->bias) % 2)
         return bad("out, residual and bias must be aligned to their types");
-    Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, s->act, t_expire_next};
+    auto whole = [&](const void* base, long long ld) {
+        return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0;
+    };
+    Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, kClamp, 0.f, 0.f,
+              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next};
+    switch (s->act) {
+        case NLLB_ACT_NONE: a.c1 = -INFINITY; break;
+        case NLLB_ACT_RELU: break;
+        case NLLB_ACT_GELU: a.kind = kGelu; break;
+        case NLLB_ACT_GELU_TANH: a.kind = kSwish, a.c1 = 2.3022082f, a.c2 = 0.10294324f; break;  // 2 sqrt(2/pi) log2 e (1, 0.044715)
+        default: a.kind = kSwish, a.c1 = kLog2e;  // SILU
+    }
     t_expire_next = false;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int device = 0, num_sms = 0;

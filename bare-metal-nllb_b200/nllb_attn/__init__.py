@@ -234,11 +234,23 @@ def ptr(x) -> Optional[int]:
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
+_TYPE_CODES: dict = {}  # of torch's types (filled by the first use: torch is not needed before)
+
+
+def _types() -> dict:
+    if not _TYPE_CODES:
+        import torch
+        _TYPE_CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, "torch.float32": torch.float32,
+                            "torch.int32": torch.int32, "torch.uint8": torch.uint8, "torch.float16": torch.float16,
+                            "torch.bfloat16": torch.bfloat16, "cuda": torch.cuda})
+    return _TYPE_CODES
+
+
 def _dtype_code(x) -> int:
-    try:
-        return {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}[str(x.dtype)]
-    except KeyError:
-        raise ValueError(f"dtype must be float32, float16 or bfloat16, not {x.dtype}") from None
+    code = _types().get(x.dtype)
+    if code is None:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, not {x.dtype}")
+    return code
 
 
 def _rows(x, name, like, axes):
@@ -254,8 +266,8 @@ def _ints(x, name, n, like, dtype="torch.int32"):
     """Address of a contiguous device array of n entries (None passes NULL)."""
     if x is None:
         return None
-    if str(x.dtype) != dtype or x.numel() != n or not x.is_contiguous() or x.device != like.device:
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} entries on q's device")
+    if x.dtype is not _types()[dtype] or x.numel() != n or not x.is_contiguous() or x.get_device() != like.get_device():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} entries on {like.device}")
     return x.data_ptr()
 
 
@@ -659,14 +671,15 @@ def linear_int8_noalloc_status(stream=None) -> int:
     return load().nllb_linear_int8_noalloc_status(stream)
 
 
-def _matrix(x, name, shape, like, dtype):
+def _matrix(x, name, rows, cols, dtype, device):
     """Address of a matrix whose rows are contiguous, and the elements from one to the next."""
-    if tuple(x.shape) != shape or x.dtype != dtype or x.device != like.device:
-        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on x's device")
-    if x.numel() and shape[1] > 1 and x.stride(1) != 1:
+    if x.dtype is not dtype or x.shape != (rows, cols) or x.get_device() != device:
+        raise ValueError(f"{name} must be a {dtype} tensor {[rows, cols]} on GPU {device}")
+    row, col = x.stride()
+    if col != 1 and cols > 1 and rows:
         raise ValueError(f"the rows of {name} must be contiguous")
     # (a single row's stride may be anything)
-    return x.data_ptr(), x.stride(0) if shape[0] > 1 else shape[1]
+    return x.data_ptr(), row if rows > 1 else (cols + 7) // 8 * 8
 
 
 def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=None, stream=None):
@@ -674,33 +687,30 @@ def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=Non
     [M][K], w [N][K], bias [N] of one 16-bit type, residual and out [M][N] of
     it or fp32 (rows may be strided).  Runs on torch's current stream of x's
     device unless `stream` names another."""
-    import torch
-    lib = load()
-    (M, K), N = x.shape, w.shape[0]
+    (M, K), N, kind, device = x.shape, w.shape[0], x.dtype, x.get_device()
+    code = _types().get(kind, F32)
+    if code == F32:
+        raise ValueError(f"x must be float16 or bfloat16, not {kind}")
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}")
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"x must be float16 or bfloat16, not {x.dtype}")
-    kind = out.dtype if out is not None else out_dtype or x.dtype
-    if kind not in (x.dtype, torch.float32) or (out_dtype is not None and kind != out_dtype):
+    out_kind = out.dtype if out is not None else out_dtype or kind
+    out_code = _TYPE_CODES.get(out_kind)
+    if (out_code != code and out_code != F32) or (out_dtype is not None and out_kind != out_dtype):
         raise ValueError("out must have x's type or float32")
-    if not x.is_cuda:
+    if device < 0:
         raise ValueError("x must be on a GPU")
     if out is None:
-        out = torch.empty((M, N), dtype=kind, device=x.device)
-    if stream is None:
-        stream = current_stream(x.device.index)
-    a = Linear16Args(bias=_ints(bias, "bias", N, x, str(x.dtype)), dtype=_dtype_code(x), out_dtype=_dtype_code(out),
-                     act=ACTIVATIONS[act], M=M, N=N, K=K)
-    (a.x, a.ldx), (a.w, a.ldw) = _matrix(x, "x", (M, K), x, x.dtype), _matrix(w, "w", (N, K), x, x.dtype)
-    if M == 1:
-        a.ldx = -(-K // 8) * 8
-    if N == 1:
-        a.ldw = -(-K // 8) * 8
-    a.out, a.ldo = _matrix(out, "out", (M, N), x, kind)
-    if residual is not None:
-        a.residual, a.ldr = _matrix(residual, "residual", (M, N), x, kind)
-    _on_device(x.device, lambda: _check(lib, lib.nllb_linear16(ctypes.byref(a), stream), "nllb_linear16"))
+        out = x.new_empty((M, N), dtype=out_kind)
+    x_at, ldx = _matrix(x, "x", M, K, kind, device)
+    w_at, ldw = _matrix(w, "w", N, K, kind, device)
+    out_at, ldo = _matrix(out, "out", M, N, out_kind, device)
+    res_at, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_kind, device)
+    if bias is not None and (bias.dtype is not kind or bias.shape != (N,) or bias.get_device() != device
+                             or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous {kind} tensor {[N]} on GPU {device}")
+    a = Linear16Args(x_at, w_at, None if bias is None else bias.data_ptr(), res_at, out_at, ldx, ldw, ldr, ldo, code,
+                     out_code, ACTIVATIONS[act], M, N, K)
+    _call(device, "nllb_linear16", a, stream)
     return out
 
 
@@ -784,13 +794,20 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     return out_tok, out_logp
 
 
-def _on_device(device, call):
-    """call(), with the tensors' GPU the current one."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        return call()
-    with torch.cuda.device(device):
-        return call()
+def _call(device, name, args, stream):
+    """A library function of (arguments, stream) with GPU `device` the current
+    one, on `stream` or torch's current stream there."""
+    cuda = _types()["cuda"]
+    lib = load()
+    if stream is None:
+        stream = current_stream(device)
+    if device == cuda.current_device():
+        rc = getattr(lib, name)(ctypes.byref(args), stream)
+    else:
+        with cuda.device(device):
+            rc = getattr(lib, name)(ctypes.byref(args), stream)
+    if rc != OK:
+        _check(lib, rc, name)
 
 
 def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entropy=None, out_top_tok=None,
@@ -801,33 +818,32 @@ def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entr
     (log-probabilities of the targets [rows] fp32 or None, entropies [rows]
     fp32 or None, likeliest tokens [rows][top_n] int32 and their
     log-probabilities fp32, or None and None for top_n 0)."""
-    lib = load()
     rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    row, col = logits.stride()
+    if vocab > 1 and col != 1:
         raise ValueError("the rows of logits must be contiguous")
     if target is None and out_logp is not None:
         raise ValueError("out_logp needs target")
     if not 0 <= top_n <= LOGPROBS_MAX_TOP:
         raise ValueError(f"top_n must lie in [0, {LOGPROBS_MAX_TOP}]")
-    import torch
-    if not logits.is_cuda:
+    if logits.get_device() < 0:
         raise ValueError("logits must be on a GPU")
-    if stream is None:
-        stream = current_stream(logits.device.index)
-
-    def buffer(given, wanted, *shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=logits.device) if given is None and wanted else given
-
-    out_logp, out_entropy = buffer(out_logp, target is not None, rows), buffer(out_entropy, entropy, rows)
-    out_top_tok = buffer(out_top_tok, top_n > 0, rows, top_n, dtype=torch.int32)
-    out_top_logp = buffer(out_top_logp, top_n > 0, rows, top_n)
+    types = _types()
+    if target is not None and out_logp is None:
+        out_logp = logits.new_empty(rows, dtype=types["torch.float32"])
+    if entropy and out_entropy is None:
+        out_entropy = logits.new_empty(rows, dtype=types["torch.float32"])
+    if top_n and out_top_tok is None:
+        out_top_tok = logits.new_empty((rows, top_n), dtype=types["torch.int32"])
+    if top_n and out_top_logp is None:
+        out_top_logp = logits.new_empty((rows, top_n), dtype=types["torch.float32"])
     f = "torch.float32"
-    a = LogprobsArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _dtype_code(logits), vocab, rows, top_n,
+    a = LogprobsArgs(logits.data_ptr(), row if rows > 1 else vocab, _dtype_code(logits), vocab, rows, top_n,
                      _ints(target, "target", rows, logits), _ints(out_logp, "out_logp", rows, logits, f),
                      _ints(out_entropy, "out_entropy", rows, logits, f),
                      _ints(out_top_tok, "out_top_tok", rows * top_n, logits),
                      _ints(out_top_logp, "out_top_logp", rows * top_n, logits, f))
-    _on_device(logits.device, lambda: _check(lib, lib.nllb_logprobs(ctypes.byref(a), stream), "nllb_logprobs"))
+    _call(logits.get_device(), "nllb_logprobs", a, stream)
     return out_logp, out_entropy, out_top_tok, out_top_logp
 
 
