@@ -59,10 +59,11 @@ cudaError_t launch_linear_tc(const LinearArgs& a, int splits, float* ws, int* ti
 // planes [2][M][K] by launch_split_planes.  K % 64 == 0, K >= 64.
 cudaError_t configure_linear_tma();
 cudaError_t encode_half_map(CUtensorMap* map, const void* base, int cols, int rows, int planes);
-// Tensor map of rows of 16-bit values `ld` elements apart (nllb_linear16), box box_cols (64) x box_rows, 128-byte swizzle;
-// what lies past the rows and columns reads as 0.
-cudaError_t encode_rows16_map(CUtensorMap* map, const void* base, bool bf16, int cols, int rows, long long ld, int box_cols,
-                              int box_rows);
+// Tensor map of rows `ld` elements apart (nllb_linear16), box box_cols x box_rows, with the 128-byte swizzle or none; what
+// lies past the rows and columns reads as 0 and is not written.
+enum class MapType { f32, f16, bf16 };
+cudaError_t encode_rows_map(CUtensorMap* map, const void* base, MapType type, int cols, int rows, long long ld, int box_cols,
+                            int box_rows, bool swizzle);
 int linear_tma_splits(int M, int N, int K, int num_sms);
 // Persistent 128 x 256-tile form (K % 32 == 0), used when the output has
 // enough tiles for its K (linear_tma_use_persistent); its tensor maps: planes box 32 x 128 x 2,

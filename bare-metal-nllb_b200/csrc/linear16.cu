@@ -40,7 +40,7 @@ struct Args {
     long long ldx, ldw, ldr, ldo;
     int M, N, K, kind;
     float c1, c2;  // of the activation
-    bool out_whole, res_whole;  // (there and) the rows start on 16 bytes
+    bool out_whole, res_whole;  // (there and) the rows start on 16 bytes, as TMA has it
     bool expire;  // test: a wait runs out
 };
 
@@ -74,23 +74,45 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return c;
 }
 
-// |y| erfc(|y| / sqrt 2) / 2, what y max 0 exceeds gelu(y) by.  With z = |y| / sqrt 2 and t = 1 / (1 + z / 2), erfc z =
-// t 2^(P(t) - z^2 log2 e); P of degree 9 is fitted to log2 (e^(z^2) erfc z / t) over z in [0, 10.2], where its largest error
-// is 4.6e-8, and 2.1e-7 when it is evaluated in fp32 (the library's erfcf takes several times as long: 471 rows of 40012
-// over k = 155 71 us).
-__device__ __forceinline__ float gelu_gap(float y) {
-    const float x = fminf(fabsf(y), 30.0f), t = rcp(fmaf(x, 0.35355339f, 1.0f));  // (0 from 15 on; finite for infinities)
-    float p = 0.20728277f;
-    p = fmaf(p, t, -0.97266638f);
-    p = fmaf(p, t, 1.6471334f);
-    p = fmaf(p, t, -0.97694308f);
-    p = fmaf(p, t, -0.13727684f);
-    p = fmaf(p, t, 0.012391086f);
-    p = fmaf(p, t, 0.046664748f);
-    p = fmaf(p, t, 0.55840427f);
-    p = fmaf(p, t, 1.4406633f);
-    p = fmaf(p, t, -1.8256532f);
-    return 0.5f * x * t * ex2(fmaf(-0.72134752f * x, x, p));
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// |y| erfc(|y| / sqrt 2) / 2, what max(y, 0) exceeds gelu(y) by, for two of them.  With z = |y| / sqrt 2 and t = 1 / (1 + z / 2),
+// erfc z = t 2^(P(t) - z^2 log2 e); P of degree 9 is fitted to log2 (e^(z^2) erfc z / t) over z in [0, 10.2], where its largest
+// error is 4.6e-8, and 2.1e-7 when it is evaluated in fp32.  (The library's erfcf, which branches: 471 rows of 40012 over
+// k = 155 65 us.)
+__device__ __forceinline__ float2 gelu_gap(float2 y) {
+    auto both = [](float c) { return make_float2(c, c); };
+    const float2 x = make_float2(fminf(fabsf(y.x), 30.0f), fminf(fabsf(y.y), 30.0f));  // (0 from 15 on; finite for infinities)
+    const float2 d = fma2(x, both(0.35355339f), both(1.0f)), t = make_float2(rcp(d.x), rcp(d.y));
+    float2 p = fma2(both(0.20728277f), t, both(-0.97266638f));
+    p = fma2(p, t, both(1.6471334f));
+    p = fma2(p, t, both(-0.97694308f));
+    p = fma2(p, t, both(-0.13727684f));
+    p = fma2(p, t, both(0.012391086f));
+    p = fma2(p, t, both(0.046664748f));
+    p = fma2(p, t, both(0.55840427f));
+    p = fma2(p, t, both(1.4406633f));
+    p = fma2(p, t, both(-2.8256532f));  // (less 1: the half)
+    p = fma2(mul2(x, both(-0.72134752f)), x, p);
+    return mul2(mul2(x, t), make_float2(ex2(p.x), ex2(p.y)));
 }
 
 // The activations, each in a form whose small results keep their relative accuracy, in three kinds of code:
@@ -100,16 +122,27 @@ __device__ __forceinline__ float gelu_gap(float y) {
 //   kGelu
 enum { kClamp = 0, kSwish = 1, kGelu = 2 };
 template <int KIND>
-__device__ __forceinline__ float activate(const Args& a, float y) {
-    if constexpr (KIND == kClamp) return max_nan(y, a.c1);
+__device__ __forceinline__ float2 activate(const Args& a, float2 y) {
+    auto both = [](float c) { return make_float2(c, c); };
+    if constexpr (KIND == kClamp) return make_float2(max_nan(y.x, a.c1), max_nan(y.y, a.c1));
     if constexpr (KIND == kSwish) {
-        y = max_nan(y, -100.f);
-        return __fdividef(y, 1.0f + ex2(-y * fmaf(a.c2 * y, y, a.c1)));
+        y = make_float2(max_nan(y.x, -100.f), max_nan(y.y, -100.f));
+        const float2 z = mul2(y, fma2(mul2(y, both(-a.c2)), y, both(-a.c1)));
+        return make_float2(__fdividef(y.x, 1.0f + ex2(z.x)), __fdividef(y.y, 1.0f + ex2(z.y)));
     }
-    return max_nan(y, 0.f) - gelu_gap(y);
+    return fma2(gelu_gap(y), both(-1.0f), make_float2(max_nan(y.x, 0.f), max_nan(y.y, 0.f)));
 }
-__device__ __forceinline__ float activate(const Args& a, float y) {
-    return a.kind == kClamp ? activate<kClamp>(a, y) : a.kind == kSwish ? activate<kSwish>(a, y) : activate<kGelu>(a, y);
+template <int KIND, int N>
+__device__ __forceinline__ void activate(const Args& a, float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const float2 y = activate<KIND>(a, make_float2(v[j], v[j + 1]));
+        v[j] = y.x, v[j + 1] = y.y;
+    }
+}
+__device__ __forceinline__ float activate(const Args& a, float x) {
+    const float2 y = make_float2(x, x);
+    return (a.kind == kClamp ? activate<kClamp>(a, y) : a.kind == kSwish ? activate<kSwish>(a, y) : activate<kGelu>(a, y)).x;
 }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------
@@ -234,16 +267,17 @@ constexpr int kRows = 128, kChunk = 64;                 // weight rows of a CTA'
 constexpr uint32_t kRowsBytes = kRows * kChunk * 2;     // 16 KB
 constexpr int kDrain = 8, kThreads = (kDrain + 2) * 32; // warps that drain accumulators; 1 that fetches, 1 that multiplies
 constexpr int kMaxStages = 10;
-constexpr int kPiece = 16, kPieceLd = 36;               // tokens that a warp drains together; floats of their rows of 32
-constexpr uint32_t kPieces = kDrain * kPiece * kPieceLd * 4;
-constexpr uint32_t kBars = (2 * kMaxStages + 6) * 8 + 16;
-constexpr uint32_t kRing = 232448 - 1024 - kBars - kPieces;  // bytes of all stages at most
+constexpr int kPiece = 16;                              // a warp drains pieces of 32 columns by 16 tokens, each through a slot
+constexpr int kMaxSlots = 8;
+constexpr uint32_t kBars = (2 * kMaxStages + 6 + kDrain * kMaxSlots) * 8 + 16;
+constexpr uint32_t kSmem = 232448 - 1024;  // of a CTA, less what the alignment takes
 
 enum { kSingle = 0, kPair = 1, kSplit = 2 };
 
 struct Tiling {
     int bn;           // tokens of a tile, a multiple of 32 up to 256
     int stages;
+    int slots;        // of a warp: 8 where residual rows of 16 bits come through them, else 4
     int tiles_n, tiles_m;
     bool tokens_first;  // tiles of the same weights follow one another (else: of the same tokens)
 };
@@ -286,14 +320,33 @@ __device__ __forceinline__ void arrive_here(uint64_t* bar) {
     asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// 16 columns of this thread's lane (warp-wide), there after tmem_wait on the same registers.
-__device__ __forceinline__ void tmem_ask16(uint32_t taddr, float (&v)[16]) {
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// All but the last N stores have read their shared memory.
+template <int N>
+__device__ __forceinline__ void stores_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// 8 or 16 columns of this thread's lane (warp-wide), there after tmem_wait on the same registers.
+__device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
           "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -302,10 +355,17 @@ __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tmem_wait(float (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])
+                 :
+                 : "memory");
+}
 
 template <typename T, typename O, int MODE, int KIND>
 __global__ void __launch_bounds__(kThreads, 1)
-    linear16_tc(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const Args a, const Tiling g,
+    linear16_tc(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                const __grid_constant__ CUtensorMap to, const __grid_constant__ CUtensorMap tr, const Args a, const Tiling g,
                 int n_split) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -313,11 +373,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int stages = g.stages;
     const uint32_t x_rows = MODE == kPair ? g.bn / 2 : g.bn, stage_bytes = kRowsBytes + x_rows * (kChunk * 2);
     const uint32_t ring = stages * stage_bytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + ring);
+    constexpr uint32_t kSlot = kPiece * 32 * sizeof(O);
+    const uint32_t slots_at = base + ring;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + ring + g.slots * (kDrain * kSlot));
     uint64_t *empty = full + kMaxStages, *ready = empty + kMaxStages, *drained = ready + 2, *done = drained + 2, *never = done + 1;
-    uint32_t* slot = reinterpret_cast<uint32_t*>(never + 1);
+    uint64_t* landed = never + 1;  // residual pieces, by warp and slot
+    uint32_t* slot = reinterpret_cast<uint32_t*>(landed + kDrain * kMaxSlots);
     volatile int* gave_up = reinterpret_cast<volatile int*>(slot + 1);
-    float* pieces = reinterpret_cast<float*>(sm + ring + kBars);
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -354,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(done, 1);
         mbar_init(never, 1);
+        for (int i = 0; i < kDrain * kMaxSlots; ++i) mbar_init(landed + i, 1);
         fence_barrier_init();
         *gave_up = 0;
     }
@@ -389,14 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- fetch
         if (lane == 0) {
             const uint32_t full0 = MODE == kPair ? map_rank(full, 0) : 0u;
-            uint32_t i = 0;
+            uint32_t i = 0, s = 0, turn = 0;  // stages so far; the next one's place, and how often it has come round
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
                 const int n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0);
                 const int m0 = tokens_at(t) + (MODE == kPair ? rank * (int)x_rows : 0);
                 for (int c = c0; c < c1; ++c, ++i) {
-                    const uint32_t s = i % stages;
-                    if (i >= (uint32_t)stages && !(ok = wait_one(empty + s, (i / stages - 1) & 1))) break;
+                    if (turn > 0 && !(ok = wait_one(empty + s, (turn - 1) & 1))) break;
                     const uint32_t at = base + s * stage_bytes;
                     if constexpr (MODE == kPair) {
                         if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * stage_bytes);
@@ -407,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tma_2d(at, &tw, c * kChunk, n0, full + s);
                         tma_2d(at + kRowsBytes, &tx, c * kChunk, m0, full + s);
                     }
+                    if (++s == (uint32_t)stages) s = 0, ++turn;
                 }
             }
             // (given up: what is in flight lands before the CTA ends)
@@ -424,15 +487,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (a.expire) ok = __all_sync(0xffffffffu, wait_one(never, 0, kTestWaitBudgetCycles));  // nothing arrives there
             uint32_t leader;
             asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
-            uint32_t i = 0, n = 0;
+            uint32_t s = 0, turn = 0, n = 0;
             for (int t = first; t < tiles && ok; t += step, ++n) {
                 const uint32_t acc = n & 1;
                 if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait_one(drained + acc, (n / 2 - 1) & 1)))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * 256;
-                for (int c = c0; c < c1; ++c, ++i) {
-                    const uint32_t s = i % stages;
-                    if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, (i / stages) & 1)))) break;
+                for (int c = c0; c < c1; ++c) {
+                    if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, turn & 1)))) break;
                     tc_fence_after();
                     const uint64_t da = umma_desc_k_sw128(base + s * stage_bytes);
                     const uint64_t db = umma_desc_k_sw128(base + s * stage_bytes + kRowsBytes);
@@ -446,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else tc_commit(empty + s);
                     }
                     __syncwarp();
+                    if (++s == (uint32_t)stages) s = 0, ++turn;
                 }
                 if (!ok) break;
                 if (leader) {
@@ -463,140 +526,112 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else {
-        // ---- drain: lane quarter warp % 4; the tile's pieces of 16 tokens in turns between the two halves
+        // ---- drain: lane quarter warp % 4, a lane to a column; the tile's pieces in turns between the two halves.  Rows that
+        // start on 16 bytes go out by TMA, and their residual comes by TMA into the same slot, slots - 2 pieces ahead and
+        // across tiles.  (Through the lanes' registers a CTA had no more than the few KB of its L1 cache on their way: 238
+        // rows of 60608 over k = 320 with a residual in fp32 46 us.)
+        constexpr int PIECE = kPiece;
         const int quarter = warp & 3, half = warp >> 2;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        // A piece goes through shared memory, from a lane to a column to 16 bytes of a row to a lane: `per` lanes to a row of
-        // the warp's 32 columns.  (Straight from the lanes' columns each value took an instruction and an address of its own:
-        // 238 rows of 60608 over k = 320 49 us.)
-        constexpr int VEC = 16 / (int)sizeof(O), PER = 32 / VEC, AT_ONCE = 32 / PER, PASSES = kPiece / AT_ONCE;
-        // Residual rows that start on 16 bytes are asked for AHEAD pieces before their use, across tiles (238 rows of 60608
-        // over k = 320 in fp32: one piece ahead 49 us), others a piece before.
-        constexpr int AHEAD = sizeof(O) == 4 ? 4 : 6;
-        float* piece = pieces + warp * kPiece * kPieceLd;
-        const int pr = lane / PER, pc = lane % PER * VEC;
-        struct Place { int n0, m0, count; };  // this warp's first column, the tile's first token, its pieces with tokens
+        const uint32_t from0 = tmem + ((uint32_t)(quarter * 32) << 16), mask = g.slots - 1, shift = g.slots == 8 ? 3 : 2;
+        const uint32_t slot0 = slots_at + warp * g.slots * kSlot;
+        O* const mem0 = reinterpret_cast<O*>(sm + (slot0 - base)) + lane;
+        uint64_t* const bars = landed + warp * kMaxSlots;
+        struct Place { int t, n0, m0, count; };  // a tile; this warp's first column, its first token, its pieces with tokens
         auto place_of = [&](int t) {
-            Place p = {0, 0, 0};
+            Place p = {t, 0, 0, 0};
             if (t < tiles) {
                 p.n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0) + quarter * 32, p.m0 = tokens_at(t);
-                p.count = (min(g.bn, a.M - p.m0) + kPiece - 1) / kPiece;
+                p.count = p.n0 < a.N ? (min(g.bn, a.M - p.m0) + PIECE - 1) / PIECE : 0;
             }
             return p;
         };
-        uint4 res[AHEAD][PASSES];
-        // piece `half` + 2 j of a tile
-        auto residual = [&](const Place& at, int j, uint4 (&to)[PASSES]) {
-            const int i = half + 2 * j, m0 = at.m0 + i * kPiece + pr;
-            if (!(i < at.count && at.n0 + 32 <= a.N)) return;
-            const O* p = static_cast<const O*>(a.residual) + m0 * a.ldr + at.n0 + pc;
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i)
-                if (m0 + i * AT_ONCE < a.M) to[i] = ld_coherent(reinterpret_cast<const uint4*>(p + i * AT_ONCE * a.ldr));
-        };
-        Place here = place_of(first);
-        uint32_t n = 0;
-        int asked = 0;  // slots that the tile before this one has filled
-        for (int t = first; t < tiles; t += step, ++n) {
-            const uint32_t acc = n & 1;
-            const Place there = place_of(t + step);  // the next tile
-            const int n0 = here.n0, m0 = here.m0, count = here.count;
-            const bool mine = n0 + lane < a.N, out_whole = a.out_whole && n0 + 32 <= a.N;
-            const bool res_whole = a.res_whole && n0 + 32 <= a.N, res_lanes = a.residual && !res_whole && mine;
-            O old[kPiece];
-            auto residual_lanes = [&](int col) {
-                const int rows = min(kPiece, a.M - m0 - col);
-                const O* p = static_cast<const O*>(a.residual) + (long long)(m0 + col) * a.ldr + n0 + lane;
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j, p += a.ldr)
-                    if (j < rows) old[j] = ld_coherent(p);
-            };
-            if (MODE != kSplit && a.residual) {
-                if (a.res_whole) {
-#pragma unroll
-                    for (int k = 0; k < AHEAD; ++k)
-                        if (k >= asked) residual(here, k, res[k]);
-                }
-                if (res_lanes && half < count) residual_lanes(half * kPiece);
+        Place here = place_of(first), there = here;
+        int next_asked = half;            // of `there`: the piece whose residual is asked for next
+        uint32_t used = 0, asked = 0;     // pieces of this warp
+        auto ask = [&] {
+            while (there.t < tiles && next_asked >= there.count) there = place_of(there.t + step), next_asked = half;
+            if (there.t >= tiles) return;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(bars + (asked & mask), kSlot);
+                tma_2d(slot0 + (asked & mask) * kSlot, &tr, there.n0, there.m0 + next_asked * PIECE, bars + (asked & mask));
             }
-            if (!__all_sync(0xffffffffu, wait_one(ready + acc, (n / 2) & 1))) break;
+            ++asked, next_asked += 2;
+        };
+        if (MODE != kSplit && a.res_whole)
+            for (int i = 0; i < g.slots - 2; ++i) ask();
+        bool ok = true;
+        uint32_t n = 0;
+        for (; here.t < tiles && ok; here = place_of(here.t + step), ++n) {
+            const uint32_t acc = n & 1, from = from0 + acc * 256;
+            if (!(ok = __all_sync(0xffffffffu, wait_one(ready + acc, (n / 2) & 1)))) break;
             tc_fence_after();
-            const uint32_t from = tmem + lanes + acc * 256;
             if constexpr (MODE == kSplit) {
                 // over the ring, which is done with and larger (a partial sum takes 64 KB at most)
                 float* part = reinterpret_cast<float*>(sm) + quarter * 32 + lane;
-                for (int col = half * kPiece; col < g.bn; col += 2 * kPiece) {
-                    float v[kPiece];
-                    tmem_ask16(from + col, v);
+                for (int col = half * PIECE; col < g.bn; col += 2 * PIECE) {
+                    float v[PIECE];
+                    tmem_ask(from + col, v);
                     tmem_wait(v);
 #pragma unroll
-                    for (int j = 0; j < kPiece; ++j) part[(col + j) * kRows] = v[j];
+                    for (int j = 0; j < PIECE; ++j) part[(col + j) * kRows] = v[j];
                 }
                 break;  // (one tile)
             } else {
-                const float bias = a.bias && mine ? as_float(ld_coherent(static_cast<const T*>(a.bias) + n0 + lane)) : 0.f;
-                float next[kPiece];
-                if (half < count) tmem_ask16(from + half * kPiece, next);
-                for (int j0 = 0; half + 2 * j0 < count; j0 += AHEAD) {
+                const bool mine = here.n0 + lane < a.N;
+                const float bias = a.bias && mine ? as_float(ld_coherent(static_cast<const T*>(a.bias) + here.n0 + lane)) : 0.f;
+                const bool res_lanes = a.residual && !a.res_whole && mine;
+                O old[PIECE];  // (asked for a piece ahead)
+                auto ask_lanes = [&](int i) {
+                    const int m0 = here.m0 + i * PIECE;
+                    const O* p = static_cast<const O*>(a.residual) + m0 * a.ldr + here.n0 + lane;
 #pragma unroll
-                    for (int k = 0; k < AHEAD; ++k) {  // (each with registers of its own for the residual)
-                        const int i = half + 2 * (j0 + k), col = i * kPiece;
-                        if (i >= count) break;
-                        float v[kPiece];
-                        tmem_wait(next);
+                    for (int j = 0; j < PIECE; ++j, p += a.ldr)
+                        if (m0 + j < a.M) old[j] = ld_coherent(p);
+                };
+                if (res_lanes && half < here.count) ask_lanes(half);
+                float next[PIECE];
+                if (half < here.count) tmem_ask(from + half * PIECE, next);
+                for (int i = half; i < here.count; i += 2, ++used) {
+                    const int m0 = here.m0 + i * PIECE, rows = min(PIECE, a.M - m0);
+                    const uint32_t at = used & mask;
+                    O* mem = mem0 + at * (kSlot / sizeof(O));
+                    float v[PIECE];
+                    tmem_wait(next);
 #pragma unroll
-                        for (int j = 0; j < kPiece; ++j) v[j] = activate<KIND>(a, next[j] + bias);
-                        if (i + 2 < count) tmem_ask16(from + col + 2 * kPiece, next);
-                        if (res_lanes) {
+                    for (int j = 0; j < PIECE; ++j) v[j] = next[j] + bias;
+                    if (i + 2 < here.count) tmem_ask(from + (i + 2) * PIECE, next);
+                    activate<KIND>(a, v);
+                    if (a.res_whole) {
+                        if (!(ok = __all_sync(0xffffffffu, wait_one(bars + at, (used >> shift) & 1)))) break;
 #pragma unroll
-                            for (int j = 0; j < kPiece; ++j) v[j] += as_float(old[j]);  // (rows past the last one: unused)
-                            if (i + 2 < count) residual_lanes(col + 2 * kPiece);
-                        }
-                        if (out_whole || res_whole) {
+                        for (int j = 0; j < PIECE; ++j) v[j] += as_float(mem[j * 32]);
+                    } else if (res_lanes) {
 #pragma unroll
-                            for (int j = 0; j < kPiece; ++j) piece[j * kPieceLd + lane] = v[j];
-                            __syncwarp();
-#pragma unroll
-                            for (int r0 = 0; r0 < PASSES; ++r0) {
-                                const int r = r0 * AT_ONCE + pr, m = m0 + col + r;
-                                float y[VEC];
-#pragma unroll
-                                for (int e = 0; e < VEC; e += 4) {
-                                    const float4 f = *reinterpret_cast<const float4*>(piece + r * kPieceLd + pc + e);
-                                    y[e] = f.x, y[e + 1] = f.y, y[e + 2] = f.z, y[e + 3] = f.w;
-                                }
-                                if (res_whole) {
-                                    float z[VEC];
-                                    rows_unpack<O>(res[k][r0], z);
-#pragma unroll
-                                    for (int e = 0; e < VEC; ++e) y[e] += z[e];
-                                }
-                                O* to = static_cast<O*>(a.out) + m * a.ldo + n0 + pc;
-                                if (m < a.M) {
-                                    if (out_whole) {
-                                        *reinterpret_cast<uint4*>(to) = rows_pack<O>(y);
-                                    } else {
-#pragma unroll
-                                        for (int e = 0; e < VEC; ++e) to[e] = rounded<O>(y[e]);
-                                    }
-                                }
-                            }
-                        } else if (mine) {
-                            const int rows = min(kPiece, a.M - m0 - col);
-                            O* p = static_cast<O*>(a.out) + (long long)(m0 + col) * a.ldo + n0 + lane;
-#pragma unroll
-                            for (int j = 0; j < kPiece; ++j, p += a.ldo)
-                                if (j < rows) *p = rounded<O>(v[j]);
-                        }
-                        if (a.res_whole) {
-                            if (half + 2 * (j0 + k + AHEAD) < count) residual(here, j0 + k + AHEAD, res[k]);
-                            else residual(there, k, res[k]);
-                        }
-                        __syncwarp();
+                        for (int j = 0; j < PIECE; ++j) v[j] += as_float(old[j]);  // (rows past the last one: unused)
+                        if (i + 2 < here.count) ask_lanes(i + 2);
                     }
+                    if (a.out_whole) {
+                        if (!a.res_whole) {  // (else the slot's last store has been waited for)
+                            if (lane == 0) stores_read<3>();
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j) mem[j * 32] = rounded<O>(v[j]);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&to, here.n0, m0, slot0 + at * kSlot);
+                            if (a.res_whole) stores_read<2>();
+                        }
+                    } else if (mine) {
+                        O* p = static_cast<O*>(a.out) + m0 * a.ldo + here.n0 + lane;
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j, p += a.ldo)
+                            if (j < rows) *p = rounded<O>(v[j]);
+                    }
+                    __syncwarp();
+                    if (a.res_whole) ask();  // into the slot of the piece before the last
                 }
-                asked = half < count ? min(AHEAD, (count - half + 1) / 2) : 0;
-                here = there;
                 tmem_wait(next);  // (what was asked for and not used)
                 tc_fence_before();
                 __syncwarp();
@@ -606,6 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+        // nothing reads or writes shared memory once the CTA has ended
+        if (lane == 0) stores_done();
+        for (; used < asked; ++used) (void)mbar_wait_bounded(bars + (used & mask), (used >> shift) & 1, kTestWaitBudgetCycles);
     }
 
     tc_fence_before();
@@ -639,7 +677,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     y[0] += h.x, y[1] += h.y, y[2] += h.z, y[3] += h.w;
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = activate<KIND>(a, y[e] + bias[e]);
+                for (int e = 0; e < 4; ++e) y[e] += bias[e];
+                activate<KIND>(a, y);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (n + e < a.N) static_cast<O*>(a.out)[m * a.ldo + n + e] = rounded<O>(a.residual ? y[e] + old[e] : y[e]);
@@ -699,23 +738,29 @@ template <typename T, typename O, int MODE, int KIND>
 cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStream_t st) {
     const int width = MODE == kPair ? 2 * kRows : kRows, x_rows = MODE == kPair ? g.bn / 2 : g.bn;
     const int stage = (int)kRowsBytes + x_rows * kChunk * 2;
-    g.stages = std::min(kMaxStages, (int)kRing / stage);
+    constexpr uint32_t kSlot = kPiece * 32 * sizeof(O);
+    g.slots = MODE == kSplit ? 0 : a.res_whole && sizeof(O) == 2 ? 8 : 4;
+    g.stages = std::min(kMaxStages, ((int)(kSmem - kBars) - g.slots * (int)(kDrain * kSlot)) / stage);
     g.tiles_n = (a.N + width - 1) / width, g.tiles_m = (a.M + g.bn - 1) / g.bn;
     g.tokens_first = (long long)a.N >= a.M;  // the larger operand is read once, while its tile is in use
-    CUtensorMap tw, tx;
-    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    cudaError_t e = encode_rows16_map(&tw, a.w, bf16, a.K, a.N, a.ldw, kChunk, kRows);
-    if (e == cudaSuccess) e = encode_rows16_map(&tx, a.x, bf16, a.K, a.M, a.ldx, kChunk, x_rows);
+    CUtensorMap tw, tx, to, tr;
+    constexpr MapType type = std::is_same<T, __nv_bfloat16>::value ? MapType::bf16 : MapType::f16;
+    constexpr MapType out_type = sizeof(O) == 4 ? MapType::f32 : type;
+    cudaError_t e = encode_rows_map(&tw, a.w, type, a.K, a.N, a.ldw, kChunk, kRows, true);
+    if (e == cudaSuccess) e = encode_rows_map(&tx, a.x, type, a.K, a.M, a.ldx, kChunk, x_rows, true);
+    to = tr = tx;  // (not looked at)
+    if (e == cudaSuccess && a.out_whole) e = encode_rows_map(&to, a.out, out_type, a.N, a.M, a.ldo, 32, kPiece, false);
+    if (e == cudaSuccess && a.res_whole) e = encode_rows_map(&tr, a.residual, out_type, a.N, a.M, a.ldr, 32, kPiece, false);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(linear16_tc<T, O, MODE, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kRing + kBars + kPieces + 1024));
+    e = cudaFuncSetAttribute(linear16_tc<T, O, MODE, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)(groups * ctas), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)g.stages * stage + kBars + kPieces + 1024;
+    cfg.dynamicSmemBytes = (size_t)g.stages * stage + g.slots * kDrain * kSlot + kBars + 1024;
     with_cluster(cfg, attr, ctas, st);
-    return cudaLaunchKernelEx(&cfg, linear16_tc<T, O, MODE, KIND>, tw, tx, a, g, ctas);
+    return cudaLaunchKernelEx(&cfg, linear16_tc<T, O, MODE, KIND>, tw, tx, to, tr, a, g, ctas);
 }
 
 template <typename T, typename O, int MODE>
@@ -806,7 +851,7 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
         reinterpret_cast<uintptr_t>(s->bias) % 2)
         return bad("out, residual and bias must be aligned to their types");
     auto whole = [&](const void* base, long long ld) {
-        return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0;
+        return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0 && ld <= 1LL << 36;
     };
     Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, kClamp, 0.f, 0.f,
               whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next};

@@ -908,17 +908,20 @@ cudaError_t encode_half_map_box(CUtensorMap* map, const void* base, int cols, in
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t encode_rows16_map(CUtensorMap* map, const void* base, bool bf16, int cols, int rows, long long ld, int box_cols,
-                              int box_rows) {
+cudaError_t encode_rows_map(CUtensorMap* map, const void* base, MapType type, int cols, int rows, long long ld, int box_cols,
+                            int box_rows, bool swizzle) {
     if (!tensor_map_encoder()) return cudaErrorNotSupported;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * (type == MapType::f32 ? 4 : 2)};
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = g_encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = g_encode(map,
+                                type == MapType::f32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : type == MapType::f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
