@@ -772,8 +772,14 @@ cudaError_t launch_kind(const Args& a, const Tiling& g, int ctas, int groups, cu
 
 template <typename T, typename O>
 cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
-    if (a.M <= 8) return launch_few<T, O, 1>(a, num_sms, st);
-    if (a.M <= 16 || a.K < kChunk) return launch_few<T, O, 2>(a, num_sms, st);
+    // Few tokens: warp-level products while the weights are few as well, for the tensor cores then take longer to start (4096 x
+    // 1024 by 1, 16 and 32 tokens 3.5, 4.2 and 7.6 us against 6.9 on the tensor cores; 1024 x 1024 by 32 4.2 against 6.8); they
+    // keep more of the weights on their way (16384 x 1024 by 1 and 16 10.2 and 14.3 us against 8.9 and 9.5).
+    const long long weights = (long long)a.N * a.K;
+    if (a.K < kChunk) return a.M <= 8 ? launch_few<T, O, 1>(a, num_sms, st) : launch_few<T, O, 2>(a, num_sms, st);
+    if (a.M <= 8 && weights < 1 << 24) return launch_few<T, O, 1>(a, num_sms, st);
+    if (a.M <= 16 && weights <= 1 << 23) return launch_few<T, O, 2>(a, num_sms, st);
+    if (a.M <= 32 && weights <= 1 << 21) return launch_few<T, O, 4>(a, num_sms, st);
     auto up = [](long long x, long long to) { return (x + to - 1) / to; };
     Tiling g = {};
     // the tile of tokens whose rounds over the SMs take the least, by the wider of products and operands
@@ -788,8 +794,9 @@ cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
     };
     const long long few_tiles = up(a.N, kRows) * up(a.M, 128);
     if (few_tiles * 2 <= num_sms) {
+        // (more than eight clusters of eight are not all at work at once: 16 tokens by 2048 x 1024 11 us)
         int split = 1;
-        while (split < 8 && few_tiles * split * 2 <= num_sms && a.K >= split * 4 * kChunk) split *= 2;
+        while (split < (few_tiles <= 8 ? 8 : 4) && few_tiles * split * 2 <= num_sms && a.K >= split * 4 * kChunk) split *= 2;
         g.bn = (int)std::min<long long>(128, up(a.M, 32) * 32);
         if (split > 1) return launch_kind<T, O, kSplit>(a, g, split, (int)few_tiles, st);
     }

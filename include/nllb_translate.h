@@ -204,8 +204,9 @@ typedef struct {
 NLLB_ATTN_API int nllb_linear16(const nllb_linear16_args* args, void* stream);
 NLLB_ATTN_API int nllb_linear16_status(void* stream);
 /* Test of the bounded device waits: if the calling thread's next nllb_linear16
- * runs on the tensor-core kernel (more than 16 rows), a wait of its runs out
- * after about 1 ms and nllb_linear16_status reports it.  Later calls are as ever. */
+ * runs on the tensor-core kernel (more than 32 rows, or 2^24 weights, of K >= 64),
+ * a wait of its runs out after about 1 ms and nllb_linear16_status reports it.
+ * Later calls are as ever. */
 NLLB_ATTN_API int nllb_linear16_test_expire_next_wait(void);
 
 /* ---- per-step vocabulary operations of the beam search --------------------

@@ -78,7 +78,8 @@ SIZES = [
     (13, 300, 8192), (3, 5003, 65), (40, 100, 1), (200, 33, 40), (70000, 5, 8),
     (17, 1, 64), (17, 128, 64), (31, 129, 100), (32, 127, 1000), (33, 1024, 4096), (64, 5003, 1024), (65, 256, 72), (100, 1000, 2048),
     (128, 128, 128), (129, 640, 513), (200, 300, 8192), (256, 20000, 96), (257, 1023, 1024), (1000, 1024, 512), (3000, 4099, 200),
-    (10000, 1024, 64), (4097, 4096, 128), (300, 40001, 64),
+    (10000, 1024, 64), (4097, 4096, 128), (300, 40001, 64), (1, 40000, 700), (16, 9001, 1000), (27, 1000, 1000), (32, 128, 8192),
+    (20, 16, 72), (12, 2048, 4104),
 ]
 
 
