@@ -14,9 +14,11 @@
 // running maximum grows anyway, which vector it came from.  Of n tokens in the
 // order (falling logit, rising index) each lies in one of the n stripes whose
 // maxima come first in that order -- n of them are ahead of any other stripe's
-// -- so those stripes alone are read again, a warp to a stripe, and what is not
-// behind the n-th maximum goes through sorted lists of 32 in registers.  A row
+// -- so of those stripes the vectors that hold the maxima are read again, and
+// the other vectors only if the largest of them is not below the n-th maximum.
+// What is not behind that goes through sorted lists of 32 in registers.  A row
 // with many equal or rising logits takes more batches of 32, never another way.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -30,11 +32,12 @@ namespace {
 
 using u64 = unsigned long long;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kUnroll = 4;         // 16-byte vectors of a thread in flight
-constexpr int kMaxCluster = 16;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kPerSm = 4;
+constexpr int kUnroll = 4;         // 16-byte vectors that a thread takes together, while as many are on their way
+constexpr int kMaxCluster = 2 * kWarps;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNoWeight = -200.0f;  // 2^-200 is 0 in fp32
+constexpr float kLag = 8.0f;          // what a running maximum may be behind by: a warp's sums are rarely moved then
 // A largest scaled logit of this size and more: what M was rounded by could be more than an exponent holds, and different
 // logits are at least 32 apart.
 constexpr float kFar = 0x1.8p28f;
@@ -49,7 +52,7 @@ struct Args {
     float* out_top_logp;
 };
 
-struct State {  // of a set of tokens: sums of 2^(y - m) and 2^(y - m) (y - m), y = l log2(e)
+struct State {  // of a set of tokens: sums of 2^(y - m) and 2^(y - m) (y - m), y = l log2(e), none above m + kLag
     float m, z, s;
 };
 
@@ -57,6 +60,8 @@ struct Shared {
     State warp[kWarps];
     State cta;
     u64 list[kWarps][32];
+    u64 kept[kWarps][64];
+    float second[kThreads];
     uint32_t top, n_top;  // beyond kFar: the largest logit's order, and how many there are
 };
 
@@ -87,6 +92,40 @@ __device__ __forceinline__ State join(State a, State b) {
     move_to(a, m);
     move_to(b, m);
     return {m, a.z + b.z, a.s + b.s};
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// The largest of a vector's logits (NaN are passed over).
+template <typename T>
+__device__ __forceinline__ float largest(uint4 u) {
+    if constexpr (std::is_same<T, float>::value) {
+        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        auto as = [](uint32_t& w) { return *reinterpret_cast<T2*>(&w); };
+        const T2 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
+        if constexpr (std::is_same<T, __half>::value) return fmaxf(__low2float(m), __high2float(m));
+        else return fmaxf(__low2float(m), __high2float(m));
+    }
 }
 
 // Bits that order like the logits (-0 as +0, NaN as -inf).
@@ -140,7 +179,7 @@ __device__ __forceinline__ float to_float(T x) {
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int C) {
+__global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a, int C) {
     constexpr int VEC = 16 / (int)sizeof(T);
     __shared__ Shared sh;
     pdl_launch_dependents();
@@ -169,83 +208,102 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int
     const int n_single = rank == 0 ? head + a.vocab - tail : 0;  // rank 0's
     auto single = [&](int i) { return i < head ? i : tail + i - head; };
     const uint4* vec = reinterpret_cast<const uint4*>(src + head);
-    const int per = (n_vec + C - 1) / C, v_end = min(n_vec, (rank + 1) * per), v_begin = min(n_vec, rank * per) + tid;
+    const int per = (n_vec + C - 1) / C, v_end = min(n_vec, (rank + 1) * per), v_first = min(n_vec, rank * per);
 
-    State st = {-INFINITY, 0.f, 0.f};
+    float m = -INFINITY;  // the warp's
+    float2 z[2], sy[2];   // 2^y and 2^y y, in four chains
+    z[0] = z[1] = sy[0] = sy[1] = make_float2(0.f, 0.f);
+    auto move = [&](float to) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            State x = {m, z[i].x, sy[i].x}, y = {m, z[i].y, sy[i].y};
+            move_to(x, to);
+            move_to(y, to);
+            z[i] = make_float2(x.z, y.z), sy[i] = make_float2(x.s, y.s);
+        }
+        m = to;
+    };
+    auto lagging = [&](float t) {  // a scaled logit of this lane; the whole warp asks
+        if (__any_sync(0xffffffffu, t > m + kLag)) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            move(t);
+        }
+    };
     float best = -INFINITY;
     uint32_t best_at = 0xffffffffu;  // the stripe's first vector that holds its maximum
-    auto batch = [&](const uint4 (&u)[kUnroll], int at) {
-        float x[kUnroll][VEC], top[kUnroll];
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            rows_unpack<T>(u[k], x[k]);
-            top[k] = x[k][0];
-#pragma unroll
-            for (int e = 1; e < VEC; ++e) top[k] = fmaxf(top[k], x[k][e]);
-        }
-        float t = top[0];
-#pragma unroll
-        for (int k = 1; k < kUnroll; ++k) t = fmaxf(t, top[k]);
-        if (t > best) {
-            best = t;
-#pragma unroll
-            for (int k = kUnroll - 1; k >= 0; --k)
-                if (top[k] == t) best_at = at + k * kThreads;
-            move_to(st, t * kLog2e);
-        }
-        const float off = -st.m;
-        float z[2] = {0.f, 0.f}, s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float y = fmaf(x[k][e], kLog2e, off);
-                const float w = weigh(y);
-                z[e & 1] += w;
-                s[e & 1] = fmaf(w, y, s[e & 1]);
-            }
-        st.z += z[0] + z[1];
-        st.s += s[0] + s[1];
-    };
-    int v = v_begin;
-    for (; v + (kUnroll - 1) * kThreads < v_end; v += kUnroll * kThreads) {
-        uint4 u[kUnroll];
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k) u[k] = ld_coherent(vec + v + k * kThreads);
-        batch(u, v);
-    }
-    if (v < v_end) {
-        // (-inf in every element: no weight, no maximum)
-        const uint32_t none = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-        uint4 u[kUnroll];
+    float second = -INFINITY;        // the largest of its other vectors' maxima
+    // (past the end: -inf in every element, no weight and no maximum)
+    constexpr uint32_t none = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    auto load = [&](uint4 (&u)[kUnroll], int v) {
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
             u[k] = v + k * kThreads < v_end ? ld_coherent(vec + v + k * kThreads) : make_uint4(none, none, none, none);
-        batch(u, v);
+    };
+    auto batch = [&](const uint4 (&u)[kUnroll], int at) {
+        float top[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            top[k] = largest<T>(u[k]);
+            if constexpr (TOP) {
+                second = fmaxf(second, fminf(best, top[k]));
+                if (top[k] > best) best = top[k], best_at = at + k * kThreads;
+            }
+        }
+        lagging(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * kLog2e);
+        const float2 off = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            float x[VEC];
+            rows_unpack<T>(u[k], x);
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+                float2 y = fma2(make_float2(x[e], x[e + 1]), scale, off), w;
+                w.x = weigh(y.x), w.y = weigh(y.y);
+                z[(e >> 1) & 1] = add2(z[(e >> 1) & 1], w);
+                sy[(e >> 1) & 1] = fma2(w, y, sy[(e >> 1) & 1]);
+            }
+        }
+    };
+    static_assert(kUnroll == 4, "four vectors together");
+    {
+        uint4 u[kUnroll], v[kUnroll];
+        constexpr int STEP = kUnroll * kThreads;
+        int at = v_first + tid;
+        const int last = v_end - warp * 32 + tid;  // (the same turns for a whole warp)
+        load(u, at);
+        while (at < last) {
+            load(v, at + STEP);
+            batch(u, at);
+            at += STEP;
+            if (at >= last) break;
+            load(u, at + STEP);
+            batch(v, at);
+            at += STEP;
+        }
     }
-    for (int i = tid; i < n_single; i += kThreads) {
-        const float l = to_float(ld_coherent(src + single(i)));
-        if (l * kLog2e > st.m) move_to(st, l * kLog2e);
-        float y = fmaf(l, kLog2e, -st.m);
+    if (n_single > 0) {  // (fewer than 32)
+        const float l = tid < n_single ? to_float(ld_coherent(src + single(tid))) : -INFINITY;
+        lagging(l * kLog2e);
+        float y = fmaf(l, kLog2e, -m);
         const float w = weigh(y);
-        st.z += w;
-        st.s = fmaf(w, y, st.s);
+        z[0].x += w;
+        sy[0].x = fmaf(w, y, sy[0].x);
     }
 
     // ---- the row's M, Z and S
+    State st = {m, (z[0].x + z[0].y) + (z[1].x + z[1].y), (sy[0].x + sy[0].y) + (sy[1].x + sy[1].y)};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        State b;
-        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        b.z = __shfl_xor_sync(0xffffffffu, st.z, o);
-        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        st = join(st, b);
+        st.z += __shfl_xor_sync(0xffffffffu, st.z, o);
+        st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
     }
     if (lane == 0) sh.warp[warp] = st;
     if (tid == 0) sh.top = sh.n_top = 0;
     u64 list = 0;
     if constexpr (TOP) {
         // the stripes whose maxima come first, by the index of the vector's first element
+        sh.second[tid] = second;
         u64 key = best_at == 0xffffffffu ? 0 : order_key(best, (uint32_t)head + best_at * VEC);
         key = merge_warps(sh, sort32(key, lane), kWarps, warp, lane);
         __syncthreads();
@@ -266,15 +324,39 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int
     }
     if constexpr (TOP) {
         const u64 bar = sh.list[0][a.top_n - 1];  // nothing behind it is among the first (0: fewer stripes)
+        const float least = logit_of((uint32_t)(bar >> 32));  // (bar 0: NaN)
+        u64* const kept = sh.kept[warp];
+        int n_kept = 0;
+        // this lane's element, of the vector whose first element gave `key`; 32 at a time go into the list
         auto take = [&](u64 key, int further, bool there) {
             const bool in = there && key >= bar && key > kNothing;
-            if (__any_sync(0xffffffffu, in)) list = merge32(list, sort32(in ? key - further : 0, lane), lane);
+            const unsigned who = __ballot_sync(0xffffffffu, in);
+            if (who == 0) return;
+            if (in) kept[n_kept + __popc(who & ((1u << lane) - 1u))] = key - further;
+            n_kept += __popc(who);
+            __syncwarp();
+            if (n_kept >= 32) {
+                n_kept -= 32;
+                list = merge32(list, sort32(kept[n_kept + lane], lane), lane);
+                __syncwarp();
+            }
         };
+        // the vectors that hold the stripes' maxima: an element to a lane
+        static_assert(kWarps * 32 >= NLLB_LOGPROBS_MAX_TOP * VEC, "one round");
+        if (warp * 32 < a.top_n * VEC) {
+            const int i = tid / VEC, e = tid % VEC;
+            const u64 stripe = i < a.top_n ? sh.list[0][i] : 0;
+            const bool there = stripe > kNothing;
+            const float l = there ? to_float(ld_coherent(src + key_index(stripe) + e)) : 0.f;
+            take(order_key(l, key_index(stripe)), e, there);
+        }
+        // the others of a stripe, where one of them may be among the first too
         for (int i = warp; i < a.top_n; i += kWarps) {
             const u64 stripe = sh.list[0][i];
             if (stripe <= kNothing) break;
-            const int t = ((int)(key_index(stripe) - head) / VEC - min(n_vec, rank * per)) % kThreads;  // whose
-            const int first = v_begin - tid + t, n = (v_end - first + kThreads - 1) / kThreads;
+            const int found = (int)(key_index(stripe) - head) / VEC, t = (found - v_first) % kThreads;
+            if (sh.second[t] < least) continue;
+            const int first = v_first + t, n = (v_end - first + kThreads - 1) / kThreads;
             for (int k0 = 0; k0 < n; k0 += 32 * kUnroll) {
                 uint4 u[kUnroll];
 #pragma unroll
@@ -285,17 +367,20 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int
 #pragma unroll
                 for (int j = 0; j < kUnroll; ++j) {
                     const int k = k0 + 32 * j + lane;
+                    const bool there = k < n && first + k * kThreads != found;
                     const uint32_t at = (uint32_t)head + (first + k * kThreads) * VEC;
+                    if (!__any_sync(0xffffffffu, there && !(largest<T>(u[j]) < least))) continue;
                     float x[VEC];
                     rows_unpack<T>(u[j], x);
                     // (an element stands behind the bar's vector, as its own vector does)
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) take(order_key(x[e], at), e, k < n);
+                    for (int e = 0; e < VEC; ++e) take(order_key(x[e], at), e, there);
                 }
             }
         }
         if (warp == kWarps - 1 && n_single > 0)
             take(lane < n_single ? order_key(to_float(ld_coherent(src + single(lane))), single(lane)) : 0, 0, lane < n_single);
+        if (n_kept > 0) list = merge32(list, sort32(lane < n_kept ? kept[lane] : 0, lane), lane);
         list = merge_warps(sh, list, kWarps, warp, lane);
         if (C > 1) {
             __syncthreads();
@@ -313,13 +398,14 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int
         }
         if constexpr (TOP) {
             if (rank == 0) {
-                list = 0;
-                if (warp < C) {
-                    const uint32_t at = map_rank(&sh.list[0][lane], warp);
-                    list = (u64)(uint32_t)ld_cluster_s32(at + 4) << 32 | (uint32_t)ld_cluster_s32(at);
-                }
+                auto of_rank = [&](int r) {
+                    const uint32_t at = map_rank(&sh.list[0][lane], r);
+                    return (u64)(uint32_t)ld_cluster_s32(at + 4) << 32 | (uint32_t)ld_cluster_s32(at);
+                };
+                list = warp < C ? of_rank(warp) : 0;
+                if (C > kWarps) list = merge32(list, of_rank(warp + kWarps), lane);
                 __syncthreads();
-                list = merge_warps(sh, list, C, warp, lane);
+                list = merge_warps(sh, list, min(C, kWarps), warp, lane);
             }
         }
     }
@@ -328,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Args a, int
     float most = 0.f;
     if (far) {
         auto each = [&](auto&& f) {
-            for (int i = v_begin; i < v_end; i += kThreads) {
+            for (int i = v_first + tid; i < v_end; i += kThreads) {
                 float x[VEC];
                 rows_unpack<T>(ld_coherent(vec + i), x);
 #pragma unroll
@@ -398,13 +484,15 @@ cudaError_t launch_one(const Args& a, int rows, int C, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch(const Args& a, int rows, int num_sms, cudaStream_t st) {
-    // CTAs of a row: what lets the last of them end first, at 22 bytes a nanosecond each and 2 us for what follows the stream
-    const double bytes = (double)a.vocab * sizeof(T);
+    // CTAs of a row, by what a call takes: the stream, at 50 bytes a nanosecond of a CTA alone and 6500 of them all, and what
+    // follows it, more where a cluster has to meet (1000 rows of 256206 in fp32 150 us by one CTA each, 159 by two; one row
+    // with 8 tokens 23, 16, 12, 10 and 11 us by 1, 2, 4, 8 and 16).
+    const double bytes = (double)a.vocab * sizeof(T), slots = (double)kPerSm * num_sms;
     int C = 1;
     double least = 1e300;
     for (int c = 1; c <= kMaxCluster; c *= 2) {
-        const long long turns = ((long long)rows * c + 2 * num_sms - 1) / (2 * num_sms);
-        const double t = (double)turns * (bytes / c / 22.0 + 2000.0);
+        const double at_work = std::min((double)rows * c, slots);
+        const double t = (double)rows * c / at_work * (bytes / c / std::min(50.0, 6500.0 / at_work) + (c == 1 ? 4000.0 : 6000.0 + 250.0 * c));
         if (t < least) least = t, C = c;
     }
     return a.top_n ? launch_one<T, true>(a, rows, C, st) : launch_one<T, false>(a, rows, C, st);
