@@ -11,8 +11,10 @@
 // Bytes bound it: each value is read and written once.  A CTA takes one token,
 // or four, with all their heads, so that a token's angles are worked out once
 // for all heads, in shared memory, and its place in the cache is looked up
-// once.  A thread turns both chunks of 16 bytes that hold its pairs; its first
-// loads are in flight before the angles are worked out.
+// once.  A thread turns both chunks of 16 bytes that hold its pairs, one unit at
+// a time: as many threads as an SM holds keep more on its way than fewer that
+// are several units ahead (20000 tokens of 32/8 heads of 128 in bf16, half of
+// each turned: 86 us, four ahead 108, two ahead 95).
 #include <algorithm>
 
 #include "rows.cuh"
@@ -21,24 +23,16 @@ namespace nllb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;  // units of a thread whose loads are in flight together
 
 enum { kNone = 0, kHalves = 1, kNeighbours = 2 };
 
-// Chunk(s) of 16 bytes of one head of one token: source, destination, whether they are turned.
-template <typename T>
-struct Unit {
-    const T* from;
-    T* to;
-    int angle;  // of its first value: into the angles of the CTA; below 0: not turned
-    bool two;   // a second chunk, half a turn's width further
-};
-
 template <typename T, int D, int PAIRS, int TOK>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendParams p) {
     constexpr int VEC = 16 / (int)sizeof(T);
-    __shared__ float2 turn[TOK * D / 2];  // cos, sin
-    __shared__ long long k_at[TOK], v_at[TOK];  // places in the cache, below 0: none
+    __shared__ __align__(16) float2 turn[TOK * D / 2];  // cos, sin
+    // of each token: where its query, key and value heads come from and go to (null: nowhere)
+    __shared__ const T* from[TOK][3];
+    __shared__ T* to[TOK][3];
     pdl_launch_dependents();
     pdl_wait_primary();
 
@@ -48,111 +42,90 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
     if (!rows_sequence<true>(r, s, sq)) return;
     const int n_tok = min(TOK, sq.qn - t0);
     if (n_tok <= 0) return;
-
-    const int n = PAIRS == kNone ? 0 : p.half;
-    // a head's units: with halves, a unit holds chunk c and chunk c + n / VEC
-    const int two = PAIRS == kHalves ? n / VEC : 0, per = D / VEC - two;
-    const int q_heads = r.q ? r.kv_heads * r.group : 0, heads = q_heads + 2 * r.kv_heads;
-    const int lanes = kThreads / per, slot = tid / per, u = tid - slot * per;  // threads [lanes * per, kThreads) have none
-    const int c = u < two ? u : u + two, total = slot < lanes ? n_tok * heads : 0;
-
-    auto unit = [&](int i) {
-        Unit<T> x;
-        const int tok = i / heads, h = i - tok * heads;
-        const long long row = sq.q0 + t0 + tok;
-        x.two = PAIRS == kHalves && u < two;
-        x.angle = PAIRS == kNone || h >= q_heads + r.kv_heads || c * VEC >= 2 * n ? -1
-                                                                                 : tok * n + (PAIRS == kHalves ? c * VEC : c * VEC / 2);
-        if (h < q_heads) {
-            x.from = static_cast<const T*>(r.q) + row * r.q_row + (long long)h * r.q_head + c * VEC;
-            x.to = static_cast<T*>(r.out) + row * r.o_row + (long long)h * r.o_head + c * VEC;
-        } else if (h < q_heads + r.kv_heads) {
-            const long long g = h - q_heads;
-            x.from = static_cast<const T*>(r.k_new) + row * r.kn_row + g * r.kn_head + c * VEC;
-            x.to = k_at[tok] < 0 ? nullptr : static_cast<T*>(r.k_w) + k_at[tok] + g * r.k_head + c * VEC;
-        } else {
-            const long long g = h - q_heads - r.kv_heads;
-            x.from = static_cast<const T*>(r.v_new) + row * r.vn_row + g * r.vn_head + c * VEC;
-            x.to = v_at[tok] < 0 ? nullptr : static_cast<T*>(r.v_w) + v_at[tok] + g * r.v_head + c * VEC;
-        }
-        return x;
-    };
-    uint4 a[kAhead], b[kAhead];
-    auto load = [&](int i0) {
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int i = i0 + k * lanes;
-            if (i >= total) continue;
-            const int tok = i / heads, h = i - tok * heads;
-            const long long row = sq.q0 + t0 + tok;
-            const T* from = h < q_heads ? static_cast<const T*>(r.q) + row * r.q_row + (long long)h * r.q_head
-                            : h < q_heads + r.kv_heads
-                                ? static_cast<const T*>(r.k_new) + row * r.kn_row + (long long)(h - q_heads) * r.kn_head
-                                : static_cast<const T*>(r.v_new) + row * r.vn_row + (long long)(h - q_heads - r.kv_heads) * r.vn_head;
-            a[k] = ld_coherent(reinterpret_cast<const uint4*>(from + c * VEC));
-            if (PAIRS == kHalves && u < two) b[k] = ld_coherent(reinterpret_cast<const uint4*>(from + c * VEC + n));
-        }
-    };
-    load(slot);
-
     if (tid < n_tok) {
         const int j = sq.kvn - sq.qn + t0 + tid, at = rows_page(r, j);
         const int pg = ld_coherent(r.table + (long long)s * r.table_ld + at);
         const bool ok = (unsigned)pg < (unsigned)r.n_pages;
         if (!ok) atomicOr(r.err, NLLB_DEV_ERR_BAD_PAGE);
-        const long long in_page = j - at * r.page;
-        k_at[tid] = ok ? pg * r.k_page + in_page * r.k_row : -1;
-        v_at[tid] = ok ? pg * r.v_page + in_page * r.v_row : -1;
+        const long long row = sq.q0 + t0 + tid, slot = j - at * r.page;
+        from[tid][0] = static_cast<const T*>(r.q) + row * r.q_row;
+        from[tid][1] = static_cast<const T*>(r.k_new) + row * r.kn_row;
+        from[tid][2] = static_cast<const T*>(r.v_new) + row * r.vn_row;
+        to[tid][0] = static_cast<T*>(r.out) + row * r.o_row;
+        to[tid][1] = ok ? static_cast<T*>(r.k_w) + pg * r.k_page + slot * r.k_row : nullptr;
+        to[tid][2] = ok ? static_cast<T*>(r.v_w) + pg * r.v_page + slot * r.v_row : nullptr;
     }
+    __syncthreads();
+
+    // A head's units: chunks of 16 bytes, or, with halves, two of them half a turn's width apart.  A thread has unit `u` of
+    // every lanes-th head, over all tokens.
+    const int n = PAIRS == kNone ? 0 : p.half;
+    const int two = PAIRS == kHalves ? n / VEC : 0, per = D / VEC - two;
+    const int q_heads = r.q ? r.kv_heads * r.group : 0, k_end = q_heads + r.kv_heads, heads = k_end + r.kv_heads;
+    const int lanes = kThreads / per, slot = tid / per, u = tid - slot * per;  // threads [lanes * per, kThreads) have none
+    const bool pair = u < two;
+    const int c = (pair ? u : u + two) * VEC;                                    // its first element
+    const int angle = c >= 2 * n ? -1 : PAIRS == kHalves ? c : c / 2;            // its first pair's (-1: not turned)
+    const int step_tok = lanes / heads, step_head = lanes - step_tok * heads;
+    int tok = slot / heads, h = slot - tok * heads;
+    if (slot >= lanes) tok = n_tok;
+    auto kind = [&](int h) { return h < q_heads ? 0 : h < k_end ? 1 : 2; };
+    uint4 a, b;
+    auto load = [&] {
+        if (tok >= n_tok) return;
+        const int x = kind(h);
+        const T* src = from[tok][x] + (x == 0 ? h * r.q_head : x == 1 ? (h - q_heads) * r.kn_head : (h - k_end) * r.vn_head) + c;
+        a = ld_coherent(reinterpret_cast<const uint4*>(src));
+        if (PAIRS == kHalves && pair) b = ld_coherent(reinterpret_cast<const uint4*>(src + n));
+    };
+    load();  // (under way while the angles are worked out)
     if constexpr (PAIRS != kNone) {
         for (int i = tid; i < n_tok * n; i += kThreads) {
-            const int tok = i / n, f = i - tok * n;
-            const int pos = p.position ? ld_coherent(p.position + sq.q0 + t0 + tok) : sq.kvn - sq.qn + t0 + tok;
+            const int t = i / n, f = i - t * n;
+            const int pos = p.position ? ld_coherent(p.position + sq.q0 + t0 + t) : sq.kvn - sq.qn + t0 + t;
             const double turns = (double)pos * (double)ld_coherent(p.inv_freq + f) * 0.15915494309189533577;
             float sin, cos;
             sincospif((float)(2.0 * (turns - rint(turns))), &sin, &cos);
             turn[i] = make_float2(cos, sin);
         }
+        __syncthreads();
     }
-    __syncthreads();
-
-    for (int i0 = slot; i0 < total; i0 += kAhead * lanes) {
-        if (i0 > slot) load(i0);
+    while (tok < n_tok) {
+        const int x = kind(h);
+        T* dst = to[tok][x];
+        if (PAIRS != kNone && angle >= 0 && x < 2) {
+            const float4* t = reinterpret_cast<const float4*>(turn + tok * n + angle);  // (two pairs)
+            float v[VEC], w[VEC];
+            rows_unpack<T>(a, v);
+            if constexpr (PAIRS == kHalves) {
+                rows_unpack<T>(b, w);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int i = i0 + k * lanes;
-            if (i >= total) continue;
-            const Unit<T> x = unit(i);
-            uint4 y = a[k], z = b[k];
-            if (PAIRS != kNone && x.angle >= 0) {
-                float v[VEC], w[VEC];
-                rows_unpack<T>(a[k], v);
-                if constexpr (PAIRS == kHalves) {
-                    rows_unpack<T>(b[k], w);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float2 t = turn[x.angle + e];
-                        const float f = v[e];
-                        v[e] = f * t.x - w[e] * t.y;
-                        w[e] = w[e] * t.x + f * t.y;
-                    }
-                    z = rows_pack<T>(w);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; e += 2) {
-                        const float2 t = turn[x.angle + e / 2];
-                        const float f = v[e];
-                        v[e] = f * t.x - v[e + 1] * t.y;
-                        v[e + 1] = v[e + 1] * t.x + f * t.y;
-                    }
+                for (int e = 0; e < VEC; e += 2) {
+                    const float4 f = t[e / 2];
+                    const float v0 = v[e], v1 = v[e + 1];
+                    v[e] = v0 * f.x - w[e] * f.y, w[e] = w[e] * f.x + v0 * f.y;
+                    v[e + 1] = v1 * f.z - w[e + 1] * f.w, w[e + 1] = w[e + 1] * f.z + v1 * f.w;
                 }
-                y = rows_pack<T>(v);
+                b = rows_pack<T>(w);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) {
+                    const float4 f = t[e / 4];
+                    const float v0 = v[e], v2 = v[e + 2];
+                    v[e] = v0 * f.x - v[e + 1] * f.y, v[e + 1] = v[e + 1] * f.x + v0 * f.y;
+                    v[e + 2] = v2 * f.z - v[e + 3] * f.w, v[e + 3] = v[e + 3] * f.z + v2 * f.w;
+                }
             }
-            if (x.to) {
-                *reinterpret_cast<uint4*>(x.to) = y;
-                if (x.two) *reinterpret_cast<uint4*>(x.to + n) = z;
-            }
+            a = rows_pack<T>(v);
         }
+        if (dst) {
+            dst += (x == 0 ? h * r.o_head : x == 1 ? (h - q_heads) * r.k_head : (h - k_end) * r.v_head) + c;
+            *reinterpret_cast<uint4*>(dst) = a;
+            if (PAIRS == kHalves && pair) *reinterpret_cast<uint4*>(dst + n) = b;
+        }
+        tok += step_tok, h += step_head;
+        if (h >= heads) h -= heads, ++tok;
+        load();
     }
 }
 
