@@ -467,15 +467,34 @@ cudaError_t launch_one(const RowsParams& p, int n_split, cudaStream_t st) {
 template <typename T, int D, int R, bool PAGED, bool WIN>
 cudaError_t launch_by_units(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long units = (long long)p.kv_heads * p.n_seq;
+    constexpr int MANY = Cfg<T, D, R, 0>::MANY, step = MANY * Cfg<T, D, R, 0>::BLK;
+    // The matrix products' sums lose up to a step of fp32 with every 16 keys, so a warp of them takes 32768 at most.
+    const int most = Cfg<T, D, R, 0>::MMA ? MANY * kWarpKeys : INT_MAX;
+    int n_split = 1;
+    if constexpr (WIN) {
+        // Windows are mostly of one length, so that CTAs end together and a round more of them costs a whole one: as many as
+        // are at work at once, which takes clusters of eight and more no further than 64 CTAs (one token, bf16, heads of 64,
+        // 16 key heads, a window of 1000: 9.0, 8.3, 6.3 and 11 us by 1, 2, 4 and 8 CTAs a head; 64 sequences of 4 key heads of
+        // 128, a window of 4000: 94, 109 and 132 us by 1, 2 and 4).
+        while (n_split < 16 && ((units * n_split * 2 <= (n_split >= 4 ? 64 : num_sms) && p.max_seen > step * n_split) ||
+                                p.max_seen / n_split > most))
+            n_split *= 2;
+        // Or a warp alone per unit, by what either takes: a round of CTAs 3.3 us and 1 us with every block of a warp, or what
+        // their bytes take; a warp alone, twelve to an SM, 1.3 us with every block (bf16, 16 key heads of 64: 100 sequences
+        // and a window of 60 41 us by many warps, 8 alone, a window of 1000 100 and 76; 40 sequences and 1000 47 and 51).
+        auto up = [](long long x, long long to) { return (double)((x + to - 1) / to); };
+        const double bytes = 2.0 * D * sizeof(T) * p.max_seen;
+        const double round = std::max(up(p.max_seen, (long long)step * n_split), bytes / n_split * std::min<double>(num_sms, (double)units * n_split) / 6.5e6);
+        const double many = up(units * n_split, num_sms) * (3.3 + round);
+        const double alone = up(units, 12LL * num_sms) * (1.0 + 1.3 * up(p.max_seen, Cfg<T, D, R, 1>::BLK));
+        if (alone < many && p.max_seen <= kWarpKeys) return launch_one<T, D, R, PAGED, 1, WIN>(p, 1, st);
+        return launch_one<T, D, R, PAGED, MANY, WIN>(p, n_split, st);
+    }
     // A warp alone per unit where that already fills the SMs and the keys are few (256 sequences of 16 heads over
     // 18..512 keys: 56 us, with four warps 75); else many warps, and as many splits as give every SM work (four CTAs
     // per SM instead of two cost 134 us against 113 over 200..8191 keys), none with less than a block per warp, one
     // cluster at most.
     if (units >= 8LL * num_sms && p.max_seen <= 1024) return launch_one<T, D, R, PAGED, 1, WIN>(p, 1, st);
-    constexpr int MANY = Cfg<T, D, R, 0>::MANY, step = MANY * Cfg<T, D, R, 0>::BLK;
-    // The matrix products' sums lose up to a step of fp32 with every 16 keys, so a warp of them takes 32768 at most.
-    const int most = Cfg<T, D, R, 0>::MMA ? MANY * kWarpKeys : INT_MAX;
-    int n_split = 1;
     while (n_split < 16 && ((units * n_split < 2LL * num_sms && p.max_seen > step * n_split) || p.max_seen / n_split > most))
         n_split *= 2;
     return launch_one<T, D, R, PAGED, MANY, WIN>(p, n_split, st);

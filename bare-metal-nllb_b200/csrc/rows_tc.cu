@@ -1052,8 +1052,15 @@ cudaError_t launch_by_tiles(const RowsParams& p, int num_sms, cudaStream_t st) {
     const long long rows = (long long)p.max_q * p.group, heads = (long long)p.kv_heads * p.n_seq;
     const bool is_long = sizeof(T) == 2 && p.max_seen > kLongKeys;
     if constexpr (sizeof(T) == 2) {
-        // two query tiles per CTA where they still give every SM one
-        if (rows > kTile && (rows + 2 * kTile - 1) / (2 * kTile) * heads >= num_sms) {
+        // Two query tiles per CTA where they still give every SM one, and, through a window, where that adds less than a twelfth
+        // to the key tiles that a row goes through (chunks of 500..1024 tokens of 32/8 heads of 64, a window of 2000: 252 us,
+        // with one tile 270; of 294..588 tokens of 16/16 heads, a window of 71 and 100 first keys: 82 and 66).
+        auto key_tiles = [&](int q_rows) {
+            const long long seen = (long long)p.sinks + p.window - 1 + (q_rows + p.group - 1) / p.group;
+            return (std::min<long long>(p.max_kv, seen) + kTile - 1) / kTile;
+        };
+        const bool pays = !WIN || key_tiles(2 * kTile) * 12 <= key_tiles(kTile) * 13;
+        if (rows > kTile && pays && (rows + 2 * kTile - 1) / (2 * kTile) * heads >= num_sms) {
             if (!is_long) return launch_tc<T, D, 2, PAGED, false, WIN>(p, 1, st);
             // (two tiles of heads of 128 fill the tensor memory)
             if constexpr (D == 64) return launch_tc<T, D, 2, PAGED, true, WIN>(p, 1, st);

@@ -234,7 +234,7 @@ def ptr(x) -> Optional[int]:
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
-_TYPE_CODES: dict = {}  # of torch's types (filled by the first use: torch is not needed before)
+_TYPE_CODES: dict = {}  # of torch's types, and what is looked up there (filled by the first use: torch is not needed before)
 
 
 def _types() -> dict:
@@ -242,7 +242,8 @@ def _types() -> dict:
         import torch
         _TYPE_CODES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, "torch.float32": torch.float32,
                             "torch.int32": torch.int32, "torch.uint8": torch.uint8, "torch.float16": torch.float16,
-                            "torch.bfloat16": torch.bfloat16, "cuda": torch.cuda})
+                            "torch.bfloat16": torch.bfloat16, "stream": torch._C._cuda_getCurrentRawStream,
+                            "current": torch.cuda.current_device, "device": torch.cuda.device})
     return _TYPE_CODES
 
 
@@ -671,10 +672,11 @@ def linear_int8_noalloc_status(stream=None) -> int:
     return load().nllb_linear_int8_noalloc_status(stream)
 
 
-def _matrix(x, name, rows, cols, dtype, device):
+def _matrix(x, name, shape, dtype, device):
     """Address of a matrix whose rows are contiguous, and the elements from one to the next."""
-    if x.dtype is not dtype or x.shape != (rows, cols) or x.get_device() != device:
-        raise ValueError(f"{name} must be a {dtype} tensor {[rows, cols]} on GPU {device}")
+    if x.dtype is not dtype or x.shape != shape or x.get_device() != device:
+        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} on GPU {device}")
+    rows, cols = shape
     row, col = x.stride()
     if col != 1 and cols > 1 and rows:
         raise ValueError(f"the rows of {name} must be contiguous")
@@ -688,7 +690,7 @@ def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=Non
     it or fp32 (rows may be strided).  Runs on torch's current stream of x's
     device unless `stream` names another."""
     (M, K), N, kind, device = x.shape, w.shape[0], x.dtype, x.get_device()
-    code = _types().get(kind, F32)
+    shape, code = (M, N), (_TYPE_CODES or _types()).get(kind, F32)
     if code == F32:
         raise ValueError(f"x must be float16 or bfloat16, not {kind}")
     if act not in ACTIVATIONS:
@@ -700,11 +702,11 @@ def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=Non
     if device < 0:
         raise ValueError("x must be on a GPU")
     if out is None:
-        out = x.new_empty((M, N), dtype=out_kind)
-    x_at, ldx = _matrix(x, "x", M, K, kind, device)
-    w_at, ldw = _matrix(w, "w", N, K, kind, device)
-    out_at, ldo = _matrix(out, "out", M, N, out_kind, device)
-    res_at, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_kind, device)
+        out = x.new_empty(shape, dtype=out_kind)
+    x_at, ldx = _matrix(x, "x", (M, K), kind, device)
+    w_at, ldw = _matrix(w, "w", (N, K), kind, device)
+    out_at, ldo = _matrix(out, "out", shape, out_kind, device)
+    res_at, ldr = (None, 0) if residual is None else _matrix(residual, "residual", shape, out_kind, device)
     if bias is not None and (bias.dtype is not kind or bias.shape != (N,) or bias.get_device() != device
                              or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous {kind} tensor {[N]} on GPU {device}")
@@ -797,14 +799,13 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
 def _call(device, name, args, stream):
     """A library function of (arguments, stream) with GPU `device` the current
     one, on `stream` or torch's current stream there."""
-    cuda = _types()["cuda"]
-    lib = load()
+    lib, torch = load(), _types()
     if stream is None:
-        stream = current_stream(device)
-    if device == cuda.current_device():
+        stream = torch["stream"](device) or 1  # (current_stream)
+    if device == torch["current"]():
         rc = getattr(lib, name)(ctypes.byref(args), stream)
     else:
-        with cuda.device(device):
+        with torch["device"](device):
             rc = getattr(lib, name)(ctypes.byref(args), stream)
     if rc != OK:
         _check(lib, rc, name)
@@ -837,13 +838,20 @@ def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entr
         out_top_tok = logits.new_empty((rows, top_n), dtype=types["torch.int32"])
     if top_n and out_top_logp is None:
         out_top_logp = logits.new_empty((rows, top_n), dtype=types["torch.float32"])
-    f = "torch.float32"
+    device, f32, i32 = logits.get_device(), types["torch.float32"], types["torch.int32"]
+
+    def at(x, name, n, kind):
+        if x is None:
+            return None
+        if x.dtype is not kind or x.numel() != n or x.get_device() != device or not x.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {kind} tensor of {n} entries on GPU {device}")
+        return x.data_ptr()
+
     a = LogprobsArgs(logits.data_ptr(), row if rows > 1 else vocab, _dtype_code(logits), vocab, rows, top_n,
-                     _ints(target, "target", rows, logits), _ints(out_logp, "out_logp", rows, logits, f),
-                     _ints(out_entropy, "out_entropy", rows, logits, f),
-                     _ints(out_top_tok, "out_top_tok", rows * top_n, logits),
-                     _ints(out_top_logp, "out_top_logp", rows * top_n, logits, f))
-    _call(logits.get_device(), "nllb_logprobs", a, stream)
+                     at(target, "target", rows, i32), at(out_logp, "out_logp", rows, f32),
+                     at(out_entropy, "out_entropy", rows, f32), at(out_top_tok, "out_top_tok", rows * top_n, i32),
+                     at(out_top_logp, "out_top_logp", rows * top_n, f32))
+    _call(device, "nllb_logprobs", a, stream)
     return out_logp, out_entropy, out_top_tok, out_top_logp
 
 
