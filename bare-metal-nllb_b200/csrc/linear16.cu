@@ -846,6 +846,7 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
     if (s->act < NLLB_ACT_NONE || s->act > NLLB_ACT_SILU) return bad("act must be one of NLLB_ACT_*");
     if (s->M < 0 || s->N < 1 || s->K < 1) return bad("M >= 0, N >= 1 and K >= 1 required");
     if (s->M > (1 << 24) || s->N > (1 << 24) || s->K > (1 << 24)) return set_error(NLLB_ATTN_ECAPACITY, "a size above 2^24");
+    if ((long long)s->M * s->N > 1LL << 40) return set_error(NLLB_ATTN_ECAPACITY, "more outputs than a call takes");
     if (s->M == 0) return NLLB_ATTN_OK;
     if (!s->x || !s->w || !s->out) return bad("x, w and out are required");
     if (s->ldx < s->K || s->ldw < s->K || s->ldo < s->N || (s->residual && s->ldr < s->N))

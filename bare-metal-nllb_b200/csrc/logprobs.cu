@@ -1,14 +1,19 @@
 // logprobs.cu -- log-probabilities of given tokens, the entropy of each row of
 // logits and its likeliest tokens (nllb_logprobs, sm_100a).
 //
-// With y_i = l_i log2(e) - M, M the largest l_i log2(e) rounded (the same for
-// every token, so that its rounding cancels):
-//   Z = sum_i 2^y_i,   S = sum_i 2^y_i y_i,
-//   log p_t = ln2 (y_t - log2 Z),   H = ln2 (log2 Z - S / Z).
+// With m the largest logit, n the number of those equal to it, and over the others
+// y_i = (l_i - m) log2(e),
+//   z = sum 2^y_i,   s = sum 2^y_i y_i:
+//   log p_t = l_t - m - ln n - log1p(z / n),
+//   H = ln n + log1p(z / n) - ln2 s / (n + z).
+// The largest are counted apart from the sums: beside their weight of 1 a sum in
+// fp32 would lose what is below 2^-24 of it, and the entropy of a row that one
+// token dominates is of that size; as they stand no term cancels another.
 //
 // The bytes of the logits bound it: they are read once, each thread keeping a
-// running M, Z and S of its stripe of 16-byte vectors, which are joined in a
-// fixed order: across the warp, the CTA and the cluster that shares the row.
+// running n, z and s of its stripe of 16-byte vectors beside its warp's m; they
+// are joined in a fixed order: across the warp, the CTA and the cluster that
+// shares the row.
 //
 // The likeliest tokens cost the stream nothing: a thread notes, where its
 // running maximum grows anyway, which vector it came from.  Of n tokens in the
@@ -37,8 +42,7 @@ constexpr int kUnroll = 4;         // 16-byte vectors that a thread takes togeth
 constexpr int kMaxCluster = 2 * kWarps;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNoWeight = -200.0f;  // 2^-200 is 0 in fp32
-constexpr float kLag = 8.0f;          // what a running maximum may be behind by: a warp's sums are rarely moved then
-// A largest scaled logit of this size and more: what M was rounded by could be more than an exponent holds, and different
+// A largest scaled logit of this size and more: what it was rounded by could be more than an exponent holds, and different
 // logits are at least 32 apart.
 constexpr float kFar = 0x1.8p28f;
 
@@ -52,8 +56,10 @@ struct Args {
     float* out_top_logp;
 };
 
-struct State {  // of a set of tokens: sums of 2^(y - m) and 2^(y - m) (y - m), y = l log2(e), none above m + kLag
-    float m, z, s;
+// A set of tokens: their largest logit, how many there are of it, and the others' sums of 2^y and 2^y y, where
+// y = l log2(e) - M with M = m log2(e) rounded: off by what M was rounded by, alike for all.
+struct __align__(16) State {
+    float m, n, z, s;
 };
 
 struct Shared {
@@ -62,7 +68,6 @@ struct Shared {
     u64 list[kWarps][32];
     u64 kept[kWarps][64];
     float second[kThreads];
-    uint32_t top, n_top;  // beyond kFar: the largest logit's order, and how many there are
 };
 
 // Weight 2^y, y <= 0 (or what infinities and NaN make of it): below kNoWeight, and for NaN, none.
@@ -73,25 +78,32 @@ __device__ __forceinline__ float weigh(float& y) {
     return e;
 }
 
-// The state's sums with its maximum moved to m >= st.m.
-__device__ __forceinline__ void move_to(State& st, float m) {
-    if (st.m == m) return;
-    float d = st.m - m;
-    if (!(d > kNoWeight)) {  // (sums beside a maximum beyond kFar may be infinite)
-        st.z = st.s = 0.f;
+// M = m log2(e), rounded (never part of a fused operation), and what it is short by.
+__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, kLog2e); }
+__device__ __forceinline__ float rounded_off(float m) { return fmaf(m, kLog2e, -scaled(m)); }
+
+// The state as others of a larger m: all in its sums.  (Nothing is left where it lies too far behind, and sums beside a
+// maximum beyond kFar, which may be infinite, do not count.)
+__device__ __forceinline__ void settle(State& st, float m) {
+    float d = scaled(st.m) - scaled(m);
+    if (!(d > kNoWeight)) {
+        st.n = st.z = st.s = 0.f;
     } else {
-        const float f = weigh(d);
-        st.s = f * fmaf(st.z, d, st.s);
+        float r = rounded_off(st.m);
+        const float w = st.n * weigh(r), f = weigh(d);
+        st.z += w;
+        st.s = f * fmaf(st.z, d, fmaf(w, r, st.s));
         st.z *= f;
+        st.n = 0.f;
     }
     st.m = m;
 }
 
 __device__ __forceinline__ State join(State a, State b) {
     const float m = fmaxf(a.m, b.m);
-    move_to(a, m);
-    move_to(b, m);
-    return {m, a.z + b.z, a.s + b.s};
+    if (a.m < m) settle(a, m);
+    if (b.m < m) settle(b, m);
+    return {m, a.n + b.n, a.z + b.z, a.s + b.s};
 }
 
 // Two fp32 operations in one instruction.
@@ -211,24 +223,25 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     const int per = (n_vec + C - 1) / C, v_end = min(n_vec, (rank + 1) * per), v_first = min(n_vec, rank * per);
 
     float m = -INFINITY;  // the warp's
-    float2 z[2], sy[2];   // 2^y and 2^y y, in four chains
+    int n = 0;
+    float2 z[2], sy[2];   // in four chains
     z[0] = z[1] = sy[0] = sy[1] = make_float2(0.f, 0.f);
-    auto move = [&](float to) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            State x = {m, z[i].x, sy[i].x}, y = {m, z[i].y, sy[i].y};
-            move_to(x, to);
-            move_to(y, to);
-            z[i] = make_float2(x.z, y.z), sy[i] = make_float2(x.s, y.s);
-        }
-        m = to;
+    auto lane_state = [&] {
+        return State{m, (float)n, (z[0].x + z[0].y) + (z[1].x + z[1].y), (sy[0].x + sy[0].y) + (sy[1].x + sy[1].y)};
     };
-    auto lagging = [&](float t) {  // a scaled logit of this lane; the whole warp asks
-        if (__any_sync(0xffffffffu, t > m + kLag)) {
+    // The largest logit of this batch in this lane, `t`: whether the warp has one as large as its m, or a larger one, which
+    // is its m from now on.
+    auto rises = [&](float t) {
+        if (!__any_sync(0xffffffffu, t >= m && t > -INFINITY)) return false;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-            move(t);
+        for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+        if (t > m) {
+            State st = lane_state();
+            settle(st, t);
+            m = t, n = 0;
+            z[0] = make_float2(st.z, 0.f), sy[0] = make_float2(st.s, 0.f), z[1] = sy[1] = make_float2(0.f, 0.f);
         }
+        return true;
     };
     float best = -INFINITY;
     uint32_t best_at = 0xffffffffu;  // the stripe's first vector that holds its maximum
@@ -250,20 +263,27 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
                 if (top[k] > best) best = top[k], best_at = at + k * kThreads;
             }
         }
-        lagging(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * kLog2e);
-        const float2 off = make_float2(-m, -m), scale = make_float2(kLog2e, kLog2e);
+        auto sum = [&](auto largest_among) {  // (whether the warp's m is among the batch's logits)
+            const float2 off = make_float2(-scaled(m), -scaled(m)), scale = make_float2(kLog2e, kLog2e);
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            float x[VEC];
-            rows_unpack<T>(u[k], x);
+            for (int k = 0; k < kUnroll; ++k) {
+                float x[VEC];
+                rows_unpack<T>(u[k], x);
 #pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-                float2 y = fma2(make_float2(x[e], x[e + 1]), scale, off), w;
-                w.x = weigh(y.x), w.y = weigh(y.y);
-                z[(e >> 1) & 1] = add2(z[(e >> 1) & 1], w);
-                sy[(e >> 1) & 1] = fma2(w, y, sy[(e >> 1) & 1]);
+                for (int e = 0; e < VEC; e += 2) {
+                    float2 y = fma2(make_float2(x[e], x[e + 1]), scale, off), w;
+                    w.x = weigh(y.x), w.y = weigh(y.y);
+                    if constexpr (decltype(largest_among)::value) {
+                        if (x[e] == m) w.x = 0.f, ++n;
+                        if (x[e + 1] == m) w.y = 0.f, ++n;
+                    }
+                    z[(e >> 1) & 1] = add2(z[(e >> 1) & 1], w);
+                    sy[(e >> 1) & 1] = fma2(w, y, sy[(e >> 1) & 1]);
+                }
             }
-        }
+        };
+        if (rises(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])))) sum(std::true_type());
+        else sum(std::false_type());
     };
     static_assert(kUnroll == 4, "four vectors together");
     {
@@ -284,22 +304,22 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     }
     if (n_single > 0) {  // (fewer than 32)
         const float l = tid < n_single ? to_float(ld_coherent(src + single(tid))) : -INFINITY;
-        lagging(l * kLog2e);
-        float y = fmaf(l, kLog2e, -m);
-        const float w = weigh(y);
+        rises(l);
+        float y = fmaf(l, kLog2e, -scaled(m)), w = weigh(y);
+        if (l == m) w = 0.f, n += tid < n_single;
         z[0].x += w;
         sy[0].x = fmaf(w, y, sy[0].x);
     }
 
-    // ---- the row's M, Z and S
-    State st = {m, (z[0].x + z[0].y) + (z[1].x + z[1].y), (sy[0].x + sy[0].y) + (sy[1].x + sy[1].y)};
+    // ---- the row's state
+    State st = lane_state();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
+        st.n += __shfl_xor_sync(0xffffffffu, st.n, o);
         st.z += __shfl_xor_sync(0xffffffffu, st.z, o);
         st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
     }
     if (lane == 0) sh.warp[warp] = st;
-    if (tid == 0) sh.top = sh.n_top = 0;
     u64 list = 0;
     if constexpr (TOP) {
         // the stripes whose maxima come first, by the index of the vector's first element
@@ -311,11 +331,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     }
     __syncthreads();
     if (warp == 0) {
-        State w = lane < kWarps ? sh.warp[lane] : State{-INFINITY, 0.f, 0.f};
+        State w = lane < kWarps ? sh.warp[lane] : State{-INFINITY, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int o = kWarps / 2; o > 0; o >>= 1) {
             State b;
             b.m = __shfl_xor_sync(0xffffffffu, w.m, o);
+            b.n = __shfl_xor_sync(0xffffffffu, w.n, o);
             b.z = __shfl_xor_sync(0xffffffffu, w.z, o);
             b.s = __shfl_xor_sync(0xffffffffu, w.s, o);
             w = join(w, b);
@@ -391,10 +412,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     else __syncthreads();
     State all = sh.cta;
     if (C > 1) {  // (the same order in every CTA)
-        all = {-INFINITY, 0.f, 0.f};
+        all = {-INFINITY, 0.f, 0.f, 0.f};
         for (int r = 0; r < C; ++r) {
-            const uint32_t at = map_rank(&sh.cta, r);
-            all = join(all, State{ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8)});
+            const float4 f = ld_cluster_f4(map_rank(&sh.cta, r));
+            all = join(all, State{f.x, f.y, f.z, f.w});
         }
         if constexpr (TOP) {
             if (rank == 0) {
@@ -409,50 +430,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
             }
         }
     }
-    // A largest logit that is infinite or far out: the logits equal to it share all the weight.
-    const bool far = !(fabsf(all.m) < kFar);
-    float most = 0.f;
-    if (far) {
-        auto each = [&](auto&& f) {
-            for (int i = v_first + tid; i < v_end; i += kThreads) {
-                float x[VEC];
-                rows_unpack<T>(ld_coherent(vec + i), x);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) f(order_of(x[e]));
-            }
-            for (int i = tid; i < n_single; i += kThreads) f(order_of(to_float(ld_coherent(src + single(i)))));
-        };
-        uint32_t top = 0, n = 0;
-        each([&](uint32_t o) { top = max(top, o); });
-        if (top) atomicMax(&sh.top, top);
-        if (C > 1) cluster_sync_all();
-        else __syncthreads();
-        for (int r = 0; r < C; ++r)
-            top = max(top, C > 1 ? (uint32_t)ld_cluster_s32(map_rank(&sh.top, r)) : *(volatile uint32_t*)&sh.top);
-        each([&](uint32_t o) { n += o == top; });
-        if (n) atomicAdd(&sh.n_top, n);
-        if (C > 1) cluster_sync_all();
-        else __syncthreads();
-        n = 0;
-        for (int r = 0; r < C; ++r)
-            n += C > 1 ? (uint32_t)ld_cluster_s32(map_rank(&sh.n_top, r)) : *(volatile uint32_t*)&sh.n_top;
-        most = logit_of(top);
-        all.z = (float)n;
-        all.s = 0.f;
-    }
     if (rank == 0 && warp == 0) {
-        const bool none = far && most == -INFINITY;
-        const float log_z = log2f(all.z);
+        // A largest logit that is infinite or far out: those equal to it share all the weight.
+        const bool none = all.m == -INFINITY, far = !(fabsf(scaled(all.m)) < kFar);
+        float r = far ? 0.f : rounded_off(all.m), back = -r;
+        const float f = weigh(back);  // (the sums without what M was rounded by)
+        const float z = far ? 0.f : f * all.z, sy = far ? 0.f : f * fmaf(-r, all.z, all.s);
+        const float log_z = logf(all.n) + log1pf(z / all.n);
         auto logp = [&](float l) {
             if (none || !(l > -INFINITY)) return -INFINITY;
-            if (far) return (l == most ? 0.f : l - most) - kLn2 * log_z;
-            // (a token far behind, whose scaled difference may leave fp32: M's rounding is nothing beside it)
-            const float y = fmaf(l, kLog2e, -all.m);
-            return y > -1e6f ? kLn2 * (y - log_z) : (l - kLn2 * all.m) - kLn2 * log_z;
+            if (far) return (l == all.m ? 0.f : l - all.m) - log_z;
+            // (a token far behind, whose scaled difference may leave fp32: what M was rounded by is nothing beside it)
+            const float y = fmaf(l, kLog2e, -scaled(all.m));
+            return l == all.m ? -log_z : y > -1e6f ? kLn2 * (y - r) - log_z : (l - all.m) - log_z;
         };
         if (lane == 0) {
             if (a.out_logp) a.out_logp[row] = target < a.vocab ? logp(to_float(ld_coherent(src + target))) : -INFINITY;
-            if (a.out_entropy) a.out_entropy[row] = none ? 0.f : kLn2 * (log_z - all.s / all.z);
+            if (a.out_entropy) a.out_entropy[row] = none ? 0.f : log_z - kLn2 * (sy / (all.n + z));
         }
         if (TOP && lane < a.top_n) {
             const bool there = list > kNothing;

@@ -17,6 +17,19 @@ using namespace nllb;
 
 namespace {
 
+// The context's device for the time of a call, then the caller's again.
+struct OnDevice {
+    int before = -1;
+    cudaError_t status;
+    explicit OnDevice(int device) {
+        status = cudaGetDevice(&before);
+        if (status == cudaSuccess && before != device) status = cudaSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
 int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -61,19 +74,6 @@ bool pages_apart(const Args& a) {
            apart(a.page_size, a.v_stride_slot, a.head_dim) && apart(a.n_kv_heads, a.v_stride_head, a.head_dim);
 }
 
-// The context's device for the time of a call, then the caller's again.
-struct OnDevice {
-    int before = -1;
-    cudaError_t status;
-    explicit OnDevice(int device) {
-        status = cudaGetDevice(&before);
-        if (status == cudaSuccess && before != device) status = cudaSetDevice(device);
-    }
-    ~OnDevice() {
-        if (before >= 0) cudaSetDevice(before);
-    }
-};
-
 // Division of a j < 2^30 by d: with 2^(b-1) < d <= 2^b the multiplier ceil(2^(30+b) / d) is too large by less than 1, so
 // the quotient by less than 2^30 / 2^(30+b) <= 1 / d: it stays below the next whole number.
 void set_division(int d, uint32_t* mul, int* shr) {
@@ -88,7 +88,8 @@ int launch(nllb_attn_ctx* c, RowsParams& p, int dtype, int head_dim, bool paged)
     if (p.n_seq == 0) return NLLB_ATTN_OK;  // nothing to do
     p.err = c->err;
     set_division(p.group, &p.group_mul, &p.group_shr);
-    cudaError_t e = cudaSetDevice(c->device);
+    OnDevice on(c->device);
+    cudaError_t e = on.status;
     p.expire = c->expire_next_rows;
     c->expire_next_rows = false;
     if (e == cudaSuccess) e = launch_rows(p, static_cast<RowType>(dtype), head_dim, paged, c->num_sms, c->stream);

@@ -188,6 +188,31 @@ def test_masked_by_a_low_value(cuda_device, dtype, mask):
     run(lg, t, 32)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gap", [4.0, 12.0, 20.0, 40.0])
+@pytest.mark.parametrize("base", [0.0, 37.7])
+def test_dominated_rows(cuda_device, dtype, gap, base):
+    """One token far ahead of very many: what is left to the others is small, and as accurate relative to its size.  Each of
+    their weights is off by 4 u, and by u of its difference and 2 u of it by log2(e)'s rounding, their sums by the chain's
+    (n / 1024 + 64) u; the logarithm of 1 + z and the quotient add 8 u."""
+    g = torch.Generator().manual_seed(int(gap))
+    for rows, vocab in ((1, 256206), (3, 50021), (200, 3001)):
+        x = base + torch.rand(rows, vocab, generator=g)
+        x[:, vocab // 3] = base + 1 + gap
+        lg = x.to(dtype).cuda()
+        t = torch.full((rows,), vocab // 3, dtype=torch.int32, device="cuda")
+        logp, h, _, _ = na.logprobs(lg, t)
+        d = lg[:, vocab // 3:vocab // 3 + 1].double() - lg.double()
+        w = torch.exp(-d)
+        w[:, vocab // 3] = 0
+        z = w.sum(1)
+        want = torch.log1p(z)
+        want_h = want + (w * d).sum(1) / (1 + z)
+        rel = U * (vocab / 1024 + 64 + 3 * (gap + 1) + 16)
+        assert ((-logp.double() / want - 1).abs() <= rel).all(), f"{rows} x {vocab}: logp"
+        assert ((h.double() / want_h - 1).abs() <= 2 * rel).all(), f"{rows} x {vocab}: entropy"
+
+
 @pytest.mark.parametrize("top", [1e6, 1e8, 2.0 ** 27 + 16, 2.0 ** 28, 1e12, 1e37])
 def test_large_logits(cuda_device, top):
     """A few of the largest, the next ones a step of the type lower, and a bulk far below; of either sign."""

@@ -25,6 +25,7 @@ def args(**kw):
     (dict(N=0), na.EINVAL, "N"),
     (dict(K=0), na.EINVAL, "K"),
     (dict(M=2 ** 24 + 1), na.ECAPACITY, "2^24"),
+    (dict(M=2 ** 24, N=2 ** 24, ldo=2 ** 24, ldr=2 ** 24), na.ECAPACITY, "outputs"),
     (dict(x=None), na.EINVAL, "required"),
     (dict(w=None), na.EINVAL, "required"),
     (dict(out=None), na.EINVAL, "required"),
