@@ -145,6 +145,11 @@ __device__ __forceinline__ float activate(const Args& a, float x) {
     return (a.kind == kClamp ? activate<kClamp>(a, y) : a.kind == kSwish ? activate<kSwish>(a, y) : activate<kGelu>(a, y)).x;
 }
 
+// The tensor cores cut what they add to a sum, so that one over K comes out up to K 2^-27 of its summands' sizes short.  Sums
+// that fp32 outputs are made of are taken over 1024 at most and those added in fp32 (4096 x 4096 by K = 8192: 9e-6 off as
+// one, 1e-6 so); of 16-bit outputs over 16384, a quarter of fp16's half step.
+constexpr int kSegment = 1024, kSegment16 = 16384;
+
 // ---- few tokens ------------------------------------------------------------------------------------------------
 
 constexpr int kFewWarps = 8, kFewRows = 16;  // warps of a CTA; weight rows of a warp
@@ -199,11 +204,21 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int
         for (int t = 0; t < NT; ++t)
             x[t] = m0 + t * 8 + lr < a.M ? static_cast<const T*>(a.x) + (m0 + t * 8 + lr) * a.ldx + 8 * lc : nullptr;
 
-        float c[NT][4];
+        float c[NT][4], total[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0.f;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[t][e] = total[t][e] = 0.f;
         constexpr int STEP = 32 * kFewBlocks;
+        int steps = 0;
         for (int k = (split * KG + kg) * STEP; k < a.K; k += n_split * KG * STEP) {
+            if (++steps > kSegment / STEP) {  // (the products cut what they add to a sum)
+                steps = 1;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) total[t][e] += c[t][e], c[t][e] = 0.f;
+            }
             uint4 u[kFewBlocks], v[kFewBlocks], b[NT][kFewBlocks];
 #pragma unroll
             for (int i = 0; i < kFewBlocks; ++i) {
@@ -227,7 +242,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[kg][t * 8 + 2 * lc + (e & 1)][rg + lr + 8 * (e >> 1)] = c[t][e];
+            for (int e = 0; e < 4; ++e) sums[kg][t * 8 + 2 * lc + (e & 1)][rg + lr + 8 * (e >> 1)] = total[t][e] + c[t][e];
         __syncthreads();
         // the warps' sums, then the splits', always in the same order
         if (n_split > 1) {
@@ -278,6 +293,8 @@ struct Tiling {
     int bn;           // tokens of a tile, a multiple of 32 up to 256
     int stages;
     int slots;        // of a warp: 8 where residual rows of 16 bits come through them, else 4
+    int segment;      // stages whose products the tensor cores add
+    int acc;          // columns of an accumulator in tensor memory; behind two of them the segments' total
     int tiles_n, tiles_m;
     bool tokens_first;  // tiles of the same weights follow one another (else: of the same tokens)
 };
@@ -334,7 +351,7 @@ __device__ __forceinline__ void stores_read() {
 }
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// 8 or 16 columns of this thread's lane (warp-wide), there after tmem_wait on the same registers.
+// 16 columns of this thread's lane (warp-wide), there after tmem_wait on the same registers.
 __device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -343,11 +360,6 @@ __device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[16]) {
           "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                 : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
@@ -355,11 +367,15 @@ __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tmem_wait(float (&v)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])
-                 :
-                 : "memory");
+// 16 columns of this thread's lane, written (warp-wide).
+__device__ __forceinline__ void tmem_put(uint32_t taddr, const float (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 template <typename T, typename O, int MODE, int KIND>
@@ -394,7 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int c1 = MODE == kSplit ? (int)((long long)(rank + 1) * chunks / n_split) : chunks;
     auto rows_at = [&](int t) { return (g.tokens_first ? t / g.tiles_m : t % g.tiles_n) * width; };
     auto tokens_at = [&](int t) { return (g.tokens_first ? t % g.tiles_m : t / g.tiles_n) * g.bn; };
-    constexpr uint32_t TMEM = MODE == kSplit ? 256 : 512;  // two accumulators of up to 256 columns, or one of up to 256
+    constexpr uint32_t TMEM = 512;  // two accumulators of up to 256 columns, or of up to 160 and the total
+    const int segments = (c1 - c0 + g.segment - 1) / g.segment;
 
     if (warp == kDrain) {
         if constexpr (MODE == kPair) {
@@ -488,35 +505,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t leader;
             asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
             uint32_t s = 0, turn = 0, n = 0;
-            for (int t = first; t < tiles && ok; t += step, ++n) {
-                const uint32_t acc = n & 1;
-                if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait_one(drained + acc, (n / 2 - 1) & 1)))) break;
-                tc_fence_after();
-                const uint32_t d = tmem + acc * 256;
-                for (int c = c0; c < c1; ++c) {
-                    if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, turn & 1)))) break;
+            for (int t = first; t < tiles && ok; t += step)
+                for (int b = c0; b < c1; b += g.segment, ++n) {
+                    const uint32_t acc = n & 1;
+                    if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait_one(drained + acc, (n / 2 - 1) & 1)))) break;
                     tc_fence_after();
-                    const uint64_t da = umma_desc_k_sw128(base + s * stage_bytes);
-                    const uint64_t db = umma_desc_k_sw128(base + s * stage_bytes + kRowsBytes);
-                    if (leader) {
+                    const uint32_t d = tmem + acc * g.acc;
+                    const int e = min(c1, b + g.segment);
+                    for (int c = b; c < e; ++c) {
+                        if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, turn & 1)))) break;
+                        tc_fence_after();
+                        const uint64_t da = umma_desc_k_sw128(base + s * stage_bytes);
+                        const uint64_t db = umma_desc_k_sw128(base + s * stage_bytes + kRowsBytes);
+                        if (leader) {
 #pragma unroll
-                        for (int k = 0; k < kChunk / 16; ++k) {
-                            if constexpr (MODE == kPair) mma_pair(d, da + 2 * k, db + 2 * k, idesc, c > c0 || k > 0);
-                            else tc_mma_f16(d, da + 2 * k, db + 2 * k, idesc, c > c0 || k > 0);
+                            for (int k = 0; k < kChunk / 16; ++k) {
+                                if constexpr (MODE == kPair) mma_pair(d, da + 2 * k, db + 2 * k, idesc, c > b || k > 0);
+                                else tc_mma_f16(d, da + 2 * k, db + 2 * k, idesc, c > b || k > 0);
+                            }
+                            if constexpr (MODE == kPair) commit_pair(empty + s);
+                            else tc_commit(empty + s);
                         }
-                        if constexpr (MODE == kPair) commit_pair(empty + s);
-                        else tc_commit(empty + s);
+                        __syncwarp();
+                        if (++s == (uint32_t)stages) s = 0, ++turn;
+                    }
+                    if (!ok) break;
+                    if (leader) {
+                        if constexpr (MODE == kPair) commit_pair(ready + acc);
+                        else tc_commit(ready + acc);
                     }
                     __syncwarp();
-                    if (++s == (uint32_t)stages) s = 0, ++turn;
                 }
-                if (!ok) break;
-                if (leader) {
-                    if constexpr (MODE == kPair) commit_pair(ready + acc);
-                    else tc_commit(ready + acc);
-                }
-                __syncwarp();
-            }
             // what was issued is over before tensor memory is given back
             if (leader) {
                 if constexpr (MODE == kPair) commit_pair(done);
@@ -560,20 +579,55 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (MODE != kSplit && a.res_whole)
             for (int i = 0; i < g.slots - 2; ++i) ask();
         bool ok = true;
-        uint32_t n = 0;
+        uint32_t n = 0;  // accumulators
+        const uint32_t total = from0 + 2 * g.acc;
+        auto release = [&](uint32_t acc) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (MODE == kPair) arrive_at(map_rank(drained + acc, 0));
+                else arrive_here(drained + acc);
+            }
+        };
         for (; here.t < tiles && ok; here = place_of(here.t + step), ++n) {
-            const uint32_t acc = n & 1, from = from0 + acc * 256;
+            // all segments but the last one are added up in tensor memory
+            for (int b = 1; b < segments; ++b, ++n) {
+                const uint32_t acc = n & 1, from = from0 + acc * g.acc;
+                if (!(ok = __all_sync(0xffffffffu, wait_one(ready + acc, (n / 2) & 1)))) break;
+                tc_fence_after();
+                for (int i = half; i < here.count; i += 2) {
+                    float v[PIECE], t[PIECE];
+                    tmem_ask(from + i * PIECE, v);
+                    if (b > 1) tmem_ask(total + i * PIECE, t);
+                    tmem_wait(v);
+                    if (b > 1) {
+                        tmem_wait(t);
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j) v[j] += t[j];
+                    }
+                    tmem_put(total + i * PIECE, v);
+                }
+                release(acc);
+            }
+            if (!ok) break;
+            const uint32_t acc = n & 1, from = from0 + acc * g.acc;
             if (!(ok = __all_sync(0xffffffffu, wait_one(ready + acc, (n / 2) & 1)))) break;
             tc_fence_after();
             if constexpr (MODE == kSplit) {
                 // over the ring, which is done with and larger (a partial sum takes 64 KB at most)
                 float* part = reinterpret_cast<float*>(sm) + quarter * 32 + lane;
-                for (int col = half * PIECE; col < g.bn; col += 2 * PIECE) {
-                    float v[PIECE];
-                    tmem_ask(from + col, v);
+                for (int i = half; i < here.count; i += 2) {
+                    float v[PIECE], t[PIECE];
+                    tmem_ask(from + i * PIECE, v);
+                    if (segments > 1) tmem_ask(total + i * PIECE, t);
                     tmem_wait(v);
+                    if (segments > 1) {
+                        tmem_wait(t);
 #pragma unroll
-                    for (int j = 0; j < PIECE; ++j) part[(col + j) * kRows] = v[j];
+                        for (int j = 0; j < PIECE; ++j) v[j] += t[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < PIECE; ++j) part[(i * PIECE + j) * kRows] = v[j];
                 }
                 break;  // (one tile)
             } else {
@@ -597,6 +651,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     O* mem = mem0 + at * (kSlot / sizeof(O));
                     float v[PIECE];
                     tmem_wait(next);
+                    if (segments > 1) {
+                        float t[PIECE];
+                        tmem_ask(total + i * PIECE, t);
+                        tmem_wait(t);
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j) next[j] += t[j];
+                    }
 #pragma unroll
                     for (int j = 0; j < PIECE; ++j) v[j] = next[j] + bias;
                     if (i + 2 < here.count) tmem_ask(from + (i + 2) * PIECE, next);
@@ -633,12 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (a.res_whole) ask();  // into the slot of the piece before the last
                 }
                 tmem_wait(next);  // (what was asked for and not used)
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (MODE == kPair) arrive_at(map_rank(drained + acc, 0));
-                    else arrive_here(drained + acc);
-                }
+                release(acc);
             }
         }
         // nothing reads or writes shared memory once the CTA has ended
@@ -741,6 +797,8 @@ cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStrea
     constexpr uint32_t kSlot = kPiece * 32 * sizeof(O);
     g.slots = MODE == kSplit ? 0 : a.res_whole && sizeof(O) == 2 ? 8 : 4;
     g.stages = std::min(kMaxStages, ((int)(kSmem - kBars) - g.slots * (int)(kDrain * kSlot)) / stage);
+    g.segment = (sizeof(O) == 4 ? kSegment : kSegment16) / kChunk;
+    g.acc = a.K > (MODE == kSplit ? ctas : 1) * g.segment * kChunk ? 160 : 256;
     g.tiles_n = (a.N + width - 1) / width, g.tiles_m = (a.M + g.bn - 1) / g.bn;
     g.tokens_first = (long long)a.N >= a.M;  // the larger operand is read once, while its tile is in use
     CUtensorMap tw, tx, to, tr;
@@ -782,10 +840,11 @@ cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
     if (a.M <= 32 && weights <= 1 << 21) return launch_few<T, O, 4>(a, num_sms, st);
     auto up = [](long long x, long long to) { return (x + to - 1) / to; };
     Tiling g = {};
+    const int widest = a.K > (sizeof(O) == 4 ? kSegment : kSegment16) ? 160 : 256;  // (the segments' total takes its room)
     // the tile of tokens whose rounds over the SMs take the least, by the wider of products and operands
     auto best = [&](int width, int groups, bool pair) {
         double least = 1e300;
-        for (int bn = 32; bn <= 256; bn += 32) {
+        for (int bn = 32; bn <= widest; bn += 32) {
             const double rounds = (double)up(up(a.N, width) * up(a.M, bn), groups);
             const double t = rounds * std::max(2.0 * bn, (16384.0 + bn * (pair ? 64 : 128)) / 64.0);
             if (t < least * 0.999) least = t, g.bn = bn;

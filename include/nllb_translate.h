@@ -178,8 +178,9 @@ NLLB_ATTN_API void nllb_linear_free(nllb_linear* layer);
  * residual [M][N] (NULL: none; may be out itself) of `out_dtype`: dtype, or
  * NLLB_F32.  Rows lie ldx, ldw, ldo, ldr elements apart; those of x and w start
  * on 16 bytes, the others anywhere.  Sums are fp32, from their start to the
- * residual, and rounded once; over K summands they may come out up to K 2^-27
- * short (relative to the sum of their sizes).  act: NONE, RELU, GELU (by erf),
+ * residual, and rounded once; they may come out short of the sum of their
+ * summands' sizes by up to K 2^-27, at most 2^-17 for NLLB_F32 outputs and 2^-13
+ * for others.  act: NONE, RELU, GELU (by erf),
  * GELU_TANH (its tanh form) or SILU.  Device pointers; asynchronous on `stream`
  * (a cudaStream_t, NULL = default); nothing is allocated and no workspace is
  * kept, so calls may overlap and be captured.  A bounded device wait that gives

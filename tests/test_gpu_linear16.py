@@ -1,8 +1,9 @@
 """nllb_linear16 on the GPU against the product in 64 bits.
 
 Tolerance, derived from the arithmetic and set before the first run.  With u = 2^-24 and A = sum |x w| + |bias|: products
-of 16-bit values are exact in fp32, the tensor cores cut off less than a step of fp32 with every 16 summands (K 2^-27 A),
-warps, splits and the bias add at most 40 roundings (40 u A).  The activations have slopes up to 1.2 and are off by 16 u of
+of 16-bit values are exact in fp32, the tensor cores cut off less than a step of fp32 with every 16 of the summands that they
+add, at most 1024 for fp32 outputs and 16384 for others (k 2^-27 A); warps, splits, those sums' sum and the bias add at most
+40 + K / 1024 roundings (u A each).  The activations have slopes up to 1.2 and are off by 16 u of
 their argument's size, the residual's sum is rounded once (u), and the result to its type: half a step, relative to it in
 the normal range, at least 2^-25 in fp16."""
 import math
@@ -35,7 +36,8 @@ def check(out, x, w, bias, residual, act, what=""):
     if bias is not None:
         y, a = y + bias.double(), a + bias.double().abs()
     z = activated(y, act)
-    tol = 1.2 * (K * 2.0 ** -27 + 40 * U) * a + 16 * U * y.abs()
+    together = min(K, 1024 if out.dtype == torch.float32 else 16384)
+    tol = 1.2 * (together * 2.0 ** -27 + (40 + K / 1024) * U) * a + 16 * U * y.abs()
     if residual is not None:
         z = z + residual.double()
         tol += U * z.abs()
@@ -79,7 +81,8 @@ SIZES = [
     (17, 1, 64), (17, 128, 64), (31, 129, 100), (32, 127, 1000), (33, 1024, 4096), (64, 5003, 1024), (65, 256, 72), (100, 1000, 2048),
     (128, 128, 128), (129, 640, 513), (200, 300, 8192), (256, 20000, 96), (257, 1023, 1024), (1000, 1024, 512), (3000, 4099, 200),
     (10000, 1024, 64), (4097, 4096, 128), (300, 40001, 64), (1, 40000, 700), (16, 9001, 1000), (27, 1000, 1000), (32, 128, 8192),
-    (20, 16, 72), (12, 2048, 4104),
+    (20, 16, 72), (12, 2048, 4104), (3, 100, 70000), (30, 60, 33000), (100, 200, 40000), (300, 20000, 1100), (2100, 4000, 2500),
+    (260, 300, 17000),
 ]
 
 
@@ -98,6 +101,25 @@ def test_epilogues(cuda_device, act, bias, residual, dtype):
     """On each of the forms: few rows, a cluster per tile, single CTAs, pairs."""
     for M, N, K in ((4, 200, 256), (50, 200, 1024), (300, 20000, 64), (4096, 8192, 128)):
         case(M, N, K, dtype, act, bias, residual)
+
+
+@pytest.mark.parametrize("M,N", [(4, 300), (30, 60), (100, 500), (600, 9000), (4096, 4096)])
+@pytest.mark.parametrize("K", [1024, 2000, 8192, 40000])
+def test_sums_of_one_sign(cuda_device, M, N, K):
+    """What the tensor cores cut has one sign here, and shows in the mean: at most 1024 2^-27 for fp32 outputs, 16384 2^-27 for
+    16-bit ones, whose roundings average out over 10000 and more outputs (half a step / sqrt(3 * 10000), four of it); the
+    additions in fp32 round to nearest, 2^-24 at most with every 1024 summands."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = (0.5 + torch.rand(M, K, generator=g, device="cuda")).to(torch.float16)
+    w = ((0.5 + torch.rand(N, K, generator=g, device="cuda")) / K).to(torch.float16)
+    some = slice(0, 500)
+    ref = x[some].double() @ w.double().T
+    for kind, together in ((torch.float32, 1024), (torch.float16, 16384)):
+        out = na.linear16(x, w, out_dtype=kind)
+        rel = out[some].double() / ref - 1
+        few = min(rel.numel(), 10000)
+        assert abs(float(rel.mean())) <= min(K, together) * 2.0 ** -27 + (2 + K / 1024) * U + 4 * half_step(kind) / (3 * few) ** 0.5
+        assert float(rel.abs().max()) <= min(K, together) * 2.0 ** -27 + (40 + K / 1024) * U + half_step(kind)
 
 
 @pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
