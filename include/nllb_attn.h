@@ -22,8 +22,8 @@
  *    run, copy outputs back and return once the outputs are written, the way
  *    the reference's call sites use their stack and heap buffers.
  *  - fp32 in, fp32 out.  head_dim must be 64 (NLLB-200: 16 heads x 64).
- *    (nllb_attn_paged and nllb_attn_cross_rows also take 16-bit types and
- *    heads of 128; their rows lie at the strides of their arguments.)
+ *    (nllb_attn_paged, _window, _cross_rows and _append also take 16-bit types
+ *    and heads of 128; their rows lie at the strides of their arguments.)
  *  - Rows of q/k/v/out hold all heads, head h at columns [64h, 64h+64), as the
  *    reference's projections produce them (decoder.c:57-59, encoder.c:159-163).
  *  - One context belongs to one device and is used by one host thread at a
@@ -198,10 +198,11 @@ NLLB_ATTN_API int nllb_attn_cross_host(nllb_attn_ctx* ctx, int layer, int n_sent
                          const float* q, float* out);
 
 /* ---- many query rows against keys of another length ----------------------
- * Two calls for a decoder that draws its tokens (nllb_sample) or scores given
- * target rows: a chunk of new tokens over a paged cache, and target rows over
- * encoder states.  No counterpart in the reference, whose decoder moves one
- * token at a time (decoder.c:48-152).
+ * Calls for a decoder that draws its tokens (nllb_sample) or scores given
+ * target rows (nllb_logprobs): a chunk of new tokens over a paged cache, over
+ * all of it or through a sliding window, target rows over encoder states, and
+ * new rows into the cache, turned by their positions.  No counterpart in the
+ * reference, whose decoder moves one token at a time (decoder.c:48-152).
  *
  * Types: q, k, v and out are all fp32, all fp16 or all bf16.  Scores, softmax
  * sums and outputs are accumulated in fp32 and an output is rounded once.

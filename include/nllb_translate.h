@@ -180,12 +180,12 @@ NLLB_ATTN_API void nllb_linear_free(nllb_linear* layer);
  * on 16 bytes, the others anywhere.  Sums are fp32, from their start to the
  * residual, and rounded once; they may come out short of the sum of their
  * summands' sizes by up to K 2^-27, at most 2^-17 for NLLB_F32 outputs and 2^-13
- * for others.  act: NONE, RELU, GELU (by erf),
- * GELU_TANH (its tanh form) or SILU.  Device pointers; asynchronous on `stream`
- * (a cudaStream_t, NULL = default); nothing is allocated and no workspace is
- * kept, so calls may overlap and be captured.  A bounded device wait that gives
- * up leaves the outputs invalid and sets a per-device error word, which
- * nllb_linear16_status (waits for `stream`) reads and clears:
+ * for others.  act: NONE, RELU, GELU (by erf), GELU_TANH (its tanh form) or
+ * SILU.  out may not overlap x, w or bias.  Device pointers; asynchronous on
+ * `stream` (a cudaStream_t, NULL = default); nothing is allocated and no
+ * workspace is kept, so calls may overlap and be captured.  A bounded device
+ * wait that gives up leaves the outputs invalid and sets a per-device error
+ * word, which nllb_linear16_status (waits for `stream`) reads and clears:
  * NLLB_ATTN_ETIMEOUT if set. */
 #define NLLB_ACT_NONE 0
 #define NLLB_ACT_RELU 1
@@ -205,9 +205,9 @@ typedef struct {
 NLLB_ATTN_API int nllb_linear16(const nllb_linear16_args* args, void* stream);
 NLLB_ATTN_API int nllb_linear16_status(void* stream);
 /* Test of the bounded device waits: if the calling thread's next nllb_linear16
- * runs on the tensor-core kernel (more than 32 rows, or 2^24 weights, of K >= 64),
- * a wait of its runs out after about 1 ms and nllb_linear16_status reports it.
- * Later calls are as ever. */
+ * runs on the tensor cores' kernel (more than 32 rows and K >= 64 do), a wait of
+ * its runs out after about 1 ms and nllb_linear16_status reports it.  Later
+ * calls are as ever. */
 NLLB_ATTN_API int nllb_linear16_test_expire_next_wait(void);
 
 /* ---- per-step vocabulary operations of the beam search --------------------
