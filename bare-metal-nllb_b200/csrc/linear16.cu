@@ -20,6 +20,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -42,6 +43,7 @@ struct Args {
     float c1, c2;  // of the activation
     bool out_whole, res_whole;  // (there and) the rows start on 16 bytes, as TMA has it
     bool expire;  // test: a wait runs out
+    int device;
 };
 
 template <typename T>
@@ -810,8 +812,14 @@ cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStrea
     if (e == cudaSuccess && a.out_whole) e = encode_rows_map(&to, a.out, out_type, a.N, a.M, a.ldo, 32, kPiece, false);
     if (e == cudaSuccess && a.res_whole) e = encode_rows_map(&tr, a.residual, out_type, a.N, a.M, a.ldr, 32, kPiece, false);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(linear16_tc<T, O, MODE, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024);
-    if (e != cudaSuccess) return e;
+    // (once per device)
+    static std::atomic<unsigned long long> configured{0};
+    const unsigned long long bit = 1ull << (a.device & 63);
+    if (!(configured.load() & bit) || a.device > 63) {
+        e = cudaFuncSetAttribute(linear16_tc<T, O, MODE, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024);
+        if (e != cudaSuccess) return e;
+        configured.fetch_or(bit);
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)(groups * ctas), 1, 1);
@@ -921,7 +929,7 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
         return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0 && ld <= 1LL << 36;
     };
     Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, kClamp, 0.f, 0.f,
-              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next};
+              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next, 0};
     switch (s->act) {
         case NLLB_ACT_NONE: a.c1 = -INFINITY; break;
         case NLLB_ACT_RELU: break;
@@ -934,6 +942,7 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
     int device = 0, num_sms = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
+    a.device = device;
     if (e == cudaSuccess) {
         const bool wide = s->out_dtype == NLLB_F32;
         if (s->dtype == NLLB_F16) e = wide ? launch<__half, float>(a, num_sms, st) : launch<__half, __half>(a, num_sms, st);

@@ -459,8 +459,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
 
 template <typename T, bool TOP>
 cudaError_t launch_one(const Args& a, int rows, int C, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
+    if (C > 8) {  // (beyond the portable size)
+        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * (unsigned)C, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
