@@ -415,6 +415,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t TMEM = 512;  // two accumulators of up to 256 columns, or of up to 160 and the total
     const int segments = (c1 - c0 + g.segment - 1) / g.segment;
 
+    if (warp == kDrain + 1 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tw)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tx)) : "memory");
+    }
     if (warp == kDrain) {
         if constexpr (MODE == kPair) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(TMEM)
@@ -709,10 +713,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     else __syncthreads();
     if constexpr (MODE == kSplit) {
         // rank z finishes the tokens z, z + n_split, ...: a warp to each, 4 columns to a lane; the sums in the order of the ranks
-        bool ok = true;
-        for (int r = 0; r < n_split; ++r) ok = ok && ld_cluster_s32(map_rank(const_cast<int*>(gave_up), r)) == 0;
+        int given_up = 0;  // (all asked for at once, as the sums are)
+        for (int r = 0; r < n_split; ++r) given_up |= ld_cluster_s32(map_rank(const_cast<int*>(gave_up), r));
         const int n = rows_at(first) + 4 * lane, m0 = tokens_at(first);
-        if (ok && warp < kDrain) {
+        if (given_up == 0 && warp < kDrain) {
             float bias[4] = {0.f, 0.f, 0.f, 0.f};
             if (a.bias) {
 #pragma unroll
@@ -728,12 +732,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int e = 0; e < 4; ++e)
                         if (n + e < a.N) old[e] = as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n + e));
                 }
+                float4 f[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    f[r] = r < n_split ? ld_cluster_f4(map_rank(part + col * kRows, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 float y[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int r = 0; r < n_split; r += 2) {  // (an even number of them)
-                    const float4 f = ld_cluster_f4(map_rank(part + col * kRows, r)), h = ld_cluster_f4(map_rank(part + col * kRows, r + 1));
-                    y[0] += f.x, y[1] += f.y, y[2] += f.z, y[3] += f.w;
-                    y[0] += h.x, y[1] += h.y, y[2] += h.z, y[3] += h.w;
-                }
+#pragma unroll
+                for (int r = 0; r < 8; ++r) y[0] += f[r].x, y[1] += f[r].y, y[2] += f[r].z, y[3] += f[r].w;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] += bias[e];
                 activate<KIND>(a, y);
