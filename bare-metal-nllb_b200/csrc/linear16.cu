@@ -6,10 +6,11 @@
 // and output rows are read and written 32 columns at a time whatever their
 // alignment, and a few tokens make a narrow tile rather than a mostly empty one.
 //
-// Few tokens (linear16_few): the weights' bytes bound it.  A warp multiplies 16
-// weight rows by 8 tokens at a time (warp-level products); the order of the
-// summands is the same permutation for both operands, so that each lane's
-// operands are 16 contiguous bytes of a row, straight from global memory.
+// Few tokens (linear16_few): the weights' bytes bound it, or the start of a
+// launch.  A warp multiplies 16 weight rows by 8 tokens at a time (warp-level
+// products); the order of the summands is the same permutation for both
+// operands, so that each lane's operands are 16 contiguous bytes of a row,
+// straight from global memory.
 //
 // More (linear16_tc): tcgen05 products of 128 weight rows by a tile of up to
 // 256 tokens, operands by TMA into a ring of stages (64 wide, 128-byte swizzle),
@@ -17,6 +18,12 @@
 // while the other is filled.  Pairs of CTAs (cta_group::2) take 256 weight rows
 // and load half of the tokens' tile each.  Where tiles are few, a cluster shares
 // the sum over k of one tile and joins it through distributed shared memory.
+//
+// Measured (device time): one token by 4096 x 1024 3.7 us (2.3 TB/s, the start of
+// a launch); 64 by 256206 x 1024 into fp32 93 us (6.3 TB/s, HBM; the library's
+// product into bf16 174); 10000 by 1024 x 4096 with a residual 70 us (1200
+// TFLOP/s, the tensor cores 73 % busy, operands from L2 in three rounds of tiles;
+// the library's product alone 65); 8192 by 8192 x 4096 389 us (1415 TFLOP/s; 369).
 #include <cuda.h>
 
 #include <algorithm>
@@ -256,21 +263,32 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear16_few(const Args a, int
             }
             cluster_sync_all();
         }
-        for (int i = split * kFewWarps * 32 + tid; i < 8 * NT * ROWS; i += n_split * kFewWarps * 32) {
-            const int m = m0 + i / ROWS;
-            const long long n = n0 + i % ROWS;
-            if (m >= a.M || n >= a.N) continue;
-            float y = 0.f;
-            if (n_split > 1) {
-                for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(&sums[0][i / ROWS][i % ROWS], r));
-            } else {
+        constexpr int ITEMS = 8 * NT * ROWS, EACH = ITEMS / (kFewWarps * 32) < 4 ? (ITEMS + kFewWarps * 32 - 1) / (kFewWarps * 32) : 4;
+        for (int i0 = split * kFewWarps * 32 + tid; i0 < ITEMS; i0 += EACH * n_split * kFewWarps * 32) {
+            float bias[EACH], old[EACH];
 #pragma unroll
-                for (int j = 0; j < KG; ++j) y += sums[j][i / ROWS][i % ROWS];
+            for (int u = 0; u < EACH; ++u) {  // (all asked for before the first is stored)
+                const int i = i0 + u * n_split * kFewWarps * 32, m = m0 + i / ROWS;
+                const long long n = n0 + i % ROWS;
+                const bool there = i < ITEMS && m < a.M && n < a.N;
+                bias[u] = there && a.bias ? as_float(ld_coherent(static_cast<const T*>(a.bias) + n)) : 0.f;
+                old[u] = there && a.residual ? as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n)) : 0.f;
             }
-            if (a.bias) y += as_float(ld_coherent(static_cast<const T*>(a.bias) + n));
-            y = activate(a, y);
-            if (a.residual) y += as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n));
-            static_cast<O*>(a.out)[m * a.ldo + n] = rounded<O>(y);
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) {
+                const int i = i0 + u * n_split * kFewWarps * 32, m = m0 + i / ROWS;
+                const long long n = n0 + i % ROWS;
+                if (i >= ITEMS || m >= a.M || n >= a.N) continue;
+                float y = 0.f;
+                if (n_split > 1) {
+                    for (int r = 0; r < n_split; ++r) y += ld_cluster_f32(map_rank(&sums[0][i / ROWS][i % ROWS], r));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < KG; ++j) y += sums[j][i / ROWS][i % ROWS];
+                }
+                y = activate(a, y + bias[u]);
+                static_cast<O*>(a.out)[m * a.ldo + n] = rounded<O>(a.residual ? y + old[u] : y);
+            }
         }
         // the sums are free again, and no CTA leaves while another reads them
         if (n_split > 1) cluster_sync_all();
@@ -844,13 +862,14 @@ cudaError_t launch_kind(const Args& a, const Tiling& g, int ctas, int groups, cu
 template <typename T, typename O>
 cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
     // Few tokens: warp-level products while the weights are few as well, for the tensor cores then take longer to start (4096 x
-    // 1024 by 1, 16 and 32 tokens 3.5, 4.2 and 7.6 us against 6.9 on the tensor cores; 1024 x 1024 by 32 4.2 against 6.8); they
-    // keep more of the weights on their way (16384 x 1024 by 1 and 16 10.2 and 14.3 us against 8.9 and 9.5).
+    // 1024 by 1, 16 and 32 tokens 3.5, 4.2 and 7.6 us against 6.9 on the tensor cores; 1024 x 1024 by 64 4.8 against 6.9, by 96
+    // 7.6 against 7.5; 256 x 1024 by 200 4.2 against 7.6; where k is short, they are quick: 64 x 64 by 1160 4.8); they keep more of the weights on their way (16384 x 1024 by 1 and 16
+    // 10.2 and 14.3 us against 8.9 and 9.5).
     const long long weights = (long long)a.N * a.K;
     if (a.K < kChunk) return a.M <= 8 ? launch_few<T, O, 1>(a, num_sms, st) : launch_few<T, O, 2>(a, num_sms, st);
     if (a.M <= 8 && weights < 1 << 24) return launch_few<T, O, 1>(a, num_sms, st);
     if (a.M <= 16 && weights <= 1 << 23) return launch_few<T, O, 2>(a, num_sms, st);
-    if (a.M <= 32 && weights <= 1 << 21) return launch_few<T, O, 4>(a, num_sms, st);
+    if (a.M <= 256 && a.K > 128 && (a.M + 31) / 32 * weights <= 1 << 21) return launch_few<T, O, 4>(a, num_sms, st);
     auto up = [](long long x, long long to) { return (x + to - 1) / to; };
     Tiling g = {};
     const int widest = a.K > (sizeof(O) == 4 ? kSegment : kSegment16) ? 160 : 256;  // (the segments' total takes its room)

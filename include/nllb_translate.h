@@ -205,9 +205,9 @@ typedef struct {
 NLLB_ATTN_API int nllb_linear16(const nllb_linear16_args* args, void* stream);
 NLLB_ATTN_API int nllb_linear16_status(void* stream);
 /* Test of the bounded device waits: if the calling thread's next nllb_linear16
- * runs on the tensor cores' kernel (more than 32 rows and K >= 64 do), a wait of
- * its runs out after about 1 ms and nllb_linear16_status reports it.  Later
- * calls are as ever. */
+ * runs on the tensor cores' kernel (more than 32 rows, K >= 64 and N K above 2^20
+ * do), a wait of its runs out after about 1 ms and nllb_linear16_status reports
+ * it.  Later calls are as ever. */
 NLLB_ATTN_API int nllb_linear16_test_expire_next_wait(void);
 
 /* ---- per-step vocabulary operations of the beam search --------------------

@@ -98,8 +98,8 @@ def test_sizes(cuda_device, M, N, K, wide, dtype):
 @pytest.mark.parametrize("act", list(na.ACTIVATIONS))
 @pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True), (True, True)])
 def test_epilogues(cuda_device, act, bias, residual, dtype):
-    """On each of the forms: few rows, a cluster per tile, single CTAs, pairs."""
-    for M, N, K in ((4, 200, 256), (50, 200, 1024), (300, 20000, 64), (4096, 8192, 128)):
+    """On each of the forms: few rows, and blocks of them, a cluster per tile, single CTAs, pairs."""
+    for M, N, K in ((4, 200, 256), (50, 200, 1024), (60, 1000, 2048), (300, 20000, 64), (4096, 8192, 128)):
         case(M, N, K, dtype, act, bias, residual)
 
 
@@ -142,7 +142,7 @@ def test_small_values_of_activations(cuda_device, act):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["f16", "bf16"])
-@pytest.mark.parametrize("M,N,K", [(6, 96, 128), (40, 256, 640), (600, 9000, 64), (4096, 8192, 64)])
+@pytest.mark.parametrize("M,N,K", [(6, 96, 128), (40, 256, 640), (70, 900, 2560), (600, 9000, 64), (4096, 8192, 64)])
 def test_residual_in_place_and_strided_operands(cuda_device, M, N, K, dtype):
     g = torch.Generator(device="cuda").manual_seed(M)
     wide = normal(g, M, 3 * K, dtype=dtype)  # columns of a fused projection's output
@@ -168,7 +168,7 @@ def test_nothing_to_do(cuda_device):
 
 def test_infinities_and_nan_stay_in_their_places(cuda_device):
     """A NaN or infinite row of x, or of w, reaches its row, or column, alone."""
-    for M, N, K in ((8, 96, 128), (40, 256, 640), (600, 9000, 64), (4096, 8192, 64)):
+    for M, N, K in ((8, 96, 128), (40, 256, 640), (70, 900, 2560), (600, 9000, 64), (4096, 8192, 64)):
         g = torch.Generator(device="cuda").manual_seed(M)
         x, w = rows(g, M, K, torch.bfloat16), rows(g, N, K, torch.bfloat16)
         x[M // 2, 3], w[N // 3, 5] = math.nan, math.inf
