@@ -14,7 +14,8 @@
 // once.  A thread turns both chunks of 16 bytes that hold its pairs, one unit at
 // a time: as many threads as an SM holds keep more on its way than fewer that
 // are several units ahead (20000 tokens of 32/8 heads of 128 in bf16, half of
-// each turned: 86 us, four ahead 108, two ahead 95).
+// each turned: 86 us, four ahead 108, two ahead 95).  Where lengths differ much the
+// CTAs take the blocks of all sequences in turn (launch_blocks).
 #include <algorithm>
 
 #include "rows.cuh"
@@ -26,18 +27,55 @@ constexpr int kThreads = 256;
 
 enum { kNone = 0, kHalves = 1, kNeighbours = 2 };
 
+// The blocks of TOK tokens of all sequences, one behind the other: which sequence's block `b` is, and its number there.  Every
+// sequence has one at least, so that its lengths are looked at.
+template <int TOK>
+struct Blocks {
+    int before;  // blocks of the sequences of the threads before this one
+    int mine;    // of this thread's sequences, [first, last)
+    int first, last, total;
+
+    static __device__ __forceinline__ int of(const RowsParams& r, int s) {
+        const int n = r.q_len ? ld_coherent(r.q_len + s) : r.max_q;
+        return n < 1 || n > r.max_q ? 1 : (n + TOK - 1) / TOK;
+    }
+    __device__ __forceinline__ explicit Blocks(const RowsParams& r) {
+        __shared__ int sums[kThreads / 32];
+        const int per = (r.n_seq + kThreads - 1) / kThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        first = min(r.n_seq, (int)threadIdx.x * per), last = min(r.n_seq, first + per), mine = 0;
+        for (int s = first; s < last; ++s) mine += of(r, s);
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        before = x - mine, total = 0;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+    }
+    __device__ __forceinline__ void find(const RowsParams& r, int b, int (&found)[2]) const {
+        if (b < before || b >= before + mine) return;
+        int at = b - before, s = first;
+        for (int n; s < last - 1 && at >= (n = of(r, s)); ++s) at -= n;
+        found[0] = s, found[1] = at;
+    }
+};
+
+// Tokens [t0, t0 + TOK) of sequence s, by a CTA.
 template <typename T, int D, int PAIRS, int TOK>
-__global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendParams p) {
+__device__ __forceinline__ void append_block(const AppendParams& p, int s, int t0) {
     constexpr int VEC = 16 / (int)sizeof(T);
     __shared__ __align__(16) float2 turn[TOK * D / 2];  // cos, sin
     // of each token: where its query, key and value heads come from and go to (null: nowhere)
     __shared__ const T* from[TOK][3];
     __shared__ T* to[TOK][3];
-    pdl_launch_dependents();
-    pdl_wait_primary();
-
     const RowsParams& r = p.rows;
-    const int s = blockIdx.y, t0 = blockIdx.x * TOK, tid = threadIdx.x;
+    const int tid = threadIdx.x;
     RowsSeq sq;
     if (!rows_sequence<true>(r, s, sq)) return;
     const int n_tok = min(TOK, sq.qn - t0);
@@ -129,14 +167,42 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendParams 
     }
 }
 
+// FLAT: the CTAs take the blocks of all sequences in turn (else: one each, of a grid of the longest sequence's by sequences).
+template <typename T, int D, int PAIRS, int TOK, bool FLAT>
+__global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendParams p) {
+    pdl_launch_dependents();
+    pdl_wait_primary();
+    if constexpr (FLAT) {
+        __shared__ int found[2];
+        const Blocks<TOK> blocks(p.rows);
+        for (int b = blockIdx.x; b < blocks.total; b += gridDim.x) {
+            __syncthreads();
+            blocks.find(p.rows, b, found);
+            __syncthreads();
+            append_block<T, D, PAIRS, TOK>(p, found[0], found[1] * TOK);
+        }
+    } else {
+        append_block<T, D, PAIRS, TOK>(p, blockIdx.y, blockIdx.x * TOK);
+    }
+}
+
+template <typename T, int D, int PAIRS, int TOK>
+cudaError_t launch_blocks(const AppendParams& p, cudaStream_t st) {
+    const RowsParams& r = p.rows;
+    const long long longest = (r.max_q + TOK - 1) / TOK, every = longest * r.n_seq, all = r.q_rows / TOK + r.n_seq;
+    // Sequences of very different lengths: a grid of their longest would be empty for the most part (one chunk of 4096 tokens
+    // among 255 single ones in bf16, 16/4 heads of 128: 77 us, flat 15).  Where each row is of one sequence, `all` CTAs have
+    // a block each at most.  The sums of blocks stay in 32 bits, and a thread counts 64 sequences at most.
+    if (every > 2 * all && every < 1ll << 31 && r.n_seq <= 64 * kThreads)
+        return launch_pdl(append_kernel<T, D, PAIRS, TOK, true>, dim3((unsigned)all), dim3(kThreads), 0, st, p);
+    return launch_pdl(append_kernel<T, D, PAIRS, TOK, false>, dim3((unsigned)longest, (unsigned)r.n_seq), dim3(kThreads), 0, st, p);
+}
+
 template <typename T, int D, int PAIRS>
 cudaError_t launch_by_tokens(const AppendParams& p, int num_sms, cudaStream_t st) {
-    const RowsParams& r = p.rows;
     // four tokens of a sequence to a CTA where that leaves every SM some
-    const bool many = r.max_q > 1 && r.q_rows >= 16 * num_sms;
-    const dim3 grid((unsigned)((r.max_q + (many ? 3 : 0)) / (many ? 4 : 1)), (unsigned)r.n_seq);
-    return many ? launch_pdl(append_kernel<T, D, PAIRS, 4>, grid, dim3(kThreads), 0, st, p)
-                : launch_pdl(append_kernel<T, D, PAIRS, 1>, grid, dim3(kThreads), 0, st, p);
+    if (p.rows.max_q > 1 && p.rows.q_rows >= 16 * num_sms) return launch_blocks<T, D, PAIRS, 4>(p, st);
+    return launch_blocks<T, D, PAIRS, 1>(p, st);
 }
 
 template <typename T, int D>

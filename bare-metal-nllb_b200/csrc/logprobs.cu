@@ -15,8 +15,9 @@
 // are joined in a fixed order: across the warp, the CTA and the cluster that
 // shares the row.
 //
-// The likeliest tokens cost the stream nothing: a thread notes, where its
-// running maximum grows anyway, which vector it came from.  Of n tokens in the
+// For the likeliest tokens a thread notes, beside the sums, its stripe's largest
+// logit, the vector that it came from and the largest of the other vectors: a few
+// selections a vector, hidden behind the bytes.  Of n tokens in the
 // order (falling logit, rising index) each lies in one of the n stripes whose
 // maxima come first in that order -- n of them are ahead of any other stripe's
 // -- so of those stripes the vectors that hold the maxima are read again, and

@@ -102,6 +102,8 @@ LENS = {
     "long": [(700, 3), (1, 5000), (301, 65)],
     "many": [(n % 5, 7 * n % 400) for n in range(1, 260)],
     "prompts": [(1500, 0), (1000, 77), (250, 1)],
+    "one prompt among tokens": [(1, 40)] * 70 + [(2000, 3), (0, 7)] + [(1 + n % 3, n) for n in range(300)] + [(700, 0)],
+    "a short prompt among tokens": [(1, 40)] * 7 + [(200, 3), (0, 7)] + [(1, n) for n in range(30)] + [(0, 0)],
 }
 
 
@@ -145,6 +147,37 @@ def test_without_queries(ctx):  # noqa: F811
     c.run(ctx, freq)
     ctx.sync()
     c.verify(freq, "halves")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lengths_that_count_for_more_than_the_rows(ctx, dtype):  # noqa: F811
+    """Without queries sequences may share rows, and a bad start leaves a long length standing: no block of another is lost."""
+    freq = frequencies(32)
+    for n in (60, 2400):  # (a token to a CTA, and four)
+        lens = [(n, 3)] + [(1, 40)] * 40 + [(n, 20)] * 3
+        c = Append(lens, 2, 2, 64, 16, dtype, seed=9, q=False)
+        c.starts = [0] + list(range(n, n + 40)) + [0, 5, 2]
+        c.rows = n + 40
+        c.k, c.v = c.k[:c.rows], c.v[:c.rows]
+        c.q_start = ints(c.starts)
+        rot = torch.zeros(c.rows, dtype=torch.int32)  # (a shared row has one position for all)
+        rot.copy_(torch.arange(c.rows) % 1000)
+        c.run(ctx, freq, position=ints(rot.tolist()))
+        ctx.sync()
+        c.verify(freq, "halves", "shared rows", rot)
+        c = Append([(n, 3)] * 12 + [(1, 40)] * 60 + [(n, 2)], 2, 2, 64, 16, dtype, seed=10)
+        short = c.rows - 11 * n
+        c.starts = [-1 - i for i in range(11)] + [0] + list(range(n, n + 60)) + [n + 60]
+        c.q, c.q_out, c.k, c.v, c.rows = c.q[:short], c.q_out[:short], c.k[:short], c.v[:short], short
+        c.pos = torch.zeros(short, dtype=torch.int32)
+        for a, (m, past) in zip(c.starts, c.lens):
+            if a >= 0:
+                c.pos[a:a + m] = torch.arange(past, past + m)
+        c.q_start = ints(c.starts)
+        c.run(ctx, freq)
+        with pytest.raises(na.NllbAttnError):
+            ctx.sync()
+        c.verify(freq, "halves", "bad starts", left_out=range(11))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
