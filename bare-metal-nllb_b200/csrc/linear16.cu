@@ -371,6 +371,12 @@ __device__ __forceinline__ void stores_read() {
 }
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // 16 columns of this thread's lane (warp-wide), there after tmem_wait on the same registers.
 __device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[16]) {
     asm volatile(
@@ -396,6 +402,92 @@ __device__ __forceinline__ void tmem_put(uint32_t taddr, const float (&v)[16]) {
         "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
         : "memory");
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Four neighbouring columns of a row, those from N on left out.  (whole: the row starts on 16 bytes)
+template <typename O>
+struct __align__(4 * sizeof(O)) Four {
+    O v[4];
+};
+template <typename O>
+__device__ __forceinline__ Four<O> load4(const O* row, int n, int N, bool whole) {
+    using Bits = typename std::conditional<sizeof(O) == 4, uint4, uint2>::type;
+    Four<O> f;
+    if (whole && n + 4 <= N) {
+        *reinterpret_cast<Bits*>(&f) = ld_coherent(reinterpret_cast<const Bits*>(row + n));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[e] = n + e < N ? ld_coherent(row + n + e) : rounded<O>(0.f);
+    }
+    return f;
+}
+template <typename O>
+__device__ __forceinline__ void store4(O* row, int n, int N, bool whole, const float (&v)[4]) {
+    if (whole && n + 4 <= N) {
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<float4*>(row + n) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<uint2*>(row + n) = make_uint2(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < N) row[n + e] = rounded<O>(v[e]);
+}
+
+// Joins the sums of S CTAs over one tile, [token][128 rows] in the shared memory of each: rank z finishes the tokens z, z + S,
+// ..., a warp to each, 4 columns to a lane, in the order of the ranks.  The cluster's shared memory gives 14 bytes a cycle, so
+// eight loads under way are enough; a kernel that runs through its code once waits for instructions, so the loop is short.
+template <typename T, typename O, int KIND, int S>
+__device__ __forceinline__ void join(const Args& a, const float* part, volatile int* gave_up, int rank, int warp, int lane, int n0,
+                                     int m0, int bn) {
+    constexpr int BATCH = 8 / S;  // tokens of a warp under way
+    const int n = n0 + 4 * lane, end = min(bn, a.M - m0);
+    Four<T> bias;
+    if (a.bias) bias = load4(static_cast<const T*>(a.bias), n, a.N, false);
+    __syncwarp();
+    cluster_sync_all();
+    if (warp < kDrain) {
+        int given_up = 0;
+        const float* mine = part + 4 * lane;
+        uint32_t from[S];
+#pragma unroll
+        for (int r = 0; r < S; ++r) {
+            given_up |= ld_cluster_s32(map_rank(const_cast<int*>(gave_up), r));
+            from[r] = map_rank(mine, r);
+        }
+#pragma unroll 1
+        for (int col = rank + S * warp; col < end; col += BATCH * S * kDrain) {
+            float4 f[BATCH][S];
+            Four<O> old[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int at = min(col + i * S * kDrain, bn - 1);
+#pragma unroll
+                for (int r = 0; r < S; ++r) f[i][r] = ld_cluster_f4(from[r] + at * (kRows * 4));
+                if (a.residual && col + i * S * kDrain < end)
+                    old[i] = load4(static_cast<const O*>(a.residual) + (long long)(m0 + at) * a.ldr, n, a.N, a.res_whole);
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < S; ++r) y[0] += f[i][r].x, y[1] += f[i][r].y, y[2] += f[i][r].z, y[3] += f[i][r].w;
+                if (a.bias) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] += as_float(bias.v[e]);
+                }
+                activate<KIND>(a, y);
+                if (a.residual) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] += as_float(old[i].v[e]);
+                }
+                const int at = col + i * S * kDrain;
+                if (at < end && given_up == 0) store4(static_cast<O*>(a.out) + (long long)(m0 + at) * a.ldo, n, a.N, a.out_whole, y);
+            }
+        }
+    }
+    __syncwarp();
+    // no CTA leaves while another reads its sums (relaxed: what was read has been used, and the stores need not be over)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 template <typename T, typename O, int MODE, int KIND>
@@ -490,17 +582,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp == kDrain) {
-        // ---- fetch
-        if (lane == 0) {
-            const uint32_t full0 = MODE == kPair ? map_rank(full, 0) : 0u;
-            uint32_t i = 0, s = 0, turn = 0;  // stages so far; the next one's place, and how often it has come round
-            bool ok = true;
-            for (int t = first; t < tiles && ok; t += step) {
-                const int n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0);
-                const int m0 = tokens_at(t) + (MODE == kPair ? rank * (int)x_rows : 0);
-                for (int c = c0; c < c1; ++c, ++i) {
-                    if (turn > 0 && !(ok = wait_one(empty + s, (turn - 1) & 1))) break;
-                    const uint32_t at = base + s * stage_bytes;
+        // ---- fetch (a warp's loop with one thread that asks: addresses and coordinates then lie in uniform registers; by a
+        // thread alone each stage took 390 cycles to ask for)
+        const uint32_t full0 = MODE == kPair ? map_rank(full, 0) : smem_u32(full);
+        uint32_t i = 0, s = 0, turn = 0;  // stages so far; the next one's place, and how often it has come round
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+            const int n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0);
+            const int m0 = tokens_at(t) + (MODE == kPair ? rank * (int)x_rows : 0);
+            for (int c = c0; c < c1; ++c, ++i) {
+                if (turn > 0 && !(ok = __all_sync(0xffffffffu, wait_one(empty + s, (turn - 1) & 1)))) break;
+                const uint32_t at = base + s * stage_bytes;
+                if (elect_one()) {
                     if constexpr (MODE == kPair) {
                         if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * stage_bytes);
                         tma_2d_pair(at, &tw, c * kChunk, n0, full0 + 8 * s);
@@ -510,14 +603,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tma_2d(at, &tw, c * kChunk, n0, full + s);
                         tma_2d(at + kRowsBytes, &tx, c * kChunk, m0, full + s);
                     }
-                    if (++s == (uint32_t)stages) s = 0, ++turn;
                 }
+                __syncwarp();
+                if (++s == (uint32_t)stages) s = 0, ++turn;
             }
-            // (given up: what is in flight lands before the CTA ends)
-            if (*gave_up && rank == 0)
-                for (uint32_t j = i > (uint32_t)stages ? i - stages : 0; j < i; ++j)
-                    (void)mbar_wait_bounded(full + j % stages, (j / stages) & 1, kTestWaitBudgetCycles);
         }
+        // (given up: what is in flight lands before the CTA ends)
+        if (lane == 0 && *gave_up && rank == 0)
+            for (uint32_t j = i > (uint32_t)stages ? i - stages : 0; j < i; ++j)
+                (void)mbar_wait_bounded(full + j % stages, (j / stages) & 1, kTestWaitBudgetCycles);
         __syncwarp();
     } else if (warp == kDrain + 1) {
         // ---- products (of both CTAs of a pair: by the first one's)
@@ -526,8 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t idesc = umma_idesc_f16(width, g.bn) | fmt;
             bool ok = true;
             if (a.expire) ok = __all_sync(0xffffffffu, wait_one(never, 0, kTestWaitBudgetCycles));  // nothing arrives there
-            uint32_t leader;
-            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+            const uint64_t da0 = umma_desc_k_sw128(base), db0 = umma_desc_k_sw128(base + kRowsBytes);
             uint32_t s = 0, turn = 0, n = 0;
             for (int t = first; t < tiles && ok; t += step)
                 for (int b = c0; b < c1; b += g.segment, ++n) {
@@ -539,9 +632,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int c = b; c < e; ++c) {
                         if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, turn & 1)))) break;
                         tc_fence_after();
-                        const uint64_t da = umma_desc_k_sw128(base + s * stage_bytes);
-                        const uint64_t db = umma_desc_k_sw128(base + s * stage_bytes + kRowsBytes);
-                        if (leader) {
+                        const uint64_t da = da0 + s * (stage_bytes / 16), db = db0 + s * (stage_bytes / 16);  // (addresses / 16)
+                        if (elect_one()) {
 #pragma unroll
                             for (int k = 0; k < kChunk / 16; ++k) {
                                 if constexpr (MODE == kPair) mma_pair(d, da + 2 * k, db + 2 * k, idesc, c > b || k > 0);
@@ -554,14 +646,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (++s == (uint32_t)stages) s = 0, ++turn;
                     }
                     if (!ok) break;
-                    if (leader) {
+                    if (elect_one()) {
                         if constexpr (MODE == kPair) commit_pair(ready + acc);
                         else tc_commit(ready + acc);
                     }
                     __syncwarp();
                 }
             // what was issued is over before tensor memory is given back
-            if (leader) {
+            if (elect_one()) {
                 if constexpr (MODE == kPair) commit_pair(done);
                 else tc_commit(done);
                 (void)mbar_wait_bounded(done, 0);
@@ -727,45 +819,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     tc_fence_before();
-    if constexpr (MODE != kSingle) cluster_sync_all();  // neither leaves while the other uses its barriers, or reads its sums
-    else __syncthreads();
+    if constexpr (MODE == kPair) cluster_sync_all();  // neither leaves while the other uses its barriers
+    else if constexpr (MODE == kSingle) __syncthreads();
     if constexpr (MODE == kSplit) {
-        // rank z finishes the tokens z, z + n_split, ...: a warp to each, 4 columns to a lane; the sums in the order of the ranks
-        int given_up = 0;  // (all asked for at once, as the sums are)
-        for (int r = 0; r < n_split; ++r) given_up |= ld_cluster_s32(map_rank(const_cast<int*>(gave_up), r));
-        const int n = rows_at(first) + 4 * lane, m0 = tokens_at(first);
-        if (given_up == 0 && warp < kDrain) {
-            float bias[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.bias) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < a.N) bias[e] = as_float(ld_coherent(static_cast<const T*>(a.bias) + n + e));
-            }
-            const float* part = reinterpret_cast<const float*>(sm) + 4 * lane;
-            for (int col = rank + n_split * warp; col < g.bn && m0 + col < a.M; col += n_split * kDrain) {
-                const long long m = m0 + col;
-                float old[4] = {0.f, 0.f, 0.f, 0.f};
-                if (a.residual) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < a.N) old[e] = as_float(ld_coherent(static_cast<const O*>(a.residual) + m * a.ldr + n + e));
-                }
-                float4 f[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    f[r] = r < n_split ? ld_cluster_f4(map_rank(part + col * kRows, r)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                float y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int r = 0; r < 8; ++r) y[0] += f[r].x, y[1] += f[r].y, y[2] += f[r].z, y[3] += f[r].w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] += bias[e];
-                activate<KIND>(a, y);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < a.N) static_cast<O*>(a.out)[m * a.ldo + n + e] = rounded<O>(a.residual ? y[e] + old[e] : y[e]);
-            }
-        }
-        cluster_sync_all();
+        const float* part = reinterpret_cast<const float*>(sm);
+        const int n0 = rows_at(first), m0 = tokens_at(first);
+        if (n_split == 2) join<T, O, KIND, 2>(a, part, gave_up, rank, warp, lane, n0, m0, g.bn);
+        else if (n_split == 4) join<T, O, KIND, 4>(a, part, gave_up, rank, warp, lane, n0, m0, g.bn);
+        else join<T, O, KIND, 8>(a, part, gave_up, rank, warp, lane, n0, m0, g.bn);
     }
     if (warp == kDrain) {
         tc_fence_after();
@@ -859,6 +920,26 @@ cudaError_t launch_kind(const Args& a, const Tiling& g, int ctas, int groups, cu
     return launch_mode<T, O, MODE, kGelu>(a, g, ctas, groups, st);
 }
 
+// How many clusters of 2, 4 or 8 CTAs a device holds at a time (asked for once; where that fails, none).
+int most_clusters(int device, int ctas) {
+    static std::atomic<int> known[64][3];
+    const int i = ctas == 2 ? 0 : ctas == 4 ? 1 : 2;
+    if (device > 63) return 0;
+    int n = known[device][i].load(std::memory_order_relaxed);
+    if (n == 0) {
+        const auto kernel = linear16_tc<__nv_bfloat16, __nv_bfloat16, kSplit, kClamp>;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        cfg.gridDim = dim3(8 * ctas, 1, 1), cfg.blockDim = dim3(kThreads, 1, 1), cfg.dynamicSmemBytes = kSmem + 1024;
+        with_cluster(cfg, attr, ctas, nullptr);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem + 1024);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        if (e != cudaSuccess) (void)cudaGetLastError(), n = 0;
+        known[device][i].store(n > 0 ? n : -1, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 template <typename T, typename O>
 cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
     // Few tokens: warp-level products while the weights are few as well, for the tensor cores then take longer to start (4096 x
@@ -870,37 +951,31 @@ cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
     if (a.M <= 8 && weights < 1 << 24) return launch_few<T, O, 1>(a, num_sms, st);
     if (a.M <= 16 && weights <= 1 << 23) return launch_few<T, O, 2>(a, num_sms, st);
     if (a.M <= 256 && a.K > 128 && (a.M + 31) / 32 * weights <= 1 << 21) return launch_few<T, O, 4>(a, num_sms, st);
-    auto up = [](long long x, long long to) { return (x + to - 1) / to; };
-    Tiling g = {};
+    // The form and the tile of tokens that take the fewest cycles, as they were measured: a stage's products or its bytes from
+    // L2; a drained tile beside the next one's products; for a shared k the sums' way through the cluster (14 bytes a cycle).
     const int widest = a.K > (sizeof(O) == 4 ? kSegment : kSegment16) ? 160 : 256;  // (the segments' total takes its room)
-    // the tile of tokens whose rounds over the SMs take the least, by the wider of products and operands
-    auto best = [&](int width, int groups, bool pair) {
-        double least = 1e300;
-        for (int bn = 32; bn <= widest; bn += 32) {
-            const double rounds = (double)up(up(a.N, width) * up(a.M, bn), groups);
-            const double t = rounds * std::max(2.0 * bn, (16384.0 + bn * (pair ? 64 : 128)) / 64.0);
-            if (t < least * 0.999) least = t, g.bn = bn;
-        }
-        return least;
+    const int chunks = (a.K + kChunk - 1) / kChunk, n_tiles = (a.N + kRows - 1) / kRows, n_pairs = (n_tiles + 1) / 2;
+    Tiling g = {};
+    int mode = kSingle, ctas = 1;
+    double least = 1e300, groups = 1.0;
+    auto take = [&](double t, int m, int c, double n, int bn) {
+        if (t < least * 0.999) least = t, mode = m, ctas = c, groups = n, g.bn = bn;
     };
-    const long long few_tiles = up(a.N, kRows) * up(a.M, 128);
-    if (few_tiles * 2 <= num_sms) {
-        // (more than eight clusters of eight are not all at work at once: 16 tokens by 2048 x 1024 11 us)
-        int split = 1;
-        while (split < (few_tiles <= 8 ? 8 : 4) && few_tiles * split * 2 <= num_sms && a.K >= split * 4 * kChunk) split *= 2;
-        g.bn = (int)std::min<long long>(128, up(a.M, 32) * 32);
-        if (split > 1) return launch_kind<T, O, kSplit>(a, g, split, (int)few_tiles, st);
+    const double sms = num_sms, half = num_sms / 2, per_sm = 1.0 / sms, per_half = 1.0 / half;
+    for (int bn = 32; bn <= widest; bn += 32) {
+        const double m_tiles = (a.M + bn - 1) / bn, tiles = n_tiles * m_tiles, pairs = n_pairs * m_tiles;
+        const double drain = 880.0 / 32 * bn, stage = std::max(2.0 * bn, 256.0 + 2.0 * bn), pair_stage = std::max(2.0 * bn, 256.0 + bn);
+        const double one = chunks * stage, two = chunks * pair_stage;
+        auto rounds = [](double x) { return std::ceil(x - 1e-7); };
+        take(rounds(tiles * per_sm) * (std::max(one, drain) + 300.0) + std::min(one, drain), kSingle, 1, std::min(tiles, sms), bn);
+        take(rounds(pairs * per_half) * (std::max(two, drain) + 300.0) + std::min(two, drain), kPair, 2, std::min(pairs, half), bn);
+        for (int split = 2; split <= 8 && bn <= 128 && chunks >= 2 * split && tiles * split <= sms && tiles <= most_clusters(a.device, split); split *= 2)
+            take((chunks + split - 1) / split * stage + 200.0 / 32 * bn + 1500.0 + bn * 512.0 / 14.0 * (split - 1) / split, kSplit, split, tiles, bn);
+        if (bn >= a.M) break;
     }
-    const double pair = best(2 * kRows, num_sms / 2, true);
-    const int pair_bn = g.bn;
-    const double single = best(kRows, num_sms, false);
-    if (pair < single) {
-        g.bn = pair_bn;
-        const long long tiles = up(a.N, 2 * kRows) * up(a.M, g.bn);
-        return launch_kind<T, O, kPair>(a, g, 2, (int)std::min<long long>(tiles, num_sms / 2), st);
-    }
-    const long long tiles = up(a.N, kRows) * up(a.M, g.bn);
-    return launch_kind<T, O, kSingle>(a, g, 1, (int)std::min<long long>(tiles, num_sms), st);
+    if (mode == kSplit) return launch_kind<T, O, kSplit>(a, g, ctas, (int)groups, st);
+    if (mode == kPair) return launch_kind<T, O, kPair>(a, g, ctas, (int)groups, st);
+    return launch_kind<T, O, kSingle>(a, g, ctas, (int)groups, st);
 }
 
 int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
