@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // (given up: what is in flight lands before the CTA ends)
-        if (lane == 0 && *gave_up && rank == 0)
+        if (lane == 0 && *gave_up && (MODE != kPair || rank == 0))
             for (uint32_t j = i > (uint32_t)stages ? i - stages : 0; j < i; ++j)
                 (void)mbar_wait_bounded(full + j % stages, (j / stages) & 1, kTestWaitBudgetCycles);
         __syncwarp();
@@ -942,15 +942,18 @@ int most_clusters(int device, int ctas) {
 
 template <typename T, typename O>
 cudaError_t launch(const Args& a, int num_sms, cudaStream_t st) {
-    // Few tokens: warp-level products while the weights are few as well, for the tensor cores then take longer to start (4096 x
-    // 1024 by 1, 16 and 32 tokens 3.5, 4.2 and 7.6 us against 6.9 on the tensor cores; 1024 x 1024 by 64 4.8 against 6.9, by 96
-    // 7.6 against 7.5; 256 x 1024 by 200 4.2 against 7.6; where k is short, they are quick: 64 x 64 by 1160 4.8); they keep more of the weights on their way (16384 x 1024 by 1 and 16
-    // 10.2 and 14.3 us against 8.9 and 9.5).
+    // Few tokens: warp-level products while the weights are few as well, for the tensor cores then take longer to start (1024 x
+    // 1024 by 1, 16 and 64 tokens 2.8, 3.4 and 4.1 us against 4.8, 4.8 and 5.5 on the tensor cores; 4096 x 1024 by 16 4.1
+    // against 6.1).  These keep more of the weights on their way (16384 x 1024 by 1 and 16 9.0 and 13.0 us against 8.7 and
+    // 8.9), and a short k is over at once there (1024 x 128 by 16 and 64 4.1 and 6.9 us against 4.1; 2048 x 256 by 128, two
+    // rounds of CTAs, 8.2 against 4.8).
     const long long weights = (long long)a.N * a.K;
     if (a.K < kChunk) return a.M <= 8 ? launch_few<T, O, 1>(a, num_sms, st) : launch_few<T, O, 2>(a, num_sms, st);
-    if (a.M <= 8 && weights < 1 << 24) return launch_few<T, O, 1>(a, num_sms, st);
-    if (a.M <= 16 && weights <= 1 << 23) return launch_few<T, O, 2>(a, num_sms, st);
-    if (a.M <= 256 && a.K > 128 && (a.M + 31) / 32 * weights <= 1 << 21) return launch_few<T, O, 4>(a, num_sms, st);
+    if (a.M <= 8 && weights <= 1 << 23) return launch_few<T, O, 1>(a, num_sms, st);
+    if (a.M > 8 && a.M <= 16 && a.K > 128 && a.N <= 8192 && weights <= 1 << 23) return launch_few<T, O, 2>(a, num_sms, st);
+    const int few_rows = a.K > 512 ? 16 : 32;  // of a CTA (launch_few)
+    if (a.M > 16 && a.K > 256 && a.K <= 1024 && (long long)((a.N + few_rows - 1) / few_rows) * ((a.M + 31) / 32) <= num_sms)
+        return launch_few<T, O, 4>(a, num_sms, st);
     // The form and the tile of tokens that take the fewest cycles, as they were measured: a stage's products or its bytes from
     // L2; a drained tile beside the next one's products; for a shared k the sums' way through the cluster (14 bytes a cycle).
     const int widest = a.K > (sizeof(O) == 4 ? kSegment : kSegment16) ? 160 : 256;  // (the segments' total takes its room)

@@ -82,7 +82,8 @@ SIZES = [
     (128, 128, 128), (129, 640, 513), (200, 300, 8192), (256, 20000, 96), (257, 1023, 1024), (1000, 1024, 512), (3000, 4099, 200),
     (10000, 1024, 64), (4097, 4096, 128), (300, 40001, 64), (1, 40000, 700), (16, 9001, 1000), (27, 1000, 1000), (32, 128, 8192),
     (20, 16, 72), (12, 2048, 4104), (3, 100, 70000), (30, 60, 33000), (100, 200, 40000), (300, 20000, 1100), (2100, 4000, 2500),
-    (260, 300, 17000),
+    (260, 300, 17000), (30000, 100, 64), (5000, 100, 500), (20000, 300, 600), (400, 1024, 4096), (700, 500, 3000), (250, 1000, 9000),
+    (1000, 1023, 4100), (21, 127, 300), (140, 260, 400), (1500, 50, 800),
 ]
 
 
@@ -99,7 +100,8 @@ def test_sizes(cuda_device, M, N, K, wide, dtype):
 @pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True), (True, True)])
 def test_epilogues(cuda_device, act, bias, residual, dtype):
     """On each of the forms: few rows, and blocks of them, a cluster per tile, single CTAs, pairs."""
-    for M, N, K in ((4, 200, 256), (50, 200, 1024), (60, 1000, 2048), (300, 20000, 64), (4096, 8192, 128)):
+    for M, N, K in ((4, 200, 256), (50, 200, 1024), (60, 1000, 2048), (300, 20000, 64), (4096, 8192, 128), (30000, 100, 64),
+                    (1000, 1024, 4096), (400, 1004, 4096)):
         case(M, N, K, dtype, act, bias, residual)
 
 
@@ -142,7 +144,8 @@ def test_small_values_of_activations(cuda_device, act):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["f16", "bf16"])
-@pytest.mark.parametrize("M,N,K", [(6, 96, 128), (40, 256, 640), (70, 900, 2560), (600, 9000, 64), (4096, 8192, 64)])
+@pytest.mark.parametrize("M,N,K", [(6, 96, 128), (40, 256, 640), (70, 900, 2560), (600, 9000, 64), (4096, 8192, 64), (400, 1024, 4096),
+                                   (5000, 100, 504)])
 def test_residual_in_place_and_strided_operands(cuda_device, M, N, K, dtype):
     g = torch.Generator(device="cuda").manual_seed(M)
     wide = normal(g, M, 3 * K, dtype=dtype)  # columns of a fused projection's output
@@ -154,7 +157,7 @@ def test_residual_in_place_and_strided_operands(cuda_device, M, N, K, dtype):
     check(out, x, w, None, before, "none")
 
 
-@pytest.mark.parametrize("M,N,K", [(7, 500, 5000), (60, 500, 5000), (500, 20000, 300), (4096, 4096, 640)])
+@pytest.mark.parametrize("M,N,K", [(7, 500, 5000), (60, 500, 5000), (1000, 1024, 4096), (20000, 300, 600), (500, 20000, 300), (4096, 4096, 640)])
 def test_runs_are_identical(cuda_device, M, N, K):
     a = case(M, N, K, torch.bfloat16, wide=True)
     for _ in range(3):
@@ -215,7 +218,8 @@ def test_streams_side_by_side_and_captured(cuda_device):
     assert na.linear16_status() == na.OK
 
 
-@pytest.mark.parametrize("M,N,K", [(60, 1000, 2048), (300, 20000, 64), (4096, 8192, 128)], ids=["cluster", "single", "pair"])
+@pytest.mark.parametrize("M,N,K", [(60, 1000, 2048), (30000, 100, 64), (300, 20000, 64), (4096, 8192, 128)],
+                         ids=["cluster", "single", "pair", "pairs"])
 def test_a_wait_that_runs_out(cuda_device, M, N, K):
     g = torch.Generator(device="cuda").manual_seed(2)
     x, w = rows(g, M, K, torch.float16), rows(g, N, K, torch.float16, K ** -0.5)
