@@ -21,9 +21,10 @@
 //
 // Measured (device time): one token by 4096 x 1024 3.7 us (2.3 TB/s, the start of
 // a launch); 64 by 256206 x 1024 into fp32 93 us (6.3 TB/s, HBM; the library's
-// product into bf16 174); 10000 by 1024 x 4096 with a residual 70 us (1200
-// TFLOP/s, the tensor cores 73 % busy, operands from L2 in three rounds of tiles;
-// the library's product alone 65); 8192 by 8192 x 4096 389 us (1415 TFLOP/s; 369).
+// product into bf16 174); 10000 by 1024 x 4096 with a residual 68 us (1230
+// TFLOP/s, the tensor cores 75 % busy, operands from L2 in three rounds of tiles;
+// the library's product alone 65); 8192 by 8192 x 4096 360 to 380 us (369);
+// 128 by 1024 x 1024 6.2 us, 512 by 256 x 256 4.9.
 #include <cuda.h>
 
 #include <algorithm>
@@ -312,7 +313,7 @@ enum { kSingle = 0, kPair = 1, kSplit = 2 };
 struct Tiling {
     int bn;           // tokens of a tile, a multiple of 32 up to 256
     int stages;
-    int slots;        // of a warp: 8 where residual rows of 16 bits come through them, else 4
+    int slots;        // of a warp: of 16 bits 8 where residual rows come through them, or k is short and draining counts, else 4
     int segment;      // stages whose products the tensor cores add
     int acc;          // columns of an accumulator in tensor memory; behind two of them the segments' total
     int tiles_n, tiles_m;
@@ -696,6 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < g.slots - 2; ++i) ask();
         bool ok = true;
         uint32_t n = 0;  // accumulators
+        const bool lean = a.out_whole && !a.residual && segments == 1;
         const uint32_t total = from0 + 2 * g.acc;
         auto release = [&](uint32_t acc) {
             tc_fence_before();
@@ -749,6 +751,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
                 const bool mine = here.n0 + lane < a.N;
                 const float bias = a.bias && mine ? as_float(ld_coherent(static_cast<const T*>(a.bias) + here.n0 + lane)) : 0.f;
+                if (lean) {
+                    // (as below, and nothing that is not needed: 6318 rows of 3200 over k = 256 20 us, there 22.5)
+                    float next[PIECE];
+                    if (half < here.count) tmem_ask(from + half * PIECE, next);
+                    for (int i = half; i < here.count; i += 2, ++used) {
+                        const uint32_t at = used & mask;
+                        O* mem = mem0 + at * (kSlot / sizeof(O));
+                        float v[PIECE];
+                        tmem_wait(next);
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j) v[j] = next[j] + bias;
+                        if (i + 2 < here.count) tmem_ask(from + (i + 2) * PIECE, next);
+                        activate<KIND>(a, v);
+                        if (lane == 0) {
+                            if (g.slots == 8) stores_read<7>();
+                            else stores_read<3>();
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < PIECE; ++j) mem[j * 32] = rounded<O>(v[j]);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tma_store_2d(&to, here.n0, here.m0 + i * PIECE, slot0 + at * kSlot);
+                        __syncwarp();
+                    }
+                    tmem_wait(next);
+                    release(acc);
+                    continue;
+                }
                 const bool res_lanes = a.residual && !a.res_whole && mine;
                 O old[PIECE];  // (asked for a piece ahead)
                 auto ask_lanes = [&](int i) {
@@ -881,7 +912,7 @@ cudaError_t launch_mode(const Args& a, Tiling g, int ctas, int groups, cudaStrea
     const int width = MODE == kPair ? 2 * kRows : kRows, x_rows = MODE == kPair ? g.bn / 2 : g.bn;
     const int stage = (int)kRowsBytes + x_rows * kChunk * 2;
     constexpr uint32_t kSlot = kPiece * 32 * sizeof(O);
-    g.slots = MODE == kSplit ? 0 : a.res_whole && sizeof(O) == 2 ? 8 : 4;
+    g.slots = MODE == kSplit ? 0 : sizeof(O) == 2 && (a.res_whole || a.K <= 1024) ? 8 : 4;
     g.stages = std::min(kMaxStages, ((int)(kSmem - kBars) - g.slots * (int)(kDrain * kSlot)) / stage);
     g.segment = (sizeof(O) == 4 ? kSegment : kSegment16) / kChunk;
     g.acc = a.K > (MODE == kSplit ? ctas : 1) * g.segment * kChunk ? 160 : 256;
