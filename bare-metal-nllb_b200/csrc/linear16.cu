@@ -372,6 +372,18 @@ __device__ __forceinline__ void stores_read() {
 }
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// Whether phase `parity` is over, without a wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -623,6 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (a.expire) ok = __all_sync(0xffffffffu, wait_one(never, 0, kTestWaitBudgetCycles));  // nothing arrives there
             const uint64_t da0 = umma_desc_k_sw128(base), db0 = umma_desc_k_sw128(base + kRowsBytes);
             uint32_t s = 0, turn = 0, n = 0;
+            bool there = false;  // the next stage is, as a look at it showed while the last one's products were issued
             for (int t = first; t < tiles && ok; t += step)
                 for (int b = c0; b < c1; b += g.segment, ++n) {
                     const uint32_t acc = n & 1;
@@ -631,9 +644,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t d = tmem + acc * g.acc;
                     const int e = min(c1, b + g.segment);
                     for (int c = b; c < e; ++c) {
-                        if (!(ok = __all_sync(0xffffffffu, wait_one(full + s, turn & 1)))) break;
+                        if (!there && !(ok = __all_sync(0xffffffffu, wait_one(full + s, turn & 1)))) break;
                         tc_fence_after();
                         const uint64_t da = da0 + s * (stage_bytes / 16), db = db0 + s * (stage_bytes / 16);  // (addresses / 16)
+                        const uint32_t next = s + 1 == (uint32_t)stages ? 0 : s + 1, next_turn = next ? turn : turn + 1;
+                        const bool look = mbar_test(full + next, next_turn & 1);
                         if (elect_one()) {
 #pragma unroll
                             for (int k = 0; k < kChunk / 16; ++k) {
@@ -643,8 +658,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if constexpr (MODE == kPair) commit_pair(empty + s);
                             else tc_commit(empty + s);
                         }
-                        __syncwarp();
-                        if (++s == (uint32_t)stages) s = 0, ++turn;
+                        there = __all_sync(0xffffffffu, look);
+                        s = next, turn = next_turn;
                     }
                     if (!ok) break;
                     if (elect_one()) {
