@@ -127,8 +127,9 @@ __device__ __forceinline__ float2 gelu_gap(float2 y) {
 
 // The activations, each in a form whose small results keep their relative accuracy, in three kinds of code:
 //   kClamp  max(y, c1): none (c1 = -inf) and RELU (0); NaN stays
-//   kSwish  y / (1 + 2^-(y (c1 + c2 y^2))): SILU, and GELU_TANH, since (1 + tanh u) / 2 = 1 / (1 + e^-2u); nothing is left at
-//           -100 (where a smaller y stops, so that infinity does not meet infinity)
+//   kSwish  y / (1 + 2^-(y (c1 + c2 y^2))): SILU, and GELU_TANH, since (1 + tanh u) / 2 = 1 / (1 + e^-2u).  Nothing is left
+//           of y at -100, where a smaller y stops, and nothing is taken from it at 100, where the exponent's stops: infinity
+//           meets neither infinity nor SILU's c2 of 0.  (Results below 2^-119 may come out as 0.)
 //   kGelu
 enum { kClamp = 0, kSwish = 1, kGelu = 2 };
 template <int KIND>
@@ -137,7 +138,8 @@ __device__ __forceinline__ float2 activate(const Args& a, float2 y) {
     if constexpr (KIND == kClamp) return make_float2(max_nan(y.x, a.c1), max_nan(y.y, a.c1));
     if constexpr (KIND == kSwish) {
         y = make_float2(max_nan(y.x, -100.f), max_nan(y.y, -100.f));
-        const float2 z = mul2(y, fma2(mul2(y, both(-a.c2)), y, both(-a.c1)));
+        const float2 x = make_float2(fminf(y.x, 100.f), fminf(y.y, 100.f));
+        const float2 z = mul2(x, fma2(mul2(x, both(-a.c2)), x, both(-a.c1)));
         return make_float2(__fdividef(y.x, 1.0f + ex2(z.x)), __fdividef(y.y, 1.0f + ex2(z.y)));
     }
     return fma2(gelu_gap(y), both(-1.0f), make_float2(max_nan(y.x, 0.f), max_nan(y.y, 0.f)));
