@@ -642,13 +642,14 @@ LINEAR_RELU = 1
 
 
 def linear_int8(x, w, weight_scale, bias=None, out=None, residual=None, relu=False, stream=None):
-    """nllb_linear_int8 on torch CUDA tensors: x [M][K] fp32, w [N][K] int8."""
+    """nllb_linear_int8 on torch CUDA tensors: x [M][K] fp32, w [N][K] int8, on
+    the legacy default stream unless `stream` names another (a handle), on
+    which an out is made too."""
     lib = load()
     M, K = x.shape
     N = w.shape[0]
     if out is None:
-        import torch
-        out = torch.empty((M, N), dtype=torch.float32, device=x.device)
+        out = _new_empty(x, (M, N), _types()["torch.float32"], stream or 0)
     _check(lib, lib.nllb_linear_int8(ptr(x), M, K, ptr(w), ptr(weight_scale), ptr(bias), N, ptr(out),
                                      ptr(residual), LINEAR_RELU if relu else 0, stream), "nllb_linear_int8")
     return out
@@ -678,6 +679,20 @@ def linear_int8_noalloc_status(stream=None) -> int:
     return load().nllb_linear_int8_noalloc_status(stream)
 
 
+def _new_empty(like, shape, dtype, stream):
+    """like.new_empty for an output or workspace of a call on `stream` (None: torch's current one), whose memory is that
+    stream's own: work queued on another may still be using what torch hands out there."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    import torch
+    handle, device = getattr(stream, "value", stream) or 1, like.device  # (as current_stream: NULL is the legacy default stream)
+    if handle == (_types()["stream"](device.index) or 1):
+        return like.new_empty(shape, dtype=dtype)
+    on = torch.cuda.default_stream(device) if handle == 1 else torch.cuda.ExternalStream(handle, device=device)
+    with torch.cuda.stream(on):
+        return like.new_empty(shape, dtype=dtype)
+
+
 def _matrix(x, name, rows, cols, dtype, device):
     """Address of a matrix whose rows are contiguous, and the elements from one to the next."""
     if x.dtype is not dtype or x.shape != (rows, cols) or x.get_device() != device:
@@ -693,7 +708,8 @@ def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=Non
     """nllb_linear16 on torch CUDA tensors: act(x w^T + bias) + residual, x
     [M][K], w [N][K], bias [N] of one 16-bit type, residual and out [M][N] of
     it or fp32 (rows may be strided).  Runs on torch's current stream of x's
-    device unless `stream` names another."""
+    device unless `stream` names another (a handle), to which an out that is
+    made here then belongs, as by torch.cuda.stream."""
     kind, device = x.dtype, x.get_device()
     code = (_TYPE_CODES or _types()).get(kind, F32)
     if code == F32:
@@ -709,7 +725,7 @@ def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=Non
     if device < 0:
         raise ValueError("x must be on a GPU")
     if out is None:
-        out = x.new_empty((M, N), dtype=out_kind)
+        out = _new_empty(x, (M, N), out_kind, stream)
     x_at, ldx = _matrix(x, "x", M, K, kind, device)
     w_at, ldw = _matrix(w, "w", N, K, kind, device)
     out_at, ldo = _matrix(out, "out", M, N, out_kind, device)
@@ -751,16 +767,18 @@ def apply_penalties(logits, tokens, n_tokens, penalty=1.2, no_repeat_ngram=2, st
 
 
 def logsoftmax_topk(logits, k=8, vocab=None, stream=None):
-    """nllb_logsoftmax_topk on a torch CUDA tensor logits [rows][ld] fp32:
-    returns (tokens [rows][k] int32, log-probabilities [rows][k] fp32)."""
+    """nllb_logsoftmax_topk on a torch CUDA tensor logits [rows][ld] fp32, on
+    the legacy default stream unless `stream` names another (a handle): returns
+    (tokens [rows][k] int32, log-probabilities [rows][k] fp32), made on that
+    stream, as by torch.cuda.stream."""
     import torch
     lib = load()
     rows = logits.shape[0]
     V = logits.shape[1] if vocab is None else vocab
-    tok = torch.empty((rows, k), dtype=torch.int32, device=logits.device)
-    lp = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
-    ws = torch.empty(max(1, lib.nllb_logsoftmax_topk_ws_bytes(V, max(rows, 1), k)), dtype=torch.uint8,
-                     device=logits.device)
+    on = stream or 0
+    tok = _new_empty(logits, (rows, k), torch.int32, on)
+    lp = _new_empty(logits, (rows, k), torch.float32, on)
+    ws = _new_empty(logits, max(1, lib.nllb_logsoftmax_topk_ws_bytes(V, max(rows, 1), k)), torch.uint8, on)
     _check(lib, lib.nllb_logsoftmax_topk(ptr(logits), logits.stride(0), V, rows, k, ptr(tok), ptr(lp), ptr(ws),
                                          stream), "nllb_logsoftmax_topk")
     return tok, lp
@@ -779,8 +797,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     """nllb_sample on torch CUDA tensors: logits [rows][vocab] (rows may be
     strided), u [rows] fp32; temperature, top_p, min_p [rows] fp32 and top_k
     [rows] int32 or None.  Runs on torch's current stream of the logits'
-    device unless `stream` names another.  Returns (tokens [rows] int32,
-    log-probabilities [rows] fp32)."""
+    device unless `stream` names another (a handle), to which outputs that are
+    made here then belong, as by torch.cuda.stream.  Returns (tokens [rows]
+    int32, log-probabilities [rows] fp32)."""
     lib = load()
     rows, vocab = logits.shape
     if vocab > 1 and logits.stride(1) != 1:
@@ -788,11 +807,10 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     import torch
     if not logits.is_cuda:
         raise ValueError("logits must be on a GPU")
+    out_tok = _new_empty(logits, rows, torch.int32, stream) if out_tok is None else out_tok
+    out_logp = _new_empty(logits, rows, torch.float32, stream) if out_logp is None else out_logp
     if stream is None:
         stream = current_stream(logits.device.index)
-    if out_tok is None or out_logp is None:
-        out_tok = torch.empty(rows, dtype=torch.int32, device=logits.device) if out_tok is None else out_tok
-        out_logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if out_logp is None else out_logp
     f = "torch.float32"
     a = SampleArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _dtype_code(logits), vocab, rows,
                    _ints(temperature, "temperature", rows, logits, f), _ints(top_k, "top_k", rows, logits),
@@ -826,7 +844,8 @@ def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entr
              out_top_logp=None, stream=None):
     """nllb_logprobs on torch CUDA tensors: logits [rows][vocab] (rows may be
     strided), target [rows] int32 or None.  Runs on torch's current stream of
-    the logits' device unless `stream` names another.  Returns
+    the logits' device unless `stream` names another (a handle), to which
+    outputs that are made here then belong, as by torch.cuda.stream.  Returns
     (log-probabilities of the targets [rows] fp32 or None, entropies [rows]
     fp32 or None, likeliest tokens [rows][top_n] int32 and their
     log-probabilities fp32, or None and None for top_n 0)."""
@@ -841,15 +860,15 @@ def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entr
     if logits.get_device() < 0:
         raise ValueError("logits must be on a GPU")
     types = _types()
-    if target is not None and out_logp is None:
-        out_logp = logits.new_empty(rows, dtype=types["torch.float32"])
-    if entropy and out_entropy is None:
-        out_entropy = logits.new_empty(rows, dtype=types["torch.float32"])
-    if top_n and out_top_tok is None:
-        out_top_tok = logits.new_empty((rows, top_n), dtype=types["torch.int32"])
-    if top_n and out_top_logp is None:
-        out_top_logp = logits.new_empty((rows, top_n), dtype=types["torch.float32"])
     device, f32, i32 = logits.get_device(), types["torch.float32"], types["torch.int32"]
+    if target is not None and out_logp is None:
+        out_logp = _new_empty(logits, rows, f32, stream)
+    if entropy and out_entropy is None:
+        out_entropy = _new_empty(logits, rows, f32, stream)
+    if top_n and out_top_tok is None:
+        out_top_tok = _new_empty(logits, (rows, top_n), i32, stream)
+    if top_n and out_top_logp is None:
+        out_top_logp = _new_empty(logits, (rows, top_n), f32, stream)
 
     def at(x, name, n, kind):
         if x is None:
@@ -889,8 +908,7 @@ class PreparedLinear:
     def __call__(self, x, out=None, residual=None, relu=False, stream=None):
         M = x.shape[0]
         if out is None:
-            import torch
-            out = torch.empty((M, self.N), dtype=torch.float32, device=x.device)
+            out = _new_empty(x, (M, self.N), _types()["torch.float32"], stream or 0)
         _check(self._lib, self._lib.nllb_linear_run(self._h, ptr(x), M, ptr(out), ptr(residual),
                                                      LINEAR_RELU if relu else 0, stream), "nllb_linear_run")
         return out
