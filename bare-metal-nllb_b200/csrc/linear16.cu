@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <mutex>
 #include <string>
 
 #include "engine_kernels.h"
@@ -41,7 +42,11 @@ int set_error(int status, const std::string& msg);  // nllb_attn.cu
 
 namespace {
 
-__device__ int g_linear16_err;  // a bounded wait gave up (nllb_linear16_status)
+// A bounded wait of a call without an error word of its own gave up; and what nllb_linear16_status last took from there.
+__device__ int g_linear16_err, g_linear16_taken;
+
+// (one step: what is set meanwhile stays for the next status)
+__global__ void linear16_take_err() { g_linear16_taken = atomicExch(&g_linear16_err, 0); }
 
 struct Args {
     const void *x, *w, *bias, *residual;
@@ -52,6 +57,7 @@ struct Args {
     bool out_whole, res_whole;  // (there and) the rows start on 16 bytes, as TMA has it
     bool expire;  // test: a wait runs out
     int device;
+    int* err;  // the caller's error word (null: the device's)
 };
 
 template <typename T>
@@ -580,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *gave_up = 1;
         if constexpr (MODE == kPair)
             asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(map_rank(const_cast<int*>(gave_up), rank ^ 1)) : "memory");
-        atomicOr(&g_linear16_err, NLLB_DEV_ERR_TIMEOUT);
+        atomicOr(a.err ? a.err : &g_linear16_err, NLLB_DEV_ERR_TIMEOUT);
     };
     // Bounded wait; false (and the CTA, or pair, gives up) once any has run out.
     auto wait_one = [&](uint64_t* bar, uint32_t parity, long long budget = kWaitBudgetCycles) -> bool {
@@ -1043,20 +1049,26 @@ extern "C" int nllb_linear16_test_expire_next_wait(void) {
 
 extern "C" int nllb_linear16_status(void* stream) {
     using namespace nllb;
+    static std::mutex one_at_a_time;  // (g_linear16_taken)
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int err = 0;
-    const int none = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(&err, g_linear16_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess && err) e = cudaMemcpyToSymbolAsync(g_linear16_err, &none, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess && err) e = cudaStreamSynchronize(st);
+    cudaError_t e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess) {
+        std::lock_guard<std::mutex> lock(one_at_a_time);
+        linear16_take_err<<<1, 1, 0, st>>>();
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&err, g_linear16_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    }
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_linear16_status: ") + cudaGetErrorString(e));
     if (err) return set_error(NLLB_ATTN_ETIMEOUT, "a bounded device wait of nllb_linear16 gave up");
     return NLLB_ATTN_OK;
 }
 
-extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
-    using namespace nllb;
+namespace nllb {
+namespace {
+
+int run(const nllb_linear16_args* s, int* error, void* stream) {
     if (!s) return bad("args is NULL");
     if (s->dtype != NLLB_F16 && s->dtype != NLLB_BF16) return bad("dtype must be NLLB_F16 or NLLB_BF16");
     if (s->out_dtype != s->dtype && s->out_dtype != NLLB_F32) return bad("out_dtype must be dtype or NLLB_F32");
@@ -1079,7 +1091,7 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
         return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0 && ld <= 1LL << 36;
     };
     Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, kClamp, 0.f, 0.f,
-              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next, 0};
+              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next, 0, error};
     switch (s->act) {
         case NLLB_ACT_NONE: a.c1 = -INFINITY; break;
         case NLLB_ACT_RELU: break;
@@ -1100,4 +1112,15 @@ extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) {
     }
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_linear16: ") + cudaGetErrorString(e));
     return NLLB_ATTN_OK;
+}
+
+}  // namespace
+}  // namespace nllb
+
+extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) { return nllb::run(s, nullptr, stream); }
+
+extern "C" int nllb_linear16_reporting(const nllb_linear16_args* s, int* error, void* stream) {
+    if (!error) return nllb::bad("error is NULL");
+    if (reinterpret_cast<uintptr_t>(error) % 4) return nllb::bad("error must be aligned to its type");
+    return nllb::run(s, error, stream);
 }

@@ -180,6 +180,7 @@ SIGNATURES = {
     "nllb_linear_test_expire_next_wait": (_c_int, [_c_void_p]),
     "nllb_linear_free": (None, [_c_void_p]),
     "nllb_linear16": (_c_int, [_c_void_p, _c_void_p]),  # (bytes of Linear16Args, or a reference to one)
+    "nllb_linear16_reporting": (_c_int, [_c_void_p, _fp, _c_void_p]),
     "nllb_linear16_status": (_c_int, [_c_void_p]),
     "nllb_linear16_test_expire_next_wait": (_c_int, []),
     "nllb_apply_penalties": (_c_int, [_fp, ctypes.c_longlong, _c_int, _fp, _c_int, _fp, ctypes.c_float, _c_int,
@@ -704,12 +705,14 @@ def _matrix(x, name, rows, cols, dtype, device):
     return x.data_ptr(), row if rows > 1 else (cols + 7) // 8 * 8
 
 
-def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=None, stream=None):
+def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=None, stream=None, error=None):
     """nllb_linear16 on torch CUDA tensors: act(x w^T + bias) + residual, x
     [M][K], w [N][K], bias [N] of one 16-bit type, residual and out [M][N] of
     it or fp32 (rows may be strided).  Runs on torch's current stream of x's
     device unless `stream` names another (a handle), to which an out that is
-    made here then belongs, as by torch.cuda.stream."""
+    made here then belongs, as by torch.cuda.stream.  error: an int32 tensor of
+    one entry on x's device, which a bounded wait that gives up makes nonzero
+    in place of the device's error word (nllb_linear16_reporting)."""
     kind, device = x.dtype, x.get_device()
     code = (_TYPE_CODES or _types()).get(kind, F32)
     if code == F32:
@@ -735,15 +738,18 @@ def linear16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=Non
         if bias.dtype is not kind or bias.shape != (N,) or bias.get_device() != device or not bias.is_contiguous():
             raise ValueError(f"bias must be a contiguous {kind} tensor {[N]} on GPU {device}")
         bias_at = bias.data_ptr()
-    _call(device, "nllb_linear16", _pack_linear16(x_at, w_at, bias_at, res_at, out_at, ldx, ldw, ldr, ldo, code, out_code,
-                                                  act_code, M, N, K), stream)
+    args = _pack_linear16(x_at, w_at, bias_at, res_at, out_at, ldx, ldw, ldr, ldo, code, out_code, act_code, M, N, K)
+    if error is None:
+        _call(device, "nllb_linear16", stream, args)
+    else:
+        _call(device, "nllb_linear16_reporting", stream, args, _ints(error, "error", 1, x))
     return out
 
 
 def linear16_status(stream=None) -> int:
     """nllb_linear16_status: waits for `stream` (torch's current one by
-    default), reads and clears the current device's error word (returns the
-    status, does not raise)."""
+    default), reads and clears the current device's error word, which is one
+    for all its streams (returns the status, does not raise)."""
     if stream is None:
         stream = current_stream(_types()["current"]())
     return load().nllb_linear16_status(stream)
@@ -825,17 +831,17 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out_
     return out_tok, out_logp
 
 
-def _call(device, name, args, stream):
-    """A library function of (packed arguments, stream) with GPU `device` the
+def _call(device, name, stream, *args):
+    """A library function of (arguments, stream) with GPU `device` the
     current one, on `stream` or torch's current stream there."""
     lib, torch = load(), _types()
     if stream is None:
         stream = torch["stream"](device) or 1  # (current_stream)
     if device == torch["current"]():
-        rc = getattr(lib, name)(args, stream)
+        rc = getattr(lib, name)(*args, stream)
     else:
         with torch["device"](device):
-            rc = getattr(lib, name)(args, stream)
+            rc = getattr(lib, name)(*args, stream)
     if rc != OK:
         _check(lib, rc, name)
 
@@ -881,7 +887,7 @@ def logprobs(logits, target=None, top_n=0, entropy=True, out_logp=None, out_entr
                        at(target, "target", rows, i32), at(out_logp, "out_logp", rows, f32),
                        at(out_entropy, "out_entropy", rows, f32), at(out_top_tok, "out_top_tok", rows * top_n, i32),
                        at(out_top_logp, "out_top_logp", rows * top_n, f32))
-    _call(device, "nllb_logprobs", a, stream)
+    _call(device, "nllb_logprobs", stream, a)
     return out_logp, out_entropy, out_top_tok, out_top_logp
 
 

@@ -184,9 +184,12 @@ NLLB_ATTN_API void nllb_linear_free(nllb_linear* layer);
  * SILU.  out may not overlap x, w or bias.  Device pointers; asynchronous on
  * `stream` (a cudaStream_t, NULL = default); nothing is allocated and no
  * workspace is kept, so calls may overlap and be captured.  A bounded device
- * wait that gives up leaves the outputs invalid and sets a per-device error
- * word, which nllb_linear16_status (waits for `stream`) reads and clears:
- * NLLB_ATTN_ETIMEOUT if set. */
+ * wait that gives up leaves the outputs invalid and sets an error word of the
+ * device, which nllb_linear16_status reads and clears in one step once all work
+ * on `stream` is over: NLLB_ATTN_ETIMEOUT if it was set.  The word is one for
+ * all streams of the device, and a status call takes what any of them has
+ * reported: where several streams have to know each for itself,
+ * nllb_linear16_reporting has them set words of their own. */
 #define NLLB_ACT_NONE 0
 #define NLLB_ACT_RELU 1
 #define NLLB_ACT_GELU 2
@@ -204,6 +207,11 @@ typedef struct {
 } nllb_linear16_args;
 NLLB_ATTN_API int nllb_linear16(const nllb_linear16_args* args, void* stream);
 NLLB_ATTN_API int nllb_linear16_status(void* stream);
+/* nllb_linear16 with an error word of the caller's, an int in device memory
+ * that is there as long as the call runs (in a graph, as often as it does): a wait
+ * that gives up makes it nonzero and leaves the device's word alone; nothing else
+ * writes it. */
+NLLB_ATTN_API int nllb_linear16_reporting(const nllb_linear16_args* args, int* error, void* stream);
 /* Test of the bounded device waits: if the calling thread's next nllb_linear16
  * runs on the tensor cores' kernel (more than 32 rows, K >= 64 and N K above 2^20
  * do), a wait of its runs out after about 1 ms and nllb_linear16_status reports
