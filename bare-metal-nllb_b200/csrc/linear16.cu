@@ -1069,6 +1069,8 @@ namespace nllb {
 namespace {
 
 int run(const nllb_linear16_args* s, int* error, void* stream) {
+    const bool expire = t_expire_next;  // (this call's, whatever becomes of it)
+    t_expire_next = false;
     if (!s) return bad("args is NULL");
     if (s->dtype != NLLB_F16 && s->dtype != NLLB_BF16) return bad("dtype must be NLLB_F16 or NLLB_BF16");
     if (s->out_dtype != s->dtype && s->out_dtype != NLLB_F32) return bad("out_dtype must be dtype or NLLB_F32");
@@ -1091,7 +1093,7 @@ int run(const nllb_linear16_args* s, int* error, void* stream) {
         return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0 && ld <= 1LL << 36;
     };
     Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, kClamp, 0.f, 0.f,
-              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), t_expire_next, 0, error};
+              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), expire, 0, error};
     switch (s->act) {
         case NLLB_ACT_NONE: a.c1 = -INFINITY; break;
         case NLLB_ACT_RELU: break;
@@ -1099,7 +1101,6 @@ int run(const nllb_linear16_args* s, int* error, void* stream) {
         case NLLB_ACT_GELU_TANH: a.kind = kSwish, a.c1 = 2.3022082f, a.c2 = 0.10294324f; break;  // 2 sqrt(2/pi) log2 e (1, 0.044715)
         default: a.kind = kSwish, a.c1 = kLog2e;  // SILU
     }
-    t_expire_next = false;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int device = 0, num_sms = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -1120,7 +1121,9 @@ int run(const nllb_linear16_args* s, int* error, void* stream) {
 extern "C" int nllb_linear16(const nllb_linear16_args* s, void* stream) { return nllb::run(s, nullptr, stream); }
 
 extern "C" int nllb_linear16_reporting(const nllb_linear16_args* s, int* error, void* stream) {
-    if (!error) return nllb::bad("error is NULL");
-    if (reinterpret_cast<uintptr_t>(error) % 4) return nllb::bad("error must be aligned to its type");
+    if (!error || reinterpret_cast<uintptr_t>(error) % 4) {
+        nllb::t_expire_next = false;
+        return nllb::bad("error must be an address, aligned to its type");
+    }
     return nllb::run(s, error, stream);
 }

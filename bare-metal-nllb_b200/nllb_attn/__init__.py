@@ -757,7 +757,7 @@ def linear16_status(stream=None) -> int:
 
 def linear16_test_expire_next_wait() -> None:
     """nllb_linear16_test_expire_next_wait: a bounded wait of this thread's
-    next linear16 on the tensor cores' kernel runs out."""
+    next linear16 runs out, if that runs on the tensor cores' kernel."""
     lib = load()
     _check(lib, lib.nllb_linear16_test_expire_next_wait(), "linear16_test_expire_next_wait")
 

@@ -213,9 +213,10 @@ NLLB_ATTN_API int nllb_linear16_status(void* stream);
  * writes it. */
 NLLB_ATTN_API int nllb_linear16_reporting(const nllb_linear16_args* args, int* error, void* stream);
 /* Test of the bounded device waits: if the calling thread's next nllb_linear16
- * runs on the tensor cores' kernel (more than 32 rows, K >= 64 and N K above 2^20
- * do), a wait of its runs out after about 1 ms and nllb_linear16_status reports
- * it.  Later calls are as ever. */
+ * runs on the tensor cores' kernel (those of more than 16 rows do where K lies in
+ * 64..256 or above 1024; of others it goes by their sizes), a wait of its runs out
+ * after about 1 ms and is reported.  Later calls are as ever, also where that next
+ * one was refused, had no rows or ran on the other kernel. */
 NLLB_ATTN_API int nllb_linear16_test_expire_next_wait(void);
 
 /* ---- per-step vocabulary operations of the beam search --------------------
