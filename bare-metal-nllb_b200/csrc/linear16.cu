@@ -606,12 +606,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- fetch (a warp's loop with one thread that asks: addresses and coordinates then lie in uniform registers; by a
         // thread alone each stage took 390 cycles to ask for)
         const uint32_t full0 = MODE == kPair ? map_rank(full, 0) : smem_u32(full);
-        uint32_t i = 0, s = 0, turn = 0;  // stages so far; the next one's place, and how often it has come round
+        uint32_t s = 0, turn = 0;  // the next stage's place, and how often it has come round
         bool ok = true;
         for (int t = first; t < tiles && ok; t += step) {
             const int n0 = rows_at(t) + (MODE == kPair ? rank * kRows : 0);
             const int m0 = tokens_at(t) + (MODE == kPair ? rank * (int)x_rows : 0);
-            for (int c = c0; c < c1; ++c, ++i) {
+            for (int c = c0; c < c1; ++c) {
                 if (turn > 0 && !(ok = __all_sync(0xffffffffu, wait_one(empty + s, (turn - 1) & 1)))) break;
                 const uint32_t at = base + s * stage_bytes;
                 if (elect_one()) {
@@ -629,11 +629,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (++s == (uint32_t)stages) s = 0, ++turn;
             }
         }
-        // (given up: what is in flight lands before the CTA ends)
-        if (lane == 0 && *gave_up && (MODE != kPair || rank == 0))
-            for (uint32_t j = i > (uint32_t)stages ? i - stages : 0; j < i; ++j)
-                (void)mbar_wait_bounded(full + j % stages, (j / stages) & 1, kTestWaitBudgetCycles);
-        __syncwarp();
     } else if (warp == kDrain + 1) {
         // ---- products (of both CTAs of a pair: by the first one's)
         if (MODE != kPair || rank == 0) {
@@ -883,6 +878,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         else join<T, O, KIND, 8>(a, part, gave_up, rank, warp, lane, n0, m0, g.bn);
     }
     if (warp == kDrain) {
+        // Given up: time for what is in flight to land before the CTA ends, whoever asked for it and has ended since (of a pair
+        // the second CTA, whose stages complete at the first, too).  Waits on their barriers, here or behind the fetching
+        // loop, would cost every launch (128 rows of 1024 over k = 1024 6.8 us instead of 6.2).
+        if (lane == 0 && *gave_up) (void)mbar_wait_bounded(never, 0, kTestWaitBudgetCycles);
+        __syncwarp();
         tc_fence_after();
         if constexpr (MODE == kPair)
             asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM) : "memory");
