@@ -29,6 +29,7 @@
 // in bf16 without 55 us (5.6 TB/s; the exponentials alone would take 34); one row
 // with 8 tokens 11 us, the latency of a cluster of eight and two merges of lists.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -462,17 +463,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Args a
     if (C > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-template <typename T, bool TOP>
-cudaError_t launch_one(const Args& a, int rows, int C, cudaStream_t st) {
-    if (C > 8) {  // (beyond the portable size)
-        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-    }
-    cudaLaunchConfig_t cfg = {};
+void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int rows, int C, cudaStream_t st) {
     cfg.gridDim = dim3((unsigned)rows * (unsigned)C, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = kPdlLaunch;
     attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -480,23 +474,46 @@ cudaError_t launch_one(const Args& a, int rows, int C, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = C > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, a, C);
 }
 
-template <typename T>
-cudaError_t launch(const Args& a, int rows, int num_sms, cudaStream_t st) {
+// CTAs of a cluster at most on this device: kMaxCluster where one of as many, beyond the portable size, has room there (a part
+// of a GPU may have none; asked for once), else 8.
+template <typename T, bool TOP>
+int widest(int device) {
+    static std::atomic<int> known[64];
+    if (device > 63) return 8;
+    int c = known[device].load(std::memory_order_relaxed);
+    if (c == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[2];
+        configure(cfg, attr, 1, kMaxCluster, nullptr);
+        int n = 0;
+        cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, logprobs_kernel<T, TOP>, &cfg);
+        if (e != cudaSuccess) (void)cudaGetLastError(), n = 0;
+        c = n > 0 ? kMaxCluster : 8;
+        known[device].store(c, std::memory_order_relaxed);
+    }
+    return c;
+}
+
+template <typename T, bool TOP>
+cudaError_t launch(const Args& a, int rows, int device, int num_sms, cudaStream_t st) {
     // CTAs of a row, by what a call takes: the stream, at 50 bytes a nanosecond of a CTA alone and 6500 of them all, and what
-    // follows it, more where a cluster has to meet (1000 rows of 256206 in fp32 150 us by one CTA each, 159 by two; one row
-    // with 8 tokens 23, 16, 12, 10 and 11 us by 1, 2, 4, 8 and 16).
+    // follows it, more where a cluster has to meet (1000 rows of 256206 in fp32 without tokens 154 us by one CTA each, 166 by two;
+    // one row with 8 tokens 21, 16, 12, 11 and 11 us by 1, 2, 4, 8 and 16; one of 820001 in bf16 49, 29, 19, 14.4 and 13.7).
     const double bytes = (double)a.vocab * sizeof(T), slots = (double)kPerSm * num_sms;
     int C = 1;
     double least = 1e300;
     for (int c = 1; c <= kMaxCluster; c *= 2) {
         const double at_work = std::min((double)rows * c, slots);
         const double t = (double)rows * c / at_work * (bytes / c / std::min(50.0, 6500.0 / at_work) + (c == 1 ? 4000.0 : 6000.0 + 250.0 * c));
-        if (t < least) least = t, C = c;
+        if (t < least && (c <= 8 || c <= widest<T, TOP>(device))) least = t, C = c;
     }
-    return a.top_n ? launch_one<T, true>(a, rows, C, st) : launch_one<T, false>(a, rows, C, st);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    configure(cfg, attr, rows, C, st);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, a, C);
 }
 
 int bad(const char* msg) { return set_error(NLLB_ATTN_EINVAL, msg); }
@@ -530,9 +547,11 @@ extern "C" int nllb_logprobs(const nllb_logprobs_args* s, void* stream) {
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess)
-        e = s->dtype == NLLB_F32   ? launch<float>(a, s->rows, num_sms, st)
-            : s->dtype == NLLB_F16 ? launch<__half>(a, s->rows, num_sms, st)
-                                   : launch<__nv_bfloat16>(a, s->rows, num_sms, st);
+        switch (s->dtype) {
+            case NLLB_F32: e = s->top_n ? launch<float, true>(a, s->rows, device, num_sms, st) : launch<float, false>(a, s->rows, device, num_sms, st); break;
+            case NLLB_F16: e = s->top_n ? launch<__half, true>(a, s->rows, device, num_sms, st) : launch<__half, false>(a, s->rows, device, num_sms, st); break;
+            default: e = s->top_n ? launch<__nv_bfloat16, true>(a, s->rows, device, num_sms, st) : launch<__nv_bfloat16, false>(a, s->rows, device, num_sms, st);
+        }
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("nllb_logprobs: ") + cudaGetErrorString(e));
     return NLLB_ATTN_OK;
 }
