@@ -35,6 +35,7 @@
 
 #include "engine_kernels.h"
 #include "nllb_translate.h"
+#include "overlap.h"
 #include "rows.cuh"
 
 namespace nllb {
@@ -1089,6 +1090,13 @@ int run(const nllb_linear16_args* s, int* error, void* stream) {
     if ((reinterpret_cast<uintptr_t>(s->out) | reinterpret_cast<uintptr_t>(s->residual)) % size ||
         reinterpret_cast<uintptr_t>(s->bias) % 2)
         return bad("out, residual and bias must be aligned to their types");
+    const MemRows out(s->out, s->M, s->ldo * (long long)size, s->N * (long long)size);
+    if (meet(out, MemRows(s->x, s->M, s->ldx * 2, s->K * 2LL)) || meet(out, MemRows(s->w, s->N, s->ldw * 2, s->K * 2LL)) ||
+        (s->bias && meet(out, MemRows(s->bias, 1, 0, s->N * 2LL))))
+        return bad("out may not overlap x, w or bias");
+    if (s->residual && !(s->residual == s->out && (s->ldr == s->ldo || s->M == 1)) &&
+        meet(out, MemRows(s->residual, s->M, s->ldr * (long long)size, s->N * (long long)size)))
+        return bad("residual may be out itself, with the same ldr, and may not overlap it otherwise");
     auto whole = [&](const void* base, long long ld) {
         return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0 && ld <= 1LL << 36;
     };

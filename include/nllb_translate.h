@@ -175,15 +175,15 @@ NLLB_ATTN_API void nllb_linear_free(nllb_linear* layer);
  * in NLLB_F16 or NLLB_BF16).  No counterpart in the reference, whose layers take
  * fp32 rows and int8 weights (nllb_linear_int8 and its prepared form here).
  * x [M][K], w [N][K] and bias [N] (NULL: none) are of `dtype`, out [M][N] and
- * residual [M][N] (NULL: none; may be out itself) of `out_dtype`: dtype, or
- * NLLB_F32.  Rows lie ldx, ldw, ldo, ldr elements apart; those of x and w start
- * on 16 bytes, the others anywhere.  Sums are fp32, from their start to the
+ * residual [M][N] (NULL: none; may be out itself, row by row) of `out_dtype`:
+ * dtype, or NLLB_F32.  Rows lie ldx, ldw, ldo, ldr elements apart; those of x and
+ * w start on 16 bytes, the others anywhere.  Sums are fp32, from their start to the
  * residual, and rounded once; they may come out short of the sum of their
  * summands' sizes by up to K 2^-27, at most 2^-17 for NLLB_F32 outputs and 2^-13
  * for others.  act: NONE, RELU, GELU (by erf), GELU_TANH (its tanh form) or
- * SILU.  out may not overlap x, w or bias.  Device pointers; asynchronous on
- * `stream` (a cudaStream_t, NULL = default); nothing is allocated and no
- * workspace is kept, so calls may overlap and be captured.  A bounded device
+ * SILU.  An out that shares memory with x, w or bias, or with a residual that is
+ * not out itself, is refused.  Device pointers; asynchronous on `stream` (a
+ * cudaStream_t, NULL = default); nothing is allocated and no workspace is kept, so calls may overlap and be captured.  A bounded device
  * wait that gives up leaves the outputs invalid and sets an error word of the
  * device, which nllb_linear16_status reads and clears in one step once all work
  * on `stream` is over: NLLB_ATTN_ETIMEOUT if it was set.  The word is one for
