@@ -7,6 +7,7 @@
 #include "attn_internal.h"
 #include "device_common.cuh"
 #include "nllb_attn.h"
+#include "overlap.h"
 #include "rows.h"
 
 namespace nllb {
@@ -72,6 +73,24 @@ bool pages_apart(const Args& a) {
     return apart(a.n_pages, a.k_stride_page, a.head_dim) && apart(a.page_size, a.k_stride_slot, a.head_dim) &&
            apart(a.n_kv_heads, a.k_stride_head, a.head_dim) && apart(a.n_pages, a.v_stride_page, a.head_dim) &&
            apart(a.page_size, a.v_stride_slot, a.head_dim) && apart(a.n_kv_heads, a.v_stride_head, a.head_dim);
+}
+
+// The memory of rows of heads, where it is rows without gaps in them (else none: not looked at).
+MemRows heads_of(const void* p, int64_t rows, int64_t row, int heads, int64_t head, int64_t dim, int size) {
+    constexpr int64_t far = 1LL << 36;
+    if (p && (heads == 1 || head == dim) && (rows == 1 || row >= heads * dim))
+        return MemRows(p, rows, std::min(row, far) * size, heads * dim * size);
+    if (p && (rows == 1 || row == dim) && head >= rows * dim) return MemRows(p, heads, std::min(head, far) * size, rows * dim * size);
+    return MemRows(p, 0, 0, 0);
+}
+
+// The memory of pages of slots of heads.
+MemRows pages_of(const void* p, int64_t pages, int64_t page, int64_t slots, int64_t slot, int heads, int64_t head, int64_t dim, int size) {
+    const bool by_slot = (heads == 1 || head == dim) && (slots == 1 || slot == heads * dim);
+    const bool by_head = (slots == 1 || slot == dim) && (heads == 1 || head == slots * dim);
+    const int64_t len = slots * heads * dim;
+    if (!p || !(by_slot || by_head) || (pages > 1 && page < len)) return MemRows(p, 0, 0, 0);
+    return MemRows(p, pages, std::min<int64_t>(page, 1LL << 36) * size, len * size);
 }
 
 // Division of a j < 2^30 by d: with 2^(b-1) < d <= 2^b the multiplier ceil(2^(30+b) / d) is too large by less than 1, so
@@ -234,6 +253,18 @@ int nllb_attn_append(nllb_attn_ctx* c, const nllb_attn_append_args* a) {
         return bad("q turned in its place keeps its strides");
     if (!pages_apart(*a)) return bad("k_pages, v_pages: strides below head_dim, the rows written would overlap");
     if (!c) return bad("ctx is NULL");
+    const int size = a->dtype == NLLB_F32 ? 4 : 2;
+    const MemRows in[3] = {heads_of(a->k_new, a->q_rows, a->k_new_stride_row, a->n_kv_heads, a->k_new_stride_head, a->head_dim, size),
+                           heads_of(a->v_new, a->q_rows, a->v_new_stride_row, a->n_kv_heads, a->v_new_stride_head, a->head_dim, size),
+                           heads_of(a->q, a->q_rows, a->q_stride_row, a->n_heads, a->q_stride_head, a->head_dim, size)};
+    const MemRows out[3] = {
+        pages_of(a->k_pages, a->n_pages, a->k_stride_page, a->page_size, a->k_stride_slot, a->n_kv_heads, a->k_stride_head, a->head_dim, size),
+        pages_of(a->v_pages, a->n_pages, a->v_stride_page, a->page_size, a->v_stride_slot, a->n_kv_heads, a->v_stride_head, a->head_dim, size),
+        heads_of(a->q_out, a->q_rows, a->q_out_stride_row, a->n_heads, a->q_out_stride_head, a->head_dim, size)};
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j < 3; ++j)
+            if ((meet(out[i], in[j]) && !(i == 2 && j == 2 && a->q == a->q_out)) || (j < i && meet(out[i], out[j])))
+                return bad("pages and q_out may not overlap q, k_new, v_new or one another (q_out may be q)");
     AppendParams p = {};
     RowsParams& r = p.rows;
     r.q = a->q, r.out = a->q_out, r.k_new = a->k_new, r.v_new = a->v_new, r.k_w = a->k_pages, r.v_w = a->v_pages;

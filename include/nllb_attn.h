@@ -330,7 +330,7 @@ NLLB_ATTN_API int nllb_attn_cross_rows(nllb_attn_ctx* ctx, const nllb_attn_cross
  * with p the token's position, or position[row] where that is given; x is
  * taken in 64 bits.  Values are left as they are.  q and q_out (both or
  * neither) may be one buffer, turned in its place; otherwise outputs may not
- * overlap inputs, nor one another.  Rows that belong to no sequence are
+ * overlap inputs, nor one another (refused where rows and pages have no gaps).  Rows that belong to no sequence are
  * neither read nor written, of page_table only the entries of written slots
  * are read; a token whose page number is bad is turned but not stored (nor are
  * its neighbours hurt), and the error word is set.  Nothing is allocated; the
