@@ -56,6 +56,7 @@ struct Args {
     int M, N, K, kind;
     float c1, c2;  // of the activation
     bool out_whole, res_whole;  // (there and) the rows start on 16 bytes, as TMA has it
+    bool out_end;  // output rows end on 16 bytes too
     bool expire;  // test: a wait runs out
     int device;
     int* err;  // the caller's error word (null: the device's)
@@ -716,7 +717,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < g.slots - 2; ++i) ask();
         bool ok = true;
         uint32_t n = 0;  // accumulators
-        const bool lean = a.out_whole && !a.residual && segments == 1;
         const uint32_t total = from0 + 2 * g.acc;
         auto release = [&](uint32_t acc) {
             tc_fence_before();
@@ -770,7 +770,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
                 const bool mine = here.n0 + lane < a.N;
                 const float bias = a.bias && mine ? as_float(ld_coherent(static_cast<const T*>(a.bias) + here.n0 + lane)) : 0.f;
-                if (lean) {
+                // (a TMA store writes the 16 bytes in which a row ends as a whole, and columns of others may follow there)
+                const bool by_tma = a.out_whole && (a.out_end || here.n0 + 32 <= a.N);
+                if (by_tma && !a.residual && segments == 1) {
                     // (as below, and nothing that is not needed: 6318 rows of 3200 over k = 256 20 us, there 22.5)
                     float next[PIECE];
                     if (half < here.count) tmem_ask(from + half * PIECE, next);
@@ -811,6 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (res_lanes && half < here.count) ask_lanes(half);
                 float next[PIECE];
                 if (half < here.count) tmem_ask(from + half * PIECE, next);
+                if (!by_tma && lane == 0) stores_read<0>();  // (of tiles before: no piece of this one waits for a slot's store)
                 for (int i = half; i < here.count; i += 2, ++used) {
                     const int m0 = here.m0 + i * PIECE, rows = min(PIECE, a.M - m0);
                     const uint32_t at = used & mask;
@@ -837,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int j = 0; j < PIECE; ++j) v[j] += as_float(old[j]);  // (rows past the last one: unused)
                         if (i + 2 < here.count) ask_lanes(i + 2);
                     }
-                    if (a.out_whole) {
+                    if (by_tma) {
                         if (!a.res_whole) {  // (else the slot's last store has been waited for)
                             if (lane == 0) stores_read<3>();
                             __syncwarp();
@@ -1101,7 +1104,7 @@ int run(const nllb_linear16_args* s, int* error, void* stream) {
         return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (long long)size)) & 15u) == 0 && ld <= 1LL << 36;
     };
     Args a = {s->x, s->w, s->bias, s->residual, s->out, s->ldx, s->ldw, s->ldr, s->ldo, s->M, s->N, s->K, kClamp, 0.f, 0.f,
-              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), expire, 0, error};
+              whole(s->out, s->ldo), s->residual && whole(s->residual, s->ldr), s->N * (long long)size % 16 == 0, expire, 0, error};
     switch (s->act) {
         case NLLB_ACT_NONE: a.c1 = -INFINITY; break;
         case NLLB_ACT_RELU: break;
