@@ -19,12 +19,15 @@
 // and load half of the tokens' tile each.  Where tiles are few, a cluster shares
 // the sum over k of one tile and joins it through distributed shared memory.
 //
-// Measured (device time): one token by 4096 x 1024 3.7 us (2.3 TB/s, the start of
-// a launch); 64 by 256206 x 1024 into fp32 93 us (6.3 TB/s, HBM; the library's
-// product into bf16 174); 10000 by 1024 x 4096 with a residual 68 us (1230
-// TFLOP/s, the tensor cores 75 % busy, operands from L2 in three rounds of tiles;
-// the library's product alone 65); 8192 by 8192 x 4096 360 to 380 us (369);
-// 128 by 1024 x 1024 6.2 us, 512 by 256 x 256 4.9.
+// Measured (device time, short replays): one token by 4096 x 1024 3.5 to 4.1 us
+// (2.4 TB/s, the start of a launch); 64 by 256206 x 1024 into fp32 93 us (6.3
+// TB/s, HBM; the library's product into bf16 174); 10000 by 1024 x 4096 with a
+// residual 68 us (1230 TFLOP/s, the tensor cores 75 % busy, operands from L2 in
+// three rounds of tiles; 81 us in a long run of them, under the power limit).
+// Under that limit 8192 by 8192 x 4096 430 us (the library's product 408).  In
+// between the library's product is ahead: 128 by 1024 x 1024 6.2 us (4.1), 512 by
+// 4096 x 1024 8.2 (6.2), 1000 by 8192 x 1024 17.8 (16.4); 128 by 1024 x 4096 8.2
+// (8.2), 4096 by 4096 x 1024 29.0 (32.1).
 #include <cuda.h>
 
 #include <algorithm>

@@ -25,9 +25,10 @@
 // What is not behind that goes through sorted lists of 32 in registers.  A row
 // with many equal or rising logits takes more batches of 32, never another way.
 //
-// Measured: 1000 rows of 256206 in fp32 with 20 tokens 161 us (6.4 TB/s), 600 rows
-// in bf16 without 55 us (5.6 TB/s; the exponentials alone would take 34); one row
-// with 8 tokens 11 us, the latency of a cluster of eight and two merges of lists.
+// Measured (device time, short replays; in long runs 7 to 10 % more): 1000 rows of
+// 256206 in fp32 with 20 tokens 161 us (6.4 TB/s), 600 rows in bf16 without 55 us
+// (5.6 TB/s; the exponentials alone would take 34); one row with 8 tokens 11 us, the
+// latency of a cluster of eight (7.5 without tokens) and of two merges of lists.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
