@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <utility>
 
 #include "attn_internal.h"
 #include "device_common.cuh"
@@ -102,6 +103,9 @@ void set_division(int d, uint32_t* mul, int* shr) {
     *mul = (uint32_t)(((1ULL << *shr) + (uint64_t)d - 1) / (uint64_t)d);
 }
 
+// Whether a wait of this call is to run out: the hook is for the next call, whatever becomes of it.
+bool take_expire(nllb_attn_ctx* c) { return c && std::exchange(c->expire_next_rows, false); }
+
 int launch(nllb_attn_ctx* c, RowsParams& p, int dtype, int head_dim, bool paged) {
     if (!c) return bad("ctx is NULL");
     if (p.n_seq == 0) return NLLB_ATTN_OK;  // nothing to do
@@ -109,8 +113,6 @@ int launch(nllb_attn_ctx* c, RowsParams& p, int dtype, int head_dim, bool paged)
     set_division(p.group, &p.group_mul, &p.group_shr);
     OnDevice on(c->device);
     cudaError_t e = on.status;
-    p.expire = c->expire_next_rows;
-    c->expire_next_rows = false;
     if (e == cudaSuccess) e = launch_rows(p, static_cast<RowType>(dtype), head_dim, paged, c->num_sms, c->stream);
     if (e != cudaSuccess) return set_error(NLLB_ATTN_ECUDA, std::string("launch_rows: ") + cudaGetErrorString(e));
     return NLLB_ATTN_OK;
@@ -131,11 +133,12 @@ int nllb_attn_test_expire_next_rows_wait(nllb_attn_ctx* c) {
 namespace {
 
 // window: 0 (every position up to its own is visible to a token), or the positions that are, and the first `sinks`.
-int attend_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a, int window, int sinks) {
+int attend_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a, int window, int sinks, bool expire) {
     int rc = check_common(a->dtype, a->head_dim, a->n_heads, a->n_kv_heads, a->n_seq, a->q_rows, a->max_q, a->max_kv,
                           a->scale);
     if (rc) return rc;
     RowsParams p = {};
+    p.expire = expire;
     if (a->n_seq == 0 || a->max_q == 0 || a->q_rows == 0) return launch(c, p, a->dtype, a->head_dim, true);
     if (!a->q || !a->k_pages || !a->v_pages || !a->out || !a->page_table || !a->kv_len)
         return bad("q, k_pages, v_pages, out, page_table and kv_len are required");
@@ -181,24 +184,28 @@ int attend_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a, int window, in
 extern "C" {
 
 int nllb_attn_paged(nllb_attn_ctx* c, const nllb_attn_paged_args* a) {
+    const bool expire = take_expire(c);
     if (!a) return bad("args is NULL");
-    return attend_paged(c, a, 0, 0);
+    return attend_paged(c, a, 0, 0, expire);
 }
 
 int nllb_attn_window(nllb_attn_ctx* c, const nllb_attn_window_args* a) {
+    const bool expire = take_expire(c);
     if (!a) return bad("args is NULL");
     if (a->window < 1) return bad("window must be >= 1");
     if (a->sinks < 0) return bad("sinks must not be negative");
-    return attend_paged(c, &a->cache, a->window, a->sinks);
+    return attend_paged(c, &a->cache, a->window, a->sinks, expire);
 }
 
 int nllb_attn_cross_rows(nllb_attn_ctx* c, const nllb_attn_cross_rows_args* a) {
+    const bool expire = take_expire(c);
     if (!a) return bad("args is NULL");
     int rc = check_common(a->dtype, a->head_dim, a->n_heads, a->n_kv_heads, a->n_seq, a->q_rows, a->max_q, a->max_kv,
                           a->scale);
     if (rc) return rc;
     if (a->kv_rows < 0) return bad("negative size");
     RowsParams p = {};
+    p.expire = expire;
     if (a->n_seq == 0 || a->max_q == 0 || a->q_rows == 0) return launch(c, p, a->dtype, a->head_dim, false);
     if (!a->q || !a->out || !a->kv_len || (a->kv_rows > 0 && (!a->k || !a->v)))
         return bad("q, k, v, out and kv_len are required");

@@ -368,7 +368,8 @@ NLLB_ATTN_API int nllb_attn_append(nllb_attn_ctx* ctx, const nllb_attn_append_ar
  * _cross_rows of this context counts as many rows, a wait of its
  * launch runs out after about 1 ms; it writes no output (paged: the chunk's
  * keys and values may be written) and the next nllb_attn_sync returns
- * NLLB_ATTN_ETIMEOUT.  The context stays usable. */
+ * NLLB_ATTN_ETIMEOUT.  The context stays usable, and calls behind that next one
+ * are as ever, also where it was refused, had no rows or counts few. */
 NLLB_ATTN_API int nllb_attn_test_expire_next_rows_wait(nllb_attn_ctx* ctx);
 
 /* ---- drop-ins for the declared single-head API (pico.h:85-92) -----------
