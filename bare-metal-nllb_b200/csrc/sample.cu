@@ -1143,6 +1143,8 @@ extern "C" int nllb_sample_test_expire_next_wait(void) {
 
 extern "C" int nllb_sample(const nllb_sample_args* s, void* stream) {
     using namespace nllb;
+    const bool expire = t_expire_next;  // (this call's, whatever becomes of it)
+    t_expire_next = false;
     if (!s) return bad("args is NULL");
     if (s->dtype != NLLB_F32 && s->dtype != NLLB_F16 && s->dtype != NLLB_BF16)
         return bad("dtype must be NLLB_F32, NLLB_F16 or NLLB_BF16");
@@ -1158,8 +1160,7 @@ extern "C" int nllb_sample(const nllb_sample_args* s, void* stream) {
     a.logits = s->logits, a.ld = s->ld, a.vocab = s->vocab;
     a.temperature = s->temperature, a.top_k = s->top_k, a.top_p = s->top_p, a.min_p = s->min_p, a.u = s->u;
     a.out_tok = s->out_tok, a.out_logp = s->out_logp;
-    a.expire = t_expire_next;
-    t_expire_next = false;
+    a.expire = expire;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int device = 0, num_sms = 0;
     cudaError_t e = cudaGetDevice(&device);

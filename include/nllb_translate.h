@@ -295,7 +295,8 @@ NLLB_ATTN_API int nllb_sample(const nllb_sample_args* args, void* stream);
 /* Test of the bounded device waits: in the calling thread's next nllb_sample,
  * if it copies its rows to shared memory (it does below 64 MB of logits), a
  * wait of every row runs out after about 1 ms, and every token is
- * NLLB_SAMPLE_TIMEOUT.  Later calls are as ever. */
+ * NLLB_SAMPLE_TIMEOUT.  Later calls are as ever, also where that next one was
+ * refused or had no rows. */
 NLLB_ATTN_API int nllb_sample_test_expire_next_wait(void);
 
 /* ---- log-probabilities of given tokens --------------------------------------
